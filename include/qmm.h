@@ -94,7 +94,8 @@ typedef enum {
   QMM_U8 = 3,
   QMM_U32 = 4,
   QMM_I32 = 5,
-  QMM_I8 = 6               /* zero points of qmm_pack_dense_* only */
+  QMM_I8 = 6,              /* zero points of qmm_pack_dense_* only */
+  QMM_E4M3 = 7             /* a paged cache's entries only (qmm_decode.h) */
 } qmm_elem;
 
 /* Which kernel family a problem is routed to (see qmm_route). */

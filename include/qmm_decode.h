@@ -142,6 +142,98 @@ int qmm_decode_attention(const void* qkv, void* k_cache, void* v_cache, void* ou
                          int64_t ctx, int64_t pos, float theta, int push_slot, int push_site,
                          const qmm_exchange* ex, void* stream);
 
+/* ---- a paged cache: append, attention, reading back -----------------------------------------
+ *
+ * Keys and values of one layer in pages of `page_size` positions, handed out to sequences by a
+ * table: position i of sequence s is row i % page_size of page table[s * table_stride + i / page_size].
+ * A sequence's entries behind its last page are never read. Contiguous keys and values of whole
+ * prompts are attended by qmm_prompt_attention without a cache.
+ *
+ * The new tokens of all sequences lie one behind the other: those of sequence s are rows
+ * cu_q[s] .. cu_q[s + 1] - 1 of q (cu_q NULL: one each, tokens == seqs), and they are the last ones of its
+ * kv_lens[s] positions, so that token i of n stands at position kv_lens[s] - n + i. Rows behind
+ * cu_q[seqs] belong to no sequence and are left as they are. Lengths, starts and tables are int32
+ * on the device and are read by the kernels: nothing is copied to the host, and a captured call
+ * may be replayed with other lengths. A page outside the cache, a length that its table has no
+ * room for and a token before position 0 are reported (QMM_DEVICE_BAD_INDEX, as QMM_ERR_SHAPE from
+ * qmm_poll_status) and never followed: such a page is read as page 0, and not written.
+ *
+ * An e4m3 cache holds a row (one position of one head) as codes under one power of two: with e the
+ * smallest whole number for which the row's largest magnitude is at most 448 * 2^e (between -117 and
+ * 119; 0 for a row of zeros), element x is e4m3(x / 2^e), rounded to nearest even, and the row's E8M0
+ * byte is e + 127. A row with an infinity or a NaN in it has the byte 255 and reads as NaN throughout.
+ * The values of such a cache are exact in bf16, which is what q has to be with it. */
+typedef struct {
+  uint32_t struct_size;     /* sizeof(qmm_paged_cache) */
+  int32_t elem;             /* QMM_BF16, QMM_F16 or QMM_E4M3 */
+  void* k;                  /* [pages, kv_heads, page_size, head_dim], 16-byte aligned */
+  void* v;
+  void* k_exp;              /* e4m3: [pages, kv_heads, page_size] E8M0 bytes, 16-byte aligned; else NULL */
+  void* v_exp;
+  int64_t pages;
+  int32_t kv_heads;
+  int32_t page_size;        /* 16, 32, 64, 128 or 256 */
+  int32_t head_dim;         /* 64 or 128 */
+  int32_t table_width;      /* entries of a sequence's row of the table */
+  const int32_t* table;     /* [seqs, table_width], rows table_stride entries apart */
+  int64_t table_stride;
+} qmm_paged_cache;
+
+/* One row of a fused projection per new token, [q heads | k heads | v heads]: every query and key head is
+ * RMS-normalised (q_norm / k_norm, where given), the first rotary_dim elements of both are rotated by the angles
+ * position * freqs[i] (taken in float64), q goes to q_out and k, v into the cache; float32 arithmetic, one rounding. */
+typedef struct {
+  uint32_t struct_size;     /* sizeof(qmm_append_args) */
+  int32_t elem;             /* QMM_BF16 or QMM_F16: of qkv, q_out, the norms' weights and a 16-bit cache */
+  const void* qkv;          /* [tokens, (heads + 2 kv_heads) * head_dim], rows row_stride elements apart (a multiple of 8) */
+  int64_t row_stride;
+  void* q_out;              /* [tokens, heads, head_dim], contiguous */
+  int64_t tokens, seqs;
+  int32_t heads;
+  int32_t rotary_dim;       /* 0: none; else a multiple of 16 up to head_dim */
+  int32_t interleaved;      /* pairs (2i, 2i + 1) instead of (i, i + rotary_dim / 2) */
+  float eps;
+  const double* freqs;      /* [rotary_dim / 2] radians per position */
+  const void* q_norm;       /* [head_dim], or NULL: no norm */
+  const void* k_norm;
+  const int32_t* kv_lens;   /* [seqs] positions, the new tokens' included */
+  const int32_t* cu_q;      /* [seqs + 1], or NULL */
+} qmm_append_args;
+int qmm_cache_append(const qmm_paged_cache* cache, const qmm_append_args* args, void* stream);
+
+/* Positions 0 .. cu_kv[s + 1] - cu_kv[s] - 1 of every sequence, as values, to rows cu_kv[s] .. of k_out and v_out
+ * [total, kv_heads, head_dim] (QMM_BF16 or QMM_F16; a 16-bit cache's own type). Rows from cu_kv[seqs] on are left as they are. */
+int qmm_cache_read(const qmm_paged_cache* cache, int64_t seqs, const int32_t* cu_kv, int64_t total, int elem, void* k_out,
+                   void* v_out, void* stream);
+
+/* out[t, h] = sum_j softmax_j(scale * q[t, h] . k[j, h / group]) v[j, h / group] over the positions j of t's sequence that t sees:
+ * those up to its own (causal), or all. What stands at other positions has no influence, whatever it is; a token that sees
+ * none is zero. float32 sums and statistics; the weights of the values are rounded to q's type. */
+typedef struct {
+  uint32_t struct_size;     /* sizeof(qmm_attention_args) */
+  int32_t elem;             /* QMM_BF16 or QMM_F16: of q, out, k and v */
+  const void* q;            /* [tokens, heads, head_dim]; strides in elements, multiples of 8; head_dim contiguous */
+  int64_t q_row, q_head;
+  const void* k;            /* qmm_prompt_attention: [tokens, kv_heads, head_dim]; NULL for qmm_paged_attention */
+  int64_t k_row, k_head;
+  const void* v;
+  int64_t v_row, v_head;
+  void* out;                /* [tokens, heads, head_dim], contiguous */
+  int64_t tokens, seqs;
+  int32_t heads, kv_heads;  /* kv_heads divides heads; at most 64 query heads per key head */
+  int32_t head_dim;         /* 64 or 128 */
+  int32_t causal;
+  float scale;              /* > 0 */
+  const int32_t* cu_q;
+  const int32_t* kv_lens;   /* qmm_paged_attention; NULL for qmm_prompt_attention */
+  void* workspace;          /* qmm_attention_workspace_bytes bytes, 16-byte aligned, in any state; not shared by calls that can overlap */
+  int64_t workspace_bytes;
+} qmm_attention_args;
+/* (reads tokens, seqs, heads, kv_heads and head_dim of `args`; negative where they are refused) */
+int64_t qmm_attention_workspace_bytes(const qmm_attention_args* args);
+int qmm_prompt_attention(const qmm_attention_args* args, void* stream);
+int qmm_paged_attention(const qmm_paged_cache* cache, const qmm_attention_args* args, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -78,6 +78,35 @@ class DecodeFusion(ctypes.Structure):
                 ("norm_weight", ctypes.c_void_p), ("eps", ctypes.c_float), ("epilogue", ctypes.c_int32), ("epilogue_out", ctypes.c_void_p)]
 
 
+class PagedCacheArgs(ctypes.Structure):
+    """`qmm_paged_cache` of include/qmm_decode.h."""
+
+    _fields_ = [("struct_size", ctypes.c_uint32), ("elem", ctypes.c_int32), ("k", ctypes.c_void_p), ("v", ctypes.c_void_p),
+                ("k_exp", ctypes.c_void_p), ("v_exp", ctypes.c_void_p), ("pages", ctypes.c_int64), ("kv_heads", ctypes.c_int32),
+                ("page_size", ctypes.c_int32), ("head_dim", ctypes.c_int32), ("table_width", ctypes.c_int32), ("table", ctypes.c_void_p),
+                ("table_stride", ctypes.c_int64)]
+
+
+class AppendArgs(ctypes.Structure):
+    """`qmm_append_args` of include/qmm_decode.h."""
+
+    _fields_ = [("struct_size", ctypes.c_uint32), ("elem", ctypes.c_int32), ("qkv", ctypes.c_void_p), ("row_stride", ctypes.c_int64),
+                ("q_out", ctypes.c_void_p), ("tokens", ctypes.c_int64), ("seqs", ctypes.c_int64), ("heads", ctypes.c_int32),
+                ("rotary_dim", ctypes.c_int32), ("interleaved", ctypes.c_int32), ("eps", ctypes.c_float), ("freqs", ctypes.c_void_p),
+                ("q_norm", ctypes.c_void_p), ("k_norm", ctypes.c_void_p), ("kv_lens", ctypes.c_void_p), ("cu_q", ctypes.c_void_p)]
+
+
+class AttentionArgs(ctypes.Structure):
+    """`qmm_attention_args` of include/qmm_decode.h."""
+
+    _fields_ = [("struct_size", ctypes.c_uint32), ("elem", ctypes.c_int32), ("q", ctypes.c_void_p), ("q_row", ctypes.c_int64), ("q_head", ctypes.c_int64),
+                ("k", ctypes.c_void_p), ("k_row", ctypes.c_int64), ("k_head", ctypes.c_int64),
+                ("v", ctypes.c_void_p), ("v_row", ctypes.c_int64), ("v_head", ctypes.c_int64), ("out", ctypes.c_void_p),
+                ("tokens", ctypes.c_int64), ("seqs", ctypes.c_int64), ("heads", ctypes.c_int32), ("kv_heads", ctypes.c_int32),
+                ("head_dim", ctypes.c_int32), ("causal", ctypes.c_int32), ("scale", ctypes.c_float), ("cu_q", ctypes.c_void_p),
+                ("kv_lens", ctypes.c_void_p), ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_int64)]
+
+
 _lib = None
 
 ctypes.pythonapi.PyCapsule_GetPointer.restype = ctypes.c_void_p
@@ -148,6 +177,12 @@ _SIGNATURES = {
                                                                    ctypes.c_int, ctypes.c_int64, ctypes.c_int64, ctypes.c_float,
                                                                    ctypes.c_int, ctypes.c_int, ctypes.POINTER(Exchange),
                                                                    ctypes.c_void_p]),
+    "qmm_cache_append": (ctypes.c_int, [ctypes.POINTER(PagedCacheArgs), ctypes.POINTER(AppendArgs), ctypes.c_void_p]),
+    "qmm_cache_read": (ctypes.c_int, [ctypes.POINTER(PagedCacheArgs), ctypes.c_int64, ctypes.c_void_p, ctypes.c_int64, ctypes.c_int, ctypes.c_void_p,
+                                      ctypes.c_void_p, ctypes.c_void_p]),
+    "qmm_attention_workspace_bytes": (ctypes.c_int64, [ctypes.POINTER(AttentionArgs)]),
+    "qmm_prompt_attention": (ctypes.c_int, [ctypes.POINTER(AttentionArgs), ctypes.c_void_p]),
+    "qmm_paged_attention": (ctypes.c_int, [ctypes.POINTER(PagedCacheArgs), ctypes.POINTER(AttentionArgs), ctypes.c_void_p]),
     "qmm_route": (ctypes.c_int, [ctypes.POINTER(Problem)]),
     "qmm_gated_matmul_pays": (ctypes.c_int, [ctypes.POINTER(Problem)]),
     "qmm_few_rows_plan": (ctypes.c_int, [ctypes.POINTER(Problem), ctypes.c_int, ctypes.POINTER(ctypes.c_int32)]),

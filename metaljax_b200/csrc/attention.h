@@ -1,0 +1,37 @@
+// The attention kernels' parameters and launchers (attention_rows.cu), and those of the cache kernels (cache_ops.cu). Host and device.
+#pragma once
+
+#include "attention_plan.cuh"
+
+namespace qmm {
+
+struct RowsParams {
+  AttentionWork work;
+  CacheView cache;             // pages
+  const uint8_t* q;
+  const uint8_t* k;            // rows
+  const uint8_t* v;
+  uint8_t* out;
+  float* partial;
+  int64_t q_row, q_head, k_row, k_head, v_row, v_head;       // elements
+  float scale_log2;
+  int32_t least_units;
+};
+
+struct JoinParams {
+  AttentionWork work;
+  uint8_t* out;
+  const float* partial;
+  int32_t ctas, least_units;
+};
+
+int attend_rows_ctas();
+int64_t attend_rows_workspace(int head_dim, int ctas);
+// `source`: 0 rows, 1 pages of 16-bit values, 2 pages of e4m3 codes; `rows`: query rows that a sequence and key head have at most, as far as is known.
+int launch_attend_rows(const RowsParams& p, int elem, int head_dim, int source, int rows, int ctas, cudaStream_t stream);
+
+int launch_append(const CacheView& c, const qmm_append_args& a, int head_dim, bool e4m3, int* status, cudaStream_t stream);
+int launch_cache_read(const CacheView& c, int64_t seqs, const int32_t* cu_kv, int64_t total, int head_dim, int elem, bool e4m3, void* k_out,
+                      void* v_out, int* status, cudaStream_t stream);
+
+}  // namespace qmm

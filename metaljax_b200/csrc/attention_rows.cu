@@ -1,0 +1,511 @@
+// Attention of query tiles of 16, 32 or 64 rows over keys and values in pages (16-bit or e4m3) or in rows, on mma.sync: what one new token a
+// sequence, or a few, take. With few rows a key is used for too little arithmetic to be anything but a stream, so the kernel is
+// built like one: 128 threads, two CTAs an SM, chunks of 64 positions on their way (cp.async, 16-byte pieces under an XOR swizzle that makes
+// ldmatrix conflict-free) while one is worked on, also across the ends of items.
+//
+// One pass: a warp holds 16 rows' queries as A fragments, takes scores of its positions of a chunk, the running maximum m and sum l of
+// 2^(s - m), and adds 2^(s - m) v to its 16 x D sums in registers. RW warps share a tile's rows; the KW = 4 / RW
+// warps on the same rows take 64 / KW positions of a chunk each, and are joined when the item ends. With one row of 16 (RW = 1) a warp reads only what it has asked
+// for itself, and the CTA does not meet but at the ends of items.
+//
+// An e4m3 chunk is turned into bf16 by the warp that asked for it (exactly: 4-bit significands under a power of two), next to the chunk in
+// shared memory.
+//
+// Masked positions: scores are selected, not added to. A value that is no number at a masked position would still be 0 * NaN in the sum, so
+// rows of v behind a sequence's end are zeros (the copies fill them in), and in chunks that some rows see and others do not infinities and NaN
+// are taken out, and put into the sums of the rows that see them at the end (`Specials`).
+#include <climits>
+#include <type_traits>
+
+#include "attention.h"
+#include "qmm_ptx.cuh"
+
+namespace qmm {
+namespace {
+
+using namespace ptx;
+
+constexpr int kThreads = 128, kChunk = 64;
+
+__device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void ldmatrix4t(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+template <typename T>
+__device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  if constexpr (std::is_same<T, __nv_bfloat16>::value)
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  else
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// Whether a pair of 16-bit floats has one without a finite value.
+template <typename T>
+__device__ __forceinline__ bool odd_pair(uint32_t w) {
+  constexpr uint32_t kExp = std::is_same<T, __nv_bfloat16>::value ? 0x7f80u : 0x7c00u;
+  return (w & kExp) == kExp || (w >> 16 & kExp) == kExp;
+}
+
+enum Source { kRowsSource, kPages16, kPages8 };
+
+template <int D, int SOURCE>
+struct RowsLayout {
+  static constexpr bool kE4m3 = SOURCE == kPages8;
+  static constexpr int kStages = kE4m3 ? 4 : 3;
+  static constexpr int kRowBytes = D * (kE4m3 ? 1 : 2);
+  static constexpr int kHalf = kChunk * kRowBytes;                       // keys of a chunk; values follow, then (e4m3) both rows' bytes
+  static constexpr int kStage = 2 * kHalf + (kE4m3 ? 2 * kChunk : 0);
+  static constexpr int kValues = kE4m3 ? 2 * kChunk * D * 2 : 0;         // an e4m3 chunk as bf16
+  static constexpr int kRing = kStages * kStage;
+  static constexpr int kSpecials = 3 * D * 4 + 16;
+  static constexpr int kStats = kChunk * 2 * 4;                          // (maximum, sum) of a warp's rows
+  static constexpr int kBytes = kRing + kValues + kSpecials + kStats + 64;
+};
+
+template <typename T, int D, int RW, int SOURCE>
+__global__ void __launch_bounds__(kThreads, 2) attend_rows_kernel(const RowsParams p) {
+  using L = RowsLayout<D, SOURCE>;
+  constexpr bool kPaged = SOURCE != kRowsSource, kE4m3 = L::kE4m3;
+  constexpr int R = 16 * RW, KW = 4 / RW, SN = kChunk / KW;               // rows of a tile; warps on the same rows; a warp's positions of a chunk
+  using Tiles = AttentionTiles<R, kChunk>;
+  extern __shared__ __align__(128) uint8_t smem[];
+  int* const special = reinterpret_cast<int*>(smem + L::kRing + L::kValues);           // first positions of +inf, -inf, NaN in each column of v
+  int* const any_special = special + 3 * D;
+  float* const stats = reinterpret_cast<float*>(smem + L::kRing + L::kValues + L::kSpecials);
+  const uint32_t ring = smem_u32(smem);
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int rw = warp / KW, kw = warp % KW;
+  const AttentionWork& w = p.work;
+
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  // every warp works out where this CTA begins by itself
+  UnitCursor c;
+  int64_t total, quota = 1;
+  const bool any = find_unit<R, kChunk>(w, [&](int64_t t) { quota = quota_of(t, gridDim.x, p.least_units); return quota * blockIdx.x; }, &total, &c);
+  if (!any) return;
+  const int64_t first_unit = quota * blockIdx.x;
+  const int count = static_cast<int>(total - first_unit < quota ? total - first_unit : quota);
+  UnitCursor load = c;                                  // where the copies are
+
+  // ---- copies: a warp asks for rows 16 * warp .. of a chunk (which lie in one page) ----
+  int64_t page = 0;                                     // of the next chunk's rows of this warp
+  auto look_up = [&](int loaded) {
+    if constexpr (kPaged) {
+      const int pos = load.u * kChunk + 16 * warp;
+      page = 0;
+      if (loaded < count && pos < load.span.len) page = page_of(p.cache, load.s, pos, w.status);
+      if (page < 0) page = 0;
+    }
+  };
+  auto request = [&](int loaded) {                      // the chunk that `load` stands at into the ring, and `load` on
+    if (loaded < count) {
+      const uint32_t stage = ring + (loaded % L::kStages) * L::kStage;
+      constexpr int kPieces = L::kRowBytes / 16;
+      const int pos0 = load.u * kChunk + 16 * warp;
+#pragma unroll
+      for (int i = 0; i < 16 * kPieces / 32; ++i) {
+        const int piece = i * 32 + lane, r = piece / kPieces, col = piece % kPieces;
+        const int pos = pos0 + r;
+        const int there = pos < load.span.len ? 16 : 0;
+        // (rows of 128 bytes and more: eight rows' pieces of one column lie in eight different banks groups)
+        const uint32_t dst = stage + (16 * warp + r) * L::kRowBytes + ((kE4m3 ? col : col ^ (r & 7)) << 4);
+        const uint8_t *ks, *vs;
+        if constexpr (kPaged) {
+          const int64_t row = ((page * w.kv_heads + load.h) << p.cache.page_shift) + (pos & ((1 << p.cache.page_shift) - 1));
+          ks = p.cache.k + row * L::kRowBytes + col * 16;
+          vs = p.cache.v + row * L::kRowBytes + col * 16;
+        } else {
+          const int64_t row = there ? load.span.q0 + pos : 0;
+          ks = p.k + (row * p.k_row + load.h * p.k_head) * 2 + col * 16;
+          vs = p.v + (row * p.v_row + load.h * p.v_head) * 2 + col * 16;
+        }
+        cp_async16(dst, ks, there);
+        cp_async16(dst + L::kHalf, vs, there);
+      }
+      if constexpr (kE4m3) {
+        if (lane < 2) {                                 // the 16 rows' exponent bytes, of k and of v (the positions behind the end: of no use)
+          const int64_t row = ((page * w.kv_heads + load.h) << p.cache.page_shift) + (pos0 & ((1 << p.cache.page_shift) - 1));
+          cp_async16(stage + 2 * L::kHalf + lane * kChunk + 16 * warp, (lane ? p.cache.v_exp : p.cache.k_exp) + row, pos0 < load.span.len ? 16 : 0);
+        }
+      }
+      if (++load.u >= load.units && loaded + 1 < count) next_item<R, kChunk>(w, load);
+      look_up(loaded + 1);
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+
+  look_up(0);
+#pragma unroll
+  for (int i = 0; i < L::kStages - 1; ++i) request(i);
+
+  uint32_t q[D / 16][4];
+  float o[D / 8][4];
+  float m[2], l[2];
+  int limit[2];                                          // last position that the thread's two rows see (-1: none)
+  int tile_first_limit = 0, tile_rows = 0;
+  int begun = 0;                                         // first unit of this item here
+
+  auto begin_item = [&]() {
+    begun = c.u;
+    const int64_t rows = static_cast<int64_t>(c.span.n) * w.group - static_cast<int64_t>(c.t) * R;
+    tile_rows = rows < R ? static_cast<int>(rows) : R;
+    const int64_t row0 = static_cast<int64_t>(c.t) * R;
+    tile_first_limit = w.causal ? c.span.len - c.span.n + static_cast<int>(row0 / w.group) : c.span.len - 1;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int r = rw * 16 + (lane >> 2) + 8 * i;
+      m[i] = -INFINITY;
+      l[i] = 0.0f;
+      limit[i] = -1;
+      const int64_t row = row0 + r;
+      const int tok = static_cast<int>(row / w.group), g = static_cast<int>(row - static_cast<int64_t>(tok) * w.group);
+      const bool live = r < tile_rows;
+      if (live) limit[i] = w.causal ? c.span.len - c.span.n + tok : c.span.len - 1;
+      const uint8_t* src = p.q + ((c.span.q0 + (live ? tok : 0)) * p.q_row + (c.h * w.group + (live ? g : 0)) * p.q_head) * 2 + (lane & 3) * 4;
+#pragma unroll
+      for (int kk = 0; kk < D / 16; ++kk) {
+        q[kk][i] = live ? __ldg(reinterpret_cast<const uint32_t*>(src + kk * 32)) : 0;
+        q[kk][i + 2] = live ? __ldg(reinterpret_cast<const uint32_t*>(src + kk * 32 + 16)) : 0;
+      }
+    }
+#pragma unroll
+    for (int n = 0; n < D / 8; ++n)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) o[n][i] = 0.0f;
+  };
+
+  if (tid == 0) *any_special = 0;
+  for (int i = tid; i < 3 * D; i += kThreads) special[i] = INT_MAX;
+  __syncthreads();
+  begin_item();
+
+  for (int done = 0; done < count; ++done) {
+    asm volatile("cp.async.wait_group %0;" ::"n"(L::kStages - 2) : "memory");
+    if constexpr (KW == 4) __syncwarp(); else __syncthreads();
+    request(done + L::kStages - 1);
+    const uint32_t stage = ring + (done % L::kStages) * L::kStage;
+    const int pos0 = c.u * kChunk;
+    uint32_t keys = stage, values = stage + L::kHalf;
+    if constexpr (kE4m3) {
+      // this warp's 16 rows of both as bf16
+      keys = ring + L::kRing;
+      values = keys + kChunk * D * 2;
+      if constexpr (KW != 4) __syncthreads();             // (the last chunk's are read by other warps)
+      constexpr int kPieces = D / 16;
+      static_assert(16 * kPieces % 32 == 0, "whole passes of a warp");
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+#pragma unroll
+        for (int i = 0; i < 16 * kPieces / 32; ++i) {
+          const int piece = i * 32 + lane, r = 16 * warp + piece / kPieces, col = piece % kPieces;
+          const uint4 codes = lds128<0>(stage + half * L::kHalf + r * D + col * 16);
+          uint32_t byte = 127;
+          if (pos0 + r < c.span.len) byte = *(smem + (stage - ring) + 2 * L::kHalf + half * kChunk + r);
+          const RowFactors f = row_factors(byte);
+          const uint2 a = row_values(codes.x, f), b = row_values(codes.y, f), d = row_values(codes.z, f), e = row_values(codes.w, f);
+          const uint32_t row = (half ? values : keys) + r * D * 2;
+          const uint32_t at0 = row + (((2 * col) ^ (r & 7)) << 4), at1 = row + (((2 * col + 1) ^ (r & 7)) << 4);
+          asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(at0), "r"(a.x), "r"(a.y), "r"(b.x), "r"(b.y) : "memory");
+          asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(at1), "r"(d.x), "r"(d.y), "r"(e.x), "r"(e.y) : "memory");
+        }
+      }
+      if constexpr (KW == 4) __syncwarp(); else __syncthreads();
+    }
+    // a chunk with positions that are this sequence's, but not every row's
+    if (pos0 + kChunk - 1 > tile_first_limit && tile_first_limit < c.span.len - 1) {
+      constexpr int kPieces = D / 8;
+      for (int i = 0; i < 16 * kPieces / 32; ++i) {
+        const int piece = i * 32 + lane, r = 16 * warp + piece / kPieces, col = piece % kPieces;
+        const uint32_t at = values + r * D * 2 + ((col ^ (r & 7)) << 4);
+        const uint4 v = lds128<0>(at);
+        if (odd_pair<T>(v.x) || odd_pair<T>(v.y) || odd_pair<T>(v.z) || odd_pair<T>(v.w)) {
+          uint32_t u[4] = {v.x, v.y, v.z, v.w};
+          for (int e = 0; e < 8; ++e) {
+            const float2 pair = unpack2<T>(u[e >> 1]);
+            const float x = e & 1 ? pair.y : pair.x;
+            if (!(fabsf(x) <= 3.402823466e38f)) {
+              atomicMin(special + (x > 0.0f ? 0 : x < 0.0f ? D : 2 * D) + col * 8 + e, pos0 + r);
+              *any_special = 1;
+              u[e >> 1] &= e & 1 ? 0x0000ffffu : 0xffff0000u;
+            }
+          }
+          asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(u[0]), "r"(u[1]), "r"(u[2]), "r"(u[3]) : "memory");
+        }
+      }
+      if constexpr (KW == 4) __syncwarp(); else __syncthreads();
+    }
+    // ---- scores of this warp's positions ----
+    float s[SN / 8][4];
+#pragma unroll
+    for (int n = 0; n < SN / 8; ++n)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) s[n][i] = 0.0f;
+#pragma unroll
+    for (int n = 0; n < SN / 16; ++n) {
+      const int r = kw * SN + n * 16 + (lane & 7) + ((lane >> 4) << 3);
+#pragma unroll
+      for (int kk = 0; kk < D / 16; ++kk) {
+        uint32_t b[4];
+        ldmatrix4(b, keys + r * D * 2 + (((kk * 2 + ((lane >> 3) & 1)) ^ (r & 7)) << 4));
+        mma16816<T>(s[2 * n], q[kk], b[0], b[1]);
+        mma16816<T>(s[2 * n + 1], q[kk], b[2], b[3]);
+      }
+    }
+    const int warp_pos = pos0 + kw * SN;
+    const bool edge = warp_pos + SN - 1 > tile_first_limit || tile_rows < R;
+    float top[2] = {m[0], m[1]};
+#pragma unroll
+    for (int n = 0; n < SN / 8; ++n)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        float x = s[n][i] * p.scale_log2;
+        if (edge && warp_pos + n * 8 + (lane & 3) * 2 + (i & 1) > limit[i >> 1]) x = -INFINITY;
+        s[n][i] = x;
+        top[i >> 1] = fmaxf(top[i >> 1], x);
+      }
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      top[i] = fmaxf(top[i], __shfl_xor_sync(0xffffffffu, top[i], 1));
+      top[i] = fmaxf(top[i], __shfl_xor_sync(0xffffffffu, top[i], 2));
+      const float base = top[i] == -INFINITY ? 0.0f : top[i];
+      const float shrink = ex2(m[i] - base);
+      m[i] = top[i];
+      l[i] *= shrink;
+#pragma unroll
+      for (int n = 0; n < D / 8; ++n) {
+        o[n][2 * i] *= shrink;
+        o[n][2 * i + 1] *= shrink;
+      }
+#pragma unroll
+      for (int n = 0; n < SN / 8; ++n)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const float x = ex2(s[n][2 * i + e] - base);
+          s[n][2 * i + e] = x;
+          l[i] += x;
+        }
+    }
+    // ---- weights times values ----
+#pragma unroll
+    for (int n = 0; n < SN / 16; ++n) {
+      const uint32_t a[4] = {pack2<T>(s[2 * n][0], s[2 * n][1]), pack2<T>(s[2 * n][2], s[2 * n][3]), pack2<T>(s[2 * n + 1][0], s[2 * n + 1][1]),
+                             pack2<T>(s[2 * n + 1][2], s[2 * n + 1][3])};
+      const int r = kw * SN + n * 16 + (lane & 7) + (((lane >> 3) & 1) << 3);
+#pragma unroll
+      for (int dd = 0; dd < D / 16; ++dd) {
+        uint32_t b[4];
+        ldmatrix4t(b, values + r * D * 2 + (((dd * 2 + (lane >> 4)) ^ (r & 7)) << 4));
+        mma16816<T>(o[2 * dd], a, b[0], b[1]);
+        mma16816<T>(o[2 * dd + 1], a, b[2], b[3]);
+      }
+    }
+    ++c.u;
+    if (c.u < c.units && done + 1 < count) continue;
+
+    // ---- the item, or this CTA's part of it, ends: its warps' sums meet where the chunk was (e4m3: where its values were) ----
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      l[i] += __shfl_xor_sync(0xffffffffu, l[i], 1);
+      l[i] += __shfl_xor_sync(0xffffffffu, l[i], 2);
+    }
+    __syncthreads();
+    float* const sums = reinterpret_cast<float*>(kE4m3 ? smem + L::kRing : smem + (stage - ring));    // [4 warps][16 rows][D]
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int r = warp * 16 + (lane >> 2) + 8 * i;
+      if ((lane & 3) == 0) {
+        stats[r] = m[i];
+        stats[kChunk + r] = l[i];
+      }
+#pragma unroll
+      for (int n = 0; n < D / 8; ++n)
+        *reinterpret_cast<float2*>(sums + r * D + ((n * 8 + (lane & 3) * 2) ^ ((r & 3) << 3))) = make_float2(o[n][2 * i], o[n][2 * i + 1]);
+    }
+    __syncthreads();
+    const bool first = begun == 0, last = c.u == c.units;
+    const bool odd = *any_special != 0;
+    float* const part = p.partial + (2 * static_cast<int64_t>(blockIdx.x) + (first ? 1 : 0)) * partial_floats<R, D>();
+    constexpr int kVec = D / 4;                           // threads of a row
+    for (int i = tid; i < tile_rows * kVec; i += kThreads) {
+      const int r = i / kVec, d = (i % kVec) * 4;
+      const int64_t row = static_cast<int64_t>(c.t) * R + r;
+      const int tok = static_cast<int>(row / w.group), g = static_cast<int>(row - static_cast<int64_t>(tok) * w.group);
+      const int seen = w.causal ? c.span.len - c.span.n + tok : c.span.len - 1;
+      float mm = -INFINITY, ll = 0.0f, v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+      for (int k = 0; k < KW; ++k) mm = fmaxf(mm, stats[((r / 16) * KW + k) * 16 + r % 16]);
+      const float base = mm == -INFINITY ? 0.0f : mm;
+#pragma unroll
+      for (int k = 0; k < KW; ++k) {
+        const int sr = ((r / 16) * KW + k) * 16 + r % 16;
+        const float f = ex2(stats[sr] - base);
+        ll = fmaf(f, stats[kChunk + sr], ll);
+        const float4 x = *reinterpret_cast<const float4*>(sums + sr * D + (d ^ ((sr & 3) << 3)));
+        v[0] = fmaf(f, x.x, v[0]);
+        v[1] = fmaf(f, x.y, v[1]);
+        v[2] = fmaf(f, x.z, v[2]);
+        v[3] = fmaf(f, x.w, v[3]);
+      }
+      if (odd) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          if (special[d + e] <= seen) v[e] += INFINITY;
+          if (special[D + d + e] <= seen) v[e] -= INFINITY;
+          if (special[2 * D + d + e] <= seen) v[e] = NAN;
+        }
+      }
+      if (first && last) {
+        // no weight at all: a row that sees nothing is zero; one that sees only scores of -inf has no softmax
+        const float inv = ll == 0.0f ? (seen < 0 ? 0.0f : NAN) : 1.0f / ll;
+        uint2 out;
+        out.x = pack2<T>(v[0] * inv, v[1] * inv);
+        out.y = pack2<T>(v[2] * inv, v[3] * inv);
+        *reinterpret_cast<uint2*>(p.out + ((static_cast<int64_t>(c.span.q0) + tok) * w.heads + c.h * w.group + g) * D * 2 + d * 2) = out;
+      } else {
+        *reinterpret_cast<float4*>(part + r * D + d) = make_float4(v[0], v[1], v[2], v[3]);
+        if (d == 0) {
+          part[R * D + r] = mm;
+          part[R * D + R + r] = ll;
+        }
+      }
+    }
+    if (odd) {
+      __syncthreads();
+      for (int i = tid; i < 3 * D; i += kThreads) special[i] = INT_MAX;
+      if (tid == 0) *any_special = 0;
+    }
+    __syncthreads();
+    if (done + 1 < count) {
+      next_item<R, kChunk>(w, c);
+      begin_item();
+    }
+  }
+  asm volatile("cp.async.wait_all;" ::: "memory");
+}
+
+// Items whose units fell to several CTAs: block b looks at the end of CTA b's share, and joins the item there if it is cut there first.
+constexpr int kJoinThreads = 512;
+template <typename T, int D, int R, int B>
+__global__ void __launch_bounds__(kJoinThreads) attend_join_kernel(const JoinParams p) {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const AttentionWork& w = p.work;
+  UnitCursor c;
+  int64_t total, quota = 1;
+  const bool any = find_unit<R, B>(w, [&](int64_t t) { quota = quota_of(t, p.ctas, p.least_units); return quota * (blockIdx.x + 1); }, &total, &c);
+  if (!any || c.u == 0 || c.u > quota) return;
+  const int64_t start = quota * (blockIdx.x + 1) - c.u;                          // the item's first unit
+  const int parts = static_cast<int>((start + c.units - 1) / quota) - blockIdx.x + 1;
+  const int64_t rows = static_cast<int64_t>(c.span.n) * w.group - static_cast<int64_t>(c.t) * R;
+  const int tile_rows = rows < R ? static_cast<int>(rows) : R;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  constexpr int V = D / 32;                                                       // elements of a lane
+  auto part_of = [&](int i) { return p.partial + (2 * (static_cast<int64_t>(blockIdx.x) + i) + (i == 0 ? 1 : 0)) * partial_floats<R, D>(); };
+  for (int r = warp; r < tile_rows; r += kJoinThreads / 32) {
+    float mm = -INFINITY;
+    for (int i = lane; i < parts; i += 32) mm = fmaxf(mm, part_of(i)[R * D + r]);
+#pragma unroll
+    for (int x = 16; x > 0; x >>= 1) mm = fmaxf(mm, __shfl_xor_sync(0xffffffffu, mm, x));
+    const float base = mm == -INFINITY ? 0.0f : mm;
+    float ll = 0.0f, v[V] = {};
+    for (int i0 = 0; i0 < parts; i0 += 32) {
+      float f = 0.0f;
+      if (i0 + lane < parts) {
+        const float* part = part_of(i0 + lane);
+        f = ex2(part[R * D + r] - base);
+        ll = fmaf(f, part[R * D + R + r], ll);
+      }
+      const int here = parts - i0 < 32 ? parts - i0 : 32;
+#pragma unroll 8
+      for (int i = 0; i < here; ++i) {
+        const float fi = __shfl_sync(0xffffffffu, f, i);
+        const float* src = part_of(i0 + i) + r * D + lane * V;
+        if constexpr (V == 4) {
+          const float4 x = *reinterpret_cast<const float4*>(src);
+          v[0] = fmaf(fi, x.x, v[0]);
+          v[1] = fmaf(fi, x.y, v[1]);
+          v[2] = fmaf(fi, x.z, v[2]);
+          v[3] = fmaf(fi, x.w, v[3]);
+        } else {
+          const float2 x = *reinterpret_cast<const float2*>(src);
+          v[0] = fmaf(fi, x.x, v[0]);
+          v[1] = fmaf(fi, x.y, v[1]);
+        }
+      }
+    }
+#pragma unroll
+    for (int x = 16; x > 0; x >>= 1) ll += __shfl_xor_sync(0xffffffffu, ll, x);
+    const int64_t row = static_cast<int64_t>(c.t) * R + r;
+    const int tok = static_cast<int>(row / w.group), g = static_cast<int>(row - static_cast<int64_t>(tok) * w.group);
+    const int seen = w.causal ? c.span.len - c.span.n + tok : c.span.len - 1;
+    const float inv = ll == 0.0f ? (seen < 0 ? 0.0f : NAN) : 1.0f / ll;
+    uint8_t* dst = p.out + ((static_cast<int64_t>(c.span.q0) + tok) * w.heads + c.h * w.group + g) * D * 2 + lane * V * 2;
+#pragma unroll
+    for (int e = 0; e < V; e += 2) *reinterpret_cast<uint32_t*>(dst + e * 2) = pack2<T>(v[e] * inv, v[e + 1] * inv);
+  }
+}
+
+template <typename T, int D, int RW, int SOURCE>
+int launch_one(const RowsParams& p, int ctas, cudaStream_t stream) {
+  static bool done[kMaxDevices] = {};
+  const int dev = current_device();
+  if (dev < 0) return QMM_ERR_DEVICE;
+  if (!done[dev]) {
+    const cudaError_t e = cudaFuncSetAttribute(attend_rows_kernel<T, D, RW, SOURCE>, cudaFuncAttributeMaxDynamicSharedMemorySize, RowsLayout<D, SOURCE>::kBytes);
+    if (e != cudaSuccess) return fail(QMM_ERR_CUDA, "cudaFuncSetAttribute: %s", cudaGetErrorString(e));
+    done[dev] = true;
+  }
+  launch_early(attend_rows_kernel<T, D, RW, SOURCE>, ctas, kThreads, RowsLayout<D, SOURCE>::kBytes, stream, p);
+  count_launch();
+  if (int rc = check_launch("attend_rows_kernel")) return rc;
+  if (ctas < 2) return QMM_OK;
+  JoinParams j = {};
+  j.work = p.work;
+  j.out = p.out;
+  j.partial = p.partial;
+  j.ctas = ctas;
+  j.least_units = p.least_units;
+  launch_early(attend_join_kernel<T, D, 16 * RW, kChunk>, ctas - 1, kJoinThreads, 0, stream, j);
+  count_launch();
+  return check_launch("attend_join_kernel");
+}
+
+template <typename T, int D, int SOURCE>
+int launch_rows_of(const RowsParams& p, int rows, int ctas, cudaStream_t stream) {
+  if (rows <= 16) return launch_one<T, D, 1, SOURCE>(p, ctas, stream);
+  if (rows <= 32) return launch_one<T, D, 2, SOURCE>(p, ctas, stream);
+  return launch_one<T, D, 4, SOURCE>(p, ctas, stream);
+}
+
+template <typename T, int D>
+int launch_source(const RowsParams& p, int source, int rows, int ctas, cudaStream_t stream) {
+  if (source == kRowsSource) return launch_one<T, D, 4, kRowsSource>(p, ctas, stream);
+  if (source == kPages16) return launch_rows_of<T, D, kPages16>(p, rows, ctas, stream);
+  if constexpr (std::is_same<T, __nv_bfloat16>::value) return launch_rows_of<T, D, kPages8>(p, rows, ctas, stream);
+  return fail(QMM_ERR_UNSUPPORTED, "attention: an e4m3 cache is attended with bf16 queries");
+}
+
+}  // namespace
+
+int attend_rows_ctas() { return 2 * device_sm_count(); }
+
+int64_t attend_rows_workspace(int head_dim, int ctas) {
+  return 2ll * ctas * (head_dim == 64 ? partial_floats<64, 64>() : partial_floats<64, 128>()) * 4;
+}
+
+int launch_attend_rows(const RowsParams& p, int elem, int head_dim, int source, int rows, int ctas, cudaStream_t stream) {
+  if (elem == QMM_BF16) return head_dim == 64 ? launch_source<__nv_bfloat16, 64>(p, source, rows, ctas, stream) : launch_source<__nv_bfloat16, 128>(p, source, rows, ctas, stream);
+  return head_dim == 64 ? launch_source<__half, 64>(p, source, rows, ctas, stream) : launch_source<__half, 128>(p, source, rows, ctas, stream);
+}
+
+}  // namespace qmm

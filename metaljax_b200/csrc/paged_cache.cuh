@@ -1,0 +1,127 @@
+// What the kernels on a paged cache share: sequences and positions of packed rows, page lookup with its checks, and the rows of an e4m3 cache.
+// Device code, but for the view.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+
+#include "../../include/qmm_decode.h"
+#include "qmm_internal.h"
+
+namespace qmm {
+
+// A checked qmm_paged_cache as the kernels take it.
+struct CacheView {
+  uint8_t* k;
+  uint8_t* v;
+  uint8_t* k_exp;
+  uint8_t* v_exp;
+  const int32_t* table;
+  int64_t table_stride;
+  int64_t pages;
+  int32_t table_width;
+  int32_t page_shift;
+  int32_t kv_heads;
+};
+
+__device__ __forceinline__ void report_index(int* status) { atomicCAS(status, 0, QMM_DEVICE_BAD_INDEX); }
+
+// Sequence of packed row `row`: the last s with starts[s] <= row, or -1 for a row of none.
+__device__ __forceinline__ int sequence_of(const int32_t* __restrict__ starts, int seqs, int row) {
+  if (row < starts[0] || row >= starts[seqs]) return -1;
+  int lo = 0, hi = seqs;                               // starts[lo] <= row < starts[hi]
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (starts[mid] <= row) lo = mid; else hi = mid;
+  }
+  return lo;
+}
+
+// Page of a position, or -1 (reported): no such entry, or a page that the cache does not have.
+__device__ __forceinline__ int64_t page_of(const CacheView& c, int seq, int pos, int* status) {
+  const int entry = pos >> c.page_shift;
+  if (pos < 0 || entry >= c.table_width) {
+    report_index(status);
+    return -1;
+  }
+  const int page = __ldg(c.table + seq * c.table_stride + entry);
+  if (page < 0 || page >= c.pages) {
+    report_index(status);
+    return -1;
+  }
+  return page;
+}
+
+// ---- rows of an e4m3 cache ----
+// The exponent e of a row whose largest magnitude is `big` (finite): the smallest whole number with big <= 448 * 2^e, 448 = 1.75 * 2^8.
+__device__ __forceinline__ int row_exponent(float big) {
+  if (big == 0.0f) return 0;
+  int x;
+  const float m = frexpf(big, &x);                     // big = m * 2^x, m in [0.5, 1); 448 = 0.875 * 2^9
+  const int e = x - (m > 0.875f ? 8 : 9);
+  return e < -117 ? -117 : e > 119 ? 119 : e;
+}
+
+__device__ __forceinline__ uint32_t e4m3_pair(float lo, float hi) {
+  uint16_t r;
+  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+
+// What turns a row's codes into bf16, as two factors (pairs of bf16): a code's bits as a bf16 are its value times 2^-120, subnormal codes
+// among them (subnormal bf16 operands are taken as they are). The second factor is 1 but for rows above 57344.
+struct RowFactors {
+  uint32_t first, second;
+};
+__device__ __forceinline__ RowFactors row_factors(uint32_t exp_byte) {
+  const int e = static_cast<int>(exp_byte) - 127;
+  const int a = e > 7 ? 127 : 120 + e;
+  const uint32_t f = exp_byte == 255 ? 0x7fc0u : static_cast<uint32_t>(a + 127) << 7;
+  const uint32_t g = static_cast<uint32_t>((exp_byte != 255 && e > 7 ? e - 7 : 0) + 127) << 7;
+  return {f | f << 16, g | g << 16};
+}
+
+__device__ __forceinline__ uint32_t mul_bf16x2(uint32_t a, uint32_t b) {
+  const __nv_bfloat162 r = __hmul2(*reinterpret_cast<const __nv_bfloat162*>(&a), *reinterpret_cast<const __nv_bfloat162*>(&b));
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
+
+// Four codes -> four bf16 (two words).
+__device__ __forceinline__ uint2 row_values(uint32_t codes, const RowFactors& f) {
+  const uint32_t x = __byte_perm(codes, 0, 0x1404), y = __byte_perm(codes, 0, 0x3424);     // a code in the upper byte of each half
+  uint32_t a = ((x >> 4) & 0x07f007f0u) | (x & 0x80008000u), b = ((y >> 4) & 0x07f007f0u) | (y & 0x80008000u);
+  a = mul_bf16x2(a, f.first);
+  b = mul_bf16x2(b, f.first);
+  if (f.second != 0x3f803f80u) {
+    a = mul_bf16x2(a, f.second);
+    b = mul_bf16x2(b, f.second);
+  }
+  return make_uint2(a, b);
+}
+
+// ---- 16-bit floats ----
+template <typename T>
+__device__ __forceinline__ float2 unpack2(uint32_t w);
+template <>
+__device__ __forceinline__ float2 unpack2<__nv_bfloat16>(uint32_t w) {
+  return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+}
+template <>
+__device__ __forceinline__ float2 unpack2<__half>(uint32_t w) {
+  return __half22float2(*reinterpret_cast<const __half2*>(&w));
+}
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi);
+template <>
+__device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float lo, float hi) {
+  const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+template <>
+__device__ __forceinline__ uint32_t pack2<__half>(float lo, float hi) {
+  const __half2 v = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+
+}  // namespace qmm
