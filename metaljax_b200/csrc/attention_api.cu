@@ -46,7 +46,10 @@ int check_attention(const char* what, const qmm_attention_args* a) {
   return QMM_OK;
 }
 
-int64_t workspace_of(const qmm_attention_args* a) { return attend_rows_workspace(a->head_dim, attend_rows_ctas()); }
+int64_t workspace_of(const qmm_attention_args* a) {
+  const int64_t rows = attend_rows_workspace(a->head_dim, attend_rows_ctas()), tc = attend_tc_workspace(a->head_dim, attend_tc_ctas());
+  return rows > tc ? rows : tc;
+}
 
 int attend(const char* what, const qmm_paged_cache* cache, const CacheView* view, const qmm_attention_args* a, cudaStream_t stream) {
   if (a->elem != QMM_BF16 && a->elem != QMM_F16) return fail(QMM_ERR_DTYPE, "%s: q is bf16 or f16", what);
@@ -86,6 +89,9 @@ int attend(const char* what, const qmm_paged_cache* cache, const CacheView* view
   }
   const int64_t rows = (a->cu_q ? a->tokens : 1) * p.work.group;
   const int source = !view ? 0 : cache->elem == QMM_E4M3 ? 2 : 1;
+  const bool tc = a->cu_q && a->tokens * p.work.group > 64 * a->seqs && source != 2 &&
+                  (!view || (static_cast<uint64_t>(p.cache.pages) * p.work.kv_heads << p.cache.page_shift) < (1ull << 31));
+  if (tc) return launch_attend_tc(p, a->elem, a->head_dim, view != nullptr, attend_tc_ctas(), stream);
   return launch_attend_rows(p, a->elem, a->head_dim, source, rows < 64 ? static_cast<int>(rows) : 64, attend_rows_ctas(), stream);
 }
 

@@ -1,7 +1,8 @@
 // How the work of an attention call is shared out, from lengths that only the device knows.
 //
 // An item is a tile of query rows of one sequence and key head: row r of a sequence's n * group rows is new token r / group, query
-// head r % group of the key head's (so that a group's heads read its keys once), R rows a tile. A unit is a block of B positions of an item's keys. All units stand in
+// head r % group of the key head's (so that a group's heads read its keys once). RowTiles takes R rows a tile, wherever tokens begin; TokenTiles (whose
+// queries come as boxes of whole tokens) two halves of tile_tokens tokens. A unit is a block of B positions of an item's keys. All units stand in
 // one order (sequence, head, tile, block), and CTA c of C works on those from c * quota on: every CTA has the same number of units whatever the lengths are. An item whose units fall to several CTAs
 // leaves a partial result with each (two slots a CTA: an item that it finishes, and one that it begins), which a second launch joins: that one works
 // out the same order. There are no atomics and no state between calls, and sums do not depend on timing.
@@ -18,6 +19,7 @@ struct AttentionWork {
   int64_t longest;             // positions that a table has room for
   int32_t seqs, heads, kv_heads, group;
   int32_t causal;
+  int32_t tile_tokens;         // TokenTiles: tokens of half a tile
   int* status;
 };
 
@@ -48,21 +50,32 @@ __device__ __forceinline__ SeqSpan span_of(const AttentionWork& w, int s) {
   return r;
 }
 
+// Positions up to which the last of a sequence's first `tokens` new tokens sees.
+__device__ __forceinline__ int seen_by(const AttentionWork& w, const SeqSpan& s, int64_t tokens) {
+  const int end = w.causal ? s.len - s.n + (tokens < s.n ? static_cast<int>(tokens) : s.n) : s.len;
+  return end < 0 ? 0 : end;
+}
+
+// (rows of a sequence can pass 2^31: 64 heads of a group times its tokens)
 template <int R, int B>
-struct AttentionTiles {
-  // (rows of a sequence can pass 2^31: 64 heads of a group times its tokens)
+struct RowTiles {
   static __device__ __forceinline__ int tiles(const AttentionWork& w, const SeqSpan& s) {
     return static_cast<int>((static_cast<int64_t>(s.n) * w.group + R - 1) / R);
   }
-  // Positions up to which the last row of tile t sees, and the units that makes: one at least, which writes the zeros of rows that see none.
-  static __device__ __forceinline__ int seen(const AttentionWork& w, const SeqSpan& s, int t) {
-    if (!w.causal) return s.len;
-    const int64_t last = ((static_cast<int64_t>(t) + 1) * R - 1) / w.group;
-    const int end = s.len - s.n + (last < s.n - 1 ? static_cast<int>(last) : s.n - 1) + 1;
-    return end < 0 ? 0 : end;
+  // One unit at least, which writes the zeros of rows that see nothing.
+  static __device__ __forceinline__ int units(const AttentionWork& w, const SeqSpan& s, int t) {
+    const int u = (seen_by(w, s, ((static_cast<int64_t>(t) + 1) * R - 1) / w.group + 1) + B - 1) / B;
+    return u < 1 ? 1 : u;
+  }
+};
+
+template <int B>
+struct TokenTiles {
+  static __device__ __forceinline__ int tiles(const AttentionWork& w, const SeqSpan& s) {
+    return (s.n + 2 * w.tile_tokens - 1) / (2 * w.tile_tokens);
   }
   static __device__ __forceinline__ int units(const AttentionWork& w, const SeqSpan& s, int t) {
-    const int u = (seen(w, s, t) + B - 1) / B;
+    const int u = (seen_by(w, s, (static_cast<int64_t>(t) + 1) * 2 * w.tile_tokens) + B - 1) / B;
     return u < 1 ? 1 : u;
   }
 };
@@ -74,9 +87,8 @@ struct UnitCursor {
 };
 
 // One warp: a sequence's units of one head, its lanes over the tiles.
-template <int R, int B>
+template <typename Tiles>
 __device__ __forceinline__ int64_t warp_units(const AttentionWork& w, const SeqSpan& s) {
-  using Tiles = AttentionTiles<R, B>;
   const int n = Tiles::tiles(w, s);
   int64_t sum = 0;
   for (int t = threadIdx.x & 31; t < n; t += 32) sum += Tiles::units(w, s, t);
@@ -86,9 +98,8 @@ __device__ __forceinline__ int64_t warp_units(const AttentionWork& w, const SeqS
 }
 
 // One warp: units of one head of 32 sequences from `base` on, a lane each (0 behind the last).
-template <int R, int B>
+template <typename Tiles>
 __device__ __forceinline__ int64_t lane_units(const AttentionWork& w, int base, SeqSpan* mine) {
-  using Tiles = AttentionTiles<R, B>;
   const int s = base + (threadIdx.x & 31);
   SeqSpan span = {0, 0, 0};
   if (s < w.seqs) span = span_of(w, s);
@@ -101,7 +112,7 @@ __device__ __forceinline__ int64_t lane_units(const AttentionWork& w, int base, 
     const int l = __ffs(many) - 1;
     many &= many - 1;
     const SeqSpan other = {__shfl_sync(0xffffffffu, span.q0, l), __shfl_sync(0xffffffffu, span.n, l), __shfl_sync(0xffffffffu, span.len, l)};
-    const int64_t all = warp_units<R, B>(w, other);
+    const int64_t all = warp_units<Tiles>(w, other);
     if ((threadIdx.x & 31) == l) sum = all;
   }
   *mine = span;
@@ -123,14 +134,13 @@ __device__ __forceinline__ int64_t warp_scan(int64_t v) {          // inclusive
 }
 
 // One warp: the units of a call, and the place of unit `index(total)` in their order (false: there is none).
-template <int R, int B, typename Index>
-__device__ bool find_unit(const AttentionWork& w, Index index, int64_t* total_out, UnitCursor* at) {
-  using Tiles = AttentionTiles<R, B>;
+template <typename Tiles, typename Index>
+__device__ __forceinline__ bool find_unit(const AttentionWork& w, Index index, int64_t* total_out, UnitCursor* at) {
   const int lane = threadIdx.x & 31;
   SeqSpan span;
   int64_t mine = 0, total = 0;
   for (int base = 0; base < w.seqs; base += 32) {
-    mine = lane_units<R, B>(w, base, &span);
+    mine = lane_units<Tiles>(w, base, &span);
     total += warp_sum(mine) * w.kv_heads;
   }
   *total_out = total;
@@ -138,7 +148,7 @@ __device__ bool find_unit(const AttentionWork& w, Index index, int64_t* total_ou
   if (left < 0 || left >= total) return false;
   int64_t per_head = 0;
   for (int base = 0; base < w.seqs; base += 32) {
-    if (w.seqs > 32) mine = lane_units<R, B>(w, base, &span);       // (the only ones are still there)
+    if (w.seqs > 32) mine = lane_units<Tiles>(w, base, &span);       // (the only ones are still there)
     const int64_t upto = warp_scan(mine) * w.kv_heads;
     const unsigned past = __ballot_sync(0xffffffffu, upto > left);
     if (past) {
@@ -151,8 +161,11 @@ __device__ bool find_unit(const AttentionWork& w, Index index, int64_t* total_ou
     }
     left -= __shfl_sync(0xffffffffu, upto, 31);
   }
-  at->h = static_cast<int>(left / per_head);
-  left -= static_cast<int64_t>(at->h) * per_head;
+  at->h = 0;
+  while (left >= per_head) {                            // (a few heads: a division of 64 bits is a call, and spills)
+    left -= per_head;
+    ++at->h;
+  }
   const int tiles = Tiles::tiles(w, at->span);
   for (int base = 0; base < tiles; base += 32) {
     const int64_t u = base + lane < tiles ? Tiles::units(w, at->span, base + lane) : 0;
@@ -171,9 +184,8 @@ __device__ bool find_unit(const AttentionWork& w, Index index, int64_t* total_ou
 }
 
 // To the first unit of the next item (which there has to be).
-template <int R, int B>
+template <typename Tiles>
 __device__ __forceinline__ void next_item(const AttentionWork& w, UnitCursor& c) {
-  using Tiles = AttentionTiles<R, B>;
   c.u = 0;
   if (++c.t >= Tiles::tiles(w, c.span)) {
     c.t = 0;
@@ -188,10 +200,17 @@ __device__ __forceinline__ void next_item(const AttentionWork& w, UnitCursor& c)
   c.units = Tiles::units(w, c.span, c.t);
 }
 
-// Units of a CTA: at least `least`, below which a CTA's share does not pay for a part of an item to be joined.
+// Units of a CTA: at least `least`, below which a CTA's share does not pay for a part of an item to be joined. (Divisions of 64 bits are calls, and spill
+// what is live around them.)
 __device__ __forceinline__ int64_t quota_of(int64_t total, int ctas, int least) {
-  const int64_t q = (total + ctas - 1) / ctas;
+  int shift = 0;
+  while ((total + ctas) >> shift >> 32) shift += 8;     // (a larger share than need be where units pass 2^32)
+  const int64_t q = shift ? (static_cast<int64_t>(static_cast<uint32_t>(total >> shift) / ctas) + 1) << shift : static_cast<uint32_t>(total + ctas - 1) / ctas;
   return q < least ? least : q;
+}
+// CTAs that have a part of an item of which `after` units lie behind the end of the first one's share.
+__device__ __forceinline__ int parts_of(int after, int64_t quota) {
+  return 1 + (quota >> 31 ? 1 : static_cast<int>((static_cast<uint32_t>(after) + static_cast<uint32_t>(quota) - 1) / static_cast<uint32_t>(quota)));
 }
 
 // A partial result in the workspace: R rows of D float32 sums, then R maxima (base 2) and R sums of weights.

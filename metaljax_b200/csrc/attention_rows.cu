@@ -76,7 +76,7 @@ __global__ void __launch_bounds__(kThreads, 2) attend_rows_kernel(const RowsPara
   using L = RowsLayout<D, SOURCE>;
   constexpr bool kPaged = SOURCE != kRowsSource, kE4m3 = L::kE4m3;
   constexpr int R = 16 * RW, KW = 4 / RW, SN = kChunk / KW;               // rows of a tile; warps on the same rows; a warp's positions of a chunk
-  using Tiles = AttentionTiles<R, kChunk>;
+  using Tiles = RowTiles<R, kChunk>;
   extern __shared__ __align__(128) uint8_t smem[];
   int* const special = reinterpret_cast<int*>(smem + L::kRing + L::kValues);           // first positions of +inf, -inf, NaN in each column of v
   int* const any_special = special + 3 * D;
@@ -91,7 +91,7 @@ __global__ void __launch_bounds__(kThreads, 2) attend_rows_kernel(const RowsPara
   // every warp works out where this CTA begins by itself
   UnitCursor c;
   int64_t total, quota = 1;
-  const bool any = find_unit<R, kChunk>(w, [&](int64_t t) { quota = quota_of(t, gridDim.x, p.least_units); return quota * blockIdx.x; }, &total, &c);
+  const bool any = find_unit<Tiles>(w, [&](int64_t t) { quota = quota_of(t, gridDim.x, p.least_units); return quota * blockIdx.x; }, &total, &c);
   if (!any) return;
   const int64_t first_unit = quota * blockIdx.x;
   const int count = static_cast<int>(total - first_unit < quota ? total - first_unit : quota);
@@ -138,7 +138,7 @@ __global__ void __launch_bounds__(kThreads, 2) attend_rows_kernel(const RowsPara
           cp_async16(stage + 2 * L::kHalf + lane * kChunk + 16 * warp, (lane ? p.cache.v_exp : p.cache.k_exp) + row, pos0 < load.span.len ? 16 : 0);
         }
       }
-      if (++load.u >= load.units && loaded + 1 < count) next_item<R, kChunk>(w, load);
+      if (++load.u >= load.units && loaded + 1 < count) next_item<Tiles>(w, load);
       look_up(loaded + 1);
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
@@ -386,7 +386,7 @@ __global__ void __launch_bounds__(kThreads, 2) attend_rows_kernel(const RowsPara
     }
     __syncthreads();
     if (done + 1 < count) {
-      next_item<R, kChunk>(w, c);
+      next_item<Tiles>(w, c);
       begin_item();
     }
   }
@@ -402,10 +402,9 @@ __global__ void __launch_bounds__(kJoinThreads) attend_join_kernel(const JoinPar
   const AttentionWork& w = p.work;
   UnitCursor c;
   int64_t total, quota = 1;
-  const bool any = find_unit<R, B>(w, [&](int64_t t) { quota = quota_of(t, p.ctas, p.least_units); return quota * (blockIdx.x + 1); }, &total, &c);
+  const bool any = find_unit<RowTiles<R, B>>(w, [&](int64_t t) { quota = quota_of(t, p.ctas, p.least_units); return quota * (blockIdx.x + 1); }, &total, &c);
   if (!any || c.u == 0 || c.u > quota) return;
-  const int64_t start = quota * (blockIdx.x + 1) - c.u;                          // the item's first unit
-  const int parts = static_cast<int>((start + c.units - 1) / quota) - blockIdx.x + 1;
+  const int parts = parts_of(c.units - c.u, quota);
   const int64_t rows = static_cast<int64_t>(c.span.n) * w.group - static_cast<int64_t>(c.t) * R;
   const int tile_rows = rows < R ? static_cast<int>(rows) : R;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;

@@ -1,0 +1,724 @@
+// Attention of query tiles of up to 2 x 128 rows on tcgen05: prompts, and chunks of new tokens over a cache.
+//
+//   S = Q K^T             both from shared memory (TMA, 128-byte swizzle), [128 x 128] float32 in tensor memory
+//   P = 2^(S scale - m)   by the thread that owns the row: tcgen05.ld -> registers -> 16-bit -> tcgen05.st over S's own columns
+//   O += P V              P is the A operand in tensor memory, V the B operand as it lies, positions by elements (MN-major)
+//
+// A tile is two halves of 128 rows (whole tokens of the group's heads, so that a key is read once for all of them) on the same keys: while one
+// half's 128 threads take the exponentials of a block of 128 positions, the tensor cores work for the other one. Tensor memory is full with both
+// halves' S and O (512 columns), so one CTA an SM, persistent: its share of the call's units is a range of their order (attention_plan.cuh).
+//
+// The running maximum is followed loosely: O is only scaled down when a row's maximum has risen by more than a factor of 2^8 (no warp does it for less),
+// so that O stays in tensor memory; weights up to 2^8 are as exact as ones below 1 in a floating format. S's barrier says that the block before has
+// been added up (MMAs complete in order), so scaling O needs none of its own.
+//
+// Masked positions: scores are selected. Two helper warps look at the blocks of v that some row does not see all of, before the tensor cores
+// do: rows behind the sequence's end become zeros (0 times what stands in a page behind the end may be NaN), and infinities and NaN that only some
+// rows see are taken out and put into those rows' sums at the end.
+//
+// Warps: 0..3 and 4..7 the halves' rows, 8 the MMAs' issuer, 9 the copies, 10 and 11 helpers. Waits are bounded, as everywhere.
+#include <climits>
+#include <type_traits>
+
+#include "attention.h"
+#include "qmm_tcgen05.cuh"
+
+namespace qmm {
+namespace {
+
+using namespace tc;
+
+constexpr int kThreads = 384, kBlock = 128, kHelpers = 2;
+using Tiles = TokenTiles<kBlock>;
+
+template <int D>
+struct TcLayout {
+  static constexpr int kTile = D / 64 * 16384;         // 128 rows: columns of 64 elements, 128 bytes a row, one behind the other
+  static constexpr int kSlots = D == 64 ? 10 : 5;
+  static constexpr int kRing = 2 * kTile;              // behind Q's halves
+  static constexpr int kSpecials = kRing + kSlots * kTile;
+  static constexpr int kBars = kSpecials + kHelpers * 3 * D * 2;           // 16-bit places, a set for each helper
+  static constexpr int kNumBars = 2 + 3 * kSlots + 8;
+  static constexpr int kWords = kBars + 8 * kNumBars;  // tensor memory's address, abort flag, and counters
+  static constexpr int kBytes = kWords + 32 + 1024;    // (what is swizzled begins at a multiple of 1024)
+};
+
+// A, B in shared memory, both K-major: D / 16 steps of 16 elements.
+#define QMM_SS(AO, BO, ACC)                                                                                  \
+  "add.u32 al, %1, " AO "; add.u32 bl, %2, " BO "; mov.b64 a, {al, %3}; mov.b64 b, {bl, %3};"               \
+  "@e tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %4, " ACC ";"
+template <int D>
+__device__ __forceinline__ void mma_scores(uint32_t d, uint32_t a_lo, uint32_t b_lo, uint32_t hi, uint32_t idesc) {
+  if constexpr (D == 64)
+    asm volatile("{ .reg .pred e, t, f; .reg .b32 al, bl; .reg .b64 a, b; elect.sync _|e, 0xffffffff; setp.eq.b32 t, 0, 0; setp.ne.b32 f, 0, 0;"
+                 QMM_SS("0", "0", "f") QMM_SS("2", "2", "t") QMM_SS("4", "4", "t") QMM_SS("6", "6", "t") "}" ::"r"(d), "r"(a_lo), "r"(b_lo), "r"(hi), "r"(idesc) : "memory");
+  else
+    asm volatile("{ .reg .pred e, t, f; .reg .b32 al, bl; .reg .b64 a, b; elect.sync _|e, 0xffffffff; setp.eq.b32 t, 0, 0; setp.ne.b32 f, 0, 0;"
+                 QMM_SS("0", "0", "f") QMM_SS("2", "2", "t") QMM_SS("4", "4", "t") QMM_SS("6", "6", "t")
+                 QMM_SS("1024", "1024", "t") QMM_SS("1026", "1026", "t") QMM_SS("1028", "1028", "t") QMM_SS("1030", "1030", "t") "}"
+                 ::"r"(d), "r"(a_lo), "r"(b_lo), "r"(hi), "r"(idesc) : "memory");
+}
+// A in tensor memory (8 columns a step of 16 positions), B in shared memory as rows of positions: 16 of them are 2048 bytes.
+#define QMM_TS(COL, BO, ACC)                                                                                 \
+  "add.u32 a, %1, " COL "; add.u32 bl, %2, " BO "; mov.b64 b, {bl, %3};"                                    \
+  "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [a], b, %4, " ACC ";"
+__device__ __forceinline__ void mma_values(uint32_t d, uint32_t a, uint32_t b_lo, uint32_t hi, uint32_t idesc, uint32_t accumulate) {
+  asm volatile("{ .reg .pred e, p, t; .reg .b32 a, bl; .reg .b64 b; elect.sync _|e, 0xffffffff; setp.ne.b32 p, %5, 0; setp.eq.b32 t, 0, 0;"
+               QMM_TS("0", "0", "p") QMM_TS("8", "128", "t") QMM_TS("16", "256", "t") QMM_TS("24", "384", "t")
+               QMM_TS("32", "512", "t") QMM_TS("40", "640", "t") QMM_TS("48", "768", "t") QMM_TS("56", "896", "t") "}"
+               ::"r"(d), "r"(a), "r"(b_lo), "r"(hi), "r"(idesc), "r"(accumulate) : "memory");
+}
+// MN-major operand in the 128-byte swizzle: columns of 64 elements (leading byte offset) and groups of 8 positions (stride byte offset).
+__device__ __forceinline__ uint32_t desc_low_mn(uint32_t saddr) { return ((saddr & 0x3FFFFu) >> 4) | ((16384u >> 4) << 16); }
+
+__device__ __forceinline__ void tma_load_3d(const CUtensorMap* map, uint32_t dst, uint32_t bar, int c0, int c1, int c2) {
+  asm volatile("cp.async.bulk.tensor.3d.shared::cta.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(dst), "l"(map), "r"(bar), "r"(c0),
+               "r"(c1), "r"(c2)
+               : "memory");
+}
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ uint64_t pack_f32(float a, float b) {
+  uint64_t v;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(a), "f"(b));
+  return v;
+}
+__device__ __forceinline__ float2 unpack_f32(uint64_t v) {
+  float2 f;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(f.x), "=f"(f.y) : "l"(v));
+  return f;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ __forceinline__ void tmem_st(uint32_t taddr, const uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
+      "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
+      "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(taddr),
+      QMM_ASM_R(0), QMM_ASM_R(8), QMM_ASM_R(16), QMM_ASM_R(24)
+      : "memory");
+}
+
+template <typename T>
+__device__ __forceinline__ bool odd_pair(uint32_t w) {
+  constexpr uint32_t kExp = std::is_same<T, __nv_bfloat16>::value ? 0x7f80u : 0x7c00u;
+  return (w & kExp) == kExp || (w >> 16 & kExp) == kExp;
+}
+
+// What a CTA does of an item: units [begin, end) of it, of which each half sees those before its own `last`.
+struct Part {
+  int begin, end, seen[2], last[2], load_end;
+  bool live;
+};
+__device__ __forceinline__ Part part_of(const AttentionWork& w, const UnitCursor& c, int left) {
+  Part r;
+  r.begin = c.u;
+  r.end = c.units - c.u < left ? c.units : c.u + left;
+  const int64_t token = static_cast<int64_t>(c.t) * 2 * w.tile_tokens;
+  r.seen[0] = seen_by(w, c.span, token + w.tile_tokens);
+  r.seen[1] = token + w.tile_tokens < c.span.n ? seen_by(w, c.span, token + 2 * w.tile_tokens) : 0;
+#pragma unroll
+  for (int x = 0; x < 2; ++x) {
+    const int u = (r.seen[x] + kBlock - 1) / kBlock;
+    r.last[x] = u < r.end ? u : r.end;
+    if (r.last[x] < r.begin) r.last[x] = r.begin;
+  }
+  r.load_end = r.last[0] > r.last[1] ? r.last[0] : r.last[1];
+  r.live = r.load_end > r.begin;
+  return r;
+}
+
+// Blocks that are looked at begin no more than 127 before the first position that the tile's first row does not see, and end less than 128 behind the
+// last that its last row sees: a place counted from here has 10 bits. (An unwritten one, 0xffff, is above every row's.)
+__device__ __forceinline__ int place_of(int first_limit) { return (first_limit > 0 ? first_limit : 0) - 127; }
+
+template <typename T, int D, bool PAGED>
+__global__ void __launch_bounds__(kThreads, 1)
+attend_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map,
+                 const RowsParams p) {
+  using L = TcLayout<D>;
+  constexpr int S = L::kSlots;
+  constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t raw = smem_u32(smem_raw);
+  const uint32_t base = (raw + 1023u) & ~1023u;
+  uint8_t* const smem = smem_raw + (base - raw);
+  uint16_t* const special = reinterpret_cast<uint16_t*>(smem + L::kSpecials);      // [helper][+inf, -inf, NaN][D]: first place with one in a column of v
+  volatile int* const words = reinterpret_cast<volatile int*>(smem + L::kWords);   // [2 + helper] item whose specials its set holds, [4] items helped with, [5] items written
+  const uint32_t ring = base + L::kRing, bars = base + L::kBars;
+  const uint32_t q_full = bars, q_empty = bars + 8, full = bars + 16, empty = full + 8 * S, clean = empty + 8 * S;
+  const uint32_t s_full = clean + 8 * S, p_full = s_full + 16, o_full = p_full + 16, o_free = o_full + 16;
+  const uint32_t tmem_slot = base + L::kWords, abort_at = tmem_slot + 4;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const AttentionWork& w = p.work;
+
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  if (tid == 0) {
+    auto init = [](uint32_t bar, int n) { asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(n)); };
+    init(q_full, 1);
+    init(q_empty, 1);
+    for (int i = 0; i < S; ++i) {
+      init(full + 8 * i, 1);
+      init(empty + 8 * i, 1);
+      init(clean + 8 * i, kHelpers);
+    }
+    for (int x = 0; x < 2; ++x) {
+      init(s_full + 8 * x, 1);
+      init(p_full + 8 * x, 4);
+      init(o_full + 8 * x, 1);
+      init(o_free + 8 * x, 4);
+    }
+    for (int i = 1; i < 8; ++i) words[i] = 0;
+    mbar_init_fence();
+  }
+  if (warp == 8) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(tmem_slot), "r"(512) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  uint32_t tmem;
+  asm volatile("ld.shared.u32 %0, [%1];" : "=r"(tmem) : "r"(tmem_slot) : "memory");
+  tmem = __shfl_sync(0xffffffffu, tmem, 0);
+
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  UnitCursor c;
+  int64_t total, quota = 1;
+  const bool any = find_unit<Tiles>(w, [&](int64_t t) { quota = quota_of(t, gridDim.x, p.least_units); return quota * blockIdx.x; }, &total, &c);
+  int left = 0;
+  if (any) {
+    const int64_t rest = total - quota * blockIdx.x;
+    left = static_cast<int>(rest < quota ? rest : quota);
+  }
+  // every lane waits, and all go on or none does
+  auto wait = [&](uint32_t bar, uint32_t parity, int where) -> bool { return __all_sync(0xffffffffu, wait_phase(bar, parity, abort_at, where)); };
+  // ... for a counter of this CTA
+  auto wait_count = [&](int word, int count, int where) -> bool {
+    bool ok = true;
+    if (words[word] < count) {
+      const long long t0 = clock64();
+      while (words[word] < count) {
+        if (words[1]) {
+          ok = false;
+          break;
+        }
+        if (clock64() - t0 > kSpinLimit) {
+          words[1] = where;
+          ok = false;
+          break;
+        }
+      }
+    }
+    __threadfence_block();
+    return __all_sync(0xffffffffu, ok);
+  };
+  bool ok = true;
+  // 168 registers a thread at the launch: 128 x 72 + 256 x 216 = 384 x 168
+  if (warp >= 8) {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+  if (warp == 9) {
+    // ---------------- copies ----------------
+    uint32_t slot = 0, ph = 0;
+    int live = 0;
+    const int page_size = 1 << p.cache.page_shift;
+    const int per_block = PAGED ? (page_size < kBlock ? kBlock / page_size : 1) : 1;       // pages of a block
+    while (ok && left > 0) {
+      const Part it = part_of(w, c, left);
+      if (it.live) {
+        if (!(ok = wait(q_empty, (live & 1) ^ 1, 31))) break;
+        if (lane == 0) {
+          const bool both = it.last[1] > it.begin;
+          mbar_expect_tx(q_full, (both ? 2 : 1) * (D / 64) * w.tile_tokens * w.group * 128);
+          const int token = c.span.q0 + c.t * 2 * w.tile_tokens;
+          for (int x = 0; x < (both ? 2 : 1); ++x)
+            for (int i = 0; i < D / 64; ++i)
+              tma_load_3d(&q_map, base + x * L::kTile + i * 16384, q_full, i * 64, c.h * w.group, token + x * w.tile_tokens);
+        }
+        __syncwarp();
+        int64_t page = 0;
+        auto look_up = [&](int u) {                    // lane i: page i of block u
+          if constexpr (PAGED) {
+            const int pos = u * kBlock + lane * page_size;
+            page = 0;
+            if (lane < per_block && u < it.load_end && pos < c.span.len) page = page_of(p.cache, c.s, pos, w.status);
+            if (page < 0) page = 0;
+          }
+        };
+        look_up(it.begin);
+        for (int u = it.begin; ok && u < it.load_end; ++u) {
+          int there = 1;                                // pages of the block that the sequence has
+          if constexpr (PAGED) {
+            const int more = (c.span.len - u * kBlock + page_size - 1) >> p.cache.page_shift;
+            there = more < per_block ? more : per_block;
+          }
+          const int64_t here = page;
+          look_up(u + 1);
+#pragma unroll
+          for (int which = 0; which < 2; ++which) {
+            if (!(ok = wait(empty + 8 * slot, ph ^ 1u, 32))) break;
+            const uint32_t dst = ring + slot * L::kTile, bar = full + 8 * slot;
+            if constexpr (PAGED) {
+              const int rows = page_size < kBlock ? page_size : kBlock;
+              if (lane == 0) mbar_expect_tx(bar, there * rows * D * 2);
+              __syncwarp();
+              if (lane < there) {
+                const int row = static_cast<int>(((here * w.kv_heads + c.h) << p.cache.page_shift) + ((u * kBlock) & (page_size - 1)));
+                for (int i = 0; i < D / 64; ++i) tma_load_2d(which ? &v_map : &k_map, dst + i * 16384 + lane * rows * 128, bar, i * 64, row);
+              }
+            } else if (lane == 0) {
+              mbar_expect_tx(bar, kBlock * D * 2);
+              for (int i = 0; i < D / 64; ++i) tma_load_3d(which ? &v_map : &k_map, dst + i * 16384, bar, i * 64, c.h, c.span.q0 + u * kBlock);
+            }
+            __syncwarp();
+            if (++slot == S) {
+              slot = 0;
+              ph ^= 1u;
+            }
+          }
+        }
+        ++live;
+      }
+      left -= it.end - it.begin;
+      if (left > 0) next_item<Tiles>(w, c);
+    }
+    if (!ok)                                            // given up: what is on its way lands first
+      for (uint32_t i = 0; i < static_cast<uint32_t>(S); ++i) mbar_drain(full + 8 * i, i < slot ? ph : ph ^ 1u);
+  } else if (warp >= 10) {
+    // ---------------- helpers: blocks of v that some row does not see all of ----------------
+    uint32_t slot = 0, ph = 0;
+    int live = 0;
+    while (ok && left > 0) {
+      const Part it = part_of(w, c, left);
+      if (it.live) {
+        const int first_limit = w.causal ? c.span.len - c.span.n + c.t * 2 * w.tile_tokens : c.span.len - 1;
+        const int place0 = place_of(first_limit);
+        uint16_t* const set = special + (warp - 10) * 3 * D;
+        bool mine = false;                              // the set is this item's
+        for (int u = it.begin; ok && u < it.load_end; ++u) {
+#pragma unroll 1
+          for (int which = 0; which < 2; ++which) {
+            if (!(ok = wait(full + 8 * slot, ph, 33))) break;
+            const int pos0 = u * kBlock;
+            if (which == 1 && pos0 + kBlock - 1 > first_limit) {
+              constexpr int kPieces = D / 8;
+#pragma unroll 2
+              for (int i = (warp - 10) * 32 + lane; i < kBlock * kPieces; i += kHelpers * 32) {
+                const int r = i / kPieces, col = i % kPieces;
+                const uint32_t at = ring + slot * L::kTile + (col >> 3) * 16384 + r * 128 + (((col & 7) ^ (r & 7)) << 4);
+                uint4 v = lds128<0>(at);
+                const bool behind = pos0 + r >= c.span.len;
+                const bool odd = !behind && (odd_pair<T>(v.x) || odd_pair<T>(v.y) || odd_pair<T>(v.z) || odd_pair<T>(v.w));
+                unsigned found = __ballot_sync(0xffffffffu, odd);
+                if (found) {
+                  if (!mine) {                          // the items before this one are written: what the set held goes
+                    if (!(ok = wait_count(5, 8 * live, 34))) break;
+                    for (int n = lane; n < 3 * D; n += 32) set[n] = 0xffff;
+                    if (lane == 0) words[2 + warp - 10] = live + 1;
+                    __syncwarp();
+                    mine = true;
+                  }
+                  while (found) {                       // a lane at a time: two may have the same column
+                    if (__ffs(found) - 1 == lane) {
+                      uint32_t word[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+                      for (int e = 0; e < 8; ++e) {
+                        const float2 pair = unpack2<T>(word[e >> 1]);
+                        const float x = e & 1 ? pair.y : pair.x;
+                        if (!(fabsf(x) <= 3.402823466e38f)) {
+                          uint16_t* const place = set + (x > 0.0f ? 0 : x < 0.0f ? D : 2 * D) + col * 8 + e;
+                          if (pos0 + r - place0 < *place) *place = static_cast<uint16_t>(pos0 + r - place0);
+                          word[e >> 1] &= e & 1 ? 0x0000ffffu : 0xffff0000u;
+                        }
+                      }
+                      v = make_uint4(word[0], word[1], word[2], word[3]);
+                    }
+                    __syncwarp();
+                    found &= found - 1;
+                  }
+                }
+                if (behind) v = make_uint4(0, 0, 0, 0);
+                if (behind || odd) asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+              }
+              fence_proxy_async();
+            }
+            __syncwarp();
+            // (also for keys, so that a slot's phases are the ring's)
+            if (lane == 0) mbar_arrive(clean + 8 * slot);
+            if (++slot == S) {
+              slot = 0;
+              ph ^= 1u;
+            }
+          }
+        }
+        __threadfence_block();
+        __syncwarp();
+        if (lane == 0) atomicAdd(const_cast<int*>(&words[4]), 1);
+        ++live;
+      }
+      left -= it.end - it.begin;
+      if (left > 0) next_item<Tiles>(w, c);
+    }
+  } else {
+    // ---------------- the MMAs' issuer ----------------
+    constexpr uint32_t kFmt = kBf16 ? 1 : 0;
+    const uint32_t id_scores = instr_desc(kFmt, 128) | (static_cast<uint32_t>(kBlock / 8) << 17);
+    const uint32_t id_values = instr_desc(kFmt, 128) | (static_cast<uint32_t>(D / 8) << 17) | (1u << 16);       // B is MN-major
+    uint32_t slot = 0, ph = 0;
+    int live = 0;
+    uint32_t items[2] = {0, 0}, p_ph[2] = {0, 0};
+    auto next_slot = [&]() {
+      if (++slot == S) {
+        slot = 0;
+        ph ^= 1u;
+      }
+    };
+    auto scores = [&](int x, uint32_t key_slot) {
+      mma_scores<D>(tmem + x * 128, desc_low(base + x * L::kTile), desc_low(ring + key_slot * L::kTile), kDescHigh, id_scores);
+      tc_commit<false>(s_full + 8 * x, 0);
+    };
+    while (ok && left > 0) {
+      const Part it = part_of(w, c, left);
+      if (it.live) {
+        if (!(ok = wait(q_full, live & 1, 35))) break;
+        if (!(ok = wait(full + 8 * slot, ph, 36))) break;
+        tc_fence_after();
+        for (int x = 0; x < 2; ++x)
+          if (it.last[x] > it.begin) scores(x, slot);
+        tc_commit<false>(empty + 8 * slot, 0);
+        next_slot();
+        for (int u = it.begin; ok && u < it.load_end; ++u) {
+          const uint32_t v_slot = slot, v_ph = ph;
+          next_slot();
+          const bool more = u + 1 < it.load_end;
+          const uint32_t k_slot = slot;
+          const uint32_t k_ph = ph;
+          if (!(ok = wait(clean + 8 * v_slot, v_ph, 37))) break;
+          if (more && !(ok = wait(full + 8 * k_slot, k_ph, 38))) break;
+          for (int x = 0; x < 2; ++x) {
+            if (u >= it.last[x]) continue;
+            if (u == it.begin) {                        // the rows' last item has been read out of O
+              if (!(ok = wait(o_free + 8 * x, (items[x] & 1) ^ 1, 39))) break;
+            }
+            if (!(ok = wait(p_full + 8 * x, p_ph[x], 40))) break;
+            p_ph[x] ^= 1u;
+            tc_fence_after();
+            mma_values(tmem + 256 + x * D, tmem + x * 128, desc_low_mn(ring + v_slot * L::kTile), kDescHigh, id_values, u > it.begin);
+            if (u + 1 < it.last[x]) {
+              scores(x, k_slot);
+            } else {
+              tc_commit<false>(o_full + 8 * x, 0);
+              ++items[x];
+            }
+          }
+          if (!ok) break;
+          tc_commit<false>(empty + 8 * v_slot, 0);
+          if (more) {
+            tc_commit<false>(empty + 8 * k_slot, 0);
+            next_slot();
+          }
+        }
+        if (ok) tc_commit<false>(q_empty, 0);
+        ++live;
+      }
+      left -= it.end - it.begin;
+      if (left > 0) next_item<Tiles>(w, c);
+    }
+    if (!ok) {                                          // given up: the MMAs issued so far complete before tensor memory goes
+      tc_commit<false>(q_empty, 0);
+      ++live;
+    }
+    if (live) mbar_drain(q_empty, (live - 1) & 1);       // (arrivals reach their barriers before the CTA leaves)
+  }
+  } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
+    // ---------------- rows ----------------
+    const int x = warp >> 2, r = (warp & 3) * 32 + lane;
+    const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
+    const uint32_t s_at = tmem + x * 128 + lanes, o_at = tmem + 256 + x * D + lanes;
+    const int tok_in = r / w.group, g = r - tok_in * w.group;
+    const uint64_t scale = pack_f32(p.scale_log2, p.scale_log2);
+    uint32_t s_ph = 0, o_ph = 0;
+    int live = 0;
+    while (ok && left > 0) {
+      const Part it = part_of(w, c, left);
+      const int tok0 = (2 * c.t + x) * w.tile_tokens, tok = tok0 + tok_in;
+      const bool mine = tok_in < w.tile_tokens && tok < c.span.n;
+      const int limit = w.causal ? c.span.len - c.span.n + tok : c.span.len - 1;
+      const int first_limit = w.causal ? c.span.len - c.span.n + tok0 : c.span.len - 1;
+      const int first_item_limit = w.causal ? c.span.len - c.span.n + 2 * c.t * w.tile_tokens : c.span.len - 1;
+      float top = -INFINITY, sum = 0.0f;                // running maximum (times the scale, base 2) that O stands for
+      for (int u = it.begin; u < it.last[x]; ++u) {
+        if (!(ok = wait(s_full + 8 * x, s_ph, 41))) break;
+        s_ph ^= 1u;
+        tc_fence_after();
+        uint32_t s[4][32];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) tmem_ld(s_at + i * 32, s[i]);
+        tmem_wait_ld();
+        if (u * kBlock + kBlock - 1 > first_limit) {
+          const int seen = limit - u * kBlock;          // columns 0 .. seen are seen
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int j = 0; j < 32; ++j)
+              if (i * 32 + j > seen) s[i][j] = 0xff800000u;
+        }
+        float m[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          m[i] = -INFINITY;
+#pragma unroll
+          for (int j = 0; j < 32; j += 2) m[i] = fmaxf(m[i], fmaxf(__uint_as_float(s[i][j]), __uint_as_float(s[i][j + 1])));
+        }
+        const float now = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3])) * p.scale_log2;
+        if (u == it.begin) {
+          top = now;
+        } else if (__any_sync(0xffffffffu, now > top + 8.0f)) {
+          float shrink = 1.0f;
+          if (now > top + 8.0f) {
+            shrink = ex2(top - now);
+            top = now;
+            sum *= shrink;
+          }
+#pragma unroll 1
+          for (int i = 0; i < D / 32; ++i) {
+            uint32_t o[32];
+            tmem_ld(o_at + i * 32, o);
+            tmem_wait_ld();
+#pragma unroll
+            for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * shrink);
+            tmem_st(o_at + i * 32, o);
+          }
+        }
+        const float off = top == -INFINITY ? 0.0f : -top;
+        const uint64_t off2 = pack_f32(off, off);
+        uint64_t sums[2] = {0, 0};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          uint32_t out[16];
+#pragma unroll
+          for (int j = 0; j < 16; ++j) {
+            const float2 e = unpack_f32(fma2(pack_f32(__uint_as_float(s[i][2 * j]), __uint_as_float(s[i][2 * j + 1])), scale, off2));
+            const float a = ex2(e.x), b = ex2(e.y);
+            sums[j & 1] = add2(sums[j & 1], pack_f32(a, b));
+            out[j] = pack2<T>(a, b);
+          }
+          tmem_st16(s_at + i * 16, out);
+        }
+        const float2 both = unpack_f32(add2(sums[0], sums[1]));
+        sum += both.x + both.y;
+        tmem_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(p_full + 8 * x);
+      }
+      if (!ok) break;
+      // ---- the item, or this CTA's part of it, ends ----
+      const bool has = it.last[x] > it.begin;
+      bool odd[kHelpers] = {};
+      if (has) {
+        if (!(ok = wait(o_full + 8 * x, o_ph, 42))) break;
+        o_ph ^= 1u;
+        tc_fence_after();
+        if (!(ok = wait_count(4, kHelpers * (live + 1), 43))) break;
+        for (int n = 0; n < kHelpers; ++n) odd[n] = words[2 + n] == live + 1;
+      }
+      const bool whole = it.begin == 0 && it.end == c.units;
+      const float inv = sum == 0.0f ? (limit < 0 ? 0.0f : NAN) : 1.0f / sum;
+      uint8_t* const out = p.out + ((static_cast<int64_t>(c.span.q0) + tok) * w.heads + c.h * w.group + g) * D * 2;
+      float4* const part = reinterpret_cast<float4*>(p.partial + (2 * static_cast<int64_t>(blockIdx.x) + (it.begin == 0 ? 1 : 0)) * partial_floats<256, D>());
+      const int row = x * 128 + r;
+#pragma unroll 1
+      for (int i = 0; i < D / 32; ++i) {
+        uint32_t o[32];
+        if (has) {
+          tmem_ld(o_at + i * 32, o);
+          tmem_wait_ld();
+        } else {
+#pragma unroll
+          for (int j = 0; j < 32; ++j) o[j] = 0;
+        }
+#pragma unroll
+        for (int n = 0; n < kHelpers; ++n)
+          if (odd[n]) {
+            const uint16_t* const set = special + n * 3 * D + i * 32;
+            const int seen = limit - place_of(first_item_limit);
+#pragma unroll
+            for (int j = 0; j < 32; ++j) {
+              float v = __uint_as_float(o[j]);
+              if (set[j] <= seen) v += INFINITY;
+              if (set[D + j] <= seen) v -= INFINITY;
+              if (set[2 * D + j] <= seen) v = NAN;
+              o[j] = __float_as_uint(v);
+            }
+          }
+        if (!mine) continue;
+        if (whole) {
+#pragma unroll
+          for (int j = 0; j < 32; j += 8) {
+            uint4 v;
+            v.x = pack2<T>(__uint_as_float(o[j]) * inv, __uint_as_float(o[j + 1]) * inv);
+            v.y = pack2<T>(__uint_as_float(o[j + 2]) * inv, __uint_as_float(o[j + 3]) * inv);
+            v.z = pack2<T>(__uint_as_float(o[j + 4]) * inv, __uint_as_float(o[j + 5]) * inv);
+            v.w = pack2<T>(__uint_as_float(o[j + 6]) * inv, __uint_as_float(o[j + 7]) * inv);
+            *reinterpret_cast<uint4*>(out + (i * 32 + j) * 2) = v;
+          }
+        } else {
+          // four elements of 256 rows side by side: neighbouring threads write neighbouring 16 bytes
+#pragma unroll
+          for (int j = 0; j < 32; j += 4)
+            part[((i * 32 + j) / 4) * 256 + row] = make_float4(__uint_as_float(o[j]), __uint_as_float(o[j + 1]), __uint_as_float(o[j + 2]), __uint_as_float(o[j + 3]));
+        }
+      }
+      if (!whole && mine) {
+        reinterpret_cast<float*>(part)[256 * D + row] = top;
+        reinterpret_cast<float*>(part)[256 * D + 256 + row] = sum;
+      }
+      if (has) {
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(o_free + 8 * x);
+      }
+      if (it.live) {
+        __threadfence_block();
+        __syncwarp();
+        if (lane == 0) atomicAdd(const_cast<int*>(&words[5]), 1);
+        ++live;
+      }
+      left -= it.end - it.begin;
+      if (left > 0) next_item<Tiles>(w, c);
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 8) {
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
+  }
+  if (tid == 0 && words[1]) atomicCAS(w.status, 0, words[1]);
+}
+
+// Items whose units fell to several CTAs: block (b, y) looks at the end of CTA b's share, and joins 16 columns of the item there if it is cut there
+// first. A thread has a row.
+constexpr int kJoinColumns = 16;
+template <typename T, int D>
+__global__ void __launch_bounds__(256) attend_tc_join_kernel(const JoinParams p) {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const AttentionWork& w = p.work;
+  UnitCursor c;
+  int64_t total, quota = 1;
+  const bool any = find_unit<Tiles>(w, [&](int64_t t) { quota = quota_of(t, p.ctas, p.least_units); return quota * (blockIdx.x + 1); }, &total, &c);
+  if (!any || c.u == 0 || c.u > quota) return;
+  const int parts = parts_of(c.units - c.u, quota);
+  const int row = threadIdx.x, x = row >> 7, r = row & 127;
+  const int tok_in = r / w.group, g = r - tok_in * w.group, tok = (2 * c.t + x) * w.tile_tokens + tok_in;
+  if (tok_in >= w.tile_tokens || tok >= c.span.n) return;
+  auto slot = [&](int i) { return p.partial + (2 * (static_cast<int64_t>(blockIdx.x) + i) + (i == 0 ? 1 : 0)) * partial_floats<256, D>(); };
+  float top = -INFINITY;
+  for (int i = 0; i < parts; ++i) top = fmaxf(top, slot(i)[256 * D + row]);
+  const float base = top == -INFINITY ? 0.0f : top;
+  float sum = 0.0f, v[kJoinColumns] = {};
+#pragma unroll 2
+  for (int i = 0; i < parts; ++i) {
+    const float* s = slot(i);
+    const float f = ex2(s[256 * D + row] - base);
+    sum = fmaf(f, s[256 * D + 256 + row], sum);
+#pragma unroll
+    for (int j = 0; j < kJoinColumns / 4; ++j) {
+      const float4 y = reinterpret_cast<const float4*>(s)[(blockIdx.y * (kJoinColumns / 4) + j) * 256 + row];
+      v[4 * j] = fmaf(f, y.x, v[4 * j]);
+      v[4 * j + 1] = fmaf(f, y.y, v[4 * j + 1]);
+      v[4 * j + 2] = fmaf(f, y.z, v[4 * j + 2]);
+      v[4 * j + 3] = fmaf(f, y.w, v[4 * j + 3]);
+    }
+  }
+  const int limit = w.causal ? c.span.len - c.span.n + tok : c.span.len - 1;
+  const float inv = sum == 0.0f ? (limit < 0 ? 0.0f : NAN) : 1.0f / sum;
+  uint8_t* const out = p.out + (((static_cast<int64_t>(c.span.q0) + tok) * w.heads + c.h * w.group + g) * D + blockIdx.y * kJoinColumns) * 2;
+#pragma unroll
+  for (int j = 0; j < kJoinColumns; j += 8)
+    *reinterpret_cast<uint4*>(out + j * 2) = make_uint4(pack2<T>(v[j] * inv, v[j + 1] * inv), pack2<T>(v[j + 2] * inv, v[j + 3] * inv),
+                                                        pack2<T>(v[j + 4] * inv, v[j + 5] * inv), pack2<T>(v[j + 6] * inv, v[j + 7] * inv));
+}
+
+template <typename T, int D, bool PAGED>
+int launch_one(const RowsParams& p, const CUtensorMap (&maps)[3], int ctas, cudaStream_t stream) {
+  static bool done[kMaxDevices] = {};
+  const int dev = current_device();
+  if (dev < 0) return QMM_ERR_DEVICE;
+  auto kernel = attend_tc_kernel<T, D, PAGED>;
+  if (!done[dev]) {
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, TcLayout<D>::kBytes);
+    if (e != cudaSuccess) return fail(QMM_ERR_CUDA, "cudaFuncSetAttribute: %s", cudaGetErrorString(e));
+    done[dev] = true;
+  }
+  launch_early(kernel, ctas, kThreads, TcLayout<D>::kBytes, stream, maps[0], maps[1], maps[2], p);
+  count_launch();
+  if (int rc = check_launch("attend_tc_kernel")) return rc;
+  if (ctas < 2) return QMM_OK;
+  JoinParams j = {};
+  j.work = p.work;
+  j.out = p.out;
+  j.partial = p.partial;
+  j.ctas = ctas;
+  j.least_units = p.least_units;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(ctas - 1, D / kJoinColumns);
+  cfg.blockDim = dim3(256);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  cudaLaunchKernelEx(&cfg, attend_tc_join_kernel<T, D>, j);
+  count_launch();
+  return check_launch("attend_tc_join_kernel");
+}
+
+template <typename T>
+int launch_of(const RowsParams& p, const CUtensorMap (&maps)[3], int head_dim, bool paged, int ctas, cudaStream_t stream) {
+  if (head_dim == 64) return paged ? launch_one<T, 64, true>(p, maps, ctas, stream) : launch_one<T, 64, false>(p, maps, ctas, stream);
+  return paged ? launch_one<T, 128, true>(p, maps, ctas, stream) : launch_one<T, 128, false>(p, maps, ctas, stream);
+}
+
+}  // namespace
+
+int attend_tc_ctas() { return device_sm_count(); }
+
+int64_t attend_tc_workspace(int head_dim, int ctas) {
+  return 2ll * ctas * (head_dim == 64 ? partial_floats<256, 64>() : partial_floats<256, 128>()) * 4;
+}
+
+int launch_attend_tc(const RowsParams& given, int elem, int head_dim, bool paged, int ctas, cudaStream_t stream) {
+  RowsParams p = given;
+  AttentionWork& w = p.work;
+  w.tile_tokens = 128 / w.group;
+  CUtensorMap maps[3];
+  if (int rc = tensor_map_3d(&maps[0], elem, p.q, head_dim, w.heads, w.tokens, p.q_head * 2, p.q_row * 2, 64, w.group, w.tile_tokens)) return rc;
+  if (paged) {
+    const int page = 1 << p.cache.page_shift, rows = page < kBlock ? page : kBlock;
+    const uint64_t all = static_cast<uint64_t>(p.cache.pages) * w.kv_heads << p.cache.page_shift;
+    if (int rc = tensor_map_2d(&maps[1], elem, p.cache.k, head_dim, all, head_dim * 2, 64, rows, 1)) return rc;
+    if (int rc = tensor_map_2d(&maps[2], elem, p.cache.v, head_dim, all, head_dim * 2, 64, rows, 1)) return rc;
+  } else {
+    if (int rc = tensor_map_3d(&maps[1], elem, p.k, head_dim, w.kv_heads, w.tokens, p.k_head * 2, p.k_row * 2, 64, 1, kBlock)) return rc;
+    if (int rc = tensor_map_3d(&maps[2], elem, p.v, head_dim, w.kv_heads, w.tokens, p.v_head * 2, p.v_row * 2, 64, 1, kBlock)) return rc;
+  }
+  return elem == QMM_BF16 ? launch_of<__nv_bfloat16>(p, maps, head_dim, paged, ctas, stream) : launch_of<__half>(p, maps, head_dim, paged, ctas, stream);
+}
+
+}  // namespace qmm

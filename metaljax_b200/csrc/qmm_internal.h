@@ -136,6 +136,10 @@ int read_status_word(int* out);
 int tensor_map_2d(void* map_out, int elem_kind, const void* base, uint64_t inner, uint64_t outer,
                   uint64_t row_bytes, uint32_t box_inner, uint32_t box_outer, int swizzle);
 
+// ... and a 3-D one in the 128-byte swizzle: `inner` x `middle` x `outer` elements, strides in bytes.
+int tensor_map_3d(void* map_out, int elem_kind, const void* base, uint64_t inner, uint64_t middle, uint64_t outer, uint64_t middle_bytes,
+                  uint64_t outer_bytes, uint32_t box_inner, uint32_t box_middle, uint32_t box_outer);
+
 // The current device's word in which kernels record a bounded wait that ran out (one word per
 // device, allocated on first use and kept), or NULL.
 int* device_status_word();

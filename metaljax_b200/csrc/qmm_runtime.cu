@@ -50,6 +50,22 @@ int tensor_map_2d(void* map_out, int elem_kind, const void* base, uint64_t inner
   return QMM_OK;
 }
 
+int tensor_map_3d(void* map_out, int elem_kind, const void* base, uint64_t inner, uint64_t middle, uint64_t outer, uint64_t middle_bytes,
+                  uint64_t outer_bytes, uint32_t box_inner, uint32_t box_middle, uint32_t box_outer) {
+  EncodeTiledFn fn = encode_fn();
+  if (!fn) return fail(QMM_ERR_CUDA, "cuTensorMapEncodeTiled is not available from the driver");
+  const CUtensorMapDataType dt = elem_kind == QMM_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : elem_kind == QMM_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
+                                                                                                                 : CU_TENSOR_MAP_DATA_TYPE_UINT8;
+  cuuint64_t dims[3] = {inner, middle, outer};
+  cuuint64_t strides[2] = {middle_bytes, outer_bytes};
+  cuuint32_t box[3] = {box_inner, box_middle, box_outer};
+  cuuint32_t estr[3] = {1, 1, 1};
+  CUresult r = fn(static_cast<CUtensorMap*>(map_out), dt, 3, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                  CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return fail(QMM_ERR_CUDA, "cuTensorMapEncodeTiled failed with CUresult %d", (int)r);
+  return QMM_OK;
+}
+
 int current_device() {
   int dev = -1;
   cudaError_t e = cudaGetDevice(&dev);
