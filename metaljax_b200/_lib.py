@@ -230,7 +230,8 @@ def native():
         loader.exec_module(module)
         module.bind(*(ctypes.cast(getattr(lib(), name), ctypes.c_void_p).value for name in ("qmm_quantized_matmul", "qmm_moe_workspace_bytes",
                                                                                              "qmm_moe_experts_checked", "qmm_moe_silu_mul", "qmm_pack_dense_layer",
-                                                                                             "qmm_gated_matmul", "qmm_gated_matmul_pays")))
+                                                                                             "qmm_gated_matmul", "qmm_gated_matmul_pays", "qmm_cache_append", "qmm_cache_read",
+                                                                                             "qmm_attention_workspace_bytes", "qmm_prompt_attention", "qmm_paged_attention")))
         _native = module
     return _native
 

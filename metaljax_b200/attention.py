@@ -55,9 +55,12 @@ class PagedCache:
     32, 64, 128 or 256, head_dim 64 or 128. Which pages are whose is the caller's: every call takes a table
     `[sequences, pages of a sequence]`."""
 
-    __slots__ = ("k", "v", "k_exp", "v_exp", "_c")
+    __slots__ = ("k", "v", "k_exp", "v_exp")
 
     def __init__(self, k, v, k_exp=None, v_exp=None):
+        self.k, self.v, self.k_exp, self.v_exp = k, v, k_exp, v_exp
+        if _lib.native().is_cache(k, v, k_exp, v_exp):
+            return
         if k.dim() != 4 or k.shape != v.shape or k.dtype != v.dtype or k.device != v.device:
             raise ValueError("PagedCache: k and v are [pages, kv_heads, page_size, head_dim] of one type and device")
         elem = _CACHE_ELEM.get(k.dtype)
@@ -67,16 +70,9 @@ class PagedCache:
             raise ValueError("PagedCache: k and v have to be contiguous")
         if (elem == 7) != (k_exp is not None) or (k_exp is None) != (v_exp is None):
             raise ValueError("PagedCache: an e4m3 cache has exponent bytes, a 16-bit one has none")
-        c = _lib.PagedCacheArgs()
-        c.struct_size, c.elem = ctypes.sizeof(c), elem
-        c.k, c.v = k.data_ptr(), v.data_ptr()
-        if k_exp is not None:
-            for e in (k_exp, v_exp):
-                if e.dtype != torch.uint8 or e.shape != k.shape[:3] or not e.is_contiguous() or e.device != k.device:
-                    raise ValueError("PagedCache: exponent bytes are uint8 [pages, kv_heads, page_size]")
-            c.k_exp, c.v_exp = k_exp.data_ptr(), v_exp.data_ptr()
-        c.pages, c.kv_heads, c.page_size, c.head_dim = k.shape
-        self.k, self.v, self.k_exp, self.v_exp, self._c = k, v, k_exp, v_exp, c
+        for e in (k_exp, v_exp) if k_exp is not None else ():
+            if e.dtype != torch.uint8 or e.shape != k.shape[:3] or not e.is_contiguous() or e.device != k.device:
+                raise ValueError("PagedCache: exponent bytes are uint8 [pages, kv_heads, page_size]")
 
     @classmethod
     def empty(cls, pages, kv_heads, page_size, head_dim, dtype=torch.bfloat16, device="cuda"):
@@ -95,7 +91,12 @@ class PagedCache:
         _index("page_table", table, self.k.device, 2)
         if table.stride(1) != 1 and table.shape[1] > 1:
             raise ValueError("page_table: a sequence's entries have to lie side by side")
-        c = _lib.PagedCacheArgs.from_buffer_copy(self._c)
+        c = _lib.PagedCacheArgs()
+        c.struct_size, c.elem = ctypes.sizeof(c), _CACHE_ELEM[self.k.dtype]
+        c.k, c.v = self.k.data_ptr(), self.v.data_ptr()
+        if self.k_exp is not None:
+            c.k_exp, c.v_exp = self.k_exp.data_ptr(), self.v_exp.data_ptr()
+        c.pages, c.kv_heads, c.page_size, c.head_dim = self.k.shape
         c.table, c.table_width = table.data_ptr(), table.shape[1]
         c.table_stride = max(table.stride(0), table.shape[1]) if table.shape[0] > 1 else table.shape[1]
         return c
@@ -144,6 +145,13 @@ def _no_grad(*tensors):
         raise RuntimeError("attention: there is no backward pass here; call it under torch.no_grad() or detach its inputs")
 
 
+def _native(done):
+    """What a native call returned: its result, or the error of its status."""
+    if done.__class__ is int:
+        _lib.check(done)
+    return done
+
+
 def append(qkv, cache: PagedCache, page_table, kv_lens, cu_q=None, *, heads: int, freqs=None, interleaved: bool = False,
            q_norm=None, k_norm=None, eps: float = 1e-6, out=None):
     """Writes the keys and values of new tokens into `cache` and returns their queries `[tokens, heads, head_dim]`.
@@ -154,6 +162,10 @@ def append(qkv, cache: PagedCache, page_table, kv_lens, cu_q=None, *, heads: int
     `rotary_frequencies`): the first `2 * len(freqs)` elements rotated, pairs half of that apart, or neighbours
     (`interleaved`). float32 arithmetic with angles from float64; rounded once, to the result's type or
     the e4m3 cache's codes. Rows behind the last sequence are neither read nor written."""
+    done = _lib.native().append(qkv, cache.k, cache.v, cache.k_exp, cache.v_exp, page_table, kv_lens, cu_q, heads, freqs, interleaved, q_norm, k_norm, eps, out)
+    if done is not None:
+        return _native(done)
+    # (what the native call leaves: tensors to be copied first, empty ones, and what is refused)
     _no_grad(qkv, q_norm, k_norm, out)
     if qkv.dim() != 2 or qkv.dtype not in (torch.bfloat16, torch.float16) or qkv.device != cache.k.device:
         raise ValueError("append: qkv is [tokens, (heads + 2 * kv_heads) * head_dim], bf16 or f16, on the cache's device")
@@ -200,6 +212,8 @@ def read_pages(cache: PagedCache, page_table, cu_kv, total: int, dtype=None, out
 
     A 16-bit cache is read as it is; an e4m3 one as bf16, which holds its values exactly (`dtype`: f16 instead, rounded,
     infinite above its range). `out`: a pair to write to. Rows from `cu_kv[-1]` on are not written."""
+    if out is None and (done := _lib.native().read_pages(cache.k, cache.v, cache.k_exp, cache.v_exp, page_table, cu_kv, total, dtype)) is not None:
+        return _native(done)
     dev = cache.k.device
     _starts("cu_kv", cu_kv, dev, page_table.shape[0])
     if dtype is None:
@@ -243,6 +257,9 @@ def prompt_attention(q, k, v, cu_seqlens, *, causal: bool = True, scale=None, ou
     rows. `scale`: of the scores, `head_dim ** -0.5` unless given. Returns `[tokens, heads, head_dim]`; rows that belong to no
     sequence are not written. A row sees its own sequence's positions, with `causal` up to its own, and nothing else has
     any influence on it."""
+    done = _lib.native().prompt_attention(q, k, v, cu_seqlens, causal, scale, out)
+    if done is not None:
+        return _native(done)
     _no_grad(q, k, v, out)
     if q.dim() != 3 or q.dtype not in (torch.bfloat16, torch.float16):
         raise ValueError("prompt_attention: q is [tokens, heads, head_dim], bf16 or f16")
@@ -264,6 +281,9 @@ def paged_attention(q, cache: PagedCache, page_table, kv_lens, cu_q=None, *, cau
     being rows `cu_q[s]` to `cu_q[s + 1] - 1` (None: one token each) and the last ones of its `kv_lens[s]` positions. A token
     sees the positions up to its own, or (not `causal`) all of them; one that sees none is zero. q has the cache's type,
     bf16 with an e4m3 cache. Returns `[tokens, heads, head_dim]`; rows that belong to no sequence are not written."""
+    done = _lib.native().paged_attention(q, cache.k, cache.v, cache.k_exp, cache.v_exp, page_table, kv_lens, cu_q, causal, scale, out)
+    if done is not None:
+        return _native(done)
     _no_grad(q, out)
     dev = cache.k.device
     if q.dim() != 3 or q.dtype not in (torch.bfloat16, torch.float16) or q.device != dev:

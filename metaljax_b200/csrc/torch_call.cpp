@@ -17,9 +17,11 @@
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <array>
+#include <cmath>
 #include <vector>
 
 #include "../../include/qmm.h"
+#include "../../include/qmm_decode.h"
 
 namespace {
 
@@ -43,6 +45,17 @@ GatedPays g_gated_pays = nullptr;
 PackLayer g_pack_layer = nullptr;
 MoeWorkspace g_moe_workspace = nullptr;
 MoeExperts g_moe_experts = nullptr;
+
+typedef int (*CacheAppend)(const qmm_paged_cache*, const qmm_append_args*, void*);
+typedef int (*CacheRead)(const qmm_paged_cache*, int64_t, const int32_t*, int64_t, int, void*, void*, void*);
+typedef int64_t (*AttentionWorkspace)(const qmm_attention_args*);
+typedef int (*PromptAttention)(const qmm_attention_args*, void*);
+typedef int (*PagedAttention)(const qmm_paged_cache*, const qmm_attention_args*, void*);
+CacheAppend g_cache_append = nullptr;
+CacheRead g_cache_read = nullptr;
+AttentionWorkspace g_attention_workspace = nullptr;
+PromptAttention g_prompt_attention = nullptr;
+PagedAttention g_paged_attention = nullptr;
 
 constexpr int kDeclined = -1;         // (the library's codes are not negative)
 
@@ -468,9 +481,232 @@ PyObject* guarded(PyObject* self, PyObject* const* a, Py_ssize_t n) {
   }
 }
 
-// bind(addresses of qmm_quantized_matmul, qmm_moe_workspace_bytes, qmm_moe_experts_checked[, qmm_moe_silu_mul[, qmm_pack_dense_layer[, qmm_gated_matmul, qmm_gated_matmul_pays]]])
+// ---- attention: what attention.py's calls come to for ordinary tensors. Each declines what its Python form would refuse or copy. ----
+
+int cache_elem(at::ScalarType t) { return t == at::kBFloat16 ? QMM_BF16 : t == at::kHalf ? QMM_F16 : t == at::kFloat8_e4m3fn ? QMM_E4M3 : -1; }
+
+bool optional_tensor(PyObject* o, const at::Tensor** t) {
+  *t = o == Py_None ? nullptr : plain_tensor(o);
+  return *t || o == Py_None;
+}
+
+bool same_device(const at::Tensor* a, const at::Tensor* b) { return !b || a->device() == b->device(); }
+
+bool aligned(const at::Tensor* t) { return !t || reinterpret_cast<uintptr_t>(t->const_data_ptr()) % 16 == 0; }
+
+// Contiguous int32, `n` of them.
+bool lengths(const at::Tensor* t, int64_t n) { return t->scalar_type() == at::kInt && t->dim() == 1 && t->size(0) == n && (n < 2 || t->stride(0) == 1); }
+
+// k, v, k_exp | None, v_exp | None as a cache, without a table.
+bool cache_of(PyObject* const* a, const at::Tensor** like, qmm_paged_cache* c) {
+  const at::Tensor *k = plain_tensor(a[0]), *v = plain_tensor(a[1]), *ke, *ve;
+  if (!k || !v || !optional_tensor(a[2], &ke) || !optional_tensor(a[3], &ve)) return false;
+  if (k->dim() != 4 || k->sizes() != v->sizes() || k->scalar_type() != v->scalar_type() || !k->is_contiguous() || !v->is_contiguous() || !same_device(k, v)) return false;
+  c->struct_size = sizeof(*c);
+  c->elem = cache_elem(k->scalar_type());
+  if (c->elem < 0 || (c->elem == QMM_E4M3) != (ke != nullptr) || !ke != !ve) return false;
+  for (const at::Tensor* e : {ke, ve}) {
+    if (!e) continue;
+    if (e->scalar_type() != at::kByte || e->dim() != 3 || !e->is_contiguous() || !same_device(k, e)) return false;
+    for (int d = 0; d < 3; ++d)
+      if (e->size(d) != k->size(d)) return false;
+  }
+  if (k->size(1) > INT32_MAX || k->size(2) > INT32_MAX || k->size(3) > INT32_MAX) return false;
+  c->k = const_cast<void*>(k->const_data_ptr());
+  c->v = const_cast<void*>(v->const_data_ptr());
+  c->k_exp = ke ? const_cast<void*>(ke->const_data_ptr()) : nullptr;
+  c->v_exp = ve ? const_cast<void*>(ve->const_data_ptr()) : nullptr;
+  c->pages = k->size(0);
+  c->kv_heads = static_cast<int32_t>(k->size(1));
+  c->page_size = static_cast<int32_t>(k->size(2));
+  c->head_dim = static_cast<int32_t>(k->size(3));
+  *like = k;
+  return true;
+}
+
+bool table_of(PyObject* o, const at::Tensor* k, qmm_paged_cache* c, int64_t* seqs) {
+  const at::Tensor* t = plain_tensor(o);
+  if (!t || t->scalar_type() != at::kInt || t->dim() != 2 || !same_device(k, t) || (t->size(1) > 1 && t->stride(1) != 1) || t->size(1) > INT32_MAX) return false;
+  c->table = static_cast<const int32_t*>(t->const_data_ptr());
+  c->table_width = static_cast<int32_t>(t->size(1));
+  c->table_stride = t->size(0) > 1 ? t->stride(0) : t->size(1);
+  *seqs = t->size(0);
+  return c->table_stride >= c->table_width;
+}
+
+// is_cache(k, v, k_exp | None, v_exp | None) -> whether they make a cache (False: perhaps, and the Python form says why not)
+PyObject* is_cache(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  qmm_paged_cache c = {};
+  const at::Tensor* k;
+  return PyBool_FromLong(n == 4 && cache_of(a, &k, &c));
+}
+
+// append(qkv, k, v, k_exp, v_exp, table, kv_lens, cu_q | None, heads, freqs | None, interleaved, q_norm | None, k_norm | None, eps, out | None)
+// -> the queries, a status code, or None (declined)
+PyObject* append(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  if (n != 15 || !g_cache_append) Py_RETURN_NONE;
+  qmm_paged_cache c = {};
+  qmm_append_args g = {};
+  const at::Tensor *x = plain_tensor(a[0]), *k, *lens = plain_tensor(a[6]), *cu, *freqs, *qn, *kn, *out;
+  if (!x || !lens || !cache_of(a + 1, &k, &c) || !table_of(a[5], k, &c, &g.seqs) || !optional_tensor(a[7], &cu) || !optional_tensor(a[9], &freqs) ||
+      !optional_tensor(a[11], &qn) || !optional_tensor(a[12], &kn) || !optional_tensor(a[14], &out))
+    Py_RETURN_NONE;
+  const long heads = PyLong_AsLong(a[8]);
+  const int interleaved = PyObject_IsTrue(a[10]);
+  const double eps = PyFloat_AsDouble(a[13]);
+  if (PyErr_Occurred()) {
+    PyErr_Clear();
+    Py_RETURN_NONE;
+  }
+  g.struct_size = sizeof(g);
+  g.elem = elem_of(x->scalar_type());
+  if ((g.elem != QMM_BF16 && g.elem != QMM_F16) || x->dim() != 2 || heads < 1 || heads > (1 << 20)) Py_RETURN_NONE;
+  for (const at::Tensor* t : {x, lens, cu, freqs, qn, kn, out})
+    if (t && !same_device(k, t)) Py_RETURN_NONE;
+  g.tokens = x->size(0);
+  g.row_stride = x->stride(0);
+  if (x->size(1) != (heads + 2 * static_cast<int64_t>(c.kv_heads)) * c.head_dim || x->stride(1) != 1 || g.row_stride % 8 || g.row_stride < x->size(1)) Py_RETURN_NONE;
+  if (!lengths(lens, g.seqs) || (cu ? !lengths(cu, g.seqs + 1) : g.tokens != g.seqs)) Py_RETURN_NONE;
+  if (freqs && (freqs->scalar_type() != at::kDouble || freqs->dim() != 1 || !freqs->is_contiguous())) Py_RETURN_NONE;
+  for (const at::Tensor* t : {qn, kn})
+    if (t && (t->scalar_type() != x->scalar_type() || t->dim() != 1 || t->size(0) != c.head_dim || !t->is_contiguous())) Py_RETURN_NONE;
+  if (!aligned(x) || !aligned(qn) || !aligned(kn)) Py_RETURN_NONE;
+  if (out && (out->scalar_type() != x->scalar_type() || !out->is_contiguous() || out->dim() != 3 || out->size(0) != g.tokens || out->size(1) != heads || out->size(2) != c.head_dim))
+    Py_RETURN_NONE;
+  g.heads = static_cast<int32_t>(heads);
+  g.rotary_dim = freqs ? static_cast<int32_t>(2 * freqs->size(0)) : 0;
+  g.interleaved = interleaved;
+  g.eps = static_cast<float>(eps);
+  g.qkv = x->const_data_ptr();
+  g.freqs = freqs ? static_cast<const double*>(freqs->const_data_ptr()) : nullptr;
+  g.q_norm = qn ? qn->const_data_ptr() : nullptr;
+  g.k_norm = kn ? kn->const_data_ptr() : nullptr;
+  g.kv_lens = static_cast<const int32_t*>(lens->const_data_ptr());
+  g.cu_q = cu ? static_cast<const int32_t*>(cu->const_data_ptr()) : nullptr;
+  at::Tensor q;
+  const int rc = unlocked([&]() -> int {
+    const c10::cuda::CUDAGuard guard(x->device());
+    q = out ? *out : at::Tensor(at::detail::empty_cuda({g.tokens, heads, c.head_dim}, x->scalar_type(), x->device(), std::nullopt));
+    g.q_out = const_cast<void*>(q.const_data_ptr());
+    return g_cache_append(&c, &g, c10::cuda::getCurrentCUDAStream(x->get_device()).stream());
+  });
+  if (rc) return PyLong_FromLong(rc);
+  return THPVariable_Wrap(std::move(q));
+}
+
+// read_pages(k, v, k_exp, v_exp, table, cu_kv, total, dtype | None) -> (k, v), a status code, or None (declined)
+PyObject* read_pages(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  if (n != 8 || !g_cache_read) Py_RETURN_NONE;
+  qmm_paged_cache c = {};
+  const at::Tensor *k, *cu = plain_tensor(a[5]);
+  int64_t seqs = 0;
+  if (!cu || !cache_of(a, &k, &c) || !table_of(a[4], k, &c, &seqs) || !same_device(k, cu) || !lengths(cu, seqs + 1)) Py_RETURN_NONE;
+  const long long total = PyLong_AsLongLong(a[6]);
+  if (PyErr_Occurred()) {
+    PyErr_Clear();
+    Py_RETURN_NONE;
+  }
+  at::ScalarType to = c.elem == QMM_F16 ? at::kHalf : at::kBFloat16;
+  if (a[7] != Py_None) {
+    if (!THPDtype_Check(a[7])) Py_RETURN_NONE;
+    to = reinterpret_cast<THPDtype*>(a[7])->scalar_type;
+  }
+  if (total < 1 || (to != at::kBFloat16 && to != at::kHalf)) Py_RETURN_NONE;
+  at::Tensor out[2];
+  const int rc = unlocked([&]() -> int {
+    const c10::cuda::CUDAGuard guard(k->device());
+    for (at::Tensor& t : out) t = at::detail::empty_cuda({static_cast<int64_t>(total), c.kv_heads, c.head_dim}, to, k->device(), std::nullopt);
+    return g_cache_read(&c, seqs, static_cast<const int32_t*>(cu->const_data_ptr()), total, elem_of(to), const_cast<void*>(out[0].const_data_ptr()),
+                        const_cast<void*>(out[1].const_data_ptr()), c10::cuda::getCurrentCUDAStream(k->get_device()).stream());
+  });
+  if (rc) return PyLong_FromLong(rc);
+  PyObject* pair = PyTuple_New(2);
+  if (!pair) return nullptr;
+  for (int i = 0; i < 2; ++i) PyTuple_SET_ITEM(pair, i, THPVariable_Wrap(std::move(out[i])));
+  return pair;
+}
+
+bool is_half(const at::Tensor* t) { return t->scalar_type() == at::kBFloat16 || t->scalar_type() == at::kHalf; }
+
+// q, k or v: heads' elements side by side, strides and address in steps of 16 bytes.
+bool heads_of(const at::Tensor* t, at::ScalarType type) {
+  return t && t->dim() == 3 && t->scalar_type() == type && t->stride(2) == 1 && t->stride(0) % 8 == 0 && t->stride(1) % 8 == 0 && t->stride(0) >= 0 && t->stride(1) >= 0 && aligned(t);
+}
+
+// The rest of both forms: result and workspace, and the call.
+PyObject* attend(qmm_attention_args* g, const at::Tensor* q, const at::Tensor* out, PyObject* causal, PyObject* scale, const qmm_paged_cache* c) {
+  g->struct_size = sizeof(*g);
+  g->elem = elem_of(q->scalar_type());
+  g->q = q->const_data_ptr();
+  g->q_row = q->stride(0);
+  g->q_head = q->stride(1);
+  g->tokens = q->size(0);
+  if (q->size(1) > INT32_MAX || (out && (out->scalar_type() != q->scalar_type() || !out->is_contiguous() || out->sizes() != q->sizes() || !same_device(q, out)))) Py_RETURN_NONE;
+  g->heads = static_cast<int32_t>(q->size(1));
+  g->head_dim = static_cast<int32_t>(q->size(2));
+  g->causal = PyObject_IsTrue(causal);
+  g->scale = scale == Py_None ? 1.0f / std::sqrt(static_cast<float>(g->head_dim)) : static_cast<float>(PyFloat_AsDouble(scale));
+  if (PyErr_Occurred()) {
+    PyErr_Clear();
+    Py_RETURN_NONE;
+  }
+  at::Tensor y;
+  const int rc = unlocked([&]() -> int {
+    const c10::cuda::CUDAGuard guard(q->device());
+    const int64_t need = g_attention_workspace(g);
+    if (need < 0) return kDeclined;
+    y = out ? *out : at::Tensor(at::detail::empty_cuda(q->sizes(), q->scalar_type(), q->device(), std::nullopt));
+    const at::Tensor work = at::detail::empty_cuda({need}, at::kByte, q->device(), std::nullopt);
+    g->out = const_cast<void*>(y.const_data_ptr());
+    g->workspace = const_cast<void*>(work.const_data_ptr());
+    g->workspace_bytes = need;
+    void* stream = c10::cuda::getCurrentCUDAStream(q->get_device()).stream();
+    return c ? g_paged_attention(c, g, stream) : g_prompt_attention(g, stream);
+  });
+  if (rc == kDeclined) Py_RETURN_NONE;
+  if (rc) return PyLong_FromLong(rc);
+  return THPVariable_Wrap(std::move(y));
+}
+
+// prompt_attention(q, k, v, cu_seqlens, causal, scale | None, out | None) -> the result, a status code, or None (declined)
+PyObject* prompt_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  if (n != 7 || !g_prompt_attention) Py_RETURN_NONE;
+  const at::Tensor *q = plain_tensor(a[0]), *k = plain_tensor(a[1]), *v = plain_tensor(a[2]), *cu = plain_tensor(a[3]), *out;
+  if (!q || !cu || !is_half(q) || !heads_of(q, q->scalar_type()) || !heads_of(k, q->scalar_type()) || !heads_of(v, q->scalar_type())) Py_RETURN_NONE;
+  if (!optional_tensor(a[6], &out) || !same_device(q, k) || !same_device(q, v) || !same_device(q, cu)) Py_RETURN_NONE;
+  if (k->sizes() != v->sizes() || k->size(0) != q->size(0) || k->size(2) != q->size(2) || cu->dim() != 1 || !lengths(cu, cu->size(0)) || k->size(1) > INT32_MAX) Py_RETURN_NONE;
+  qmm_attention_args g = {};
+  g.seqs = cu->size(0) - 1;
+  g.kv_heads = static_cast<int32_t>(k->size(1));
+  g.k = k->const_data_ptr();
+  g.k_row = k->stride(0);
+  g.k_head = k->stride(1);
+  g.v = v->const_data_ptr();
+  g.v_row = v->stride(0);
+  g.v_head = v->stride(1);
+  g.cu_q = static_cast<const int32_t*>(cu->const_data_ptr());
+  return attend(&g, q, out, a[4], a[5], nullptr);
+}
+
+// paged_attention(q, k, v, k_exp, v_exp, table, kv_lens, cu_q | None, causal, scale | None, out | None) -> the result, a status code, or None
+PyObject* paged_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  if (n != 11 || !g_paged_attention) Py_RETURN_NONE;
+  qmm_paged_cache c = {};
+  qmm_attention_args g = {};
+  const at::Tensor *q = plain_tensor(a[0]), *k, *lens = plain_tensor(a[6]), *cu, *out;
+  if (!q || !lens || !is_half(q) || !heads_of(q, q->scalar_type()) || !cache_of(a + 1, &k, &c) || !table_of(a[5], k, &c, &g.seqs)) Py_RETURN_NONE;
+  if (!optional_tensor(a[7], &cu) || !optional_tensor(a[10], &out) || !same_device(q, k) || !same_device(q, lens) || !same_device(q, cu)) Py_RETURN_NONE;
+  if (!lengths(lens, g.seqs) || (cu && !lengths(cu, g.seqs + 1)) || q->size(2) != c.head_dim) Py_RETURN_NONE;
+  g.kv_heads = c.kv_heads;
+  g.kv_lens = static_cast<const int32_t*>(lens->const_data_ptr());
+  g.cu_q = cu ? static_cast<const int32_t*>(cu->const_data_ptr()) : nullptr;
+  return attend(&g, q, out, a[8], a[9], &c);
+}
+
+// bind(addresses of qmm_quantized_matmul, qmm_moe_workspace_bytes, qmm_moe_experts_checked[, qmm_moe_silu_mul[, qmm_pack_dense_layer[, qmm_gated_matmul, qmm_gated_matmul_pays
+// [, qmm_cache_append, qmm_cache_read, qmm_attention_workspace_bytes, qmm_prompt_attention, qmm_paged_attention]]]])
 PyObject* bind(PyObject*, PyObject* const* a, Py_ssize_t n) {
-  if (n < 3 || n > 7) {
+  if (n < 3 || n > 12) {
     PyErr_SetString(PyExc_TypeError, "bind takes the entry points' addresses");
     return nullptr;
   }
@@ -481,6 +717,13 @@ PyObject* bind(PyObject*, PyObject* const* a, Py_ssize_t n) {
   if (n > 4) g_pack_layer = reinterpret_cast<PackLayer>(PyLong_AsVoidPtr(a[4]));
   if (n > 5) g_gated_matmul = reinterpret_cast<GatedMatmul>(PyLong_AsVoidPtr(a[5]));
   if (n > 6) g_gated_pays = reinterpret_cast<GatedPays>(PyLong_AsVoidPtr(a[6]));
+  if (n == 12) {
+    g_cache_append = reinterpret_cast<CacheAppend>(PyLong_AsVoidPtr(a[7]));
+    g_cache_read = reinterpret_cast<CacheRead>(PyLong_AsVoidPtr(a[8]));
+    g_attention_workspace = reinterpret_cast<AttentionWorkspace>(PyLong_AsVoidPtr(a[9]));
+    g_prompt_attention = reinterpret_cast<PromptAttention>(PyLong_AsVoidPtr(a[10]));
+    g_paged_attention = reinterpret_cast<PagedAttention>(PyLong_AsVoidPtr(a[11]));
+  }
   if (PyErr_Occurred()) return nullptr;
   Py_RETURN_NONE;
 }
@@ -491,6 +734,11 @@ PyMethodDef kMethods[] = {
     {"moe_experts", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(guarded<moe_experts>)), METH_FASTCALL, nullptr},
     {"pack_layer", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(guarded<pack_layer>)), METH_FASTCALL, nullptr},
     {"run_steps", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(guarded<run_steps>)), METH_FASTCALL, nullptr},
+    {"is_cache", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(guarded<is_cache>)), METH_FASTCALL, nullptr},
+    {"append", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(guarded<append>)), METH_FASTCALL, nullptr},
+    {"read_pages", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(guarded<read_pages>)), METH_FASTCALL, nullptr},
+    {"prompt_attention", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(guarded<prompt_attention>)), METH_FASTCALL, nullptr},
+    {"paged_attention", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(guarded<paged_attention>)), METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr}};
 
 PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_native", nullptr, -1, kMethods, nullptr, nullptr, nullptr, nullptr};
