@@ -12,6 +12,7 @@ struct RowsParams {
   const uint8_t* k;            // rows
   const uint8_t* v;
   uint8_t* out;
+  JoinNote* notes;
   float* partial;
   int64_t q_row, q_head, k_row, k_head, v_row, v_head;       // elements
   float scale_log2;
@@ -21,8 +22,8 @@ struct RowsParams {
 struct JoinParams {
   AttentionWork work;
   uint8_t* out;
+  const JoinNote* notes;
   const float* partial;
-  int32_t ctas, least_units;
 };
 
 int attend_rows_ctas();

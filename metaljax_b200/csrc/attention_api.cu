@@ -74,7 +74,7 @@ int attend(const char* what, const qmm_paged_cache* cache, const CacheView* view
   p.k = static_cast<const uint8_t*>(a->k);
   p.v = static_cast<const uint8_t*>(a->v);
   p.out = static_cast<uint8_t*>(a->out);
-  p.partial = static_cast<float*>(a->workspace);
+  p.notes = static_cast<JoinNote*>(a->workspace);
   p.q_row = a->q_row;
   p.q_head = a->q_head;
   p.k_row = a->k_row;
@@ -91,8 +91,10 @@ int attend(const char* what, const qmm_paged_cache* cache, const CacheView* view
   const int source = !view ? 0 : cache->elem == QMM_E4M3 ? 2 : 1;
   const bool tc = a->cu_q && a->tokens * p.work.group > 64 * a->seqs && source != 2 &&
                   (!view || (static_cast<uint64_t>(p.cache.pages) * p.work.kv_heads << p.cache.page_shift) < (1ull << 31));
-  if (tc) return launch_attend_tc(p, a->elem, a->head_dim, view != nullptr, attend_tc_ctas(), stream);
-  return launch_attend_rows(p, a->elem, a->head_dim, source, rows < 64 ? static_cast<int>(rows) : 64, attend_rows_ctas(), stream);
+  const int ctas = tc ? attend_tc_ctas() : attend_rows_ctas();
+  p.partial = reinterpret_cast<float*>(p.notes + ctas);
+  if (tc) return launch_attend_tc(p, a->elem, a->head_dim, view != nullptr, ctas, stream);
+  return launch_attend_rows(p, a->elem, a->head_dim, source, rows < 64 ? static_cast<int>(rows) : 64, ctas, stream);
 }
 
 }  // namespace

@@ -213,6 +213,16 @@ __device__ __forceinline__ int parts_of(int after, int64_t quota) {
   return 1 + (quota >> 31 ? 1 : static_cast<int>((static_cast<uint32_t>(after) + static_cast<uint32_t>(quota) - 1) / static_cast<uint32_t>(quota)));
 }
 
+// The workspace: a note of every CTA, written by each, then two partial results a CTA. The note says what the second launch has to join at the end of a
+// CTA's share: the item that it began and did not finish, and how many CTAs have a part of it (0: there is none).
+struct JoinNote {
+  int32_t parts, q0, n, len, h, t, pad[2];
+};
+__device__ __forceinline__ JoinNote note_of(const UnitCursor& c, int begun, int ended, int64_t quota) {
+  const int parts = begun == 0 && ended < c.units ? parts_of(c.units - ended, quota) : 0;
+  return {parts, c.span.q0, c.span.n, c.span.len, c.h, c.t, {0, 0}};
+}
+
 // A partial result in the workspace: R rows of D float32 sums, then R maxima (base 2) and R sums of weights.
 template <int R, int D>
 constexpr int64_t partial_floats() { return static_cast<int64_t>(R) * (D + 2); }

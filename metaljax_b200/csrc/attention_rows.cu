@@ -92,7 +92,10 @@ __global__ void __launch_bounds__(kThreads, 2) attend_rows_kernel(const RowsPara
   UnitCursor c;
   int64_t total, quota = 1;
   const bool any = find_unit<Tiles>(w, [&](int64_t t) { quota = quota_of(t, gridDim.x, p.least_units); return quota * blockIdx.x; }, &total, &c);
-  if (!any) return;
+  if (!any) {
+    if (tid == 0) p.notes[blockIdx.x].parts = 0;
+    return;
+  }
   const int64_t first_unit = quota * blockIdx.x;
   const int count = static_cast<int>(total - first_unit < quota ? total - first_unit : quota);
   UnitCursor load = c;                                  // where the copies are
@@ -388,70 +391,68 @@ __global__ void __launch_bounds__(kThreads, 2) attend_rows_kernel(const RowsPara
     if (done + 1 < count) {
       next_item<Tiles>(w, c);
       begin_item();
+    } else if (tid == 0) {
+      p.notes[blockIdx.x] = note_of(c, begun, c.u, quota);
     }
   }
   asm volatile("cp.async.wait_all;" ::: "memory");
 }
 
-// Items whose units fell to several CTAs: block b looks at the end of CTA b's share, and joins the item there if it is cut there first.
-constexpr int kJoinThreads = 512;
-template <typename T, int D, int R, int B>
+// Items whose units fell to several CTAs: block (b, y) joins eight rows of the one that CTA b began and did not finish, a warp each.
+constexpr int kJoinThreads = 256, kJoinRows = kJoinThreads / 32;
+template <typename T, int D, int R>
 __global__ void __launch_bounds__(kJoinThreads) attend_join_kernel(const JoinParams p) {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const AttentionWork& w = p.work;
-  UnitCursor c;
-  int64_t total, quota = 1;
-  const bool any = find_unit<RowTiles<R, B>>(w, [&](int64_t t) { quota = quota_of(t, p.ctas, p.least_units); return quota * (blockIdx.x + 1); }, &total, &c);
-  if (!any || c.u == 0 || c.u > quota) return;
-  const int parts = parts_of(c.units - c.u, quota);
-  const int64_t rows = static_cast<int64_t>(c.span.n) * w.group - static_cast<int64_t>(c.t) * R;
-  const int tile_rows = rows < R ? static_cast<int>(rows) : R;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const JoinNote c = p.notes[blockIdx.x];
+  const int64_t row = static_cast<int64_t>(c.t) * R + blockIdx.y * kJoinRows + (threadIdx.x >> 5);
+  if (c.parts == 0 || row >= static_cast<int64_t>(c.n) * w.group) return;
+  const int r = blockIdx.y * kJoinRows + (threadIdx.x >> 5), lane = threadIdx.x & 31;
   constexpr int V = D / 32;                                                       // elements of a lane
-  auto part_of = [&](int i) { return p.partial + (2 * (static_cast<int64_t>(blockIdx.x) + i) + (i == 0 ? 1 : 0)) * partial_floats<R, D>(); };
-  for (int r = warp; r < tile_rows; r += kJoinThreads / 32) {
-    float mm = -INFINITY;
-    for (int i = lane; i < parts; i += 32) mm = fmaxf(mm, part_of(i)[R * D + r]);
+  // (the first part lies behind this CTA's finished item, the others are the first of theirs)
+  const float* const first = p.partial + (2 * static_cast<int64_t>(blockIdx.x) + 1) * partial_floats<R, D>();
+  const float* const others = p.partial + 2 * static_cast<int64_t>(blockIdx.x) * partial_floats<R, D>();
+  auto part_of = [&](int i) { return i == 0 ? first : others + 2ll * i * partial_floats<R, D>(); };
+  float mm = -INFINITY;
+  for (int i = lane; i < c.parts; i += 32) mm = fmaxf(mm, part_of(i)[R * D + r]);
 #pragma unroll
-    for (int x = 16; x > 0; x >>= 1) mm = fmaxf(mm, __shfl_xor_sync(0xffffffffu, mm, x));
-    const float base = mm == -INFINITY ? 0.0f : mm;
-    float ll = 0.0f, v[V] = {};
-    for (int i0 = 0; i0 < parts; i0 += 32) {
-      float f = 0.0f;
-      if (i0 + lane < parts) {
-        const float* part = part_of(i0 + lane);
-        f = ex2(part[R * D + r] - base);
-        ll = fmaf(f, part[R * D + R + r], ll);
-      }
-      const int here = parts - i0 < 32 ? parts - i0 : 32;
+  for (int x = 16; x > 0; x >>= 1) mm = fmaxf(mm, __shfl_xor_sync(0xffffffffu, mm, x));
+  const float base = mm == -INFINITY ? 0.0f : mm;
+  float ll = 0.0f, v[V] = {};
+  for (int i0 = 0; i0 < c.parts; i0 += 32) {
+    float f = 0.0f;
+    if (i0 + lane < c.parts) {
+      const float* part = part_of(i0 + lane);
+      f = ex2(part[R * D + r] - base);
+      ll = fmaf(f, part[R * D + R + r], ll);
+    }
+    const int here = c.parts - i0 < 32 ? c.parts - i0 : 32;
 #pragma unroll 8
-      for (int i = 0; i < here; ++i) {
-        const float fi = __shfl_sync(0xffffffffu, f, i);
-        const float* src = part_of(i0 + i) + r * D + lane * V;
-        if constexpr (V == 4) {
-          const float4 x = *reinterpret_cast<const float4*>(src);
-          v[0] = fmaf(fi, x.x, v[0]);
-          v[1] = fmaf(fi, x.y, v[1]);
-          v[2] = fmaf(fi, x.z, v[2]);
-          v[3] = fmaf(fi, x.w, v[3]);
-        } else {
-          const float2 x = *reinterpret_cast<const float2*>(src);
-          v[0] = fmaf(fi, x.x, v[0]);
-          v[1] = fmaf(fi, x.y, v[1]);
-        }
+    for (int i = 0; i < here; ++i) {
+      const float fi = __shfl_sync(0xffffffffu, f, i);
+      const float* src = part_of(i0 + i) + r * D + lane * V;
+      if constexpr (V == 4) {
+        const float4 x = *reinterpret_cast<const float4*>(src);
+        v[0] = fmaf(fi, x.x, v[0]);
+        v[1] = fmaf(fi, x.y, v[1]);
+        v[2] = fmaf(fi, x.z, v[2]);
+        v[3] = fmaf(fi, x.w, v[3]);
+      } else {
+        const float2 x = *reinterpret_cast<const float2*>(src);
+        v[0] = fmaf(fi, x.x, v[0]);
+        v[1] = fmaf(fi, x.y, v[1]);
       }
     }
-#pragma unroll
-    for (int x = 16; x > 0; x >>= 1) ll += __shfl_xor_sync(0xffffffffu, ll, x);
-    const int64_t row = static_cast<int64_t>(c.t) * R + r;
-    const int tok = static_cast<int>(row / w.group), g = static_cast<int>(row - static_cast<int64_t>(tok) * w.group);
-    const int seen = w.causal ? c.span.len - c.span.n + tok : c.span.len - 1;
-    const float inv = ll == 0.0f ? (seen < 0 ? 0.0f : NAN) : 1.0f / ll;
-    uint8_t* dst = p.out + ((static_cast<int64_t>(c.span.q0) + tok) * w.heads + c.h * w.group + g) * D * 2 + lane * V * 2;
-#pragma unroll
-    for (int e = 0; e < V; e += 2) *reinterpret_cast<uint32_t*>(dst + e * 2) = pack2<T>(v[e] * inv, v[e + 1] * inv);
   }
+#pragma unroll
+  for (int x = 16; x > 0; x >>= 1) ll += __shfl_xor_sync(0xffffffffu, ll, x);
+  const int tok = static_cast<int>(row / w.group), g = static_cast<int>(row - static_cast<int64_t>(tok) * w.group);
+  const int seen = w.causal ? c.len - c.n + tok : c.len - 1;
+  const float inv = ll == 0.0f ? (seen < 0 ? 0.0f : NAN) : 1.0f / ll;
+  uint8_t* dst = p.out + ((static_cast<int64_t>(c.q0) + tok) * w.heads + c.h * w.group + g) * D * 2 + lane * V * 2;
+#pragma unroll
+  for (int e = 0; e < V; e += 2) *reinterpret_cast<uint32_t*>(dst + e * 2) = pack2<T>(v[e] * inv, v[e + 1] * inv);
 }
 
 template <typename T, int D, int RW, int SOURCE>
@@ -468,13 +469,8 @@ int launch_one(const RowsParams& p, int ctas, cudaStream_t stream) {
   count_launch();
   if (int rc = check_launch("attend_rows_kernel")) return rc;
   if (ctas < 2) return QMM_OK;
-  JoinParams j = {};
-  j.work = p.work;
-  j.out = p.out;
-  j.partial = p.partial;
-  j.ctas = ctas;
-  j.least_units = p.least_units;
-  launch_early(attend_join_kernel<T, D, 16 * RW, kChunk>, ctas - 1, kJoinThreads, 0, stream, j);
+  JoinParams j = {p.work, p.out, p.notes, p.partial};
+  launch_early(attend_join_kernel<T, D, 16 * RW>, dim3(ctas - 1, 16 * RW / kJoinRows), kJoinThreads, 0, stream, j);
   count_launch();
   return check_launch("attend_join_kernel");
 }
@@ -499,7 +495,7 @@ int launch_source(const RowsParams& p, int source, int rows, int ctas, cudaStrea
 int attend_rows_ctas() { return 2 * device_sm_count(); }
 
 int64_t attend_rows_workspace(int head_dim, int ctas) {
-  return 2ll * ctas * (head_dim == 64 ? partial_floats<64, 64>() : partial_floats<64, 128>()) * 4;
+  return ctas * (sizeof(JoinNote) + 2ll * (head_dim == 64 ? partial_floats<64, 64>() : partial_floats<64, 128>()) * 4);
 }
 
 int launch_attend_rows(const RowsParams& p, int elem, int head_dim, int source, int rows, int ctas, cudaStream_t stream) {

@@ -34,13 +34,14 @@ using Tiles = TokenTiles<kBlock>;
 template <int D>
 struct TcLayout {
   static constexpr int kTile = D / 64 * 16384;         // 128 rows: columns of 64 elements, 128 bytes a row, one behind the other
-  static constexpr int kSlots = D == 64 ? 10 : 5;
-  static constexpr int kRing = 2 * kTile;              // behind Q's halves
-  static constexpr int kSpecials = kRing + kSlots * kTile;
+  static constexpr int kKeys = D == 64 ? 5 : 2, kValues = D == 64 ? 5 : 3;       // blocks on their way or at work
+  static constexpr int kKeyRing = 2 * kTile;           // behind Q's halves
+  static constexpr int kValueRing = kKeyRing + kKeys * kTile;
+  static constexpr int kSpecials = kValueRing + kValues * kTile;
   static constexpr int kBars = kSpecials + kHelpers * 3 * D * 2;           // 16-bit places, a set for each helper
-  static constexpr int kNumBars = 2 + 3 * kSlots + 8;
+  static constexpr int kNumBars = 2 * kKeys + 3 * kValues + 13;
   static constexpr int kWords = kBars + 8 * kNumBars;  // tensor memory's address, abort flag, and counters
-  static constexpr int kBytes = kWords + 32 + 1024;    // (what is swizzled begins at a multiple of 1024)
+  static constexpr int kBytes = kWords + 64 + 1024;    // (what is swizzled begins at a multiple of 1024)
 };
 
 // A, B in shared memory, both K-major: D / 16 steps of 16 elements.
@@ -116,6 +117,20 @@ __device__ __forceinline__ bool odd_pair(uint32_t w) {
   return (w & kExp) == kExp || (w >> 16 & kExp) == kExp;
 }
 
+// A place in a ring. Keys and values have rings of their own: a wait knows a phase only from the one before it, so whoever waits for a ring's copies has
+// to wait for each of them in turn (or could take the phase before for the one it wants: copies do not land in order), and has to hold up the
+// next ones (or could be lapped). The issuer does so for keys, the helpers for values.
+template <int N>
+struct Slot {
+  uint32_t slot, phase;
+  __device__ __forceinline__ void next() {
+    if (++slot == N) {
+      slot = 0;
+      phase ^= 1u;
+    }
+  }
+};
+
 // What a CTA does of an item: units [begin, end) of it, of which each half sees those before its own `last`.
 struct Part {
   int begin, end, seen[2], last[2], load_end;
@@ -148,17 +163,18 @@ __global__ void __launch_bounds__(kThreads, 1)
 attend_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map,
                  const RowsParams p) {
   using L = TcLayout<D>;
-  constexpr int S = L::kSlots;
   constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw = smem_u32(smem_raw);
   const uint32_t base = (raw + 1023u) & ~1023u;
   uint8_t* const smem = smem_raw + (base - raw);
   uint16_t* const special = reinterpret_cast<uint16_t*>(smem + L::kSpecials);      // [helper][+inf, -inf, NaN][D]: first place with one in a column of v
-  volatile int* const words = reinterpret_cast<volatile int*>(smem + L::kWords);   // [2 + helper] item whose specials its set holds, [4] items helped with, [5] items written
-  const uint32_t ring = base + L::kRing, bars = base + L::kBars;
-  const uint32_t q_full = bars, q_empty = bars + 8, full = bars + 16, empty = full + 8 * S, clean = empty + 8 * S;
-  const uint32_t s_full = clean + 8 * S, p_full = s_full + 16, o_full = p_full + 16, o_free = o_full + 16;
+  // [2 + helper] item whose specials its set holds, [4 + helper] items it has been through, [6 + warp of rows] items it has written
+  volatile int* const words = reinterpret_cast<volatile int*>(smem + L::kWords);
+  const uint32_t key_ring = base + L::kKeyRing, value_ring = base + L::kValueRing, bars = base + L::kBars;
+  const uint32_t q_full = bars, q_empty = bars + 16, k_full = bars + 32, k_empty = k_full + 8 * L::kKeys;
+  const uint32_t v_full = k_empty + 8 * L::kKeys, v_empty = v_full + 8 * L::kValues, v_clean = v_empty + 8 * L::kValues;
+  const uint32_t s_full = v_clean + 8 * L::kValues, p_full = s_full + 16, o_full = p_full + 16, o_free = o_full + 16, done = o_free + 16;
   const uint32_t tmem_slot = base + L::kWords, abort_at = tmem_slot + 4;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const AttentionWork& w = p.work;
@@ -166,20 +182,25 @@ attend_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constan
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   if (tid == 0) {
     auto init = [](uint32_t bar, int n) { asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(n)); };
-    init(q_full, 1);
-    init(q_empty, 1);
-    for (int i = 0; i < S; ++i) {
-      init(full + 8 * i, 1);
-      init(empty + 8 * i, 1);
-      init(clean + 8 * i, kHelpers);
+    for (int i = 0; i < L::kKeys; ++i) {
+      init(k_full + 8 * i, 1);
+      init(k_empty + 8 * i, 1);
+    }
+    for (int i = 0; i < L::kValues; ++i) {
+      init(v_full + 8 * i, 1);
+      init(v_empty + 8 * i, 1);
+      init(v_clean + 8 * i, kHelpers);
     }
     for (int x = 0; x < 2; ++x) {
+      init(q_full + 8 * x, 1);
+      init(q_empty + 8 * x, 1);
       init(s_full + 8 * x, 1);
       init(p_full + 8 * x, 4);
       init(o_full + 8 * x, 1);
       init(o_free + 8 * x, 4);
     }
-    for (int i = 1; i < 8; ++i) words[i] = 0;
+    init(done, 1);
+    for (int i = 1; i < 16; ++i) words[i] = 0;
     mbar_init_fence();
   }
   if (warp == 8) {
@@ -204,12 +225,12 @@ attend_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constan
   }
   // every lane waits, and all go on or none does
   auto wait = [&](uint32_t bar, uint32_t parity, int where) -> bool { return __all_sync(0xffffffffu, wait_phase(bar, parity, abort_at, where)); };
-  // ... for a counter of this CTA
-  auto wait_count = [&](int word, int count, int where) -> bool {
+  // ... for `n` counters of this CTA, a lane each
+  auto wait_count = [&](int word, int n, int count, int where) -> bool {
     bool ok = true;
-    if (words[word] < count) {
+    if (lane < n && words[word + lane] < count) {
       const long long t0 = clock64();
-      while (words[word] < count) {
+      while (words[word + lane] < count) {
         if (words[1]) {
           ok = false;
           break;
@@ -221,32 +242,37 @@ attend_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constan
         }
       }
     }
+    ok = __all_sync(0xffffffffu, ok);
     __threadfence_block();
-    return __all_sync(0xffffffffu, ok);
+    return ok;
   };
   bool ok = true;
-  // 168 registers a thread at the launch: 128 x 72 + 256 x 216 = 384 x 168
+  // 168 registers a thread at the launch: 128 x 104 + 256 x 200 = 384 x 168
   if (warp >= 8) {
-  asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");
   if (warp == 9) {
     // ---------------- copies ----------------
-    uint32_t slot = 0, ph = 0;
-    int live = 0;
+    if (lane == 0) p.notes[blockIdx.x].parts = 0;         // (also where this CTA gives up)
+    Slot<L::kKeys> key = {0, 0};
+    Slot<L::kValues> value = {0, 0};
+    int items[2] = {0, 0};
     const int page_size = 1 << p.cache.page_shift;
     const int per_block = PAGED ? (page_size < kBlock ? kBlock / page_size : 1) : 1;       // pages of a block
     while (ok && left > 0) {
       const Part it = part_of(w, c, left);
       if (it.live) {
-        if (!(ok = wait(q_empty, (live & 1) ^ 1, 31))) break;
-        if (lane == 0) {
-          const bool both = it.last[1] > it.begin;
-          mbar_expect_tx(q_full, (both ? 2 : 1) * (D / 64) * w.tile_tokens * w.group * 128);
-          const int token = c.span.q0 + c.t * 2 * w.tile_tokens;
-          for (int x = 0; x < (both ? 2 : 1); ++x)
+        for (int x = 0; x < 2; ++x) {
+          if (it.last[x] == it.begin) continue;
+          if (!(ok = wait(q_empty + 8 * x, (items[x] & 1) ^ 1, 31))) break;
+          ++items[x];
+          if (lane == 0) {
+            mbar_expect_tx(q_full + 8 * x, (D / 64) * w.tile_tokens * w.group * 128);
             for (int i = 0; i < D / 64; ++i)
-              tma_load_3d(&q_map, base + x * L::kTile + i * 16384, q_full, i * 64, c.h * w.group, token + x * w.tile_tokens);
+              tma_load_3d(&q_map, base + x * L::kTile + i * 16384, q_full + 8 * x, i * 64, c.h * w.group, c.span.q0 + (2 * c.t + x) * w.tile_tokens);
+          }
+          __syncwarp();
         }
-        __syncwarp();
+        if (!ok) break;
         int64_t page = 0;
         auto look_up = [&](int u) {                    // lane i: page i of block u
           if constexpr (PAGED) {
@@ -267,8 +293,9 @@ attend_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constan
           look_up(u + 1);
 #pragma unroll
           for (int which = 0; which < 2; ++which) {
-            if (!(ok = wait(empty + 8 * slot, ph ^ 1u, 32))) break;
-            const uint32_t dst = ring + slot * L::kTile, bar = full + 8 * slot;
+            const uint32_t slot = which ? value.slot : key.slot;
+            if (!(ok = wait((which ? v_empty : k_empty) + 8 * slot, (which ? value.phase : key.phase) ^ 1u, 32))) break;
+            const uint32_t dst = (which ? value_ring : key_ring) + slot * L::kTile, bar = (which ? v_full : k_full) + 8 * slot;
             if constexpr (PAGED) {
               const int rows = page_size < kBlock ? page_size : kBlock;
               if (lane == 0) mbar_expect_tx(bar, there * rows * D * 2);
@@ -282,22 +309,26 @@ attend_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constan
               for (int i = 0; i < D / 64; ++i) tma_load_3d(which ? &v_map : &k_map, dst + i * 16384, bar, i * 64, c.h, c.span.q0 + u * kBlock);
             }
             __syncwarp();
-            if (++slot == S) {
-              slot = 0;
-              ph ^= 1u;
-            }
+            if (which) value.next(); else key.next();
           }
         }
-        ++live;
       }
       left -= it.end - it.begin;
       if (left > 0) next_item<Tiles>(w, c);
+      else if (lane == 0) p.notes[blockIdx.x] = note_of(c, it.begin, it.end, quota);
     }
-    if (!ok)                                            // given up: what is on its way lands first
-      for (uint32_t i = 0; i < static_cast<uint32_t>(S); ++i) mbar_drain(full + 8 * i, i < slot ? ph : ph ^ 1u);
+    if (!ok) {                                          // given up: what is on its way lands first
+      auto drain = [&](uint32_t bars_of, int n, uint32_t slot, uint32_t phase) {
+        for (int i = 0; i < n; ++i) mbar_drain(bars_of + 8 * i, i < static_cast<int>(slot) ? phase : phase ^ 1u);
+      };
+      drain(k_full, L::kKeys, key.slot, key.phase);
+      drain(v_full, L::kValues, value.slot, value.phase);
+      for (int x = 0; x < 2; ++x)
+        if (items[x]) mbar_drain(q_full + 8 * x, (items[x] - 1) & 1);
+    }
   } else if (warp >= 10) {
     // ---------------- helpers: blocks of v that some row does not see all of ----------------
-    uint32_t slot = 0, ph = 0;
+    Slot<L::kValues> at = {0, 0};
     int live = 0;
     while (ok && left > 0) {
       const Part it = part_of(w, c, left);
@@ -307,64 +338,73 @@ attend_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constan
         uint16_t* const set = special + (warp - 10) * 3 * D;
         bool mine = false;                              // the set is this item's
         for (int u = it.begin; ok && u < it.load_end; ++u) {
-#pragma unroll 1
-          for (int which = 0; which < 2; ++which) {
-            if (!(ok = wait(full + 8 * slot, ph, 33))) break;
-            const int pos0 = u * kBlock;
-            if (which == 1 && pos0 + kBlock - 1 > first_limit) {
-              constexpr int kPieces = D / 8;
-#pragma unroll 2
-              for (int i = (warp - 10) * 32 + lane; i < kBlock * kPieces; i += kHelpers * 32) {
-                const int r = i / kPieces, col = i % kPieces;
-                const uint32_t at = ring + slot * L::kTile + (col >> 3) * 16384 + r * 128 + (((col & 7) ^ (r & 7)) << 4);
-                uint4 v = lds128<0>(at);
-                const bool behind = pos0 + r >= c.span.len;
-                const bool odd = !behind && (odd_pair<T>(v.x) || odd_pair<T>(v.y) || odd_pair<T>(v.z) || odd_pair<T>(v.w));
-                unsigned found = __ballot_sync(0xffffffffu, odd);
-                if (found) {
-                  if (!mine) {                          // the items before this one are written: what the set held goes
-                    if (!(ok = wait_count(5, 8 * live, 34))) break;
-                    for (int n = lane; n < 3 * D; n += 32) set[n] = 0xffff;
-                    if (lane == 0) words[2 + warp - 10] = live + 1;
-                    __syncwarp();
-                    mine = true;
-                  }
-                  while (found) {                       // a lane at a time: two may have the same column
-                    if (__ffs(found) - 1 == lane) {
-                      uint32_t word[4] = {v.x, v.y, v.z, v.w};
+          const uint32_t slot = at.slot;
+          if (!(ok = wait(v_full + 8 * slot, at.phase, 33))) break;
+          const int pos0 = u * kBlock;
+          if (pos0 + kBlock - 1 > first_limit) {
+            constexpr int kPieces = D / 8;
+            const int some = first_limit + 1 > pos0 ? first_limit + 1 - pos0 : 0;                                   // rows up to here: seen by all
+            const int seen = it.seen[0] > it.seen[1] ? it.seen[0] : it.seen[1];
+            const int none = seen - pos0 < kBlock ? seen - pos0 : kBlock;                                           // from here on: by none
+            auto place = [&](int i) {
+              const int r = i / kPieces, col = i % kPieces;
+              return value_ring + slot * L::kTile + (col >> 3) * 16384 + r * 128 + (((col & 7) ^ (r & 7)) << 4);
+            };
+            const int mine0 = (warp - 10) * 32 + lane;
+            for (int i = none * kPieces + mine0; i < kBlock * kPieces; i += kHelpers * 32)
+              asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(place(i)), "r"(0) : "memory");
+            constexpr int kBatch = 4;
+            for (int i0 = some * kPieces; i0 < none * kPieces; i0 += kBatch * kHelpers * 32) {
+              uint4 v[kBatch];
+              unsigned odd = 0;
 #pragma unroll
-                      for (int e = 0; e < 8; ++e) {
-                        const float2 pair = unpack2<T>(word[e >> 1]);
-                        const float x = e & 1 ? pair.y : pair.x;
-                        if (!(fabsf(x) <= 3.402823466e38f)) {
-                          uint16_t* const place = set + (x > 0.0f ? 0 : x < 0.0f ? D : 2 * D) + col * 8 + e;
-                          if (pos0 + r - place0 < *place) *place = static_cast<uint16_t>(pos0 + r - place0);
-                          word[e >> 1] &= e & 1 ? 0x0000ffffu : 0xffff0000u;
-                        }
+              for (int b = 0; b < kBatch; ++b) {
+                const int i = i0 + b * kHelpers * 32 + mine0;
+                v[b] = i < none * kPieces ? lds128<0>(place(i)) : make_uint4(0, 0, 0, 0);
+              }
+#pragma unroll
+              for (int b = 0; b < kBatch; ++b)
+                if (odd_pair<T>(v[b].x) || odd_pair<T>(v[b].y) || odd_pair<T>(v[b].z) || odd_pair<T>(v[b].w)) odd |= 1u << b;
+              if (!__any_sync(0xffffffffu, odd)) continue;
+              if (!mine) {                            // the items before this one are written: what the set held goes
+                if (!(ok = wait_count(6, 8, live, 34))) break;
+                for (int n = lane; n < 3 * D; n += 32) set[n] = 0xffff;
+                if (lane == 0) words[2 + warp - 10] = live + 1;
+                __syncwarp();
+                mine = true;
+              }
+              for (int l = 0; l < 32; ++l) {          // a lane at a time: two may have the same column
+                if (l == lane && odd) {
+#pragma unroll
+                  for (int b = 0; b < kBatch; ++b) {
+                    if (!(odd >> b & 1)) continue;
+                    const int i = i0 + b * kHelpers * 32 + mine0, r = i / kPieces, col = i % kPieces;
+                    uint32_t word[4] = {v[b].x, v[b].y, v[b].z, v[b].w};
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                      const float2 pair = unpack2<T>(word[e >> 1]);
+                      const float x = e & 1 ? pair.y : pair.x;
+                      if (!(fabsf(x) <= 3.402823466e38f)) {
+                        uint16_t* const first = set + (x > 0.0f ? 0 : x < 0.0f ? D : 2 * D) + col * 8 + e;
+                        if (pos0 + r - place0 < *first) *first = static_cast<uint16_t>(pos0 + r - place0);
+                        word[e >> 1] &= e & 1 ? 0x0000ffffu : 0xffff0000u;
                       }
-                      v = make_uint4(word[0], word[1], word[2], word[3]);
                     }
-                    __syncwarp();
-                    found &= found - 1;
+                    asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(place(i)), "r"(word[0]), "r"(word[1]), "r"(word[2]), "r"(word[3]) : "memory");
                   }
                 }
-                if (behind) v = make_uint4(0, 0, 0, 0);
-                if (behind || odd) asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+                __syncwarp();
               }
-              fence_proxy_async();
             }
-            __syncwarp();
-            // (also for keys, so that a slot's phases are the ring's)
-            if (lane == 0) mbar_arrive(clean + 8 * slot);
-            if (++slot == S) {
-              slot = 0;
-              ph ^= 1u;
-            }
+            fence_proxy_async();
           }
+          __syncwarp();
+          if (lane == 0) mbar_arrive(v_clean + 8 * slot);
+          at.next();
         }
         __threadfence_block();
         __syncwarp();
-        if (lane == 0) atomicAdd(const_cast<int*>(&words[4]), 1);
+        if (lane == 0) words[4 + warp - 10] = live + 1;
         ++live;
       }
       left -= it.end - it.begin;
@@ -375,37 +415,31 @@ attend_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constan
     constexpr uint32_t kFmt = kBf16 ? 1 : 0;
     const uint32_t id_scores = instr_desc(kFmt, 128) | (static_cast<uint32_t>(kBlock / 8) << 17);
     const uint32_t id_values = instr_desc(kFmt, 128) | (static_cast<uint32_t>(D / 8) << 17) | (1u << 16);       // B is MN-major
-    uint32_t slot = 0, ph = 0;
-    int live = 0;
+    Slot<L::kKeys> key = {0, 0};
+    Slot<L::kValues> value = {0, 0};
     uint32_t items[2] = {0, 0}, p_ph[2] = {0, 0};
-    auto next_slot = [&]() {
-      if (++slot == S) {
-        slot = 0;
-        ph ^= 1u;
-      }
-    };
-    auto scores = [&](int x, uint32_t key_slot) {
-      mma_scores<D>(tmem + x * 128, desc_low(base + x * L::kTile), desc_low(ring + key_slot * L::kTile), kDescHigh, id_scores);
+    auto scores = [&](int x, uint32_t key_slot, bool last) {
+      mma_scores<D>(tmem + x * 128, desc_low(base + x * L::kTile), desc_low(key_ring + key_slot * L::kTile), kDescHigh, id_scores);
       tc_commit<false>(s_full + 8 * x, 0);
+      if (last) tc_commit<false>(q_empty + 8 * x, 0);    // the next item's queries may come
     };
     while (ok && left > 0) {
       const Part it = part_of(w, c, left);
       if (it.live) {
-        if (!(ok = wait(q_full, live & 1, 35))) break;
-        if (!(ok = wait(full + 8 * slot, ph, 36))) break;
-        tc_fence_after();
-        for (int x = 0; x < 2; ++x)
-          if (it.last[x] > it.begin) scores(x, slot);
-        tc_commit<false>(empty + 8 * slot, 0);
-        next_slot();
+        if (!(ok = wait(k_full + 8 * key.slot, key.phase, 36))) break;
+        for (int x = 0; x < 2; ++x) {
+          if (it.last[x] == it.begin) continue;
+          if (!(ok = wait(q_full + 8 * x, items[x] & 1, 35))) break;
+          tc_fence_after();
+          scores(x, key.slot, it.begin + 1 == it.last[x]);
+        }
+        if (!ok) break;
+        tc_commit<false>(k_empty + 8 * key.slot, 0);
+        key.next();
         for (int u = it.begin; ok && u < it.load_end; ++u) {
-          const uint32_t v_slot = slot, v_ph = ph;
-          next_slot();
           const bool more = u + 1 < it.load_end;
-          const uint32_t k_slot = slot;
-          const uint32_t k_ph = ph;
-          if (!(ok = wait(clean + 8 * v_slot, v_ph, 37))) break;
-          if (more && !(ok = wait(full + 8 * k_slot, k_ph, 38))) break;
+          if (!(ok = wait(v_clean + 8 * value.slot, value.phase, 37))) break;
+          if (more && !(ok = wait(k_full + 8 * key.slot, key.phase, 38))) break;
           for (int x = 0; x < 2; ++x) {
             if (u >= it.last[x]) continue;
             if (u == it.begin) {                        // the rows' last item has been read out of O
@@ -414,35 +448,32 @@ attend_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constan
             if (!(ok = wait(p_full + 8 * x, p_ph[x], 40))) break;
             p_ph[x] ^= 1u;
             tc_fence_after();
-            mma_values(tmem + 256 + x * D, tmem + x * 128, desc_low_mn(ring + v_slot * L::kTile), kDescHigh, id_values, u > it.begin);
+            mma_values(tmem + 256 + x * D, tmem + x * 128, desc_low_mn(value_ring + value.slot * L::kTile), kDescHigh, id_values, u > it.begin);
             if (u + 1 < it.last[x]) {
-              scores(x, k_slot);
+              scores(x, key.slot, u + 2 == it.last[x]);
             } else {
               tc_commit<false>(o_full + 8 * x, 0);
               ++items[x];
             }
           }
           if (!ok) break;
-          tc_commit<false>(empty + 8 * v_slot, 0);
+          tc_commit<false>(v_empty + 8 * value.slot, 0);
+          value.next();
           if (more) {
-            tc_commit<false>(empty + 8 * k_slot, 0);
-            next_slot();
+            tc_commit<false>(k_empty + 8 * key.slot, 0);
+            key.next();
           }
         }
-        if (ok) tc_commit<false>(q_empty, 0);
-        ++live;
       }
       left -= it.end - it.begin;
       if (left > 0) next_item<Tiles>(w, c);
     }
-    if (!ok) {                                          // given up: the MMAs issued so far complete before tensor memory goes
-      tc_commit<false>(q_empty, 0);
-      ++live;
-    }
-    if (live) mbar_drain(q_empty, (live - 1) & 1);       // (arrivals reach their barriers before the CTA leaves)
+    // The arrivals of all MMAs so far, given up or not, reach their barriers before the CTA leaves.
+    tc_commit<false>(done, 0);
+    mbar_drain(done, 0);
   }
   } else {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
     // ---------------- rows ----------------
     const int x = warp >> 2, r = (warp & 3) * 32 + lane;
     const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
@@ -532,7 +563,7 @@ attend_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constan
         if (!(ok = wait(o_full + 8 * x, o_ph, 42))) break;
         o_ph ^= 1u;
         tc_fence_after();
-        if (!(ok = wait_count(4, kHelpers * (live + 1), 43))) break;
+        if (!(ok = wait_count(4, kHelpers, live + 1, 43))) break;
         for (int n = 0; n < kHelpers; ++n) odd[n] = words[2 + n] == live + 1;
       }
       const bool whole = it.begin == 0 && it.end == c.units;
@@ -594,7 +625,7 @@ attend_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constan
       if (it.live) {
         __threadfence_block();
         __syncwarp();
-        if (lane == 0) atomicAdd(const_cast<int*>(&words[5]), 1);
+        if (lane == 0) words[6 + warp] = live + 1;
         ++live;
       }
       left -= it.end - it.begin;
@@ -618,21 +649,18 @@ __global__ void __launch_bounds__(256) attend_tc_join_kernel(const JoinParams p)
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const AttentionWork& w = p.work;
-  UnitCursor c;
-  int64_t total, quota = 1;
-  const bool any = find_unit<Tiles>(w, [&](int64_t t) { quota = quota_of(t, p.ctas, p.least_units); return quota * (blockIdx.x + 1); }, &total, &c);
-  if (!any || c.u == 0 || c.u > quota) return;
-  const int parts = parts_of(c.units - c.u, quota);
+  const JoinNote c = p.notes[blockIdx.x];
+  if (c.parts == 0) return;
   const int row = threadIdx.x, x = row >> 7, r = row & 127;
   const int tok_in = r / w.group, g = r - tok_in * w.group, tok = (2 * c.t + x) * w.tile_tokens + tok_in;
-  if (tok_in >= w.tile_tokens || tok >= c.span.n) return;
+  if (tok_in >= w.tile_tokens || tok >= c.n) return;
   auto slot = [&](int i) { return p.partial + (2 * (static_cast<int64_t>(blockIdx.x) + i) + (i == 0 ? 1 : 0)) * partial_floats<256, D>(); };
   float top = -INFINITY;
-  for (int i = 0; i < parts; ++i) top = fmaxf(top, slot(i)[256 * D + row]);
+  for (int i = 0; i < c.parts; ++i) top = fmaxf(top, slot(i)[256 * D + row]);
   const float base = top == -INFINITY ? 0.0f : top;
   float sum = 0.0f, v[kJoinColumns] = {};
 #pragma unroll 2
-  for (int i = 0; i < parts; ++i) {
+  for (int i = 0; i < c.parts; ++i) {
     const float* s = slot(i);
     const float f = ex2(s[256 * D + row] - base);
     sum = fmaf(f, s[256 * D + 256 + row], sum);
@@ -645,9 +673,9 @@ __global__ void __launch_bounds__(256) attend_tc_join_kernel(const JoinParams p)
       v[4 * j + 3] = fmaf(f, y.w, v[4 * j + 3]);
     }
   }
-  const int limit = w.causal ? c.span.len - c.span.n + tok : c.span.len - 1;
+  const int limit = w.causal ? c.len - c.n + tok : c.len - 1;
   const float inv = sum == 0.0f ? (limit < 0 ? 0.0f : NAN) : 1.0f / sum;
-  uint8_t* const out = p.out + (((static_cast<int64_t>(c.span.q0) + tok) * w.heads + c.h * w.group + g) * D + blockIdx.y * kJoinColumns) * 2;
+  uint8_t* const out = p.out + (((static_cast<int64_t>(c.q0) + tok) * w.heads + c.h * w.group + g) * D + blockIdx.y * kJoinColumns) * 2;
 #pragma unroll
   for (int j = 0; j < kJoinColumns; j += 8)
     *reinterpret_cast<uint4*>(out + j * 2) = make_uint4(pack2<T>(v[j] * inv, v[j + 1] * inv), pack2<T>(v[j + 2] * inv, v[j + 3] * inv),
@@ -669,22 +697,8 @@ int launch_one(const RowsParams& p, const CUtensorMap (&maps)[3], int ctas, cuda
   count_launch();
   if (int rc = check_launch("attend_tc_kernel")) return rc;
   if (ctas < 2) return QMM_OK;
-  JoinParams j = {};
-  j.work = p.work;
-  j.out = p.out;
-  j.partial = p.partial;
-  j.ctas = ctas;
-  j.least_units = p.least_units;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(ctas - 1, D / kJoinColumns);
-  cfg.blockDim = dim3(256);
-  cfg.stream = stream;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  cudaLaunchKernelEx(&cfg, attend_tc_join_kernel<T, D>, j);
+  JoinParams j = {p.work, p.out, p.notes, p.partial};
+  launch_early(attend_tc_join_kernel<T, D>, dim3(ctas - 1, D / kJoinColumns), 256, 0, stream, j);
   count_launch();
   return check_launch("attend_tc_join_kernel");
 }
@@ -700,7 +714,7 @@ int launch_of(const RowsParams& p, const CUtensorMap (&maps)[3], int head_dim, b
 int attend_tc_ctas() { return device_sm_count(); }
 
 int64_t attend_tc_workspace(int head_dim, int ctas) {
-  return 2ll * ctas * (head_dim == 64 ? partial_floats<256, 64>() : partial_floats<256, 128>()) * 4;
+  return ctas * (sizeof(JoinNote) + 2ll * (head_dim == 64 ? partial_floats<256, 64>() : partial_floats<256, 128>()) * 4);
 }
 
 int launch_attend_tc(const RowsParams& given, int elem, int head_dim, bool paged, int ctas, cudaStream_t stream) {

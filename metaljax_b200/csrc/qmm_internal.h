@@ -164,9 +164,9 @@ int max_active_clusters(const void* kernel, const cudaLaunchConfig_t& cfg, int c
 // Launches with programmatic stream serialization: a kernel that begins with griddepcontrol.wait is scheduled while the one
 // before it drains. A failure stays as the last error (check_launch reports it).
 template <typename... Params, typename... Args>
-void launch_early(void (*kernel)(Params...), unsigned grid, unsigned threads, size_t smem, cudaStream_t stream, Args&&... args) {
+void launch_early(void (*kernel)(Params...), dim3 grid, unsigned threads, size_t smem, cudaStream_t stream, Args&&... args) {
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(grid);
+  cfg.gridDim = grid;
   cfg.blockDim = dim3(threads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;

@@ -143,6 +143,36 @@ def test_long_cache():
     _check_paged([64], [30000], 8, 2, 128, 128, BF, BF)
 
 
+@pytest.mark.parametrize("page", [16, 128])
+def test_a_chunk_of_a_long_prompt(page):
+    """Thousands of blocks a CTA on the tensor-core kernel, whose roles must not lap one another."""
+    gen = _gen(8)
+    heads, kv, dim, new, length = 32, 8, 128, 1024, 32768
+    cache, table, ks, vs = _paged([length], kv, dim, page, BF, gen)
+    q = torch.randn((new, heads, dim), generator=gen, device=DEV).to(BF)
+    for _ in range(4):
+        got = attention.paged_attention(q, cache, table, R.lengths([length], DEV), R.starts([new], DEV))
+    at = torch.tensor([0, 1, 63, 64, 500, 1023], device=DEV)
+    for i in at.tolist():
+        want, size = R.attend_fast(q[i: i + 1].double(), ks[0][: length - new + i + 1], vs[0][: length - new + i + 1], length - new + i, True, dim ** -0.5)
+        R.close(got[i: i + 1], want, size, BF)
+
+
+def test_calls_one_behind_the_other():
+    """Hundreds of calls with nothing between them, so that the copies of keys and values are late now and then: no role of the kernel may take one
+    of them for another (a wait that ran out would be reported)."""
+    gen = _gen(9)
+    heads, kv, dim, n = 32, 8, 128, 4096
+    x = torch.randn((n, heads + 2 * kv, dim), generator=gen, device=DEV).to(BF)
+    q, k, v = x.split([heads, kv, kv], dim=1)
+    cu = R.starts([n], DEV)
+    first = attention.prompt_attention(q, k, v, cu)
+    outs = [attention.prompt_attention(q, k, v, cu) for _ in range(500)][::50]
+    assert all(torch.equal(o, first) for o in outs)
+    want, size = R.attend_fast(*(y[:600].double() for y in (q, k, v)), 0, True, dim ** -0.5)
+    R.close(first[:600], want, size, BF)
+
+
 def test_offsets_beyond_32_bits():
     """A sequence in the last pages of a cache of 4.6 GB a side."""
     gen = _gen(5)
