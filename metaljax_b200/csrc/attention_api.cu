@@ -41,6 +41,7 @@ int check_attention(const char* what, const qmm_attention_args* a) {
   if (!a || a->struct_size != sizeof(qmm_attention_args)) return fail(QMM_ERR_NULL, "%s: qmm_attention_args with their struct_size are required", what);
   if (a->tokens < 0 || a->tokens > (1 << 30) || a->seqs < 0 || a->seqs > (1 << 30)) return fail(QMM_ERR_SHAPE, "%s: bad number of tokens or sequences", what);
   if (a->heads < 1 || a->kv_heads < 1 || a->heads % a->kv_heads) return fail(QMM_ERR_SHAPE, "%s: the key heads must divide the query heads", what);
+  if (a->tokens * (a->heads / a->kv_heads) > (1ll << 31) - 256) return fail(QMM_ERR_TOO_LARGE, "%s: a key head has less than 2^31 rows of queries", what);
   if (a->heads / a->kv_heads > 64) return fail(QMM_ERR_UNSUPPORTED, "%s: at most 64 query heads per key head", what);
   if (a->head_dim != 64 && a->head_dim != 128) return fail(QMM_ERR_UNSUPPORTED, "%s: head_dim must be 64 or 128", what);
   return QMM_OK;
@@ -82,7 +83,6 @@ int attend(const char* what, const qmm_paged_cache* cache, const CacheView* view
   p.v_row = a->v_row;
   p.v_head = a->v_head;
   p.scale_log2 = a->scale * 1.4426950408889634f;
-  p.least_units = 2;
   if (view) {
     p.cache = *view;
     p.work.longest = static_cast<int64_t>(cache->table_width) << view->page_shift;
@@ -91,6 +91,7 @@ int attend(const char* what, const qmm_paged_cache* cache, const CacheView* view
   const int source = !view ? 0 : cache->elem == QMM_E4M3 ? 2 : 1;
   const bool tc = a->cu_q && a->tokens * p.work.group > 64 * a->seqs && source != 2 &&
                   (!view || (static_cast<uint64_t>(p.cache.pages) * p.work.kv_heads << p.cache.page_shift) < (1ull << 31));
+  p.least = tc ? 8 : 4;
   const int ctas = tc ? attend_tc_ctas() : attend_rows_ctas();
   p.partial = reinterpret_cast<float*>(p.notes + ctas);
   if (tc) return launch_attend_tc(p, a->elem, a->head_dim, view != nullptr, ctas, stream);

@@ -2,10 +2,11 @@
 //
 // An item is a tile of query rows of one sequence and key head: row r of a sequence's n * group rows is new token r / group, query
 // head r % group of the key head's (so that a group's heads read its keys once). RowTiles takes R rows a tile, wherever tokens begin; TokenTiles (whose
-// queries come as boxes of whole tokens) two halves of tile_tokens tokens. A unit is a block of B positions of an item's keys. All units stand in
-// one order (sequence, head, tile, block), and CTA c of C works on those from c * quota on: every CTA has the same number of units whatever the lengths are. An item whose units fall to several CTAs
-// leaves a partial result with each (two slots a CTA: an item that it finishes, and one that it begins), which a second launch joins: that one works
-// out the same order. There are no atomics and no state between calls, and sums do not depend on timing.
+// queries come as boxes of whole tokens) two halves of tile_tokens tokens. A unit is a block of B positions of an item's keys. An item weighs its units
+// and kCost more (queries in, results out). All items stand in one order (sequence, head, tile), and CTA c of C takes the weights from c * quota to
+// (c + 1) * quota, so that every CTA has about as much to do whatever the lengths are. Items of fewer than kWhole units go to one CTA, that of their beginning; longer
+// ones are cut where a share ends, and each CTA leaves a partial result (two slots a CTA: an item that it finishes, and one that it begins), which a second
+// launch joins. There are no atomics and no state between calls, and sums do not depend on timing.
 #pragma once
 
 #include "paged_cache.cuh"
@@ -51,72 +52,49 @@ __device__ __forceinline__ SeqSpan span_of(const AttentionWork& w, int s) {
 }
 
 // Positions up to which the last of a sequence's first `tokens` new tokens sees.
-__device__ __forceinline__ int seen_by(const AttentionWork& w, const SeqSpan& s, int64_t tokens) {
-  const int end = w.causal ? s.len - s.n + (tokens < s.n ? static_cast<int>(tokens) : s.n) : s.len;
+__device__ __forceinline__ int seen_by(const AttentionWork& w, const SeqSpan& s, int tokens) {
+  const int end = w.causal ? s.len - s.n + (tokens < s.n ? tokens : s.n) : s.len;
   return end < 0 ? 0 : end;
 }
 
-// (rows of a sequence can pass 2^31: 64 heads of a group times its tokens)
+// (a sequence's rows are fewer than 2^31: the entry points see to that)
 template <int R, int B>
 struct RowTiles {
-  static __device__ __forceinline__ int tiles(const AttentionWork& w, const SeqSpan& s) {
-    return static_cast<int>((static_cast<int64_t>(s.n) * w.group + R - 1) / R);
-  }
+  static constexpr int kCost = 2, kWhole = 2;
+  static __device__ __forceinline__ int tiles(const AttentionWork& w, const SeqSpan& s) { return static_cast<int>((static_cast<unsigned>(s.n) * w.group + R - 1) / R); }
   // One unit at least, which writes the zeros of rows that see nothing.
   static __device__ __forceinline__ int units(const AttentionWork& w, const SeqSpan& s, int t) {
-    const int u = (seen_by(w, s, ((static_cast<int64_t>(t) + 1) * R - 1) / w.group + 1) + B - 1) / B;
+    const int u = (seen_by(w, s, static_cast<int>((static_cast<unsigned>(t) * R + R - 1) / static_cast<unsigned>(w.group)) + 1) + B - 1) / B;
     return u < 1 ? 1 : u;
   }
 };
 
 template <int B>
 struct TokenTiles {
+  static constexpr int kCost = 3, kWhole = 8;
   static __device__ __forceinline__ int tiles(const AttentionWork& w, const SeqSpan& s) {
-    return (s.n + 2 * w.tile_tokens - 1) / (2 * w.tile_tokens);
+    return static_cast<int>((s.n + 2u * w.tile_tokens - 1) / (2u * w.tile_tokens));
   }
   static __device__ __forceinline__ int units(const AttentionWork& w, const SeqSpan& s, int t) {
-    const int u = (seen_by(w, s, (static_cast<int64_t>(t) + 1) * 2 * w.tile_tokens) + B - 1) / B;
+    const int u = (seen_by(w, s, (t + 1) * 2 * w.tile_tokens) + B - 1) / B;
     return u < 1 ? 1 : u;
   }
 };
 
-// A place in the order of units.
+// A CTA's place in the order: units u to before `end` of an item are its; `room`: weights from the item's beginning to the end of its share.
 struct UnitCursor {
-  int s, h, t, u, units;
+  int s, h, t, u, end, units;
   SeqSpan span;
+  int64_t room;
 };
 
-// One warp: a sequence's units of one head, its lanes over the tiles.
+// Units of an item before the place `room` weights behind its beginning, where one share ends and the next begins: no share of a single unit.
 template <typename Tiles>
-__device__ __forceinline__ int64_t warp_units(const AttentionWork& w, const SeqSpan& s) {
-  const int n = Tiles::tiles(w, s);
-  int64_t sum = 0;
-  for (int t = threadIdx.x & 31; t < n; t += 32) sum += Tiles::units(w, s, t);
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-  return sum;
-}
-
-// One warp: units of one head of 32 sequences from `base` on, a lane each (0 behind the last).
-template <typename Tiles>
-__device__ __forceinline__ int64_t lane_units(const AttentionWork& w, int base, SeqSpan* mine) {
-  const int s = base + (threadIdx.x & 31);
-  SeqSpan span = {0, 0, 0};
-  if (s < w.seqs) span = span_of(w, s);
-  const int tiles = Tiles::tiles(w, span);
-  int64_t sum = 0;
-  if (tiles <= 4)
-    for (int t = 0; t < tiles; ++t) sum += Tiles::units(w, span, t);
-  unsigned many = __ballot_sync(0xffffffffu, tiles > 4);
-  while (many) {
-    const int l = __ffs(many) - 1;
-    many &= many - 1;
-    const SeqSpan other = {__shfl_sync(0xffffffffu, span.q0, l), __shfl_sync(0xffffffffu, span.n, l), __shfl_sync(0xffffffffu, span.len, l)};
-    const int64_t all = warp_units<Tiles>(w, other);
-    if ((threadIdx.x & 31) == l) sum = all;
-  }
-  *mine = span;
-  return sum;
+__device__ __forceinline__ int cut(int units, int64_t room) {
+  if (room >= units + Tiles::kCost) return units;
+  if (units < Tiles::kWhole) return room > 0 ? units : 0;
+  const int u = static_cast<int>(room) - Tiles::kCost;
+  return u < 2 ? 0 : units - u < 2 ? units : u;
 }
 
 __device__ __forceinline__ int64_t warp_sum(int64_t v) {
@@ -133,22 +111,83 @@ __device__ __forceinline__ int64_t warp_scan(int64_t v) {          // inclusive
   return v;
 }
 
-// One warp: the units of a call, and the place of unit `index(total)` in their order (false: there is none).
-template <typename Tiles, typename Index>
-__device__ __forceinline__ bool find_unit(const AttentionWork& w, Index index, int64_t* total_out, UnitCursor* at) {
+// One warp: weight of one head's items of 32 sequences from `base` on, a lane each (0 behind the last).
+template <typename Tiles>
+__device__ __forceinline__ int64_t lane_weights(const AttentionWork& w, int base, SeqSpan* mine) {
+  const int lane = threadIdx.x & 31, s = base + lane;
+  SeqSpan span = {0, 0, 0};
+  if (s < w.seqs) span = span_of(w, s);
+  const int tiles = Tiles::tiles(w, span);
+  int64_t sum = 0;
+  if (tiles <= 32)
+    for (int t = 0; t < tiles; ++t) sum += Tiles::units(w, span, t) + Tiles::kCost;
+  unsigned many = __ballot_sync(0xffffffffu, tiles > 32);
+  while (many) {                                        // long ones: all lanes over the tiles
+    const int l = __ffs(many) - 1;
+    many &= many - 1;
+    const SeqSpan other = {__shfl_sync(0xffffffffu, span.q0, l), __shfl_sync(0xffffffffu, span.n, l), __shfl_sync(0xffffffffu, span.len, l)};
+    const int n = Tiles::tiles(w, other);
+    int64_t part = 0;
+    for (int t = lane; t < n; t += 32) part += Tiles::units(w, other, t) + Tiles::kCost;
+    part = warp_sum(part);
+    if (lane == l) sum = part;
+  }
+  *mine = span;
+  return sum;
+}
+
+// Weights of a CTA's share: at least `least`. (Divisions of 64 bits are calls, and spill what is live around them.)
+__device__ __forceinline__ int64_t quota_of(int64_t total, int ctas, int least) {
+  int shift = 0;
+  while ((total + ctas) >> shift >> 32) shift += 8;     // (a larger share than need be where weights pass 2^32)
+  const int64_t q = shift ? (static_cast<int64_t>(static_cast<uint32_t>(total >> shift) / ctas) + 1) << shift : static_cast<uint32_t>(total + ctas - 1) / ctas;
+  return q < least ? least : q;
+}
+
+// To the beginning of the next item; whether there is one.
+template <typename Tiles>
+__device__ __forceinline__ bool step_item(const AttentionWork& w, UnitCursor& c) {
+  if (++c.t >= Tiles::tiles(w, c.span)) {
+    c.t = 0;
+    if (++c.h >= w.kv_heads) {
+      c.h = 0;
+      do {
+        if (++c.s >= w.seqs) return false;
+        c.span = span_of(w, c.s);
+      } while (c.span.n == 0);
+    }
+  }
+  c.units = Tiles::units(w, c.span, c.t);
+  return true;
+}
+
+// To this CTA's part of the next item; whether it has one.
+template <typename Tiles>
+__device__ __forceinline__ bool next_item(const AttentionWork& w, UnitCursor& c) {
+  c.room -= c.units + Tiles::kCost;
+  if (c.room <= 0 || !step_item<Tiles>(w, c)) return false;
+  c.u = 0;
+  c.end = cut<Tiles>(c.units, c.room);
+  return c.end > 0;
+}
+
+// One warp: where CTA `cta` of `ctas` begins; false where it has nothing to do. `share`: what a CTA takes.
+template <typename Tiles>
+__device__ __forceinline__ bool find_share(const AttentionWork& w, int cta, int ctas, int least, UnitCursor* at, int64_t* share) {
   const int lane = threadIdx.x & 31;
   SeqSpan span;
   int64_t mine = 0, total = 0;
   for (int base = 0; base < w.seqs; base += 32) {
-    mine = lane_units<Tiles>(w, base, &span);
+    mine = lane_weights<Tiles>(w, base, &span);
     total += warp_sum(mine) * w.kv_heads;
   }
-  *total_out = total;
-  int64_t left = index(total);
-  if (left < 0 || left >= total) return false;
+  const int64_t quota = quota_of(total, ctas, least);
+  *share = quota;
+  int64_t left = quota * cta;
+  if (left >= total) return false;
   int64_t per_head = 0;
   for (int base = 0; base < w.seqs; base += 32) {
-    if (w.seqs > 32) mine = lane_units<Tiles>(w, base, &span);       // (the only ones are still there)
+    if (w.seqs > 32) mine = lane_weights<Tiles>(w, base, &span);    // (the only ones are still there)
     const int64_t upto = warp_scan(mine) * w.kv_heads;
     const unsigned past = __ballot_sync(0xffffffffu, upto > left);
     if (past) {
@@ -162,55 +201,30 @@ __device__ __forceinline__ bool find_unit(const AttentionWork& w, Index index, i
     left -= __shfl_sync(0xffffffffu, upto, 31);
   }
   at->h = 0;
-  while (left >= per_head) {                            // (a few heads: a division of 64 bits is a call, and spills)
+  while (left >= per_head) {
     left -= per_head;
     ++at->h;
   }
   const int tiles = Tiles::tiles(w, at->span);
   for (int base = 0; base < tiles; base += 32) {
-    const int64_t u = base + lane < tiles ? Tiles::units(w, at->span, base + lane) : 0;
-    const int64_t upto = warp_scan(u);
+    const int units = base + lane < tiles ? Tiles::units(w, at->span, base + lane) : 0;
+    const int64_t upto = warp_scan(base + lane < tiles ? units + Tiles::kCost : 0);
     const unsigned past = __ballot_sync(0xffffffffu, upto > left);
     if (past) {
       const int l = __ffs(past) - 1;
       at->t = base + l;
-      at->units = static_cast<int>(__shfl_sync(0xffffffffu, u, l));
-      at->u = static_cast<int>(left - (__shfl_sync(0xffffffffu, upto, l) - at->units));
-      return true;
+      at->units = __shfl_sync(0xffffffffu, units, l);
+      left -= __shfl_sync(0xffffffffu, upto, l) - (at->units + Tiles::kCost);
+      break;
     }
     left -= __shfl_sync(0xffffffffu, upto, 31);
   }
-  return false;                                        // (not reached: the sums are the same)
-}
-
-// To the first unit of the next item (which there has to be).
-template <typename Tiles>
-__device__ __forceinline__ void next_item(const AttentionWork& w, UnitCursor& c) {
-  c.u = 0;
-  if (++c.t >= Tiles::tiles(w, c.span)) {
-    c.t = 0;
-    if (++c.h >= w.kv_heads) {
-      c.h = 0;
-      do {
-        ++c.s;
-        c.span = c.s < w.seqs ? span_of(w, c.s) : SeqSpan{0, 1, 0};
-      } while (c.span.n == 0);
-    }
-  }
-  c.units = Tiles::units(w, c.span, c.t);
-}
-
-// Units of a CTA: at least `least`, below which a CTA's share does not pay for a part of an item to be joined. (Divisions of 64 bits are calls, and spill
-// what is live around them.)
-__device__ __forceinline__ int64_t quota_of(int64_t total, int ctas, int least) {
-  int shift = 0;
-  while ((total + ctas) >> shift >> 32) shift += 8;     // (a larger share than need be where units pass 2^32)
-  const int64_t q = shift ? (static_cast<int64_t>(static_cast<uint32_t>(total >> shift) / ctas) + 1) << shift : static_cast<uint32_t>(total + ctas - 1) / ctas;
-  return q < least ? least : q;
-}
-// CTAs that have a part of an item of which `after` units lie behind the end of the first one's share.
-__device__ __forceinline__ int parts_of(int after, int64_t quota) {
-  return 1 + (quota >> 31 ? 1 : static_cast<int>((static_cast<uint32_t>(after) + static_cast<uint32_t>(quota) - 1) / static_cast<uint32_t>(quota)));
+  // `left` weights into the item
+  at->u = left > 0 ? cut<Tiles>(at->units, left) : 0;
+  at->room = quota + left;
+  if (at->u == at->units) return next_item<Tiles>(w, *at);
+  at->end = cut<Tiles>(at->units, at->room);
+  return at->end > at->u;
 }
 
 // The workspace: a note of every CTA, written by each, then two partial results a CTA. The note says what the second launch has to join at the end of a
@@ -218,8 +232,13 @@ __device__ __forceinline__ int parts_of(int after, int64_t quota) {
 struct JoinNote {
   int32_t parts, q0, n, len, h, t, pad[2];
 };
-__device__ __forceinline__ JoinNote note_of(const UnitCursor& c, int begun, int ended, int64_t quota) {
-  const int parts = begun == 0 && ended < c.units ? parts_of(c.units - ended, quota) : 0;
+// (the shares behind the first one's end take `share` units each, the last one what is left, and a single unit more)
+__device__ __forceinline__ JoinNote note_of(const UnitCursor& c, int begun, int64_t share) {
+  int parts = 0;
+  if (begun == 0 && c.end < c.units) {
+    const int rest = c.units - 1 - c.end;
+    parts = 1 + (share > rest ? 1 : static_cast<int>((static_cast<uint32_t>(rest) + static_cast<uint32_t>(share) - 1) / static_cast<uint32_t>(share)));
+  }
   return {parts, c.span.q0, c.span.n, c.span.len, c.h, c.t, {0, 0}};
 }
 

@@ -88,30 +88,26 @@ __global__ void __launch_bounds__(kThreads, 2) attend_rows_kernel(const RowsPara
 
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");
+  if (tid == 0) p.notes[blockIdx.x].parts = 0;
   // every warp works out where this CTA begins by itself
   UnitCursor c;
-  int64_t total, quota = 1;
-  const bool any = find_unit<Tiles>(w, [&](int64_t t) { quota = quota_of(t, gridDim.x, p.least_units); return quota * blockIdx.x; }, &total, &c);
-  if (!any) {
-    if (tid == 0) p.notes[blockIdx.x].parts = 0;
-    return;
-  }
-  const int64_t first_unit = quota * blockIdx.x;
-  const int count = static_cast<int>(total - first_unit < quota ? total - first_unit : quota);
+  int64_t share;
+  if (!find_share<Tiles>(w, blockIdx.x, gridDim.x, p.least, &c, &share)) return;
   UnitCursor load = c;                                  // where the copies are
+  bool loading = true;
 
   // ---- copies: a warp asks for rows 16 * warp .. of a chunk (which lie in one page) ----
   int64_t page = 0;                                     // of the next chunk's rows of this warp
-  auto look_up = [&](int loaded) {
+  auto look_up = [&]() {
     if constexpr (kPaged) {
       const int pos = load.u * kChunk + 16 * warp;
       page = 0;
-      if (loaded < count && pos < load.span.len) page = page_of(p.cache, load.s, pos, w.status);
+      if (loading && pos < load.span.len) page = page_of(p.cache, load.s, pos, w.status);
       if (page < 0) page = 0;
     }
   };
   auto request = [&](int loaded) {                      // the chunk that `load` stands at into the ring, and `load` on
-    if (loaded < count) {
+    if (loading) {
       const uint32_t stage = ring + (loaded % L::kStages) * L::kStage;
       constexpr int kPieces = L::kRowBytes / 16;
       const int pos0 = load.u * kChunk + 16 * warp;
@@ -141,13 +137,13 @@ __global__ void __launch_bounds__(kThreads, 2) attend_rows_kernel(const RowsPara
           cp_async16(stage + 2 * L::kHalf + lane * kChunk + 16 * warp, (lane ? p.cache.v_exp : p.cache.k_exp) + row, pos0 < load.span.len ? 16 : 0);
         }
       }
-      if (++load.u >= load.units && loaded + 1 < count) next_item<Tiles>(w, load);
-      look_up(loaded + 1);
+      if (++load.u >= load.end) loading = next_item<Tiles>(w, load);
+      look_up();
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
 
-  look_up(0);
+  look_up();
 #pragma unroll
   for (int i = 0; i < L::kStages - 1; ++i) request(i);
 
@@ -160,18 +156,16 @@ __global__ void __launch_bounds__(kThreads, 2) attend_rows_kernel(const RowsPara
 
   auto begin_item = [&]() {
     begun = c.u;
-    const int64_t rows = static_cast<int64_t>(c.span.n) * w.group - static_cast<int64_t>(c.t) * R;
-    tile_rows = rows < R ? static_cast<int>(rows) : R;
-    const int64_t row0 = static_cast<int64_t>(c.t) * R;
-    tile_first_limit = w.causal ? c.span.len - c.span.n + static_cast<int>(row0 / w.group) : c.span.len - 1;
+    const int row0 = c.t * R, rows = c.span.n * w.group - row0;
+    tile_rows = rows < R ? rows : R;
+    tile_first_limit = w.causal ? c.span.len - c.span.n + row0 / w.group : c.span.len - 1;
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       const int r = rw * 16 + (lane >> 2) + 8 * i;
       m[i] = -INFINITY;
       l[i] = 0.0f;
       limit[i] = -1;
-      const int64_t row = row0 + r;
-      const int tok = static_cast<int>(row / w.group), g = static_cast<int>(row - static_cast<int64_t>(tok) * w.group);
+      const int tok = (row0 + r) / w.group, g = row0 + r - tok * w.group;
       const bool live = r < tile_rows;
       if (live) limit[i] = w.causal ? c.span.len - c.span.n + tok : c.span.len - 1;
       const uint8_t* src = p.q + ((c.span.q0 + (live ? tok : 0)) * p.q_row + (c.h * w.group + (live ? g : 0)) * p.q_head) * 2 + (lane & 3) * 4;
@@ -192,7 +186,7 @@ __global__ void __launch_bounds__(kThreads, 2) attend_rows_kernel(const RowsPara
   __syncthreads();
   begin_item();
 
-  for (int done = 0; done < count; ++done) {
+  for (int done = 0;; ++done) {
     asm volatile("cp.async.wait_group %0;" ::"n"(L::kStages - 2) : "memory");
     if constexpr (KW == 4) __syncwarp(); else __syncthreads();
     request(done + L::kStages - 1);
@@ -313,7 +307,7 @@ __global__ void __launch_bounds__(kThreads, 2) attend_rows_kernel(const RowsPara
       }
     }
     ++c.u;
-    if (c.u < c.units && done + 1 < count) continue;
+    if (c.u < c.end) continue;
 
     // ---- the item, or this CTA's part of it, ends: its warps' sums meet where the chunk was (e4m3: where its values were) ----
 #pragma unroll
@@ -341,8 +335,7 @@ __global__ void __launch_bounds__(kThreads, 2) attend_rows_kernel(const RowsPara
     constexpr int kVec = D / 4;                           // threads of a row
     for (int i = tid; i < tile_rows * kVec; i += kThreads) {
       const int r = i / kVec, d = (i % kVec) * 4;
-      const int64_t row = static_cast<int64_t>(c.t) * R + r;
-      const int tok = static_cast<int>(row / w.group), g = static_cast<int>(row - static_cast<int64_t>(tok) * w.group);
+      const int tok = (c.t * R + r) / w.group, g = c.t * R + r - tok * w.group;
       const int seen = w.causal ? c.span.len - c.span.n + tok : c.span.len - 1;
       float mm = -INFINITY, ll = 0.0f, v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
@@ -388,12 +381,9 @@ __global__ void __launch_bounds__(kThreads, 2) attend_rows_kernel(const RowsPara
       if (tid == 0) *any_special = 0;
     }
     __syncthreads();
-    if (done + 1 < count) {
-      next_item<Tiles>(w, c);
-      begin_item();
-    } else if (tid == 0) {
-      p.notes[blockIdx.x] = note_of(c, begun, c.u, quota);
-    }
+    if (c.end < c.units && tid == 0) p.notes[blockIdx.x] = note_of(c, begun, share);
+    if (!next_item<Tiles>(w, c)) break;
+    begin_item();
   }
   asm volatile("cp.async.wait_all;" ::: "memory");
 }
@@ -406,9 +396,8 @@ __global__ void __launch_bounds__(kJoinThreads) attend_join_kernel(const JoinPar
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const AttentionWork& w = p.work;
   const JoinNote c = p.notes[blockIdx.x];
-  const int64_t row = static_cast<int64_t>(c.t) * R + blockIdx.y * kJoinRows + (threadIdx.x >> 5);
-  if (c.parts == 0 || row >= static_cast<int64_t>(c.n) * w.group) return;
-  const int r = blockIdx.y * kJoinRows + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+  const int r = blockIdx.y * kJoinRows + (threadIdx.x >> 5), lane = threadIdx.x & 31, row = c.t * R + r;
+  if (c.parts == 0 || row >= c.n * w.group) return;
   constexpr int V = D / 32;                                                       // elements of a lane
   // (the first part lies behind this CTA's finished item, the others are the first of theirs)
   const float* const first = p.partial + (2 * static_cast<int64_t>(blockIdx.x) + 1) * partial_floats<R, D>();
@@ -447,7 +436,7 @@ __global__ void __launch_bounds__(kJoinThreads) attend_join_kernel(const JoinPar
   }
 #pragma unroll
   for (int x = 16; x > 0; x >>= 1) ll += __shfl_xor_sync(0xffffffffu, ll, x);
-  const int tok = static_cast<int>(row / w.group), g = static_cast<int>(row - static_cast<int64_t>(tok) * w.group);
+  const int tok = row / w.group, g = row - tok * w.group;
   const int seen = w.causal ? c.len - c.n + tok : c.len - 1;
   const float inv = ll == 0.0f ? (seen < 0 ? 0.0f : NAN) : 1.0f / ll;
   uint8_t* dst = p.out + ((static_cast<int64_t>(c.q0) + tok) * w.heads + c.h * w.group + g) * D * 2 + lane * V * 2;

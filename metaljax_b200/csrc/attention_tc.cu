@@ -39,7 +39,7 @@ struct TcLayout {
   static constexpr int kValueRing = kKeyRing + kKeys * kTile;
   static constexpr int kSpecials = kValueRing + kValues * kTile;
   static constexpr int kBars = kSpecials + kHelpers * 3 * D * 2;           // 16-bit places, a set for each helper
-  static constexpr int kNumBars = 2 * kKeys + 3 * kValues + 13;
+  static constexpr int kNumBars = 2 * kKeys + 3 * kValues + 15;
   static constexpr int kWords = kBars + 8 * kNumBars;  // tensor memory's address, abort flag, and counters
   static constexpr int kBytes = kWords + 64 + 1024;    // (what is swizzled begins at a multiple of 1024)
 };
@@ -65,8 +65,7 @@ __device__ __forceinline__ void mma_scores(uint32_t d, uint32_t a_lo, uint32_t b
   "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [a], b, %4, " ACC ";"
 __device__ __forceinline__ void mma_values(uint32_t d, uint32_t a, uint32_t b_lo, uint32_t hi, uint32_t idesc, uint32_t accumulate) {
   asm volatile("{ .reg .pred e, p, t; .reg .b32 a, bl; .reg .b64 b; elect.sync _|e, 0xffffffff; setp.ne.b32 p, %5, 0; setp.eq.b32 t, 0, 0;"
-               QMM_TS("0", "0", "p") QMM_TS("8", "128", "t") QMM_TS("16", "256", "t") QMM_TS("24", "384", "t")
-               QMM_TS("32", "512", "t") QMM_TS("40", "640", "t") QMM_TS("48", "768", "t") QMM_TS("56", "896", "t") "}"
+               QMM_TS("0", "0", "p") QMM_TS("8", "128", "t") QMM_TS("16", "256", "t") QMM_TS("24", "384", "t") "}"
                ::"r"(d), "r"(a), "r"(b_lo), "r"(hi), "r"(idesc), "r"(accumulate) : "memory");
 }
 // MN-major operand in the 128-byte swizzle: columns of 64 elements (leading byte offset) and groups of 8 positions (stride byte offset).
@@ -80,6 +79,11 @@ __device__ __forceinline__ void tma_load_3d(const CUtensorMap* map, uint32_t dst
 __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float y;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
   return y;
 }
 __device__ __forceinline__ uint64_t pack_f32(float a, float b) {
@@ -131,22 +135,27 @@ struct Slot {
   }
 };
 
-// What a CTA does of an item: units [begin, end) of it, of which each half sees those before its own `last`.
+// A sector of a row at once (16-byte aligned at least: two stores where it is not 32).
+__device__ __forceinline__ void store32(uint8_t* at, const uint32_t (&v)[8]) {
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(at), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
+               : "memory");
+}
+
+// What a CTA does of an item: units from `begin` on, of which each half sees those before its own `last`.
 struct Part {
-  int begin, end, seen[2], last[2], load_end;
+  int begin, seen[2], last[2], load_end;
   bool live;
 };
-__device__ __forceinline__ Part part_of(const AttentionWork& w, const UnitCursor& c, int left) {
+__device__ __forceinline__ Part part_of(const AttentionWork& w, const UnitCursor& c) {
   Part r;
   r.begin = c.u;
-  r.end = c.units - c.u < left ? c.units : c.u + left;
-  const int64_t token = static_cast<int64_t>(c.t) * 2 * w.tile_tokens;
+  const int token = c.t * 2 * w.tile_tokens;
   r.seen[0] = seen_by(w, c.span, token + w.tile_tokens);
   r.seen[1] = token + w.tile_tokens < c.span.n ? seen_by(w, c.span, token + 2 * w.tile_tokens) : 0;
 #pragma unroll
   for (int x = 0; x < 2; ++x) {
     const int u = (r.seen[x] + kBlock - 1) / kBlock;
-    r.last[x] = u < r.end ? u : r.end;
+    r.last[x] = u < c.end ? u : c.end;
     if (r.last[x] < r.begin) r.last[x] = r.begin;
   }
   r.load_end = r.last[0] > r.last[1] ? r.last[0] : r.last[1];
@@ -174,7 +183,7 @@ attend_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constan
   const uint32_t key_ring = base + L::kKeyRing, value_ring = base + L::kValueRing, bars = base + L::kBars;
   const uint32_t q_full = bars, q_empty = bars + 16, k_full = bars + 32, k_empty = k_full + 8 * L::kKeys;
   const uint32_t v_full = k_empty + 8 * L::kKeys, v_empty = v_full + 8 * L::kValues, v_clean = v_empty + 8 * L::kValues;
-  const uint32_t s_full = v_clean + 8 * L::kValues, p_full = s_full + 16, o_full = p_full + 16, o_free = o_full + 16, done = o_free + 16;
+  const uint32_t s_full = v_clean + 8 * L::kValues, p_full = s_full + 16, o_full = p_full + 32, o_free = o_full + 16, done = o_free + 16;
   const uint32_t tmem_slot = base + L::kWords, abort_at = tmem_slot + 4;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const AttentionWork& w = p.work;
@@ -195,7 +204,8 @@ attend_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constan
       init(q_full + 8 * x, 1);
       init(q_empty + 8 * x, 1);
       init(s_full + 8 * x, 1);
-      init(p_full + 8 * x, 4);
+      init(p_full + 16 * x, 4);
+      init(p_full + 16 * x + 8, 4);
       init(o_full + 8 * x, 1);
       init(o_free + 8 * x, 4);
     }
@@ -216,13 +226,8 @@ attend_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constan
 
   asm volatile("griddepcontrol.wait;" ::: "memory");
   UnitCursor c;
-  int64_t total, quota = 1;
-  const bool any = find_unit<Tiles>(w, [&](int64_t t) { quota = quota_of(t, gridDim.x, p.least_units); return quota * blockIdx.x; }, &total, &c);
-  int left = 0;
-  if (any) {
-    const int64_t rest = total - quota * blockIdx.x;
-    left = static_cast<int>(rest < quota ? rest : quota);
-  }
+  int64_t share;
+  bool more = find_share<Tiles>(w, blockIdx.x, gridDim.x, p.least, &c, &share);
   // every lane waits, and all go on or none does
   auto wait = [&](uint32_t bar, uint32_t parity, int where) -> bool { return __all_sync(0xffffffffu, wait_phase(bar, parity, abort_at, where)); };
   // ... for `n` counters of this CTA, a lane each
@@ -258,8 +263,8 @@ attend_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constan
     int items[2] = {0, 0};
     const int page_size = 1 << p.cache.page_shift;
     const int per_block = PAGED ? (page_size < kBlock ? kBlock / page_size : 1) : 1;       // pages of a block
-    while (ok && left > 0) {
-      const Part it = part_of(w, c, left);
+    while (ok && more) {
+      const Part it = part_of(w, c);
       if (it.live) {
         for (int x = 0; x < 2; ++x) {
           if (it.last[x] == it.begin) continue;
@@ -286,8 +291,8 @@ attend_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constan
         for (int u = it.begin; ok && u < it.load_end; ++u) {
           int there = 1;                                // pages of the block that the sequence has
           if constexpr (PAGED) {
-            const int more = (c.span.len - u * kBlock + page_size - 1) >> p.cache.page_shift;
-            there = more < per_block ? more : per_block;
+            const int pages = (c.span.len - u * kBlock + page_size - 1) >> p.cache.page_shift;
+            there = pages < per_block ? pages : per_block;
           }
           const int64_t here = page;
           look_up(u + 1);
@@ -313,9 +318,8 @@ attend_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constan
           }
         }
       }
-      left -= it.end - it.begin;
-      if (left > 0) next_item<Tiles>(w, c);
-      else if (lane == 0) p.notes[blockIdx.x] = note_of(c, it.begin, it.end, quota);
+      if (c.end < c.units && lane == 0) p.notes[blockIdx.x] = note_of(c, it.begin, share);
+      more = next_item<Tiles>(w, c);
     }
     if (!ok) {                                          // given up: what is on its way lands first
       auto drain = [&](uint32_t bars_of, int n, uint32_t slot, uint32_t phase) {
@@ -330,8 +334,8 @@ attend_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constan
     // ---------------- helpers: blocks of v that some row does not see all of ----------------
     Slot<L::kValues> at = {0, 0};
     int live = 0;
-    while (ok && left > 0) {
-      const Part it = part_of(w, c, left);
+    while (ok && more) {
+      const Part it = part_of(w, c);
       if (it.live) {
         const int first_limit = w.causal ? c.span.len - c.span.n + c.t * 2 * w.tile_tokens : c.span.len - 1;
         const int place0 = place_of(first_limit);
@@ -407,8 +411,7 @@ attend_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constan
         if (lane == 0) words[4 + warp - 10] = live + 1;
         ++live;
       }
-      left -= it.end - it.begin;
-      if (left > 0) next_item<Tiles>(w, c);
+      more = next_item<Tiles>(w, c);
     }
   } else {
     // ---------------- the MMAs' issuer ----------------
@@ -423,8 +426,8 @@ attend_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constan
       tc_commit<false>(s_full + 8 * x, 0);
       if (last) tc_commit<false>(q_empty + 8 * x, 0);    // the next item's queries may come
     };
-    while (ok && left > 0) {
-      const Part it = part_of(w, c, left);
+    while (ok && more) {
+      const Part it = part_of(w, c);
       if (it.live) {
         if (!(ok = wait(k_full + 8 * key.slot, key.phase, 36))) break;
         for (int x = 0; x < 2; ++x) {
@@ -437,18 +440,22 @@ attend_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constan
         tc_commit<false>(k_empty + 8 * key.slot, 0);
         key.next();
         for (int u = it.begin; ok && u < it.load_end; ++u) {
-          const bool more = u + 1 < it.load_end;
+          const bool next = u + 1 < it.load_end;
           if (!(ok = wait(v_clean + 8 * value.slot, value.phase, 37))) break;
-          if (more && !(ok = wait(k_full + 8 * key.slot, key.phase, 38))) break;
+          if (next && !(ok = wait(k_full + 8 * key.slot, key.phase, 38))) break;
           for (int x = 0; x < 2; ++x) {
             if (u >= it.last[x]) continue;
             if (u == it.begin) {                        // the rows' last item has been read out of O
               if (!(ok = wait(o_free + 8 * x, (items[x] & 1) ^ 1, 39))) break;
             }
-            if (!(ok = wait(p_full + 8 * x, p_ph[x], 40))) break;
+            for (int part = 0; part < 2; ++part) {      // P comes in two parts of 64 positions
+              if (!(ok = wait(p_full + 16 * x + 8 * part, p_ph[x], 40))) break;
+              tc_fence_after();
+              mma_values(tmem + 256 + x * D, tmem + x * 128 + part * 32, desc_low_mn(value_ring + value.slot * L::kTile + part * 8192), kDescHigh, id_values,
+                         part | (u > it.begin));
+            }
+            if (!ok) break;
             p_ph[x] ^= 1u;
-            tc_fence_after();
-            mma_values(tmem + 256 + x * D, tmem + x * 128, desc_low_mn(value_ring + value.slot * L::kTile), kDescHigh, id_values, u > it.begin);
             if (u + 1 < it.last[x]) {
               scores(x, key.slot, u + 2 == it.last[x]);
             } else {
@@ -459,14 +466,13 @@ attend_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constan
           if (!ok) break;
           tc_commit<false>(v_empty + 8 * value.slot, 0);
           value.next();
-          if (more) {
+          if (next) {
             tc_commit<false>(k_empty + 8 * key.slot, 0);
             key.next();
           }
         }
       }
-      left -= it.end - it.begin;
-      if (left > 0) next_item<Tiles>(w, c);
+      more = next_item<Tiles>(w, c);
     }
     // The arrivals of all MMAs so far, given up or not, reach their barriers before the CTA leaves.
     tc_commit<false>(done, 0);
@@ -482,8 +488,8 @@ attend_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constan
     const uint64_t scale = pack_f32(p.scale_log2, p.scale_log2);
     uint32_t s_ph = 0, o_ph = 0;
     int live = 0;
-    while (ok && left > 0) {
-      const Part it = part_of(w, c, left);
+    while (ok && more) {
+      const Part it = part_of(w, c);
       const int tok0 = (2 * c.t + x) * w.tile_tokens, tok = tok0 + tok_in;
       const bool mine = tok_in < w.tile_tokens && tok < c.span.n;
       const int limit = w.causal ? c.span.len - c.span.n + tok : c.span.len - 1;
@@ -499,21 +505,21 @@ attend_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constan
         for (int i = 0; i < 4; ++i) tmem_ld(s_at + i * 32, s[i]);
         tmem_wait_ld();
         if (u * kBlock + kBlock - 1 > first_limit) {
-          const int seen = limit - u * kBlock;          // columns 0 .. seen are seen
 #pragma unroll
-          for (int i = 0; i < 4; ++i)
+          for (int i = 0; i < 4; ++i) {
+            const int seen = limit - u * kBlock - i * 32;             // columns 0 .. seen of these 32 are seen: a bit each
+            const uint32_t mask = seen < 0 ? 0u : seen >= 31 ? ~0u : (2u << seen) - 1u;
 #pragma unroll
             for (int j = 0; j < 32; ++j)
-              if (i * 32 + j > seen) s[i][j] = 0xff800000u;
+              if (!(mask & 1u << j)) s[i][j] = 0xff800000u;
+          }
         }
-        float m[4];
+        float m[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          m[i] = -INFINITY;
+        for (int i = 0; i < 4; ++i)
 #pragma unroll
-          for (int j = 0; j < 32; j += 2) m[i] = fmaxf(m[i], fmaxf(__uint_as_float(s[i][j]), __uint_as_float(s[i][j + 1])));
-        }
-        const float now = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3])) * p.scale_log2;
+          for (int j = 0; j < 32; j += 2) m[j >> 1 & 3] = max3(m[j >> 1 & 3], __uint_as_float(s[i][j]), __uint_as_float(s[i][j + 1]));
+        const float now = fmaxf(max3(m[0], m[1], m[2]), m[3]) * p.scale_log2;
         if (u == it.begin) {
           top = now;
         } else if (__any_sync(0xffffffffu, now > top + 8.0f)) {
@@ -537,23 +543,26 @@ attend_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constan
         const uint64_t off2 = pack_f32(off, off);
         uint64_t sums[2] = {0, 0};
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          uint32_t out[16];
+        for (int part = 0; part < 2; ++part) {
+          uint32_t out[32];
 #pragma unroll
-          for (int j = 0; j < 16; ++j) {
-            const float2 e = unpack_f32(fma2(pack_f32(__uint_as_float(s[i][2 * j]), __uint_as_float(s[i][2 * j + 1])), scale, off2));
-            const float a = ex2(e.x), b = ex2(e.y);
-            sums[j & 1] = add2(sums[j & 1], pack_f32(a, b));
-            out[j] = pack2<T>(a, b);
-          }
-          tmem_st16(s_at + i * 16, out);
+          for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int j = 0; j < 16; ++j) {
+              const uint32_t(&v)[32] = s[2 * part + i];
+              const float2 e = unpack_f32(fma2(pack_f32(__uint_as_float(v[2 * j]), __uint_as_float(v[2 * j + 1])), scale, off2));
+              const float a = ex2(e.x), b = ex2(e.y);
+              sums[j & 1] = add2(sums[j & 1], pack_f32(a, b));
+              out[i * 16 + j] = pack2<T>(a, b);
+            }
+          tmem_st(s_at + part * 32, out);
+          tmem_wait_st();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(p_full + 16 * x + 8 * part);
         }
         const float2 both = unpack_f32(add2(sums[0], sums[1]));
         sum += both.x + both.y;
-        tmem_wait_st();
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(p_full + 8 * x);
       }
       if (!ok) break;
       // ---- the item, or this CTA's part of it, ends ----
@@ -566,7 +575,7 @@ attend_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constan
         if (!(ok = wait_count(4, kHelpers, live + 1, 43))) break;
         for (int n = 0; n < kHelpers; ++n) odd[n] = words[2 + n] == live + 1;
       }
-      const bool whole = it.begin == 0 && it.end == c.units;
+      const bool whole = it.begin == 0 && c.end == c.units;
       const float inv = sum == 0.0f ? (limit < 0 ? 0.0f : NAN) : 1.0f / sum;
       uint8_t* const out = p.out + ((static_cast<int64_t>(c.span.q0) + tok) * w.heads + c.h * w.group + g) * D * 2;
       float4* const part = reinterpret_cast<float4*>(p.partial + (2 * static_cast<int64_t>(blockIdx.x) + (it.begin == 0 ? 1 : 0)) * partial_floats<256, D>());
@@ -598,13 +607,11 @@ attend_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constan
         if (!mine) continue;
         if (whole) {
 #pragma unroll
-          for (int j = 0; j < 32; j += 8) {
-            uint4 v;
-            v.x = pack2<T>(__uint_as_float(o[j]) * inv, __uint_as_float(o[j + 1]) * inv);
-            v.y = pack2<T>(__uint_as_float(o[j + 2]) * inv, __uint_as_float(o[j + 3]) * inv);
-            v.z = pack2<T>(__uint_as_float(o[j + 4]) * inv, __uint_as_float(o[j + 5]) * inv);
-            v.w = pack2<T>(__uint_as_float(o[j + 6]) * inv, __uint_as_float(o[j + 7]) * inv);
-            *reinterpret_cast<uint4*>(out + (i * 32 + j) * 2) = v;
+          for (int j = 0; j < 32; j += 16) {
+            uint32_t v[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] = pack2<T>(__uint_as_float(o[j + 2 * e]) * inv, __uint_as_float(o[j + 2 * e + 1]) * inv);
+            store32(out + (i * 32 + j) * 2, v);
           }
         } else {
           // four elements of 256 rows side by side: neighbouring threads write neighbouring 16 bytes
@@ -628,8 +635,7 @@ attend_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constan
         if (lane == 0) words[6 + warp] = live + 1;
         ++live;
       }
-      left -= it.end - it.begin;
-      if (left > 0) next_item<Tiles>(w, c);
+      more = next_item<Tiles>(w, c);
     }
   }
   tc_fence_before();
