@@ -91,7 +91,7 @@ int attend(const char* what, const qmm_paged_cache* cache, const CacheView* view
   const int source = !view ? 0 : cache->elem == QMM_E4M3 ? 2 : 1;
   const bool tc = a->cu_q && a->tokens * p.work.group > 64 * a->seqs && source != 2 &&
                   (!view || (static_cast<uint64_t>(p.cache.pages) * p.work.kv_heads << p.cache.page_shift) < (1ull << 31));
-  p.least = tc ? 8 : 4;
+  p.least = 4;
   const int ctas = tc ? attend_tc_ctas() : attend_rows_ctas();
   p.partial = reinterpret_cast<float*>(p.notes + ctas);
   if (tc) return launch_attend_tc(p, a->elem, a->head_dim, view != nullptr, ctas, stream);

@@ -102,10 +102,11 @@ __device__ __forceinline__ int64_t warp_sum(int64_t v) {
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
   return v;
 }
-__device__ __forceinline__ int64_t warp_scan(int64_t v) {          // inclusive
+template <typename I>
+__device__ __forceinline__ I warp_scan(I v) {                      // inclusive
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const int64_t x = __shfl_up_sync(0xffffffffu, v, o);
+    const I x = __shfl_up_sync(0xffffffffu, v, o);
     if ((threadIdx.x & 31) >= o) v += x;
   }
   return v;
@@ -177,9 +178,11 @@ __device__ __forceinline__ bool find_share(const AttentionWork& w, int cta, int 
   const int lane = threadIdx.x & 31;
   SeqSpan span;
   int64_t mine = 0, total = 0;
+  bool small = w.seqs <= 32;                            // ordinary calls: sums fit 32 bits, and the one warp-full of sequences is looked at once
   for (int base = 0; base < w.seqs; base += 32) {
     mine = lane_weights<Tiles>(w, base, &span);
-    total += warp_sum(mine) * w.kv_heads;
+    small = small && __all_sync(0xffffffffu, mine < (1 << 25) / w.kv_heads);
+    total += small ? __reduce_add_sync(0xffffffffu, static_cast<int>(mine) * w.kv_heads) : warp_sum(mine) * w.kv_heads;
   }
   const int64_t quota = quota_of(total, ctas, least);
   *share = quota;
@@ -187,8 +190,8 @@ __device__ __forceinline__ bool find_share(const AttentionWork& w, int cta, int 
   if (left >= total) return false;
   int64_t per_head = 0;
   for (int base = 0; base < w.seqs; base += 32) {
-    if (w.seqs > 32) mine = lane_weights<Tiles>(w, base, &span);    // (the only ones are still there)
-    const int64_t upto = warp_scan(mine) * w.kv_heads;
+    if (w.seqs > 32) mine = lane_weights<Tiles>(w, base, &span);
+    const int64_t upto = small ? warp_scan(static_cast<int>(mine)) * w.kv_heads : warp_scan(mine) * w.kv_heads;
     const unsigned past = __ballot_sync(0xffffffffu, upto > left);
     if (past) {
       const int l = __ffs(past) - 1;
@@ -208,7 +211,7 @@ __device__ __forceinline__ bool find_share(const AttentionWork& w, int cta, int 
   const int tiles = Tiles::tiles(w, at->span);
   for (int base = 0; base < tiles; base += 32) {
     const int units = base + lane < tiles ? Tiles::units(w, at->span, base + lane) : 0;
-    const int64_t upto = warp_scan(base + lane < tiles ? units + Tiles::kCost : 0);
+    const int upto = warp_scan(base + lane < tiles ? units + Tiles::kCost : 0);        // (32 items: fewer than 2^30)
     const unsigned past = __ballot_sync(0xffffffffu, upto > left);
     if (past) {
       const int l = __ffs(past) - 1;

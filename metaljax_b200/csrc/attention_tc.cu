@@ -135,10 +135,15 @@ struct Slot {
   }
 };
 
-// A sector of a row at once (16-byte aligned at least: two stores where it is not 32).
-__device__ __forceinline__ void store32(uint8_t* at, const uint32_t (&v)[8]) {
-  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(at), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
-               : "memory");
+// 32 bytes of a row: a sector at once where the result is aligned to that, else (16 bytes) in two stores.
+__device__ __forceinline__ void store32(uint8_t* at, const uint32_t (&v)[8], bool sector) {
+  if (sector) {
+    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(at), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
+                 : "memory");
+  } else {
+    reinterpret_cast<uint4*>(at)[0] = make_uint4(v[0], v[1], v[2], v[3]);
+    reinterpret_cast<uint4*>(at)[1] = make_uint4(v[4], v[5], v[6], v[7]);
+  }
 }
 
 // What a CTA does of an item: units from `begin` on, of which each half sees those before its own `last`.
@@ -565,7 +570,9 @@ attend_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constan
         sum += both.x + both.y;
       }
       if (!ok) break;
-      // ---- the item, or this CTA's part of it, ends ----
+      // ---- the item, or this CTA's part of it, ends (the next one is worked out while its last product runs) ----
+      UnitCursor after = c;
+      const bool again = next_item<Tiles>(w, after);
       const bool has = it.last[x] > it.begin;
       bool odd[kHelpers] = {};
       if (has) {
@@ -575,49 +582,53 @@ attend_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constan
         if (!(ok = wait_count(4, kHelpers, live + 1, 43))) break;
         for (int n = 0; n < kHelpers; ++n) odd[n] = words[2 + n] == live + 1;
       }
+      const bool sector = (reinterpret_cast<uintptr_t>(p.out) & 31) == 0;
       const bool whole = it.begin == 0 && c.end == c.units;
       const float inv = sum == 0.0f ? (limit < 0 ? 0.0f : NAN) : 1.0f / sum;
       uint8_t* const out = p.out + ((static_cast<int64_t>(c.span.q0) + tok) * w.heads + c.h * w.group + g) * D * 2;
       float4* const part = reinterpret_cast<float4*>(p.partial + (2 * static_cast<int64_t>(blockIdx.x) + (it.begin == 0 ? 1 : 0)) * partial_floats<256, D>());
       const int row = x * 128 + r;
 #pragma unroll 1
-      for (int i = 0; i < D / 32; ++i) {
-        uint32_t o[32];
+      for (int i = 0; i < D / 64; ++i) {
+        uint32_t o[2][32];
         if (has) {
-          tmem_ld(o_at + i * 32, o);
+          tmem_ld(o_at + i * 64, o[0]);
+          tmem_ld(o_at + i * 64 + 32, o[1]);
           tmem_wait_ld();
         } else {
 #pragma unroll
-          for (int j = 0; j < 32; ++j) o[j] = 0;
+          for (int j = 0; j < 64; ++j) o[j >> 5][j & 31] = 0;
         }
 #pragma unroll
         for (int n = 0; n < kHelpers; ++n)
           if (odd[n]) {
-            const uint16_t* const set = special + n * 3 * D + i * 32;
+            const uint16_t* const set = special + n * 3 * D + i * 64;
             const int seen = limit - place_of(first_item_limit);
 #pragma unroll
-            for (int j = 0; j < 32; ++j) {
-              float v = __uint_as_float(o[j]);
+            for (int j = 0; j < 64; ++j) {
+              float v = __uint_as_float(o[j >> 5][j & 31]);
               if (set[j] <= seen) v += INFINITY;
               if (set[D + j] <= seen) v -= INFINITY;
               if (set[2 * D + j] <= seen) v = NAN;
-              o[j] = __float_as_uint(v);
+              o[j >> 5][j & 31] = __float_as_uint(v);
             }
           }
         if (!mine) continue;
         if (whole) {
 #pragma unroll
-          for (int j = 0; j < 32; j += 16) {
+          for (int j = 0; j < 64; j += 16) {
             uint32_t v[8];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) v[e] = pack2<T>(__uint_as_float(o[j + 2 * e]) * inv, __uint_as_float(o[j + 2 * e + 1]) * inv);
-            store32(out + (i * 32 + j) * 2, v);
+            for (int e = 0; e < 8; ++e)
+              v[e] = pack2<T>(__uint_as_float(o[j >> 5][(j & 31) + 2 * e]) * inv, __uint_as_float(o[j >> 5][(j & 31) + 2 * e + 1]) * inv);
+            store32(out + (i * 64 + j) * 2, v, sector);
           }
         } else {
           // four elements of 256 rows side by side: neighbouring threads write neighbouring 16 bytes
 #pragma unroll
-          for (int j = 0; j < 32; j += 4)
-            part[((i * 32 + j) / 4) * 256 + row] = make_float4(__uint_as_float(o[j]), __uint_as_float(o[j + 1]), __uint_as_float(o[j + 2]), __uint_as_float(o[j + 3]));
+          for (int j = 0; j < 64; j += 4)
+            part[((i * 64 + j) / 4) * 256 + row] = make_float4(__uint_as_float(o[j >> 5][j & 31]), __uint_as_float(o[j >> 5][(j & 31) + 1]),
+                                                               __uint_as_float(o[j >> 5][(j & 31) + 2]), __uint_as_float(o[j >> 5][(j & 31) + 3]));
         }
       }
       if (!whole && mine) {
@@ -635,7 +646,8 @@ attend_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constan
         if (lane == 0) words[6 + warp] = live + 1;
         ++live;
       }
-      more = next_item<Tiles>(w, c);
+      more = again;
+      c = after;
     }
   }
   tc_fence_before();

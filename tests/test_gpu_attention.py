@@ -572,6 +572,37 @@ def test_rows_that_are_not_aligned():
     assert torch.equal(a, b) and all(torch.equal(m, n) for m, n in zip(*(attention.read_pages(c, table, cu, 59) for c in caches)))
 
 
+@pytest.mark.parametrize("offset", [8, 16, 24])
+def test_results_at_every_alignment(offset):
+    """Results, queries, keys, values and caches that begin at any multiple of 16 bytes."""
+    gen = _gen(26)
+    news, heads, kv, dim = [150, 9], 4, 2, 128
+
+    def at_offset(t):
+        flat = torch.empty((t.numel() + 64,), dtype=t.dtype, device=DEV)
+        view = flat[offset * 2 // t.element_size():][: t.numel()].view(t.shape)
+        assert view.data_ptr() % 16 == 0 and (offset % 16 == 0 or view.data_ptr() % 32 != 0)
+        return view.copy_(t)
+
+    q, k, v = (torch.randn((159, n, dim), generator=gen, device=DEV).to(BF) for n in (heads, kv, kv))
+    cu = R.starts(news, DEV)
+    want = attention.prompt_attention(q, k, v, cu)
+    out = at_offset(torch.zeros_like(q))
+    assert torch.equal(attention.prompt_attention(*(at_offset(t) for t in (q, k, v)), cu, out=out), want)
+    cache, table, _, _ = _paged([200, 40], kv, dim, 32, BF, gen)
+    lens = R.lengths([200, 40], DEV)
+    other = PagedCache(at_offset(cache.k), at_offset(cache.v))
+    for rows, starts in ((q, cu), (q[:2], None), (q[:5], R.starts([3, 2], DEV))):
+        want = attention.paged_attention(rows, cache, table, lens, starts)
+        assert torch.equal(attention.paged_attention(at_offset(rows), other, table, lens, starts, out=at_offset(torch.zeros_like(rows))), want)
+    x = torch.randn((2, (heads + 2 * kv) * dim), generator=gen, device=DEV).to(BF)
+    a = attention.append(x, cache, table, lens, heads=heads)
+    assert torch.equal(attention.append(at_offset(x), other, table, lens, heads=heads, out=at_offset(torch.zeros_like(a))), a)
+    cu_kv = R.starts([200, 40], DEV)
+    outs = tuple(at_offset(torch.zeros((240, kv, dim), dtype=BF, device=DEV)) for _ in range(2))
+    assert all(torch.equal(m, n) for m, n in zip(attention.read_pages(other, table, cu_kv, 240, out=outs), attention.read_pages(cache, table, cu_kv, 240)))
+
+
 def test_no_sequences():
     cache = PagedCache.empty(1, 2, 16, 64, BF, DEV)
     none = torch.zeros((0,), dtype=torch.int32, device=DEV)
