@@ -1,9 +1,12 @@
 // Writing new tokens into a paged cache and reading a cache's rows back.
 //
-// append: one CTA per token. A head's row of D elements is D / 8 lanes of 16 bytes, so that norm, largest magnitude and rotation
-// stay within one group of lanes (shuffles), and a CTA of 256 threads works on 16 or 32 heads' rows at once. A token's angles are the same for all of its
-// heads: one thread each takes position * frequency in float64 (a position of 10^5 times a float32 frequency is off by 0.006 radians), reduces it to a
-// fraction of a turn there, and leaves sine and cosine in shared memory.
+// Both are streams of rows, bound by memory where there are many and by a chain of dependent loads (starts, length, table, row) where there are few, so a warp works by
+// itself, without a barrier: it looks up its token or positions (32 starts at a time), and has the loads of several rows on their way at once.
+//
+// append: a head's row of D elements is D / 8 lanes of 16 bytes, so that norm, largest magnitude and rotation stay within a group of lanes (shuffles). A
+// token's angles are the same for all of its heads: two lanes' worth each take position * frequency in float64 (a position of 10^5 times a float32 frequency
+// is off by 0.006 radians), reduce it to a fraction of a turn there, and hand sine and cosine round through shared memory. A token's heads go to one
+// warp, or to up to eight where there are few tokens.
 #include <type_traits>
 
 #include "paged_cache.cuh"
@@ -11,7 +14,28 @@
 namespace qmm {
 namespace {
 
-constexpr int kThreads = 256;
+constexpr int kThreads = 256, kWarps = kThreads / 32;
+
+// One warp: sequence of packed row `row`, as sequence_of.
+__device__ __forceinline__ int warp_sequence_of(const int32_t* __restrict__ starts, int seqs, int row, int* end) {
+  const int lane = threadIdx.x & 31;
+  int lo = 0, n = seqs + 1;                            // among starts[lo .. lo + n), of which the first is <= row
+  for (;;) {
+    const int step = (n + 31) / 32, at = lane * step;
+    const int v = at < n ? __ldg(starts + lo + at) : 0x7fffffff;
+    const unsigned below = __ballot_sync(0xffffffffu, at < n && v <= row);
+    if (!below) return -1;
+    const int k = 31 - __clz(below);                   // (starts that fall would still leave it within them)
+    if (step == 1) {
+      lo += k;
+      const int next = __shfl_sync(0xffffffffu, v, k + 1 < 32 ? k + 1 : 31);
+      *end = k + 1 < n && k + 1 < 32 ? next : lo < seqs ? __ldg(starts + lo + 1) : 0;
+      return lo < seqs && row < *end ? lo : -1;
+    }
+    lo += k * step;
+    n = n - k * step < step ? n - k * step : step;
+  }
+}
 
 struct AppendParams {
   CacheView c;
@@ -25,6 +49,7 @@ struct AppendParams {
   int* status;
   int64_t row_stride;          // elements
   int32_t seqs, heads, rotary_dim, interleaved;
+  int32_t tokens, token_warps;  // warps of a token
   float eps;
 };
 
@@ -48,107 +73,124 @@ template <typename T, int D, bool E4M3>
 __global__ void __launch_bounds__(kThreads) append_kernel(const AppendParams p) {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  constexpr int kLanes = D / 8;                        // of a head's row
-  constexpr int kRows = kThreads / kLanes;             // heads' rows at once
-  __shared__ float2 turn[D / 2];                       // (sine, cosine) of the token's angles
-  __shared__ int where[2];                             // its sequence and position
-  const int token = blockIdx.x, tid = threadIdx.x;
-  const int lane = tid % kLanes, slot = tid / kLanes;
-  const int all = p.heads + 2 * p.c.kv_heads;
-  if (tid == 0) {
-    const int seq = p.cu_q ? sequence_of(p.cu_q, p.seqs, token) : token;
-    where[0] = seq;
-    where[1] = seq < 0 ? 0 : p.kv_lens[seq] - (p.cu_q ? p.cu_q[seq + 1] - token : 1);
+  constexpr int kLanes = D / 8, kRows = 32 / kLanes;   // lanes of a head's row; rows of a warp
+  constexpr int kBatch = 4;                            // rows whose loads are on their way at once, kRows heads each
+  __shared__ float2 turns[kWarps][D / 2];              // (sine, cosine) of a token's angles
+  const int warp = threadIdx.x >> 5, lane32 = threadIdx.x & 31, lane = lane32 % kLanes, slot = lane32 / kLanes;
+  const int id = blockIdx.x * kWarps + warp, token = id / p.token_warps, part = id - token * p.token_warps;
+  if (token >= p.tokens) return;
+  const int all = p.heads + 2 * p.c.kv_heads, stride = p.token_warps * kRows;
+  const uint4* const rows = reinterpret_cast<const uint4*>(p.qkv) + token * p.row_stride / 8 + lane;
+  uint4 x[kBatch];
+  auto fetch = [&](int head0) {
+#pragma unroll
+    for (int b = 0; b < kBatch; ++b) {
+      const int head = head0 + b * stride;
+      x[b] = head < all ? __ldg(rows + static_cast<int64_t>(head) * kLanes) : make_uint4(0, 0, 0, 0);
+    }
+  };
+  fetch(part * kRows + slot);
+  int seq = token, end = 0, pos;
+  if (p.cu_q) {
+    seq = warp_sequence_of(p.cu_q, p.seqs, token, &end);
+    if (seq < 0) return;                               // a row behind the last sequence
+    pos = __ldg(p.kv_lens + seq) - (end - token);
+  } else {
+    pos = __ldg(p.kv_lens + seq) - 1;
   }
-  __syncthreads();
-  const int seq = where[0], pos = where[1];
-  if (seq < 0) return;                                 // a row behind the last sequence
-  for (int i = tid; i < p.rotary_dim / 2; i += kThreads) {
-    // a fraction of a turn, exact to 2^-30 for positions up to 2^31, before it becomes a float
-    const double turns = static_cast<double>(pos) * (p.freqs[i] * 0.15915494309189533576888376337251);
-    float s, c;
-    sincospif(2.0f * static_cast<float>(turns - rint(turns)), &s, &c);
-    turn[i] = make_float2(s, c);
-  }
-  __syncthreads();
   const int64_t page = page_of(p.c, seq, pos, p.status);
   const int row = pos & ((1 << p.c.page_shift) - 1);
+  for (int i = lane32; i < p.rotary_dim / 2; i += 32) {
+    // a fraction of a turn, exact to 2^-30 for positions up to 2^31, before it becomes a float
+    const double turned = static_cast<double>(pos) * (__ldg(p.freqs + i) * 0.15915494309189533576888376337251);
+    float s, c;
+    sincospif(2.0f * static_cast<float>(turned - rint(turned)), &s, &c);
+    turns[warp][i] = make_float2(s, c);
+  }
+  __syncwarp();
   const int pairs = p.rotary_dim / 16;                 // lanes of the first elements of split pairs
-  for (int head0 = 0; head0 < all; head0 += kRows) {
-    const int head = head0 + slot;
-    const bool live = head < all;
-    float f[8] = {};
-    if (live) unpack8<T>(__ldg(reinterpret_cast<const uint4*>(p.qkv) + (token * p.row_stride + head * D) / 8 + lane), f);
-    const bool is_q = head < p.heads, is_v = head >= p.heads + p.c.kv_heads;
-    const uint8_t* weight = is_v ? nullptr : is_q ? p.q_norm : p.k_norm;
-    float ss = 0.0f;
+  const bool first = lane < pairs, turned = lane < 2 * pairs;
+  const int partner = first ? lane + pairs : lane - pairs;
+  float2 t[8];                                          // this lane's angles: of eight split pairs, or of four neighbouring ones
 #pragma unroll
-    for (int i = 0; i < 8; ++i) ss = fmaf(f[i], f[i], ss);
+  for (int i = 0; i < 8; ++i) {
+    const int at = p.interleaved ? lane * 4 + (i & 3) : (first ? lane : partner) * 8 + i;
+    t[i] = turned ? turns[warp][at] : make_float2(0.0f, 1.0f);
+    if (!p.interleaved && first) t[i].x = -t[i].x;      // the first of a pair takes the sine with the other sign
+  }
+  for (int head0 = part * kRows + slot; __any_sync(0xffffffffu, head0 < all); head0 += kBatch * stride) {
+    uint4 now[kBatch];
 #pragma unroll
-    for (int o = kLanes / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-    if (weight) {
-      float w[8];
-      unpack8<T>(__ldg(reinterpret_cast<const uint4*>(weight) + lane), w);
-      const float inv = rsqrtf(ss / static_cast<float>(D) + p.eps);
+    for (int b = 0; b < kBatch; ++b) now[b] = x[b];
+    fetch(head0 + kBatch * stride);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) f[i] = f[i] * inv * w[i];
-    }
-    // the partner's elements for split pairs: rotary_dim / 16 lanes further on or back
-    const int partner = lane < pairs ? lane + pairs : lane - pairs;
-    const bool turned = !is_v && lane < 2 * pairs;
-    float other[8];
+    for (int b = 0; b < kBatch; ++b) {
+      const int head = head0 + b * stride;
+      if (!__any_sync(0xffffffffu, head < all)) break;
+      const bool live = head < all, is_q = head < p.heads, is_v = head >= p.heads + p.c.kv_heads;
+      float f[8];
+      unpack8<T>(now[b], f);
+      if (__any_sync(0xffffffffu, !is_v)) {
+        const uint8_t* const weight = is_v ? nullptr : is_q ? p.q_norm : p.k_norm;
+        if (p.q_norm || p.k_norm) {
+          float ss = 0.0f;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) other[i] = __shfl_sync(0xffffffffu, f[i], turned ? partner : lane, kLanes);
-    if (turned) {
-      if (p.interleaved) {
+          for (int i = 0; i < 8; ++i) ss = fmaf(f[i], f[i], ss);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float2 t = turn[lane * 4 + i];
-          const float a = f[2 * i], b = f[2 * i + 1];
-          f[2 * i] = a * t.y - b * t.x;
-          f[2 * i + 1] = b * t.y + a * t.x;
+          for (int o = kLanes / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+          if (weight) {
+            float w[8];
+            unpack8<T>(__ldg(reinterpret_cast<const uint4*>(weight) + lane), w);
+            const float inv = rsqrtf(ss / static_cast<float>(D) + p.eps);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) f[i] = f[i] * inv * w[i];
+          }
         }
-      } else {
+        if (p.interleaved) {
+          if (turned && !is_v) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const float a = f[2 * i], c = f[2 * i + 1];
+              f[2 * i] = a * t[i].y - c * t[i].x;
+              f[2 * i + 1] = c * t[i].y + a * t[i].x;
+            }
+          }
+        } else if (pairs) {
+          float other[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) other[i] = __shfl_sync(0xffffffffu, f[i], turned ? partner : lane, kLanes);
+          if (turned && !is_v) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) f[i] = fmaf(f[i], t[i].y, other[i] * t[i].x);
+          }
+        }
+      }
+      const int64_t at = ((page * p.c.kv_heads + (head - p.heads - (is_v ? p.c.kv_heads : 0))) << p.c.page_shift) + row;     // (of keys and values)
+      if constexpr (E4M3) {
+        float big = 0.0f;
+        bool fine = true;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          const float2 t = turn[(lane % pairs) * 8 + i];
-          f[i] = lane < pairs ? f[i] * t.y - other[i] * t.x : f[i] * t.y + other[i] * t.x;
+          big = fmaxf(big, fabsf(f[i]));
+          fine = fine && fabsf(f[i]) <= 3.402823466e38f;
         }
-      }
-    }
-    if constexpr (E4M3) {
-      float big = 0.0f;
-      bool fine = true;
+        if (!fine) big = INFINITY;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        big = fmaxf(big, fabsf(f[i]));
-        fine = fine && fabsf(f[i]) <= 3.402823466e38f;
-      }
+        for (int o = kLanes / 2; o > 0; o >>= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, o));
+        fine = big <= 3.402823466e38f;
+        if (live && !is_q && page >= 0) {
+          const int e = fine ? row_exponent(big) : 0;
+          const float down = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);      // 2^-e: a normal number, and the product is exact
+          uint32_t u[4];
 #pragma unroll
-      for (int o = kLanes / 2; o > 0; o >>= 1) {
-        big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, o));
-        fine = __shfl_xor_sync(0xffffffffu, fine ? 1 : 0, o) && fine;
-      }
-      if (live && !is_q && page >= 0) {
-        const int e = fine ? row_exponent(big) : 0;
-        const float down = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);      // 2^-e: a normal number, and the product is exact
-        const int64_t at = ((page * p.c.kv_heads + (head - p.heads - (is_v ? p.c.kv_heads : 0))) << p.c.page_shift) + row;
-        uint32_t u[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) u[i] = fine ? e4m3_pair(f[2 * i] * down, f[2 * i + 1] * down) : 0;
-        reinterpret_cast<uint2*>(is_v ? p.c.v : p.c.k)[at * kLanes + lane] = make_uint2(u[0] | u[1] << 16, u[2] | u[3] << 16);
-        if (lane == 0) (is_v ? p.c.v_exp : p.c.k_exp)[at] = static_cast<uint8_t>(fine ? e + 127 : 255);
-      }
-      if (live && is_q) reinterpret_cast<uint4*>(p.q_out)[(static_cast<int64_t>(token) * p.heads + head) * kLanes + lane] = pack8<T>(f);
-    } else {
-      if (live) {
-        const uint4 w = pack8<T>(f);
-        if (is_q) {
-          reinterpret_cast<uint4*>(p.q_out)[(static_cast<int64_t>(token) * p.heads + head) * kLanes + lane] = w;
-        } else if (page >= 0) {
-          const int64_t at = ((page * p.c.kv_heads + (head - p.heads - (is_v ? p.c.kv_heads : 0))) << p.c.page_shift) + row;
-          reinterpret_cast<uint4*>(is_v ? p.c.v : p.c.k)[at * kLanes + lane] = w;
+          for (int i = 0; i < 4; ++i) u[i] = fine ? e4m3_pair(f[2 * i] * down, f[2 * i + 1] * down) : 0;
+          reinterpret_cast<uint2*>(is_v ? p.c.v : p.c.k)[at * kLanes + lane] = make_uint2(u[0] | u[1] << 16, u[2] | u[3] << 16);
+          if (lane == 0) (is_v ? p.c.v_exp : p.c.k_exp)[at] = static_cast<uint8_t>(fine ? e + 127 : 255);
         }
+        if (live && is_q) reinterpret_cast<uint4*>(p.q_out)[(static_cast<int64_t>(token) * p.heads + head) * kLanes + lane] = pack8<T>(f);
+      } else if (live) {
+        if (is_q) reinterpret_cast<uint4*>(p.q_out)[(static_cast<int64_t>(token) * p.heads + head) * kLanes + lane] = pack8<T>(f);
+        else if (page >= 0) reinterpret_cast<uint4*>(is_v ? p.c.v : p.c.k)[at * kLanes + lane] = pack8<T>(f);
       }
     }
   }
@@ -160,45 +202,72 @@ struct ReadParams {
   uint8_t* v_out;
   const int32_t* cu_kv;
   int* status;
-  int32_t seqs;
+  int32_t seqs, warp_rows;     // positions of a warp
   int64_t total;
 };
 
-// A position's row of all heads at a time: kv_heads * D / 8 threads of 16 bytes (of k, then of v).
+// A warp takes warp_rows positions one behind the other, all heads of each; a lane's pieces are 16 bytes of the cache.
 template <typename T, int D, bool E4M3>
 __global__ void __launch_bounds__(kThreads) read_kernel(const ReadParams p) {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  constexpr int kLanes = D / 8;
-  const int per_row = p.c.kv_heads * kLanes;
-  const int64_t pieces = p.total * per_row;
-  for (int64_t i = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x; i < pieces; i += static_cast<int64_t>(gridDim.x) * kThreads) {
-    const int64_t out_row = i / per_row;
-    const int piece = static_cast<int>(i - out_row * per_row), head = piece / kLanes, lane = piece % kLanes;
-    const int seq = sequence_of(p.cu_kv, p.seqs, static_cast<int>(out_row));
-    if (seq < 0) continue;
-    const int pos = static_cast<int>(out_row) - p.cu_kv[seq];
+  constexpr int kLanes = D / (E4M3 ? 16 : 8), kRows = 32 / kLanes;      // lanes of a head's row; heads of a warp
+  constexpr int kBatch = 2;                                             // loads of k, and as many of v, on their way at once
+  const int lane32 = threadIdx.x & 31, lane = lane32 % kLanes, slot = lane32 / kLanes;
+  const int64_t first = (static_cast<int64_t>(blockIdx.x) * kWarps + (threadIdx.x >> 5)) * p.warp_rows;
+  int seq = -1, start = 0, end = 0;
+  for (int64_t out_row = first; out_row < first + p.warp_rows && out_row < p.total; ++out_row) {
+    if (seq < 0 || out_row >= end) {
+      seq = warp_sequence_of(p.cu_kv, p.seqs, static_cast<int>(out_row), &end);
+      if (seq < 0) continue;                            // a row of no sequence
+      start = __ldg(p.cu_kv + seq);
+    }
+    const int pos = static_cast<int>(out_row) - start;
     int64_t page = page_of(p.c, seq, pos, p.status);
     if (page < 0) page = 0;
-    const int64_t at = ((page * p.c.kv_heads + head) << p.c.page_shift) + (pos & ((1 << p.c.page_shift) - 1));
+    const int64_t row0 = ((page * p.c.kv_heads) << p.c.page_shift) + (pos & ((1 << p.c.page_shift) - 1));
+    for (int head0 = slot; head0 < p.c.kv_heads; head0 += kBatch * kRows) {
+      uint4 w[2][kBatch];
+      uint32_t byte[2][kBatch];
 #pragma unroll
-    for (int which = 0; which < 2; ++which) {
-      const uint8_t* src = which ? p.c.v : p.c.k;
-      uint4 w;
-      if constexpr (E4M3) {
-        const uint2 codes = __ldg(reinterpret_cast<const uint2*>(src) + at * kLanes + lane);
-        const RowFactors f = row_factors(__ldg((which ? p.c.v_exp : p.c.k_exp) + at));
-        const uint2 a = row_values(codes.x, f), b = row_values(codes.y, f);
-        w = make_uint4(a.x, a.y, b.x, b.y);
-        if constexpr (!std::is_same<T, __nv_bfloat16>::value) {
-          float v[8];
-          unpack8<__nv_bfloat16>(w, v);
-          w = pack8<T>(v);
+      for (int b = 0; b < kBatch; ++b) {
+        const int head = head0 + b * kRows;
+        const int64_t at = row0 + (static_cast<int64_t>(head) << p.c.page_shift);
+#pragma unroll
+        for (int which = 0; which < 2; ++which) {
+          if (head < p.c.kv_heads) {
+            w[which][b] = __ldg(reinterpret_cast<const uint4*>(which ? p.c.v : p.c.k) + at * kLanes + lane);
+            if constexpr (E4M3) byte[which][b] = __ldg((which ? p.c.v_exp : p.c.k_exp) + at);
+          }
         }
-      } else {
-        w = __ldg(reinterpret_cast<const uint4*>(src) + at * kLanes + lane);
       }
-      reinterpret_cast<uint4*>(which ? p.v_out : p.k_out)[i] = w;
+#pragma unroll
+      for (int b = 0; b < kBatch; ++b) {
+        const int head = head0 + b * kRows;
+        if (head >= p.c.kv_heads) break;
+        const int64_t to = (out_row * p.c.kv_heads + head) * (D / 8) + lane * (E4M3 ? 2 : 1);
+#pragma unroll
+        for (int which = 0; which < 2; ++which) {
+          uint4* const out = reinterpret_cast<uint4*>(which ? p.v_out : p.k_out) + to;
+          if constexpr (E4M3) {
+            const RowFactors f = row_factors(byte[which][b]);
+            const uint32_t codes[4] = {w[which][b].x, w[which][b].y, w[which][b].z, w[which][b].w};
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              const uint2 lo = row_values(codes[2 * i], f), hi = row_values(codes[2 * i + 1], f);
+              uint4 v = make_uint4(lo.x, lo.y, hi.x, hi.y);
+              if constexpr (!std::is_same<T, __nv_bfloat16>::value) {
+                float e[8];
+                unpack8<__nv_bfloat16>(v, e);
+                v = pack8<T>(e);
+              }
+              out[i] = v;
+            }
+          } else {
+            *out = w[which][b];
+          }
+        }
+      }
     }
   }
 }
@@ -224,6 +293,10 @@ int launch_append(const CacheView& c, const qmm_append_args& a, int head_dim, bo
   p.cu_q = a.cu_q;
   p.status = status;
   p.row_stride = a.row_stride;
+  p.tokens = static_cast<int32_t>(a.tokens);
+  // a warp a token fills the machine from some 2000 tokens on; fewer share their heads out
+  p.token_warps = 1;
+  while (p.token_warps < kWarps && a.tokens * p.token_warps < 12ll * device_sm_count()) p.token_warps *= 2;
   p.seqs = static_cast<int32_t>(a.seqs);
   p.heads = a.heads;
   p.rotary_dim = a.rotary_dim;
@@ -237,7 +310,7 @@ int launch_append(const CacheView& c, const qmm_append_args& a, int head_dim, bo
     if (e4m3) kernel = head_dim == 64 ? append_kernel<__half, 64, true> : append_kernel<__half, 128, true>;
     else kernel = head_dim == 64 ? append_kernel<__half, 64, false> : append_kernel<__half, 128, false>;
   }
-  return launch("append_kernel", kernel, a.tokens, stream, p);
+  return launch("append_kernel", kernel, (a.tokens * p.token_warps + kWarps - 1) / kWarps, stream, p);
 }
 
 int launch_cache_read(const CacheView& c, int64_t seqs, const int32_t* cu_kv, int64_t total, int head_dim, int elem, bool e4m3, void* k_out,
@@ -254,10 +327,9 @@ int launch_cache_read(const CacheView& c, int64_t seqs, const int32_t* cu_kv, in
   if (!e4m3) kernel = head_dim == 64 ? read_kernel<__nv_bfloat16, 64, false> : read_kernel<__nv_bfloat16, 128, false>;    // (16-bit rows are copied, whatever they hold)
   else if (elem == QMM_BF16) kernel = head_dim == 64 ? read_kernel<__nv_bfloat16, 64, true> : read_kernel<__nv_bfloat16, 128, true>;
   else kernel = head_dim == 64 ? read_kernel<__half, 64, true> : read_kernel<__half, 128, true>;
-  const int64_t pieces = total * c.kv_heads * (head_dim / 8);
-  int64_t blocks = (pieces + kThreads - 1) / kThreads;
-  const int64_t most = static_cast<int64_t>(device_sm_count()) * 16;
-  return launch("read_kernel", kernel, blocks < most ? blocks : most, stream, p);
+  // four positions a warp (one look into the starts), one where that would leave warps without any
+  p.warp_rows = total >= 4ll * 48 * device_sm_count() ? 4 : 1;
+  return launch("read_kernel", kernel, (total + static_cast<int64_t>(p.warp_rows) * kWarps - 1) / (static_cast<int64_t>(p.warp_rows) * kWarps), stream, p);
 }
 
 }  // namespace qmm
