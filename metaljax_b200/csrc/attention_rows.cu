@@ -8,8 +8,10 @@
 // warps on the same rows take 64 / KW positions of a chunk each, and are joined when the item ends. With one row of 16 (RW = 1) a warp reads only what it has asked
 // for itself, and the CTA does not meet but at the ends of items.
 //
-// An e4m3 chunk is turned into bf16 by the warp that asked for it (exactly: 4-bit significands under a power of two), next to the chunk in
-// shared memory.
+// e4m3 codes become bf16 exactly (4-bit significands), five instructions a pair. With one row of 16 a warp takes them straight into its B
+// fragments: of keys four codes of a row a step (the queries' elements in the order that makes), of values the codes of its four positions, paired by a byte
+// permutation that the conversion needs anyway; the rows' powers of two go to the scores and to the weights, in float32. Where warps share
+// positions, the one that asked for a chunk's rows turns them into bf16 next to the chunk in shared memory.
 //
 // Masked positions: scores are selected, not added to. A value that is no number at a masked position would still be 0 * NaN in the sum, so
 // rows of v behind a sequence's end are zeros (the copies fill them in), and in chunks that some rows see and others do not infinities and NaN
@@ -41,6 +43,11 @@ __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], 
   else
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t lds16(uint32_t addr) {
+  uint16_t v;
+  asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(addr));
+  return v;
 }
 __device__ __forceinline__ float ex2(float x) {
   float y;
@@ -76,6 +83,7 @@ __global__ void __launch_bounds__(kThreads, 2) attend_rows_kernel(const RowsPara
   using L = RowsLayout<D, SOURCE>;
   constexpr bool kPaged = SOURCE != kRowsSource, kE4m3 = L::kE4m3;
   constexpr int R = 16 * RW, KW = 4 / RW, SN = kChunk / KW;               // rows of a tile; warps on the same rows; a warp's positions of a chunk
+  constexpr bool kDirect = kE4m3 && RW == 1;                              // codes straight into fragments: no other warp wants them
   using Tiles = RowTiles<R, kChunk>;
   extern __shared__ __align__(128) uint8_t smem[];
   int* const special = reinterpret_cast<int*>(smem + L::kRing + L::kValues);           // first positions of +inf, -inf, NaN in each column of v
@@ -117,7 +125,9 @@ __global__ void __launch_bounds__(kThreads, 2) attend_rows_kernel(const RowsPara
         const int pos = pos0 + r;
         const int there = pos < load.span.len ? 16 : 0;
         // (rows of 128 bytes and more: eight rows' pieces of one column lie in eight different banks groups)
-        const uint32_t dst = stage + (16 * warp + r) * L::kRowBytes + ((kE4m3 ? col : col ^ (r & 7)) << 4);
+        const uint32_t line = stage + (16 * warp + r) * L::kRowBytes;
+        const int k_col = kDirect ? (D == 128 ? col ^ ((r & 1) << 2) : col) : kE4m3 ? col : col ^ (r & 7);
+        const int v_col = kDirect ? (D == 128 ? col ^ (r & 6) : col ^ (r & 2)) : k_col;
         const uint8_t *ks, *vs;
         if constexpr (kPaged) {
           const int64_t row = ((page * w.kv_heads + load.h) << p.cache.page_shift) + (pos & ((1 << p.cache.page_shift) - 1));
@@ -128,8 +138,8 @@ __global__ void __launch_bounds__(kThreads, 2) attend_rows_kernel(const RowsPara
           ks = p.k + (row * p.k_row + load.h * p.k_head) * 2 + col * 16;
           vs = p.v + (row * p.v_row + load.h * p.v_head) * 2 + col * 16;
         }
-        cp_async16(dst, ks, there);
-        cp_async16(dst + L::kHalf, vs, there);
+        cp_async16(line + (k_col << 4), ks, there);
+        cp_async16(line + (v_col << 4) + L::kHalf, vs, there);
       }
       if constexpr (kE4m3) {
         if (lane < 2) {                                 // the 16 rows' exponent bytes, of k and of v (the positions behind the end: of no use)
@@ -168,11 +178,21 @@ __global__ void __launch_bounds__(kThreads, 2) attend_rows_kernel(const RowsPara
       const int tok = (row0 + r) / w.group, g = row0 + r - tok * w.group;
       const bool live = r < tile_rows;
       if (live) limit[i] = w.causal ? c.span.len - c.span.n + tok : c.span.len - 1;
-      const uint8_t* src = p.q + ((c.span.q0 + (live ? tok : 0)) * p.q_row + (c.h * w.group + (live ? g : 0)) * p.q_head) * 2 + (lane & 3) * 4;
+      const uint8_t* src = p.q + ((c.span.q0 + (live ? tok : 0)) * p.q_row + (c.h * w.group + (live ? g : 0)) * p.q_head) * 2;
+      if constexpr (kDirect) {
+        // elements in the order in which codes come: 16 of a piece a lane, four a step, even ones before odd ones
 #pragma unroll
-      for (int kk = 0; kk < D / 16; ++kk) {
-        q[kk][i] = live ? __ldg(reinterpret_cast<const uint32_t*>(src + kk * 32)) : 0;
-        q[kk][i + 2] = live ? __ldg(reinterpret_cast<const uint32_t*>(src + kk * 32 + 16)) : 0;
+        for (int kk = 0; kk < D / 16; ++kk) {
+          const uint2 x = live ? __ldg(reinterpret_cast<const uint2*>(src + ((kk / 4 * 4 + (lane & 3)) * 16 + kk % 4 * 4) * 2)) : make_uint2(0, 0);
+          q[kk][i] = __byte_perm(x.x, x.y, 0x5410);
+          q[kk][i + 2] = __byte_perm(x.x, x.y, 0x7632);
+        }
+      } else {
+#pragma unroll
+        for (int kk = 0; kk < D / 16; ++kk) {
+          q[kk][i] = live ? __ldg(reinterpret_cast<const uint32_t*>(src + (lane & 3) * 4 + kk * 32)) : 0;
+          q[kk][i + 2] = live ? __ldg(reinterpret_cast<const uint32_t*>(src + (lane & 3) * 4 + kk * 32 + 16)) : 0;
+        }
       }
     }
 #pragma unroll
@@ -193,7 +213,7 @@ __global__ void __launch_bounds__(kThreads, 2) attend_rows_kernel(const RowsPara
     const uint32_t stage = ring + (done % L::kStages) * L::kStage;
     const int pos0 = c.u * kChunk;
     uint32_t keys = stage, values = stage + L::kHalf;
-    if constexpr (kE4m3) {
+    if constexpr (kE4m3 && !kDirect) {
       // this warp's 16 rows of both as bf16
       keys = ring + L::kRing;
       values = keys + kChunk * D * 2;
@@ -218,8 +238,8 @@ __global__ void __launch_bounds__(kThreads, 2) attend_rows_kernel(const RowsPara
       }
       if constexpr (KW == 4) __syncwarp(); else __syncthreads();
     }
-    // a chunk with positions that are this sequence's, but not every row's
-    if (pos0 + kChunk - 1 > tile_first_limit && tile_first_limit < c.span.len - 1) {
+    // a chunk with positions that are this sequence's, but not every row's (codes by themselves are always numbers)
+    if (!kDirect && pos0 + kChunk - 1 > tile_first_limit && tile_first_limit < c.span.len - 1) {
       constexpr int kPieces = D / 8;
       for (int i = 0; i < 16 * kPieces / 32; ++i) {
         const int piece = i * 32 + lane, r = 16 * warp + piece / kPieces, col = piece % kPieces;
@@ -247,6 +267,31 @@ __global__ void __launch_bounds__(kThreads, 2) attend_rows_kernel(const RowsPara
     for (int n = 0; n < SN / 8; ++n)
 #pragma unroll
       for (int i = 0; i < 4; ++i) s[n][i] = 0.0f;
+    float k_scale[SN / 8][2], v_scale[SN / 8][2];         // (codes: of the thread's columns; positions behind the end: 1)
+    if constexpr (kDirect) {
+#pragma unroll
+      for (int n = 0; n < SN / 8; ++n) {
+        const int at = kw * SN + n * 8 + (lane & 3) * 2, there = c.span.len - pos0 - at;
+        const uint32_t k2 = lds16(stage + 2 * L::kHalf + at), v2 = lds16(stage + 2 * L::kHalf + kChunk + at);
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          k_scale[n][e] = (e < there ? row_scale(k2 >> (8 * e) & 255) : 1.0f) * p.scale_log2;
+          v_scale[n][e] = e < there ? row_scale(v2 >> (8 * e) & 255) : 1.0f;
+        }
+        const int r = kw * SN + n * 8 + (lane >> 2);
+#pragma unroll
+        for (int h = 0; h < D / 64; ++h) {
+          const int piece = h * 4 + (lane & 3);
+          const uint4 codes = lds128<0>(keys + r * D + ((D == 128 ? piece ^ ((r & 1) << 2) : piece) << 4));
+          const uint32_t word[4] = {codes.x, codes.y, codes.z, codes.w};
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const uint2 b = code_values(word[i]);
+            mma16816<T>(s[n], q[h * 4 + i], b.x, b.y);
+          }
+        }
+      }
+    } else
 #pragma unroll
     for (int n = 0; n < SN / 16; ++n) {
       const int r = kw * SN + n * 16 + (lane & 7) + ((lane >> 4) << 3);
@@ -260,12 +305,12 @@ __global__ void __launch_bounds__(kThreads, 2) attend_rows_kernel(const RowsPara
     }
     const int warp_pos = pos0 + kw * SN;
     const bool edge = warp_pos + SN - 1 > tile_first_limit || tile_rows < R;
-    float top[2] = {m[0], m[1]};
+    float top[2] = {-INFINITY, -INFINITY};
 #pragma unroll
     for (int n = 0; n < SN / 8; ++n)
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        float x = s[n][i] * p.scale_log2;
+        float x = s[n][i] * (kDirect ? k_scale[n][i & 1] : p.scale_log2);
         if (edge && warp_pos + n * 8 + (lane & 3) * 2 + (i & 1) > limit[i >> 1]) x = -INFINITY;
         s[n][i] = x;
         top[i >> 1] = fmaxf(top[i >> 1], x);
@@ -274,22 +319,36 @@ __global__ void __launch_bounds__(kThreads, 2) attend_rows_kernel(const RowsPara
     for (int i = 0; i < 2; ++i) {
       top[i] = fmaxf(top[i], __shfl_xor_sync(0xffffffffu, top[i], 1));
       top[i] = fmaxf(top[i], __shfl_xor_sync(0xffffffffu, top[i], 2));
-      const float base = top[i] == -INFINITY ? 0.0f : top[i];
-      const float shrink = ex2(m[i] - base);
-      m[i] = top[i];
-      l[i] *= shrink;
+    }
+    // the maximum is followed loosely: sums are scaled down when a row's has risen by more than a factor of 2^8, for all rows of the warp at once
+    if (__any_sync(0xffffffffu, top[0] > m[0] + 8.0f || top[1] > m[1] + 8.0f)) {
 #pragma unroll
-      for (int n = 0; n < D / 8; ++n) {
-        o[n][2 * i] *= shrink;
-        o[n][2 * i + 1] *= shrink;
+      for (int i = 0; i < 2; ++i) {
+        const float now = fmaxf(m[i], top[i]), shrink = ex2(m[i] - (now == -INFINITY ? 0.0f : now));
+        m[i] = now;
+        l[i] *= shrink;
+#pragma unroll
+        for (int n = 0; n < D / 8; ++n) {
+          o[n][2 * i] *= shrink;
+          o[n][2 * i + 1] *= shrink;
+        }
       }
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const float base = m[i] == -INFINITY ? 0.0f : m[i];
 #pragma unroll
       for (int n = 0; n < SN / 8; ++n)
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          const float x = ex2(s[n][2 * i + e] - base);
-          s[n][2 * i + e] = x;
+          float x = ex2(s[n][2 * i + e] - base);
           l[i] += x;
+          if constexpr (kDirect) {
+            // the values' power of two goes to their weights; a masked weight is zero whatever that is
+            if (edge && warp_pos + n * 8 + (lane & 3) * 2 + e > limit[i]) x = 0.0f;
+            else x *= v_scale[n][e];
+          }
+          s[n][2 * i + e] = x;
         }
     }
     // ---- weights times values ----
@@ -297,13 +356,42 @@ __global__ void __launch_bounds__(kThreads, 2) attend_rows_kernel(const RowsPara
     for (int n = 0; n < SN / 16; ++n) {
       const uint32_t a[4] = {pack2<T>(s[2 * n][0], s[2 * n][1]), pack2<T>(s[2 * n][2], s[2 * n][3]), pack2<T>(s[2 * n + 1][0], s[2 * n + 1][1]),
                              pack2<T>(s[2 * n + 1][2], s[2 * n + 1][3])};
-      const int r = kw * SN + n * 16 + (lane & 7) + (((lane >> 3) & 1) << 3);
+      if constexpr (kDirect) {
+        // a thread's D / 8 codes of the four positions that its B fragments hold: column `lane / 4` of every fragment
+        const int r = kw * SN + n * 16 + (lane & 3) * 2, g = lane >> 2;
+        uint32_t codes[4][D / 32];
 #pragma unroll
-      for (int dd = 0; dd < D / 16; ++dd) {
-        uint32_t b[4];
-        ldmatrix4t(b, values + r * D * 2 + (((dd * 2 + (lane >> 4)) ^ (r & 7)) << 4));
-        mma16816<T>(o[2 * dd], a, b[0], b[1]);
-        mma16816<T>(o[2 * dd + 1], a, b[2], b[3]);
+        for (int i = 0; i < 4; ++i) {
+          const int row = r + (i & 1) + (i >> 1) * 8;
+          const uint32_t at = values + row * D;
+          if constexpr (D == 128) {
+            const uint4 v = lds128<0>(at + ((g ^ (row & 6)) << 4));
+            codes[i][0] = v.x;
+            codes[i][1] = v.y;
+            codes[i][2] = v.z;
+            codes[i][3] = v.w;
+          } else {
+            const uint2 v = lds64<0>(at + (((g >> 1) ^ (row & 2)) << 4) + (g & 1) * 8);
+            codes[i][0] = v.x;
+            codes[i][1] = v.y;
+          }
+        }
+#pragma unroll
+        for (int x = 0; x < D / 32; ++x) {
+          mma16816<T>(o[4 * x], a, code_pair<0>(codes[0][x], codes[1][x]), code_pair<0>(codes[2][x], codes[3][x]));
+          mma16816<T>(o[4 * x + 1], a, code_pair<1>(codes[0][x], codes[1][x]), code_pair<1>(codes[2][x], codes[3][x]));
+          mma16816<T>(o[4 * x + 2], a, code_pair<2>(codes[0][x], codes[1][x]), code_pair<2>(codes[2][x], codes[3][x]));
+          mma16816<T>(o[4 * x + 3], a, code_pair<3>(codes[0][x], codes[1][x]), code_pair<3>(codes[2][x], codes[3][x]));
+        }
+      } else {
+        const int r = kw * SN + n * 16 + (lane & 7) + (((lane >> 3) & 1) << 3);
+#pragma unroll
+        for (int dd = 0; dd < D / 16; ++dd) {
+          uint32_t b[4];
+          ldmatrix4t(b, values + r * D * 2 + (((dd * 2 + (lane >> 4)) ^ (r & 7)) << 4));
+          mma16816<T>(o[2 * dd], a, b[0], b[1]);
+          mma16816<T>(o[2 * dd + 1], a, b[2], b[3]);
+        }
       }
     }
     ++c.u;
@@ -346,11 +434,16 @@ __global__ void __launch_bounds__(kThreads, 2) attend_rows_kernel(const RowsPara
         const int sr = ((r / 16) * KW + k) * 16 + r % 16;
         const float f = ex2(stats[sr] - base);
         ll = fmaf(f, stats[kChunk + sr], ll);
-        const float4 x = *reinterpret_cast<const float4*>(sums + sr * D + (d ^ ((sr & 3) << 3)));
-        v[0] = fmaf(f, x.x, v[0]);
-        v[1] = fmaf(f, x.y, v[1]);
-        v[2] = fmaf(f, x.z, v[2]);
-        v[3] = fmaf(f, x.w, v[3]);
+        if constexpr (kDirect) {                          // fragment t, column n: element n * D / 8 + t
+#pragma unroll
+          for (int e = 0; e < 4; ++e) v[e] = fmaf(f, sums[sr * D + (((d + e) % (D / 8) * 8 + d / (D / 8)) ^ ((sr & 3) << 3))], v[e]);
+        } else {
+          const float4 x = *reinterpret_cast<const float4*>(sums + sr * D + (d ^ ((sr & 3) << 3)));
+          v[0] = fmaf(f, x.x, v[0]);
+          v[1] = fmaf(f, x.y, v[1]);
+          v[2] = fmaf(f, x.z, v[2]);
+          v[3] = fmaf(f, x.w, v[3]);
+        }
       }
       if (odd) {
 #pragma unroll
