@@ -26,10 +26,10 @@ struct JoinParams {
   const float* partial;
 };
 
-int attend_rows_ctas();
+int attend_rows_ctas();             // at most
 int64_t attend_rows_workspace(int head_dim, int ctas);
 // `source`: 0 rows, 1 pages of 16-bit values, 2 pages of e4m3 codes; `rows`: query rows that a sequence and key head have at most, as far as is known.
-int launch_attend_rows(const RowsParams& p, int elem, int head_dim, int source, int rows, int ctas, cudaStream_t stream);
+int launch_attend_rows(const RowsParams& p, int elem, int head_dim, int source, int rows, cudaStream_t stream);
 
 // 128-row halves on tcgen05: prompts (not `paged`) and 16-bit pages. A cache's rows have to be fewer than 2^31.
 int attend_tc_ctas();

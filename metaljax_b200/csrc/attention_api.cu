@@ -95,7 +95,7 @@ int attend(const char* what, const qmm_paged_cache* cache, const CacheView* view
   const int ctas = tc ? attend_tc_ctas() : attend_rows_ctas();
   p.partial = reinterpret_cast<float*>(p.notes + ctas);
   if (tc) return launch_attend_tc(p, a->elem, a->head_dim, view != nullptr, ctas, stream);
-  return launch_attend_rows(p, a->elem, a->head_dim, source, rows < 64 ? static_cast<int>(rows) : 64, ctas, stream);
+  return launch_attend_rows(p, a->elem, a->head_dim, source, rows < 64 ? static_cast<int>(rows) : 64, stream);
 }
 
 }  // namespace

@@ -8,10 +8,11 @@
 // warps on the same rows take 64 / KW positions of a chunk each, and are joined when the item ends. With one row of 16 (RW = 1) a warp reads only what it has asked
 // for itself, and the CTA does not meet but at the ends of items.
 //
-// e4m3 codes become bf16 exactly (4-bit significands), five instructions a pair. With one row of 16 a warp takes them straight into its B
-// fragments: of keys four codes of a row a step (the queries' elements in the order that makes), of values the codes of its four positions, paired by a byte
-// permutation that the conversion needs anyway; the rows' powers of two go to the scores and to the weights, in float32. Where warps share
-// positions, the one that asked for a chunk's rows turns them into bf16 next to the chunk in shared memory.
+// e4m3 codes: with one row of 16 a warp takes them straight into its B fragments as f16, one conversion a pair (a bf16 takes five
+// instructions a pair, which bound this form: 249 us for 64 sequences of 2000 to 8000 positions, against 197): of keys four codes of a row a step (the queries' elements in the order that makes),
+// of values the codes of its four positions, paired by a byte permutation. The queries become f16 under a power of two, the rows' powers of two go to the
+// scores and to the weights. Where warps share positions, the one that asked for a chunk's rows turns them into bf16 (exactly) next to the chunk in
+// shared memory.
 //
 // Masked positions: scores are selected, not added to. A value that is no number at a masked position would still be 0 * NaN in the sum, so
 // rows of v behind a sequence's end are zeros (the copies fill them in), and in chunks that some rows see and others do not infinities and NaN
@@ -44,6 +45,11 @@ __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], 
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
+__device__ __forceinline__ uint32_t lds8(uint32_t addr) {
+  uint32_t v;
+  asm volatile("ld.shared.u8 %0, [%1];" : "=r"(v) : "r"(addr));
+  return v;
+}
 __device__ __forceinline__ uint32_t lds16(uint32_t addr) {
   uint16_t v;
   asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(addr));
@@ -64,14 +70,16 @@ __device__ __forceinline__ bool odd_pair(uint32_t w) {
 
 enum Source { kRowsSource, kPages16, kPages8 };
 
-template <int D, int SOURCE>
+template <int D, int SOURCE, int RW>
 struct RowsLayout {
-  static constexpr bool kE4m3 = SOURCE == kPages8;
+  static constexpr bool kE4m3 = SOURCE == kPages8, kDirect = kE4m3 && RW == 1;
+  static constexpr int kCtas = kDirect ? 3 : 2;                          // an SM
+
   static constexpr int kStages = kE4m3 ? 4 : 3;
   static constexpr int kRowBytes = D * (kE4m3 ? 1 : 2);
   static constexpr int kHalf = kChunk * kRowBytes;                       // keys of a chunk; values follow, then (e4m3) both rows' bytes
   static constexpr int kStage = 2 * kHalf + (kE4m3 ? 2 * kChunk : 0);
-  static constexpr int kValues = kE4m3 ? 2 * kChunk * D * 2 : 0;         // an e4m3 chunk as bf16
+  static constexpr int kValues = kE4m3 && !kDirect ? 2 * kChunk * D * 2 : 0;         // an e4m3 chunk as bf16
   static constexpr int kRing = kStages * kStage;
   static constexpr int kSpecials = 3 * D * 4 + 16;
   static constexpr int kStats = kChunk * 2 * 4;                          // (maximum, sum) of a warp's rows
@@ -79,11 +87,12 @@ struct RowsLayout {
 };
 
 template <typename T, int D, int RW, int SOURCE>
-__global__ void __launch_bounds__(kThreads, 2) attend_rows_kernel(const RowsParams p) {
-  using L = RowsLayout<D, SOURCE>;
+__global__ void __launch_bounds__(kThreads, (RowsLayout<D, SOURCE, RW>::kCtas)) attend_rows_kernel(const RowsParams p) {
+  using L = RowsLayout<D, SOURCE, RW>;
   constexpr bool kPaged = SOURCE != kRowsSource, kE4m3 = L::kE4m3;
   constexpr int R = 16 * RW, KW = 4 / RW, SN = kChunk / KW;               // rows of a tile; warps on the same rows; a warp's positions of a chunk
-  constexpr bool kDirect = kE4m3 && RW == 1;                              // codes straight into fragments: no other warp wants them
+  constexpr bool kDirect = L::kDirect;                                    // codes straight into fragments: no other warp wants them
+  using MT = typename std::conditional<kDirect, __half, T>::type;         // ... f16, which holds a code in one conversion of two
   using Tiles = RowTiles<R, kChunk>;
   extern __shared__ __align__(128) uint8_t smem[];
   int* const special = reinterpret_cast<int*>(smem + L::kRing + L::kValues);           // first positions of +inf, -inf, NaN in each column of v
@@ -119,33 +128,37 @@ __global__ void __launch_bounds__(kThreads, 2) attend_rows_kernel(const RowsPara
       const uint32_t stage = ring + (loaded % L::kStages) * L::kStage;
       constexpr int kPieces = L::kRowBytes / 16;
       const int pos0 = load.u * kChunk + 16 * warp;
+      // (16 positions of a page are one run of bytes)
+      const int64_t run = kPaged ? ((page * w.kv_heads + load.h) << p.cache.page_shift) + (pos0 & ((1 << p.cache.page_shift) - 1)) : 0;
+      const bool whole = pos0 + 16 <= load.span.len;
 #pragma unroll
       for (int i = 0; i < 16 * kPieces / 32; ++i) {
         const int piece = i * 32 + lane, r = piece / kPieces, col = piece % kPieces;
-        const int pos = pos0 + r;
-        const int there = pos < load.span.len ? 16 : 0;
-        // (rows of 128 bytes and more: eight rows' pieces of one column lie in eight different banks groups)
         const uint32_t line = stage + (16 * warp + r) * L::kRowBytes;
         const int k_col = kDirect ? (D == 128 ? col ^ ((r & 1) << 2) : col) : kE4m3 ? col : col ^ (r & 7);
         const int v_col = kDirect ? (D == 128 ? col ^ (r & 6) : col ^ (r & 2)) : k_col;
-        const uint8_t *ks, *vs;
+        const uint32_t k_dst = line + (k_col << 4), v_dst = line + (v_col << 4) + L::kHalf;
         if constexpr (kPaged) {
-          const int64_t row = ((page * w.kv_heads + load.h) << p.cache.page_shift) + (pos & ((1 << p.cache.page_shift) - 1));
-          ks = p.cache.k + row * L::kRowBytes + col * 16;
-          vs = p.cache.v + row * L::kRowBytes + col * 16;
+          const uint8_t* const ks = p.cache.k + run * L::kRowBytes + piece * 16;
+          const uint8_t* const vs = p.cache.v + run * L::kRowBytes + piece * 16;
+          if (whole) {
+            cp_async16(k_dst, ks);
+            cp_async16(v_dst, vs);
+          } else {
+            const int there = pos0 + r < load.span.len ? 16 : 0;
+            cp_async16(k_dst, ks, there);
+            cp_async16(v_dst, vs, there);
+          }
         } else {
-          const int64_t row = there ? load.span.q0 + pos : 0;
-          ks = p.k + (row * p.k_row + load.h * p.k_head) * 2 + col * 16;
-          vs = p.v + (row * p.v_row + load.h * p.v_head) * 2 + col * 16;
+          const int there = pos0 + r < load.span.len ? 16 : 0;
+          const int64_t row = there ? load.span.q0 + pos0 + r : 0;
+          cp_async16(k_dst, p.k + (row * p.k_row + load.h * p.k_head) * 2 + col * 16, there);
+          cp_async16(v_dst, p.v + (row * p.v_row + load.h * p.v_head) * 2 + col * 16, there);
         }
-        cp_async16(line + (k_col << 4), ks, there);
-        cp_async16(line + (v_col << 4) + L::kHalf, vs, there);
       }
       if constexpr (kE4m3) {
-        if (lane < 2) {                                 // the 16 rows' exponent bytes, of k and of v (the positions behind the end: of no use)
-          const int64_t row = ((page * w.kv_heads + load.h) << p.cache.page_shift) + (pos0 & ((1 << p.cache.page_shift) - 1));
-          cp_async16(stage + 2 * L::kHalf + lane * kChunk + 16 * warp, (lane ? p.cache.v_exp : p.cache.k_exp) + row, pos0 < load.span.len ? 16 : 0);
-        }
+        if (lane < 2)                                   // the 16 rows' exponent bytes, of k and of v (the positions behind the end: of no use)
+          cp_async16(stage + 2 * L::kHalf + lane * kChunk + 16 * warp, (lane ? p.cache.v_exp : p.cache.k_exp) + run, pos0 < load.span.len ? 16 : 0);
       }
       if (++load.u >= load.end) loading = next_item<Tiles>(w, load);
       look_up();
@@ -163,12 +176,15 @@ __global__ void __launch_bounds__(kThreads, 2) attend_rows_kernel(const RowsPara
   int limit[2];                                          // last position that the thread's two rows see (-1: none)
   int tile_first_limit = 0, tile_rows = 0;
   int begun = 0;                                         // first unit of this item here
+  [[maybe_unused]] float q_scale = 0.0f;                 // (codes) the queries' power of two and the scale
+  [[maybe_unused]] int v_top = 0;                        // (codes) the largest exponent of a row of values so far: the sums are in units of 2^v_top
 
   auto begin_item = [&]() {
     begun = c.u;
     const int row0 = c.t * R, rows = c.span.n * w.group - row0;
     tile_rows = rows < R ? rows : R;
     tile_first_limit = w.causal ? c.span.len - c.span.n + row0 / w.group : c.span.len - 1;
+    [[maybe_unused]] float big = 0.0f;
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       const int r = rw * 16 + (lane >> 2) + 8 * i;
@@ -180,12 +196,18 @@ __global__ void __launch_bounds__(kThreads, 2) attend_rows_kernel(const RowsPara
       if (live) limit[i] = w.causal ? c.span.len - c.span.n + tok : c.span.len - 1;
       const uint8_t* src = p.q + ((c.span.q0 + (live ? tok : 0)) * p.q_row + (c.h * w.group + (live ? g : 0)) * p.q_head) * 2;
       if constexpr (kDirect) {
-        // elements in the order in which codes come: 16 of a piece a lane, four a step, even ones before odd ones
+        // elements in the order in which codes come: 16 of a piece a lane, four a step
 #pragma unroll
         for (int kk = 0; kk < D / 16; ++kk) {
           const uint2 x = live ? __ldg(reinterpret_cast<const uint2*>(src + ((kk / 4 * 4 + (lane & 3)) * 16 + kk % 4 * 4) * 2)) : make_uint2(0, 0);
-          q[kk][i] = __byte_perm(x.x, x.y, 0x5410);
-          q[kk][i + 2] = __byte_perm(x.x, x.y, 0x7632);
+          q[kk][i] = x.x;
+          q[kk][i + 2] = x.y;
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const float2 f = unpack2<T>(e ? x.y : x.x);
+            if (fabsf(f.x) <= 3.402823466e38f) big = fmaxf(big, fabsf(f.x));
+            if (fabsf(f.y) <= 3.402823466e38f) big = fmaxf(big, fabsf(f.y));
+          }
         }
       } else {
 #pragma unroll
@@ -199,6 +221,24 @@ __global__ void __launch_bounds__(kThreads, 2) attend_rows_kernel(const RowsPara
     for (int n = 0; n < D / 8; ++n)
 #pragma unroll
       for (int i = 0; i < 4; ++i) o[n][i] = 0.0f;
+    if constexpr (kDirect) {
+      // f16 under a power of two that brings the tile's largest element to [2^14, 2^15): elements down to 2^-31 of it keep all their bits
+#pragma unroll
+      for (int x = 16; x > 0; x >>= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, x));
+      int e = 0;
+      if (big > 0.0f) frexpf(big, &e);
+      e = e < -100 ? -100 : e;
+      const float up = __uint_as_float(static_cast<uint32_t>(15 - e + 127) << 23);
+      q_scale = __uint_as_float(static_cast<uint32_t>(e - 15 + 127) << 23) * p.scale_log2;
+#pragma unroll
+      for (int kk = 0; kk < D / 16; ++kk)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float2 f = unpack2<T>(q[kk][i]);
+          q[kk][i] = pack2<__half>(f.x * up, f.y * up);
+        }
+      v_top = -1000;
+    }
   };
 
   if (tid == 0) *any_special = 0;
@@ -268,15 +308,34 @@ __global__ void __launch_bounds__(kThreads, 2) attend_rows_kernel(const RowsPara
 #pragma unroll
       for (int i = 0; i < 4; ++i) s[n][i] = 0.0f;
     float k_scale[SN / 8][2], v_scale[SN / 8][2];         // (codes: of the thread's columns; positions behind the end: 1)
+    [[maybe_unused]] bool wide = false;
     if constexpr (kDirect) {
+      // The weights of the values are f16 too: p * 2^(e - v_top + 6), e a row's exponent. Rows more than 2^12 below the largest would lose bits where that one's
+      // weight is small: then these positions' products are taken in bf16 (`wide`).
+      const int mine = lane < SN && kw * SN + lane < c.span.len - pos0 ? static_cast<int>(lds8(stage + 2 * L::kHalf + kChunk + kw * SN + (lane & (SN - 1)))) : 255;
+      const int high = __reduce_max_sync(0xffffffffu, mine == 255 ? -1000 : mine - 127), low = __reduce_min_sync(0xffffffffu, mine == 255 ? 1000 : mine - 127);
+      if (high > v_top) {
+        if (v_top > -1000) {
+          const float down = high - v_top > 126 ? 0.0f : __uint_as_float(static_cast<uint32_t>(127 + v_top - high) << 23);
+#pragma unroll
+          for (int n = 0; n < D / 8; ++n)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) o[n][i] *= down;
+        }
+        v_top = high;
+      }
+      wide = v_top - low > 12;
+      // (2^(e - v_top + 6) in two steps that are both in range)
+      const float unit = __uint_as_float(static_cast<uint32_t>(127 + 6 - (v_top > 64 ? 64 : v_top < -64 ? -64 : v_top)) << 23);
+      const float rest = __uint_as_float(static_cast<uint32_t>(127 - (v_top > 64 ? v_top - 64 : v_top < -64 ? (v_top < -127 ? -63 : v_top + 64) : 0)) << 23);
 #pragma unroll
       for (int n = 0; n < SN / 8; ++n) {
         const int at = kw * SN + n * 8 + (lane & 3) * 2, there = c.span.len - pos0 - at;
         const uint32_t k2 = lds16(stage + 2 * L::kHalf + at), v2 = lds16(stage + 2 * L::kHalf + kChunk + at);
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          k_scale[n][e] = (e < there ? row_scale(k2 >> (8 * e) & 255) : 1.0f) * p.scale_log2;
-          v_scale[n][e] = e < there ? row_scale(v2 >> (8 * e) & 255) : 1.0f;
+          k_scale[n][e] = (e < there ? row_scale(k2 >> (8 * e) & 255) : 1.0f) * q_scale;
+          v_scale[n][e] = (e < there ? row_scale(v2 >> (8 * e) & 255) : 0.0f) * unit * rest;
         }
         const int r = kw * SN + n * 8 + (lane >> 2);
 #pragma unroll
@@ -285,10 +344,7 @@ __global__ void __launch_bounds__(kThreads, 2) attend_rows_kernel(const RowsPara
           const uint4 codes = lds128<0>(keys + r * D + ((D == 128 ? piece ^ ((r & 1) << 2) : piece) << 4));
           const uint32_t word[4] = {codes.x, codes.y, codes.z, codes.w};
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const uint2 b = code_values(word[i]);
-            mma16816<T>(s[n], q[h * 4 + i], b.x, b.y);
-          }
+          for (int i = 0; i < 4; ++i) mma16816<MT>(s[n], q[h * 4 + i], code_half2(word[i]), code_half2(word[i] >> 16));
         }
       }
     } else
@@ -299,8 +355,8 @@ __global__ void __launch_bounds__(kThreads, 2) attend_rows_kernel(const RowsPara
       for (int kk = 0; kk < D / 16; ++kk) {
         uint32_t b[4];
         ldmatrix4(b, keys + r * D * 2 + (((kk * 2 + ((lane >> 3) & 1)) ^ (r & 7)) << 4));
-        mma16816<T>(s[2 * n], q[kk], b[0], b[1]);
-        mma16816<T>(s[2 * n + 1], q[kk], b[2], b[3]);
+        mma16816<MT>(s[2 * n], q[kk], b[0], b[1]);
+        mma16816<MT>(s[2 * n + 1], q[kk], b[2], b[3]);
       }
     }
     const int warp_pos = pos0 + kw * SN;
@@ -354,8 +410,8 @@ __global__ void __launch_bounds__(kThreads, 2) attend_rows_kernel(const RowsPara
     // ---- weights times values ----
 #pragma unroll
     for (int n = 0; n < SN / 16; ++n) {
-      const uint32_t a[4] = {pack2<T>(s[2 * n][0], s[2 * n][1]), pack2<T>(s[2 * n][2], s[2 * n][3]), pack2<T>(s[2 * n + 1][0], s[2 * n + 1][1]),
-                             pack2<T>(s[2 * n + 1][2], s[2 * n + 1][3])};
+      const uint32_t a[4] = {pack2<MT>(s[2 * n][0], s[2 * n][1]), pack2<MT>(s[2 * n][2], s[2 * n][3]), pack2<MT>(s[2 * n + 1][0], s[2 * n + 1][1]),
+                             pack2<MT>(s[2 * n + 1][2], s[2 * n + 1][3])};
       if constexpr (kDirect) {
         // a thread's D / 8 codes of the four positions that its B fragments hold: column `lane / 4` of every fragment
         const int r = kw * SN + n * 16 + (lane & 3) * 2, g = lane >> 2;
@@ -376,12 +432,24 @@ __global__ void __launch_bounds__(kThreads, 2) attend_rows_kernel(const RowsPara
             codes[i][1] = v.y;
           }
         }
+        if (!wide) {
 #pragma unroll
-        for (int x = 0; x < D / 32; ++x) {
-          mma16816<T>(o[4 * x], a, code_pair<0>(codes[0][x], codes[1][x]), code_pair<0>(codes[2][x], codes[3][x]));
-          mma16816<T>(o[4 * x + 1], a, code_pair<1>(codes[0][x], codes[1][x]), code_pair<1>(codes[2][x], codes[3][x]));
-          mma16816<T>(o[4 * x + 2], a, code_pair<2>(codes[0][x], codes[1][x]), code_pair<2>(codes[2][x], codes[3][x]));
-          mma16816<T>(o[4 * x + 3], a, code_pair<3>(codes[0][x], codes[1][x]), code_pair<3>(codes[2][x], codes[3][x]));
+          for (int x = 0; x < D / 32; ++x) {
+            mma16816<MT>(o[4 * x], a, code_half2<0>(codes[0][x], codes[1][x]), code_half2<0>(codes[2][x], codes[3][x]));
+            mma16816<MT>(o[4 * x + 1], a, code_half2<1>(codes[0][x], codes[1][x]), code_half2<1>(codes[2][x], codes[3][x]));
+            mma16816<MT>(o[4 * x + 2], a, code_half2<2>(codes[0][x], codes[1][x]), code_half2<2>(codes[2][x], codes[3][x]));
+            mma16816<MT>(o[4 * x + 3], a, code_half2<3>(codes[0][x], codes[1][x]), code_half2<3>(codes[2][x], codes[3][x]));
+          }
+        } else {
+          const uint32_t b[4] = {pack2<T>(s[2 * n][0], s[2 * n][1]), pack2<T>(s[2 * n][2], s[2 * n][3]), pack2<T>(s[2 * n + 1][0], s[2 * n + 1][1]),
+                                 pack2<T>(s[2 * n + 1][2], s[2 * n + 1][3])};
+#pragma unroll
+          for (int x = 0; x < D / 32; ++x) {
+            mma16816<T>(o[4 * x], b, code_pair<0>(codes[0][x], codes[1][x]), code_pair<0>(codes[2][x], codes[3][x]));
+            mma16816<T>(o[4 * x + 1], b, code_pair<1>(codes[0][x], codes[1][x]), code_pair<1>(codes[2][x], codes[3][x]));
+            mma16816<T>(o[4 * x + 2], b, code_pair<2>(codes[0][x], codes[1][x]), code_pair<2>(codes[2][x], codes[3][x]));
+            mma16816<T>(o[4 * x + 3], b, code_pair<3>(codes[0][x], codes[1][x]), code_pair<3>(codes[2][x], codes[3][x]));
+          }
         }
       } else {
         const int r = kw * SN + n * 16 + (lane & 7) + (((lane >> 3) & 1) << 3);
@@ -389,8 +457,8 @@ __global__ void __launch_bounds__(kThreads, 2) attend_rows_kernel(const RowsPara
         for (int dd = 0; dd < D / 16; ++dd) {
           uint32_t b[4];
           ldmatrix4t(b, values + r * D * 2 + (((dd * 2 + (lane >> 4)) ^ (r & 7)) << 4));
-          mma16816<T>(o[2 * dd], a, b[0], b[1]);
-          mma16816<T>(o[2 * dd + 1], a, b[2], b[3]);
+          mma16816<MT>(o[2 * dd], a, b[0], b[1]);
+          mma16816<MT>(o[2 * dd + 1], a, b[2], b[3]);
         }
       }
     }
@@ -403,68 +471,83 @@ __global__ void __launch_bounds__(kThreads, 2) attend_rows_kernel(const RowsPara
       l[i] += __shfl_xor_sync(0xffffffffu, l[i], 1);
       l[i] += __shfl_xor_sync(0xffffffffu, l[i], 2);
     }
-    __syncthreads();
-    float* const sums = reinterpret_cast<float*>(kE4m3 ? smem + L::kRing : smem + (stage - ring));    // [4 warps][16 rows][D]
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int r = warp * 16 + (lane >> 2) + 8 * i;
-      if ((lane & 3) == 0) {
-        stats[r] = m[i];
-        stats[kChunk + r] = l[i];
-      }
+    if constexpr (kDirect) {
+      const float unit = v_top > -1000 ? ldexpf(1.0f, v_top - 6) : 1.0f;
 #pragma unroll
       for (int n = 0; n < D / 8; ++n)
-        *reinterpret_cast<float2*>(sums + r * D + ((n * 8 + (lane & 3) * 2) ^ ((r & 3) << 3))) = make_float2(o[n][2 * i], o[n][2 * i + 1]);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) o[n][i] *= unit;
     }
     __syncthreads();
+    float* const sums = reinterpret_cast<float*>(kE4m3 && !kDirect ? smem + L::kRing : smem + (stage - ring));
+    constexpr int kPasses = kDirect ? 2 : 1, kPart = 16 / kPasses;       // a stage of codes holds eight rows of each warp's sums, the other places all sixteen
     const bool first = begun == 0, last = c.u == c.units;
     const bool odd = *any_special != 0;
     float* const part = p.partial + (2 * static_cast<int64_t>(blockIdx.x) + (first ? 1 : 0)) * partial_floats<R, D>();
     constexpr int kVec = D / 4;                           // threads of a row
-    for (int i = tid; i < tile_rows * kVec; i += kThreads) {
-      const int r = i / kVec, d = (i % kVec) * 4;
-      const int tok = (c.t * R + r) / w.group, g = c.t * R + r - tok * w.group;
-      const int seen = w.causal ? c.span.len - c.span.n + tok : c.span.len - 1;
-      float mm = -INFINITY, ll = 0.0f, v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-      for (int k = 0; k < KW; ++k) mm = fmaxf(mm, stats[((r / 16) * KW + k) * 16 + r % 16]);
-      const float base = mm == -INFINITY ? 0.0f : mm;
+    for (int pass = 0; pass < kPasses; ++pass) {
+      if (pass * kPart >= tile_rows) break;
+      if (pass) __syncthreads();
 #pragma unroll
-      for (int k = 0; k < KW; ++k) {
-        const int sr = ((r / 16) * KW + k) * 16 + r % 16;
-        const float f = ex2(stats[sr] - base);
-        ll = fmaf(f, stats[kChunk + sr], ll);
-        if constexpr (kDirect) {                          // fragment t, column n: element n * D / 8 + t
+      for (int i = 0; i < 2; ++i) {
+        const int r = (lane >> 2) + 8 * i, sr = warp * kPart + (kDirect ? lane >> 2 : r);
+        if (pass == 0 && (lane & 3) == 0) {
+          stats[warp * 16 + r] = m[i];
+          stats[kChunk + warp * 16 + r] = l[i];
+        }
+        if (kDirect && i != pass) continue;
 #pragma unroll
-          for (int e = 0; e < 4; ++e) v[e] = fmaf(f, sums[sr * D + (((d + e) % (D / 8) * 8 + d / (D / 8)) ^ ((sr & 3) << 3))], v[e]);
+        for (int n = 0; n < D / 8; ++n)
+          *reinterpret_cast<float2*>(sums + sr * D + ((n * 8 + (lane & 3) * 2) ^ ((sr & 3) << 3))) = make_float2(o[n][2 * i], o[n][2 * i + 1]);
+      }
+      __syncthreads();
+      const int row_end = kDirect && tile_rows > (pass + 1) * kPart ? (pass + 1) * kPart : tile_rows;
+      for (int i = pass * kPart * kVec + tid; i < row_end * kVec; i += kThreads) {
+        const int r = i / kVec, d = (i % kVec) * 4;
+        const int tok = (c.t * R + r) / w.group, g = c.t * R + r - tok * w.group;
+        const int seen = w.causal ? c.span.len - c.span.n + tok : c.span.len - 1;
+        float mm = -INFINITY, ll = 0.0f, v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int k = 0; k < KW; ++k) mm = fmaxf(mm, stats[((r / 16) * KW + k) * 16 + r % 16]);
+        const float base = mm == -INFINITY ? 0.0f : mm;
+#pragma unroll
+        for (int k = 0; k < KW; ++k) {
+          const int at = ((r / 16) * KW + k) * 16 + r % 16, sr = ((r / 16) * KW + k) * kPart + r % kPart;
+          const float f = ex2(stats[at] - base);
+          ll = fmaf(f, stats[kChunk + at], ll);
+          if constexpr (kDirect) {                        // fragment t, column n: element n * D / 8 + t
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] = fmaf(f, sums[sr * D + (((d + e) % (D / 8) * 8 + d / (D / 8)) ^ ((sr & 3) << 3))], v[e]);
+          } else {
+            const float4 x = *reinterpret_cast<const float4*>(sums + sr * D + (d ^ ((sr & 3) << 3)));
+            v[0] = fmaf(f, x.x, v[0]);
+            v[1] = fmaf(f, x.y, v[1]);
+            v[2] = fmaf(f, x.z, v[2]);
+            v[3] = fmaf(f, x.w, v[3]);
+          }
+        }
+        if (odd) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            if (special[d + e] <= seen) v[e] += INFINITY;
+            if (special[D + d + e] <= seen) v[e] -= INFINITY;
+            if (special[2 * D + d + e] <= seen) v[e] = NAN;
+          }
+        }
+        if (first && last) {
+          // no weight at all: a row that sees nothing is zero; one that sees only scores of -inf has no softmax
+          const float inv = ll == 0.0f ? (seen < 0 ? 0.0f : NAN) : 1.0f / ll;
+          uint2 out;
+          out.x = pack2<T>(v[0] * inv, v[1] * inv);
+          out.y = pack2<T>(v[2] * inv, v[3] * inv);
+          *reinterpret_cast<uint2*>(p.out + ((static_cast<int64_t>(c.span.q0) + tok) * w.heads + c.h * w.group + g) * D * 2 + d * 2) = out;
         } else {
-          const float4 x = *reinterpret_cast<const float4*>(sums + sr * D + (d ^ ((sr & 3) << 3)));
-          v[0] = fmaf(f, x.x, v[0]);
-          v[1] = fmaf(f, x.y, v[1]);
-          v[2] = fmaf(f, x.z, v[2]);
-          v[3] = fmaf(f, x.w, v[3]);
-        }
-      }
-      if (odd) {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          if (special[d + e] <= seen) v[e] += INFINITY;
-          if (special[D + d + e] <= seen) v[e] -= INFINITY;
-          if (special[2 * D + d + e] <= seen) v[e] = NAN;
-        }
-      }
-      if (first && last) {
-        // no weight at all: a row that sees nothing is zero; one that sees only scores of -inf has no softmax
-        const float inv = ll == 0.0f ? (seen < 0 ? 0.0f : NAN) : 1.0f / ll;
-        uint2 out;
-        out.x = pack2<T>(v[0] * inv, v[1] * inv);
-        out.y = pack2<T>(v[2] * inv, v[3] * inv);
-        *reinterpret_cast<uint2*>(p.out + ((static_cast<int64_t>(c.span.q0) + tok) * w.heads + c.h * w.group + g) * D * 2 + d * 2) = out;
-      } else {
-        *reinterpret_cast<float4*>(part + r * D + d) = make_float4(v[0], v[1], v[2], v[3]);
-        if (d == 0) {
-          part[R * D + r] = mm;
-          part[R * D + R + r] = ll;
+          *reinterpret_cast<float4*>(part + r * D + d) = make_float4(v[0], v[1], v[2], v[3]);
+          if (d == 0) {
+            part[R * D + r] = mm;
+            part[R * D + R + r] = ll;
+          }
         }
       }
     }
@@ -538,16 +621,17 @@ __global__ void __launch_bounds__(kJoinThreads) attend_join_kernel(const JoinPar
 }
 
 template <typename T, int D, int RW, int SOURCE>
-int launch_one(const RowsParams& p, int ctas, cudaStream_t stream) {
+int launch_one(const RowsParams& p, cudaStream_t stream) {
+  const int ctas = RowsLayout<D, SOURCE, RW>::kCtas * device_sm_count();
   static bool done[kMaxDevices] = {};
   const int dev = current_device();
   if (dev < 0) return QMM_ERR_DEVICE;
   if (!done[dev]) {
-    const cudaError_t e = cudaFuncSetAttribute(attend_rows_kernel<T, D, RW, SOURCE>, cudaFuncAttributeMaxDynamicSharedMemorySize, RowsLayout<D, SOURCE>::kBytes);
+    const cudaError_t e = cudaFuncSetAttribute(attend_rows_kernel<T, D, RW, SOURCE>, cudaFuncAttributeMaxDynamicSharedMemorySize, RowsLayout<D, SOURCE, RW>::kBytes);
     if (e != cudaSuccess) return fail(QMM_ERR_CUDA, "cudaFuncSetAttribute: %s", cudaGetErrorString(e));
     done[dev] = true;
   }
-  launch_early(attend_rows_kernel<T, D, RW, SOURCE>, ctas, kThreads, RowsLayout<D, SOURCE>::kBytes, stream, p);
+  launch_early(attend_rows_kernel<T, D, RW, SOURCE>, ctas, kThreads, RowsLayout<D, SOURCE, RW>::kBytes, stream, p);
   count_launch();
   if (int rc = check_launch("attend_rows_kernel")) return rc;
   if (ctas < 2) return QMM_OK;
@@ -558,31 +642,31 @@ int launch_one(const RowsParams& p, int ctas, cudaStream_t stream) {
 }
 
 template <typename T, int D, int SOURCE>
-int launch_rows_of(const RowsParams& p, int rows, int ctas, cudaStream_t stream) {
-  if (rows <= 16) return launch_one<T, D, 1, SOURCE>(p, ctas, stream);
-  if (rows <= 32) return launch_one<T, D, 2, SOURCE>(p, ctas, stream);
-  return launch_one<T, D, 4, SOURCE>(p, ctas, stream);
+int launch_rows_of(const RowsParams& p, int rows, cudaStream_t stream) {
+  if (rows <= 16) return launch_one<T, D, 1, SOURCE>(p, stream);
+  if (rows <= 32) return launch_one<T, D, 2, SOURCE>(p, stream);
+  return launch_one<T, D, 4, SOURCE>(p, stream);
 }
 
 template <typename T, int D>
-int launch_source(const RowsParams& p, int source, int rows, int ctas, cudaStream_t stream) {
-  if (source == kRowsSource) return launch_one<T, D, 4, kRowsSource>(p, ctas, stream);
-  if (source == kPages16) return launch_rows_of<T, D, kPages16>(p, rows, ctas, stream);
-  if constexpr (std::is_same<T, __nv_bfloat16>::value) return launch_rows_of<T, D, kPages8>(p, rows, ctas, stream);
+int launch_source(const RowsParams& p, int source, int rows, cudaStream_t stream) {
+  if (source == kRowsSource) return launch_one<T, D, 4, kRowsSource>(p, stream);
+  if (source == kPages16) return launch_rows_of<T, D, kPages16>(p, rows, stream);
+  if constexpr (std::is_same<T, __nv_bfloat16>::value) return launch_rows_of<T, D, kPages8>(p, rows, stream);
   return fail(QMM_ERR_UNSUPPORTED, "attention: an e4m3 cache is attended with bf16 queries");
 }
 
 }  // namespace
 
-int attend_rows_ctas() { return 2 * device_sm_count(); }
+int attend_rows_ctas() { return 3 * device_sm_count(); }
 
 int64_t attend_rows_workspace(int head_dim, int ctas) {
   return ctas * (sizeof(JoinNote) + 2ll * (head_dim == 64 ? partial_floats<64, 64>() : partial_floats<64, 128>()) * 4);
 }
 
-int launch_attend_rows(const RowsParams& p, int elem, int head_dim, int source, int rows, int ctas, cudaStream_t stream) {
-  if (elem == QMM_BF16) return head_dim == 64 ? launch_source<__nv_bfloat16, 64>(p, source, rows, ctas, stream) : launch_source<__nv_bfloat16, 128>(p, source, rows, ctas, stream);
-  return head_dim == 64 ? launch_source<__half, 64>(p, source, rows, ctas, stream) : launch_source<__half, 128>(p, source, rows, ctas, stream);
+int launch_attend_rows(const RowsParams& p, int elem, int head_dim, int source, int rows, cudaStream_t stream) {
+  if (elem == QMM_BF16) return head_dim == 64 ? launch_source<__nv_bfloat16, 64>(p, source, rows, stream) : launch_source<__nv_bfloat16, 128>(p, source, rows, stream);
+  return head_dim == 64 ? launch_source<__half, 64>(p, source, rows, stream) : launch_source<__half, 128>(p, source, rows, stream);
 }
 
 }  // namespace qmm

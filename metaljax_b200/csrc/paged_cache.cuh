@@ -100,16 +100,20 @@ __device__ __forceinline__ uint2 row_values(uint32_t codes, const RowFactors& f)
   return make_uint2(a, b);
 }
 
-// ... without the power of two: a word's codes 0 and 2, and 1 and 3, as bf16 (2^120 brings the exponent there; subnormal codes among them).
-__device__ __forceinline__ uint2 code_values(uint32_t codes) {
-  const uint32_t even = codes << 8;
-  return make_uint2(mul_bf16x2(((even >> 4) & 0x07f007f0u) | (even & 0x80008000u), 0x7b807b80u), mul_bf16x2(((codes >> 4) & 0x07f007f0u) | (codes & 0x80008000u), 0x7b807b80u));
-}
-// ... code i of two words.
+// ... without the power of two: code I of two words, as bf16 (2^120 brings the exponent there; subnormal codes among them), and as f16, which holds a code as it is.
 template <int I>
 __device__ __forceinline__ uint32_t code_pair(uint32_t a, uint32_t b) {
   const uint32_t x = __byte_perm(a, b, (4 + I) << 12 | I << 4);         // (what stands in the lower bytes is masked off)
   return mul_bf16x2(((x >> 4) & 0x07f007f0u) | (x & 0x80008000u), 0x7b807b80u);
+}
+__device__ __forceinline__ uint32_t code_half2(uint32_t two) {         // the lower two
+  uint32_t h;
+  asm("{ .reg .b16 l, u; mov.b32 {l, u}, %1; cvt.rn.f16x2.e4m3x2 %0, l; }" : "=r"(h) : "r"(two));
+  return h;
+}
+template <int I>
+__device__ __forceinline__ uint32_t code_half2(uint32_t a, uint32_t b) {
+  return code_half2(__byte_perm(a, b, (4 + I) << 4 | I));
 }
 __device__ __forceinline__ float row_scale(uint32_t exp_byte) {
   return __uint_as_float(exp_byte == 255 ? 0x7fc00000u : exp_byte == 0 ? 0x00400000u : exp_byte << 23);

@@ -314,6 +314,29 @@ def test_e4m3_values_of_every_size():
         R.close(got[0], want.mean(0, keepdim=True), want.abs().mean(0, keepdim=True), BF)
 
 
+@pytest.mark.parametrize("heads", [4, 16])
+@pytest.mark.parametrize("spread", [3, 8, 40])
+def test_e4m3_rows_of_very_different_sizes(heads, spread):
+    """Powers of two that differ between the rows of a sequence, growing along it, falling, and in no order: none loses bits beside the others."""
+    gen = _gen(15)
+    lens = [333, 333, 333, 1000]
+    cache, table, ks, vs = _paged(lens, 1, 128, 32, E4M3, gen)
+    for s, n in enumerate(lens):
+        pos = torch.arange(n, device=DEV)
+        at, off = table[s].long()[pos // 32], pos % 32
+        shift = (pos * spread // n, (n - 1 - pos) * spread // n, torch.randint(0, spread, (n,), generator=gen, device=DEV))[s % 3] - spread // 2
+        cache.v_exp[at, 0, off] = (cache.v_exp[at, 0, off].int() + shift).to(torch.uint8)
+        vs[s] = R.dequantized(cache.v[at, :, off], cache.v_exp[at, :, off])
+        # keys shrink as values grow, so that scores stay in their range
+        cache.k_exp[at, 0, off] = (cache.k_exp[at, 0, off].int() - (shift > 0).int() * 3).to(torch.uint8)
+        ks[s] = R.dequantized(cache.k[at, :, off], cache.k_exp[at, :, off])
+    q = (torch.randn((len(lens), heads, 128), generator=gen, device=DEV) * torch.exp2(torch.arange(heads, device=DEV) % 5 - 4.0)[None, :, None]).to(BF)
+    got = attention.paged_attention(q, cache, table, R.lengths(lens, DEV))
+    for s in range(len(lens)):
+        want, size = R.attend_fast(q[s: s + 1].double(), ks[s], vs[s], lens[s] - 1, True, 128 ** -0.5)
+        R.close(got[s: s + 1], want, size, BF, products=16.0 * 8)          # (keys here are up to eight times N(0, 1))
+
+
 # ---- append and read back ----
 
 
