@@ -60,7 +60,7 @@ __device__ __forceinline__ int seen_by(const AttentionWork& w, const SeqSpan& s,
 // (a sequence's rows are fewer than 2^31: the entry points see to that)
 template <int R, int B>
 struct RowTiles {
-  static constexpr int kCost = 2, kWhole = 2;
+  static constexpr int kCost = 3, kWhole = 2;
   static __device__ __forceinline__ int tiles(const AttentionWork& w, const SeqSpan& s) { return static_cast<int>((static_cast<unsigned>(s.n) * w.group + R - 1) / R); }
   // One unit at least, which writes the zeros of rows that see nothing.
   static __device__ __forceinline__ int units(const AttentionWork& w, const SeqSpan& s, int t) {
@@ -114,7 +114,7 @@ __device__ __forceinline__ I warp_scan(I v) {                      // inclusive
 
 // One warp: weight of one head's items of 32 sequences from `base` on, a lane each (0 behind the last).
 template <typename Tiles>
-__device__ __forceinline__ int64_t lane_weights(const AttentionWork& w, int base, SeqSpan* mine) {
+__device__ __forceinline__ int64_t lane_weights(const AttentionWork& w, int base) {
   const int lane = threadIdx.x & 31, s = base + lane;
   SeqSpan span = {0, 0, 0};
   if (s < w.seqs) span = span_of(w, s);
@@ -133,7 +133,6 @@ __device__ __forceinline__ int64_t lane_weights(const AttentionWork& w, int base
     part = warp_sum(part);
     if (lane == l) sum = part;
   }
-  *mine = span;
   return sum;
 }
 
@@ -172,43 +171,23 @@ __device__ __forceinline__ bool next_item(const AttentionWork& w, UnitCursor& c)
   return c.end > 0;
 }
 
-// One warp: where CTA `cta` of `ctas` begins; false where it has nothing to do. `share`: what a CTA takes.
+// `left` weights into its item, and `quota` of them this CTA's: where it begins; false where it has nothing to do.
 template <typename Tiles>
-__device__ __forceinline__ bool find_share(const AttentionWork& w, int cta, int ctas, int least, UnitCursor* at, int64_t* share) {
-  const int lane = threadIdx.x & 31;
-  SeqSpan span;
-  int64_t mine = 0, total = 0;
-  bool small = w.seqs <= 32;                            // ordinary calls: sums fit 32 bits, and the one warp-full of sequences is looked at once
-  for (int base = 0; base < w.seqs; base += 32) {
-    mine = lane_weights<Tiles>(w, base, &span);
-    small = small && __all_sync(0xffffffffu, mine < (1 << 25) / w.kv_heads);
-    total += small ? __reduce_add_sync(0xffffffffu, static_cast<int>(mine) * w.kv_heads) : warp_sum(mine) * w.kv_heads;
-  }
-  const int64_t quota = quota_of(total, ctas, least);
-  *share = quota;
-  int64_t left = quota * cta;
-  if (left >= total) return false;
-  int64_t per_head = 0;
-  for (int base = 0; base < w.seqs; base += 32) {
-    if (w.seqs > 32) mine = lane_weights<Tiles>(w, base, &span);
-    const int64_t upto = small ? warp_scan(static_cast<int>(mine)) * w.kv_heads : warp_scan(mine) * w.kv_heads;
-    const unsigned past = __ballot_sync(0xffffffffu, upto > left);
-    if (past) {
-      const int l = __ffs(past) - 1;
-      at->s = base + l;
-      at->span = {__shfl_sync(0xffffffffu, span.q0, l), __shfl_sync(0xffffffffu, span.n, l), __shfl_sync(0xffffffffu, span.len, l)};
-      per_head = __shfl_sync(0xffffffffu, mine, l);
-      left -= __shfl_sync(0xffffffffu, upto, l) - per_head * w.kv_heads;
-      break;
-    }
-    left -= __shfl_sync(0xffffffffu, upto, 31);
-  }
-  at->h = 0;
-  while (left >= per_head) {
-    left -= per_head;
-    ++at->h;
-  }
-  const int tiles = Tiles::tiles(w, at->span);
+__device__ __forceinline__ bool begin_share(const AttentionWork& w, int64_t left, int64_t quota, UnitCursor* at) {
+  at->u = left > 0 ? cut<Tiles>(at->units, left) : 0;
+  at->room = quota + left;
+  if (at->u == at->units) return next_item<Tiles>(w, *at);
+  at->end = cut<Tiles>(at->units, at->room);
+  return at->end > at->u;
+}
+
+// One warp: the item of a sequence at->s and head at->h that is `left` weights behind its first one's beginning; returns what is left of them.
+template <typename Tiles, typename I>
+__device__ __forceinline__ I find_tile(const AttentionWork& w, I left, UnitCursor* at) {
+  const int lane = threadIdx.x & 31, tiles = Tiles::tiles(w, at->span);
+  at->t = 0;
+  at->units = Tiles::units(w, at->span, 0);
+  if (tiles == 1) return left;
   for (int base = 0; base < tiles; base += 32) {
     const int units = base + lane < tiles ? Tiles::units(w, at->span, base + lane) : 0;
     const int upto = warp_scan(base + lane < tiles ? units + Tiles::kCost : 0);        // (32 items: fewer than 2^30)
@@ -217,17 +196,84 @@ __device__ __forceinline__ bool find_share(const AttentionWork& w, int cta, int 
       const int l = __ffs(past) - 1;
       at->t = base + l;
       at->units = __shfl_sync(0xffffffffu, units, l);
-      left -= __shfl_sync(0xffffffffu, upto, l) - (at->units + Tiles::kCost);
-      break;
+      return left - (__shfl_sync(0xffffffffu, upto, l) - (at->units + Tiles::kCost));
     }
     left -= __shfl_sync(0xffffffffu, upto, 31);
   }
-  // `left` weights into the item
-  at->u = left > 0 ? cut<Tiles>(at->units, left) : 0;
-  at->room = quota + left;
-  if (at->u == at->units) return next_item<Tiles>(w, *at);
-  at->end = cut<Tiles>(at->units, at->room);
-  return at->end > at->u;
+  return left;                                          // (not reached: the sums are the same)
+}
+
+// One warp: where CTA `cta` of `ctas` begins; false where it has nothing to do. `share`: what a CTA takes.
+template <typename Tiles>
+__device__ __forceinline__ bool find_share(const AttentionWork& w, int cta, int ctas, int least, UnitCursor* at, int64_t* share) {
+  // ordinary calls: up to 128 sequences, looked at once, and sums of 32 bits (a call waits 2 us for this, and more with 64-bit sums over two looks)
+  constexpr int kGroups = 4;
+  if (w.seqs <= 32 * kGroups) {
+    int mine[kGroups], sum = 0;
+    bool small = true;
+#pragma unroll
+    for (int i = 0; i < kGroups; ++i) {
+      mine[i] = 0;
+      if (i * 32 >= w.seqs) continue;
+      const int64_t weight = lane_weights<Tiles>(w, i * 32);
+      small = small && weight < (1 << 23) / w.kv_heads;
+      mine[i] = static_cast<int>(weight) * w.kv_heads;
+      sum += mine[i];
+    }
+    if (__all_sync(0xffffffffu, small)) {
+      const int total = __reduce_add_sync(0xffffffffu, sum);
+      int quota = static_cast<int>(static_cast<unsigned>(total + ctas - 1) / static_cast<unsigned>(ctas));
+      if (quota < least) quota = least;
+      *share = quota;
+      if (static_cast<int64_t>(quota) * cta >= total) return false;
+      int left = quota * cta;
+#pragma unroll
+      for (int i = 0; i < kGroups; ++i) {
+        if (i * 32 >= w.seqs) break;
+        const int upto = warp_scan(mine[i]);
+        const unsigned past = __ballot_sync(0xffffffffu, upto > left);
+        if (past) {
+          const int l = __ffs(past) - 1, all = __shfl_sync(0xffffffffu, mine[i], l);
+          at->s = i * 32 + l;
+          at->span = span_of(w, at->s);
+          left -= __shfl_sync(0xffffffffu, upto, l) - all;
+          const unsigned per_head = static_cast<unsigned>(all) / static_cast<unsigned>(w.kv_heads);
+          at->h = static_cast<int>(static_cast<unsigned>(left) / per_head);
+          left = find_tile<Tiles>(w, left - at->h * static_cast<int>(per_head), at);
+          return begin_share<Tiles>(w, left, quota, at);
+        }
+        left -= __shfl_sync(0xffffffffu, upto, 31);
+      }
+      return false;                                     // (not reached)
+    }
+  }
+  int64_t total = 0;
+  for (int base = 0; base < w.seqs; base += 32) total += warp_sum(lane_weights<Tiles>(w, base)) * w.kv_heads;
+  const int64_t quota = quota_of(total, ctas, least);
+  *share = quota;
+  int64_t left = quota * cta;
+  if (left >= total) return false;
+  for (int base = 0; base < w.seqs; base += 32) {
+    const int64_t mine = lane_weights<Tiles>(w, base);
+    const int64_t upto = warp_scan(mine) * w.kv_heads;
+    const unsigned past = __ballot_sync(0xffffffffu, upto > left);
+    if (past) {
+      const int l = __ffs(past) - 1;
+      at->s = base + l;
+      at->span = span_of(w, at->s);
+      const int64_t per_head = __shfl_sync(0xffffffffu, mine, l);
+      left -= __shfl_sync(0xffffffffu, upto, l) - per_head * w.kv_heads;
+      at->h = 0;
+      while (left >= per_head) {
+        left -= per_head;
+        ++at->h;
+      }
+      left = find_tile<Tiles>(w, left, at);
+      return begin_share<Tiles>(w, left, quota, at);
+    }
+    left -= __shfl_sync(0xffffffffu, upto, 31);
+  }
+  return false;                                         // (not reached)
 }
 
 // The workspace: a note of every CTA, written by each, then two partial results a CTA. The note says what the second launch has to join at the end of a

@@ -114,13 +114,14 @@ __global__ void __launch_bounds__(kThreads, (RowsLayout<D, SOURCE, RW>::kCtas)) 
   bool loading = true;
 
   // ---- copies: a warp asks for rows 16 * warp .. of a chunk (which lie in one page) ----
-  int64_t page = 0;                                     // of the next chunk's rows of this warp
+  int pages = 0, pages_at = 0;                          // lane i: the page of this warp's rows of chunk pages_at + i
   auto look_up = [&]() {
     if constexpr (kPaged) {
-      const int pos = load.u * kChunk + 16 * warp;
-      page = 0;
-      if (loading && pos < load.span.len) page = page_of(p.cache, load.s, pos, w.status);
-      if (page < 0) page = 0;
+      pages_at = load.u;
+      const int u = load.u + lane, pos = u * kChunk + 16 * warp;
+      int64_t page = 0;
+      if (u < load.end && pos < load.span.len) page = page_of(p.cache, load.s, pos, w.status);
+      pages = page < 0 ? 0 : static_cast<int>(page);
     }
   };
   auto request = [&](int loaded) {                      // the chunk that `load` stands at into the ring, and `load` on
@@ -129,6 +130,7 @@ __global__ void __launch_bounds__(kThreads, (RowsLayout<D, SOURCE, RW>::kCtas)) 
       constexpr int kPieces = L::kRowBytes / 16;
       const int pos0 = load.u * kChunk + 16 * warp;
       // (16 positions of a page are one run of bytes)
+      const int64_t page = kPaged ? __shfl_sync(0xffffffffu, pages, load.u - pages_at) : 0;
       const int64_t run = kPaged ? ((page * w.kv_heads + load.h) << p.cache.page_shift) + (pos0 & ((1 << p.cache.page_shift) - 1)) : 0;
       const bool whole = pos0 + 16 <= load.span.len;
 #pragma unroll
@@ -160,15 +162,17 @@ __global__ void __launch_bounds__(kThreads, (RowsLayout<D, SOURCE, RW>::kCtas)) 
         if (lane < 2)                                   // the 16 rows' exponent bytes, of k and of v (the positions behind the end: of no use)
           cp_async16(stage + 2 * L::kHalf + lane * kChunk + 16 * warp, (lane ? p.cache.v_exp : p.cache.k_exp) + run, pos0 < load.span.len ? 16 : 0);
       }
-      if (++load.u >= load.end) loading = next_item<Tiles>(w, load);
-      look_up();
+      if (++load.u >= load.end) {
+        loading = next_item<Tiles>(w, load);
+        if (loading) look_up();
+      } else if (load.u - pages_at == 32) {
+        look_up();
+      }
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
 
   look_up();
-#pragma unroll
-  for (int i = 0; i < L::kStages - 1; ++i) request(i);
 
   uint32_t q[D / 16][4];
   float o[D / 8][4];
@@ -241,10 +245,12 @@ __global__ void __launch_bounds__(kThreads, (RowsLayout<D, SOURCE, RW>::kCtas)) 
     }
   };
 
+  begin_item();                                          // (its queries before the stream of keys and values, which they would wait behind)
+#pragma unroll
+  for (int i = 0; i < L::kStages - 1; ++i) request(i);
   if (tid == 0) *any_special = 0;
   for (int i = tid; i < 3 * D; i += kThreads) special[i] = INT_MAX;
   __syncthreads();
-  begin_item();
 
   for (int done = 0;; ++done) {
     asm volatile("cp.async.wait_group %0;" ::"n"(L::kStages - 2) : "memory");
@@ -309,6 +315,7 @@ __global__ void __launch_bounds__(kThreads, (RowsLayout<D, SOURCE, RW>::kCtas)) 
       for (int i = 0; i < 4; ++i) s[n][i] = 0.0f;
     float k_scale[SN / 8][2], v_scale[SN / 8][2];         // (codes: of the thread's columns; positions behind the end: 1)
     [[maybe_unused]] bool wide = false;
+    [[maybe_unused]] float s2[SN / 8][4] = {};            // (two chains of products)
     if constexpr (kDirect) {
       // The weights of the values are f16 too: p * 2^(e - v_top + 6), e a row's exponent. Rows more than 2^12 below the largest would lose bits where that one's
       // weight is small: then these positions' products are taken in bf16 (`wide`).
@@ -344,7 +351,11 @@ __global__ void __launch_bounds__(kThreads, (RowsLayout<D, SOURCE, RW>::kCtas)) 
           const uint4 codes = lds128<0>(keys + r * D + ((D == 128 ? piece ^ ((r & 1) << 2) : piece) << 4));
           const uint32_t word[4] = {codes.x, codes.y, codes.z, codes.w};
 #pragma unroll
-          for (int i = 0; i < 4; ++i) mma16816<MT>(s[n], q[h * 4 + i], code_half2(word[i]), code_half2(word[i] >> 16));
+          for (int i = 0; i < 4; ++i) mma16816<MT>(h == 0 ? s[n] : s2[n], q[h * 4 + i], code_half2(word[i]), code_half2(word[i] >> 16));
+        }
+        if constexpr (D == 128) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) s[n][i] += s2[n][i];
         }
       }
     } else
@@ -579,39 +590,46 @@ __global__ void __launch_bounds__(kJoinThreads) attend_join_kernel(const JoinPar
   const float* const first = p.partial + (2 * static_cast<int64_t>(blockIdx.x) + 1) * partial_floats<R, D>();
   const float* const others = p.partial + 2 * static_cast<int64_t>(blockIdx.x) * partial_floats<R, D>();
   auto part_of = [&](int i) { return i == 0 ? first : others + 2ll * i * partial_floats<R, D>(); };
-  float mm = -INFINITY;
-  for (int i = lane; i < c.parts; i += 32) mm = fmaxf(mm, part_of(i)[R * D + r]);
+  // eight parts' loads on their way at once
+  constexpr int kBatch = 8;
+  float mm = -INFINITY, ll = 0.0f, v[V] = {};
+  for (int i0 = 0; i0 < c.parts; i0 += kBatch) {
+    float x[kBatch][V], m[kBatch], l[kBatch];
 #pragma unroll
-  for (int x = 16; x > 0; x >>= 1) mm = fmaxf(mm, __shfl_xor_sync(0xffffffffu, mm, x));
-  const float base = mm == -INFINITY ? 0.0f : mm;
-  float ll = 0.0f, v[V] = {};
-  for (int i0 = 0; i0 < c.parts; i0 += 32) {
-    float f = 0.0f;
-    if (i0 + lane < c.parts) {
-      const float* part = part_of(i0 + lane);
-      f = ex2(part[R * D + r] - base);
-      ll = fmaf(f, part[R * D + R + r], ll);
-    }
-    const int here = c.parts - i0 < 32 ? c.parts - i0 : 32;
-#pragma unroll 8
-    for (int i = 0; i < here; ++i) {
-      const float fi = __shfl_sync(0xffffffffu, f, i);
-      const float* src = part_of(i0 + i) + r * D + lane * V;
+    for (int i = 0; i < kBatch; ++i) {
+      const float* const part = part_of(i0 + i < c.parts ? i0 + i : i0);
+      m[i] = part[R * D + r];
+      l[i] = part[R * D + R + r];
       if constexpr (V == 4) {
-        const float4 x = *reinterpret_cast<const float4*>(src);
-        v[0] = fmaf(fi, x.x, v[0]);
-        v[1] = fmaf(fi, x.y, v[1]);
-        v[2] = fmaf(fi, x.z, v[2]);
-        v[3] = fmaf(fi, x.w, v[3]);
+        const float4 y = *reinterpret_cast<const float4*>(part + r * D + lane * V);
+        x[i][0] = y.x;
+        x[i][1] = y.y;
+        x[i][2] = y.z;
+        x[i][3] = y.w;
       } else {
-        const float2 x = *reinterpret_cast<const float2*>(src);
-        v[0] = fmaf(fi, x.x, v[0]);
-        v[1] = fmaf(fi, x.y, v[1]);
+        const float2 y = *reinterpret_cast<const float2*>(part + r * D + lane * V);
+        x[i][0] = y.x;
+        x[i][1] = y.y;
       }
     }
-  }
+    float top = mm;
 #pragma unroll
-  for (int x = 16; x > 0; x >>= 1) ll += __shfl_xor_sync(0xffffffffu, ll, x);
+    for (int i = 0; i < kBatch; ++i)
+      if (i0 + i < c.parts) top = fmaxf(top, m[i]);
+    const float base = top == -INFINITY ? 0.0f : top, shrink = ex2(mm - base);
+    mm = top;
+    ll *= shrink;
+#pragma unroll
+    for (int e = 0; e < V; ++e) v[e] *= shrink;
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i)
+      if (i0 + i < c.parts) {
+        const float f = ex2(m[i] - base);
+        ll = fmaf(f, l[i], ll);
+#pragma unroll
+        for (int e = 0; e < V; ++e) v[e] = fmaf(f, x[i][e], v[e]);
+      }
+  }
   const int tok = row / w.group, g = row - tok * w.group;
   const int seen = w.causal ? c.len - c.n + tok : c.len - 1;
   const float inv = ll == 0.0f ? (seen < 0 ? 0.0f : NAN) : 1.0f / ll;
