@@ -75,7 +75,7 @@ struct RowsLayout {
   static constexpr bool kE4m3 = SOURCE == kPages8, kDirect = kE4m3 && RW == 1;
   static constexpr int kCtas = kDirect ? 3 : 2;                          // an SM
 
-  static constexpr int kStages = kE4m3 ? 4 : 3;
+  static constexpr int kStages = 3;
   static constexpr int kRowBytes = D * (kE4m3 ? 1 : 2);
   static constexpr int kHalf = kChunk * kRowBytes;                       // keys of a chunk; values follow, then (e4m3) both rows' bytes
   static constexpr int kStage = 2 * kHalf + (kE4m3 ? 2 * kChunk : 0);
@@ -181,6 +181,7 @@ __global__ void __launch_bounds__(kThreads, (RowsLayout<D, SOURCE, RW>::kCtas)) 
   int tile_first_limit = 0, tile_rows = 0;
   int begun = 0;                                         // first unit of this item here
   [[maybe_unused]] float q_scale = 0.0f;                 // (codes) the queries' power of two and the scale
+  [[maybe_unused]] float v_unit = 1.0f, v_rest = 1.0f;
   [[maybe_unused]] int v_top = 0;                        // (codes) the largest exponent of a row of values so far: the sums are in units of 2^v_top
 
   auto begin_item = [&]() {
@@ -242,6 +243,7 @@ __global__ void __launch_bounds__(kThreads, (RowsLayout<D, SOURCE, RW>::kCtas)) 
           q[kk][i] = pack2<__half>(f.x * up, f.y * up);
         }
       v_top = -1000;
+      v_unit = v_rest = 1.0f;
     }
   };
 
@@ -319,8 +321,10 @@ __global__ void __launch_bounds__(kThreads, (RowsLayout<D, SOURCE, RW>::kCtas)) 
     if constexpr (kDirect) {
       // The weights of the values are f16 too: p * 2^(e - v_top + 6), e a row's exponent. Rows more than 2^12 below the largest would lose bits where that one's
       // weight is small: then these positions' products are taken in bf16 (`wide`).
-      const int mine = lane < SN && kw * SN + lane < c.span.len - pos0 ? static_cast<int>(lds8(stage + 2 * L::kHalf + kChunk + kw * SN + (lane & (SN - 1)))) : 255;
-      const int high = __reduce_max_sync(0xffffffffu, mine == 255 ? -1000 : mine - 127), low = __reduce_min_sync(0xffffffffu, mine == 255 ? 1000 : mine - 127);
+      const uint32_t bytes = stage + 2 * L::kHalf + kw * SN;
+      const bool there = lane < SN && kw * SN + lane < c.span.len - pos0;
+      const int k_byte = there ? static_cast<int>(lds8(bytes + lane)) : 127, v_byte = there ? static_cast<int>(lds8(bytes + kChunk + lane)) : 255;
+      const int high = __reduce_max_sync(0xffffffffu, v_byte == 255 ? -1000 : v_byte - 127), low = __reduce_min_sync(0xffffffffu, v_byte == 255 ? 1000 : v_byte - 127);
       if (high > v_top) {
         if (v_top > -1000) {
           const float down = high - v_top > 126 ? 0.0f : __uint_as_float(static_cast<uint32_t>(127 + v_top - high) << 23);
@@ -330,19 +334,28 @@ __global__ void __launch_bounds__(kThreads, (RowsLayout<D, SOURCE, RW>::kCtas)) 
             for (int i = 0; i < 4; ++i) o[n][i] *= down;
         }
         v_top = high;
+        // 2^(6 - v_top), in two steps that are both in range
+        const int near = v_top > 64 ? 64 : v_top < -64 ? -64 : v_top;
+        v_unit = __uint_as_float(static_cast<uint32_t>(127 + 6 - near) << 23);
+        v_rest = __uint_as_float(static_cast<uint32_t>(127 + near - (v_top < -127 ? -127 : v_top)) << 23);
       }
       wide = v_top - low > 12;
-      // (2^(e - v_top + 6) in two steps that are both in range)
-      const float unit = __uint_as_float(static_cast<uint32_t>(127 + 6 - (v_top > 64 ? 64 : v_top < -64 ? -64 : v_top)) << 23);
-      const float rest = __uint_as_float(static_cast<uint32_t>(127 - (v_top > 64 ? v_top - 64 : v_top < -64 ? (v_top < -127 ? -63 : v_top + 64) : 0)) << 23);
+      // ordinary rows: all there, and numbers
+      const bool plain = __all_sync(0xffffffffu, lane >= SN || (there && k_byte != 255 && k_byte != 0 && v_byte != 255 && v_byte != 0));
 #pragma unroll
       for (int n = 0; n < SN / 8; ++n) {
-        const int at = kw * SN + n * 8 + (lane & 3) * 2, there = c.span.len - pos0 - at;
-        const uint32_t k2 = lds16(stage + 2 * L::kHalf + at), v2 = lds16(stage + 2 * L::kHalf + kChunk + at);
+        const uint32_t k2 = lds16(bytes + n * 8 + (lane & 3) * 2), v2 = lds16(bytes + kChunk + n * 8 + (lane & 3) * 2);
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          k_scale[n][e] = (e < there ? row_scale(k2 >> (8 * e) & 255) : 1.0f) * q_scale;
-          v_scale[n][e] = (e < there ? row_scale(v2 >> (8 * e) & 255) : 0.0f) * unit * rest;
+          const uint32_t kb = e ? k2 >> 8 : k2 & 255, vb = e ? v2 >> 8 : v2 & 255;
+          if (plain) {
+            k_scale[n][e] = __uint_as_float(kb << 23) * q_scale;
+            v_scale[n][e] = __uint_as_float(vb << 23) * v_unit * v_rest;
+          } else {
+            const bool in = kw * SN + n * 8 + (lane & 3) * 2 + e < c.span.len - pos0;
+            k_scale[n][e] = (in ? row_scale(kb) : 1.0f) * q_scale;
+            v_scale[n][e] = (in ? row_scale(vb) : 0.0f) * v_unit * v_rest;
+          }
         }
         const int r = kw * SN + n * 8 + (lane >> 2);
 #pragma unroll
@@ -377,11 +390,19 @@ __global__ void __launch_bounds__(kThreads, (RowsLayout<D, SOURCE, RW>::kCtas)) 
     for (int n = 0; n < SN / 8; ++n)
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        float x = s[n][i] * (kDirect ? k_scale[n][i & 1] : p.scale_log2);
-        if (edge && warp_pos + n * 8 + (lane & 3) * 2 + (i & 1) > limit[i >> 1]) x = -INFINITY;
-        s[n][i] = x;
-        top[i >> 1] = fmaxf(top[i >> 1], x);
+        s[n][i] *= kDirect ? k_scale[n][i & 1] : p.scale_log2;
       }
+    if (edge) {
+#pragma unroll
+      for (int n = 0; n < SN / 8; ++n)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (warp_pos + n * 8 + (lane & 3) * 2 + (i & 1) > limit[i >> 1]) s[n][i] = -INFINITY;
+    }
+#pragma unroll
+    for (int n = 0; n < SN / 8; ++n)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) top[i >> 1] = fmaxf(top[i >> 1], s[n][i]);
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       top[i] = fmaxf(top[i], __shfl_xor_sync(0xffffffffu, top[i], 1));
@@ -408,15 +429,17 @@ __global__ void __launch_bounds__(kThreads, (RowsLayout<D, SOURCE, RW>::kCtas)) 
       for (int n = 0; n < SN / 8; ++n)
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          float x = ex2(s[n][2 * i + e] - base);
+          const float x = ex2(s[n][2 * i + e] - base);
           l[i] += x;
-          if constexpr (kDirect) {
-            // the values' power of two goes to their weights; a masked weight is zero whatever that is
-            if (edge && warp_pos + n * 8 + (lane & 3) * 2 + e > limit[i]) x = 0.0f;
-            else x *= v_scale[n][e];
-          }
-          s[n][2 * i + e] = x;
+          s[n][2 * i + e] = kDirect ? x * v_scale[n][e] : x;           // (the values' power of two goes to their weights)
         }
+    }
+    if (kDirect && edge) {                                // a masked weight is zero whatever that is
+#pragma unroll
+      for (int n = 0; n < SN / 8; ++n)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (warp_pos + n * 8 + (lane & 3) * 2 + (i & 1) > limit[i >> 1]) s[n][i] = 0.0f;
     }
     // ---- weights times values ----
 #pragma unroll
