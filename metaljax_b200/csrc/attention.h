@@ -31,10 +31,10 @@ int64_t attend_rows_workspace(int head_dim, int ctas);
 // `source`: 0 rows, 1 pages of 16-bit values, 2 pages of e4m3 codes; `rows`: query rows that a sequence and key head have at most, as far as is known.
 int launch_attend_rows(const RowsParams& p, int elem, int head_dim, int source, int rows, cudaStream_t stream);
 
-// 128-row halves on tcgen05: prompts (not `paged`) and 16-bit pages. A cache's rows have to be fewer than 2^31.
+// 128-row halves on tcgen05. A cache's rows have to be fewer than 2^31.
 int attend_tc_ctas();
 int64_t attend_tc_workspace(int head_dim, int ctas);
-int launch_attend_tc(const RowsParams& p, int elem, int head_dim, bool paged, int ctas, cudaStream_t stream);
+int launch_attend_tc(const RowsParams& p, int elem, int head_dim, int source, int ctas, cudaStream_t stream);
 
 int launch_append(const CacheView& c, const qmm_append_args& a, int head_dim, bool e4m3, int* status, cudaStream_t stream);
 int launch_cache_read(const CacheView& c, int64_t seqs, const int32_t* cu_kv, int64_t total, int head_dim, int elem, bool e4m3, void* k_out,

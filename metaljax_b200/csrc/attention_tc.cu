@@ -16,7 +16,10 @@
 // do: rows behind the sequence's end become zeros (0 times what stands in a page behind the end may be NaN), and infinities and NaN that only some
 // rows see are taken out and put into those rows' sums at the end.
 //
-// Warps: 0..3 and 4..7 the halves' rows, 8 the MMAs' issuer, 9 the copies, 10 and 11 helpers. Waits are bounded, as everywhere.
+// An e4m3 cache's blocks arrive as codes, and six helpers turn them into bf16 in the products' layout (exactly); there the only values that are no numbers
+// are rows whose exponent byte says so.
+//
+// Warps: 0..3 and 4..7 the halves' rows, 8 the MMAs' issuer, 9 the copies, from 10 on helpers. Waits are bounded, as everywhere.
 #include <climits>
 #include <type_traits>
 
@@ -28,20 +31,26 @@ namespace {
 
 using namespace tc;
 
-constexpr int kThreads = 384, kBlock = 128, kHelpers = 2;
+constexpr int kBlock = 128;
+enum Source { kRowsSource, kPages16, kPages8 };
 using Tiles = TokenTiles<kBlock>;
 
-template <int D>
+template <int D, int SOURCE>
 struct TcLayout {
+  static constexpr bool kE4m3 = SOURCE == kPages8;
+  static constexpr int kHelpers = kE4m3 ? 6 : 2, kThreads = (10 + kHelpers) * 32;
   static constexpr int kTile = D / 64 * 16384;         // 128 rows: columns of 64 elements, 128 bytes a row, one behind the other
-  static constexpr int kKeys = D == 64 ? 5 : 2, kValues = D == 64 ? 5 : 3;       // blocks on their way or at work
+  static constexpr int kKeys = D == 64 ? (kE4m3 ? 3 : 5) : 2, kValues = D == 64 ? (kE4m3 ? 3 : 5) : kE4m3 ? 2 : 3;       // blocks on their way or at work
+  static constexpr int kCodes = kE4m3 ? 2 : 0;         // blocks of codes on their way, keys and values in turn
   static constexpr int kKeyRing = 2 * kTile;           // behind Q's halves
   static constexpr int kValueRing = kKeyRing + kKeys * kTile;
-  static constexpr int kSpecials = kValueRing + kValues * kTile;
-  static constexpr int kBars = kSpecials + kHelpers * 3 * D * 2;           // 16-bit places, a set for each helper
-  static constexpr int kNumBars = 2 * kKeys + 3 * kValues + 15;
+  static constexpr int kCodeRing = kValueRing + kValues * kTile;
+  static constexpr int kExps = kCodeRing + kCodes * kBlock * D;          // the codes' rows' exponent bytes
+  static constexpr int kSpecials = kExps + kCodes * kBlock;
+  static constexpr int kBars = kSpecials + (kE4m3 ? 0 : kHelpers * 3 * D * 2);           // 16-bit places, a set for each helper
+  static constexpr int kNumBars = 2 * kKeys + 3 * kValues + 2 * kCodes + 15;
   static constexpr int kWords = kBars + 8 * kNumBars;  // tensor memory's address, abort flag, and counters
-  static constexpr int kBytes = kWords + 64 + 1024;    // (what is swizzled begins at a multiple of 1024)
+  static constexpr int kBytes = kWords + 128 + 1024;   // (what is swizzled begins at a multiple of 1024)
 };
 
 // A, B in shared memory, both K-major: D / 16 steps of 16 elements.
@@ -75,6 +84,9 @@ __device__ __forceinline__ void tma_load_3d(const CUtensorMap* map, uint32_t dst
   asm volatile("cp.async.bulk.tensor.3d.shared::cta.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(dst), "l"(map), "r"(bar), "r"(c0),
                "r"(c1), "r"(c2)
                : "memory");
+}
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {       // 16-byte aligned, a multiple of 16 bytes
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
 }
 __device__ __forceinline__ float ex2(float x) {
   float y;
@@ -172,23 +184,26 @@ __device__ __forceinline__ Part part_of(const AttentionWork& w, const UnitCursor
 // last that its last row sees: a place counted from here has 10 bits. (An unwritten one, 0xffff, is above every row's.)
 __device__ __forceinline__ int place_of(int first_limit) { return (first_limit > 0 ? first_limit : 0) - 127; }
 
-template <typename T, int D, bool PAGED>
-__global__ void __launch_bounds__(kThreads, 1)
+template <typename T, int D, int SOURCE>
+__global__ void __launch_bounds__((TcLayout<D, SOURCE>::kThreads), 1)
 attend_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map,
                  const RowsParams p) {
-  using L = TcLayout<D>;
+  using L = TcLayout<D, SOURCE>;
+  constexpr bool PAGED = SOURCE != kRowsSource, kE4m3 = L::kE4m3;
+  constexpr int kHelpers = L::kHelpers, kTags = 2, kHelped = 8, kWritten = 14, kNanPlace = 22;      // words
   constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw = smem_u32(smem_raw);
   const uint32_t base = (raw + 1023u) & ~1023u;
   uint8_t* const smem = smem_raw + (base - raw);
   uint16_t* const special = reinterpret_cast<uint16_t*>(smem + L::kSpecials);      // [helper][+inf, -inf, NaN][D]: first place with one in a column of v
-  // [2 + helper] item whose specials its set holds, [4 + helper] items it has been through, [6 + warp of rows] items it has written
+  // [kTags + helper] item whose specials its set holds, [kHelped + helper] items it has been through, [kWritten + warp of rows] items it has written
   volatile int* const words = reinterpret_cast<volatile int*>(smem + L::kWords);
   const uint32_t key_ring = base + L::kKeyRing, value_ring = base + L::kValueRing, bars = base + L::kBars;
   const uint32_t q_full = bars, q_empty = bars + 16, k_full = bars + 32, k_empty = k_full + 8 * L::kKeys;
   const uint32_t v_full = k_empty + 8 * L::kKeys, v_empty = v_full + 8 * L::kValues, v_clean = v_empty + 8 * L::kValues;
-  const uint32_t s_full = v_clean + 8 * L::kValues, p_full = s_full + 16, o_full = p_full + 32, o_free = o_full + 16, done = o_free + 16;
+  const uint32_t c_full = v_clean + 8 * L::kValues, c_empty = c_full + 8 * L::kCodes;
+  const uint32_t s_full = c_empty + 8 * L::kCodes, p_full = s_full + 16, o_full = p_full + 32, o_free = o_full + 16, done = o_free + 16;
   const uint32_t tmem_slot = base + L::kWords, abort_at = tmem_slot + 4;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const AttentionWork& w = p.work;
@@ -197,13 +212,17 @@ attend_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constan
   if (tid == 0) {
     auto init = [](uint32_t bar, int n) { asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(n)); };
     for (int i = 0; i < L::kKeys; ++i) {
-      init(k_full + 8 * i, 1);
+      init(k_full + 8 * i, kE4m3 ? kHelpers : 1);
       init(k_empty + 8 * i, 1);
     }
     for (int i = 0; i < L::kValues; ++i) {
       init(v_full + 8 * i, 1);
       init(v_empty + 8 * i, 1);
       init(v_clean + 8 * i, kHelpers);
+    }
+    for (int i = 0; i < L::kCodes; ++i) {
+      init(c_full + 8 * i, 1);
+      init(c_empty + 8 * i, kHelpers);
     }
     for (int x = 0; x < 2; ++x) {
       init(q_full + 8 * x, 1);
@@ -215,7 +234,7 @@ attend_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constan
       init(o_free + 8 * x, 4);
     }
     init(done, 1);
-    for (int i = 1; i < 16; ++i) words[i] = 0;
+    for (int i = 1; i < 32; ++i) words[i] = 0;
     mbar_init_fence();
   }
   if (warp == 8) {
@@ -257,14 +276,16 @@ attend_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constan
     return ok;
   };
   bool ok = true;
-  // 168 registers a thread at the launch: 128 x 104 + 256 x 200 = 384 x 168
+  // registers a thread at the launch: 168 (128 x 104 + 256 x 200 = 384 x 168), or with more helpers 128 (256 x 64 + 256 x 192 = 512 x 128)
   if (warp >= 8) {
-  asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");
+  if constexpr (kE4m3) asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
+  else asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");
   if (warp == 9) {
     // ---------------- copies ----------------
     if (lane == 0) p.notes[blockIdx.x].parts = 0;         // (also where this CTA gives up)
     Slot<L::kKeys> key = {0, 0};
     Slot<L::kValues> value = {0, 0};
+    [[maybe_unused]] Slot<kE4m3 ? L::kCodes : 1> code = {0, 0};
     int items[2] = {0, 0};
     const int page_size = 1 << p.cache.page_shift;
     const int per_block = PAGED ? (page_size < kBlock ? kBlock / page_size : 1) : 1;       // pages of a block
@@ -303,6 +324,21 @@ attend_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constan
           look_up(u + 1);
 #pragma unroll
           for (int which = 0; which < 2; ++which) {
+            if constexpr (kE4m3) {
+              if (!(ok = wait(c_empty + 8 * code.slot, code.phase ^ 1u, 32))) break;
+              const uint32_t dst = base + L::kCodeRing + code.slot * (kBlock * D), exps = base + L::kExps + code.slot * kBlock, bar = c_full + 8 * code.slot;
+              const int rows = page_size < kBlock ? page_size : kBlock;
+              if (lane == 0) mbar_expect_tx(bar, there * rows * (D + 1));
+              __syncwarp();
+              if (lane < there) {
+                const int64_t row = ((here * w.kv_heads + c.h) << p.cache.page_shift) + ((u * kBlock) & (page_size - 1));
+                tma_load_2d(which ? &v_map : &k_map, dst + lane * rows * D, bar, 0, static_cast<int>(row));
+                bulk_load(exps + lane * rows, (which ? p.cache.v_exp : p.cache.k_exp) + row, rows, bar);
+              }
+              __syncwarp();
+              code.next();
+              continue;
+            }
             const uint32_t slot = which ? value.slot : key.slot;
             if (!(ok = wait((which ? v_empty : k_empty) + 8 * slot, (which ? value.phase : key.phase) ^ 1u, 32))) break;
             const uint32_t dst = (which ? value_ring : key_ring) + slot * L::kTile, bar = (which ? v_full : k_full) + 8 * slot;
@@ -330,10 +366,79 @@ attend_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constan
       auto drain = [&](uint32_t bars_of, int n, uint32_t slot, uint32_t phase) {
         for (int i = 0; i < n; ++i) mbar_drain(bars_of + 8 * i, i < static_cast<int>(slot) ? phase : phase ^ 1u);
       };
-      drain(k_full, L::kKeys, key.slot, key.phase);
-      drain(v_full, L::kValues, value.slot, value.phase);
+      if constexpr (kE4m3) {
+        drain(c_full, L::kCodes, code.slot, code.phase);
+      } else {
+        drain(k_full, L::kKeys, key.slot, key.phase);
+        drain(v_full, L::kValues, value.slot, value.phase);
+      }
       for (int x = 0; x < 2; ++x)
         if (items[x]) mbar_drain(q_full + 8 * x, (items[x] - 1) & 1);
+    }
+  } else if (kE4m3 && warp >= 10) {
+    // ---------------- helpers: codes into bf16, in the products' layout ----------------
+    Slot<L::kKeys> key = {0, 0};
+    Slot<L::kValues> value = {0, 0};
+    Slot<kE4m3 ? L::kCodes : 1> code = {0, 0};
+    int live = 0;
+    while (ok && more) {
+      const Part it = part_of(w, c);
+      if (it.live) {
+        const int first_limit = w.causal ? c.span.len - c.span.n + c.t * 2 * w.tile_tokens : c.span.len - 1;
+        const int seen = it.seen[0] > it.seen[1] ? it.seen[0] : it.seen[1];
+        bool mine = false;                              // the first row of no numbers is this item's
+        for (int u = it.begin; ok && u < it.load_end; ++u) {
+#pragma unroll 1
+          for (int which = 0; which < 2; ++which) {
+            if (!(ok = wait(c_full + 8 * code.slot, code.phase, 33))) break;
+            if (!(ok = wait((which ? v_empty : k_empty) + 8 * (which ? value.slot : key.slot), (which ? value.phase : key.phase) ^ 1u, 45))) break;
+            const uint32_t from = base + L::kCodeRing + code.slot * (kBlock * D), exps = base + L::kExps + code.slot * kBlock;
+            const uint32_t to = which ? value_ring + value.slot * L::kTile : key_ring + key.slot * L::kTile;
+            const int pos0 = u * kBlock;
+            constexpr int kPieces = D / 16;
+            // rows of values that some rows see and others do not, or none
+            const int some = which ? (first_limit + 1 > pos0 ? first_limit + 1 - pos0 : 0) : kBlock, none = which ? seen - pos0 : kBlock;
+#pragma unroll 2
+            for (int i = (warp - 10) * 32 + lane; i < kBlock * kPieces; i += kHelpers * 32) {
+              const int r = i / kPieces, col = i % kPieces;
+              const uint4 codes = lds128<0>(from + i * 16);
+              uint32_t byte = lds8(exps + r);
+              bool odd = false;
+              if (r >= some) {
+                odd = byte == 255 && r < none;
+                if (odd || r >= none) byte = 0x100;     // zeros
+              }
+              if (__any_sync(0xffffffffu, odd) && !mine) {
+                if (!(ok = wait_count(kWritten, 8, live, 34))) break;
+                if (lane == 0) words[kNanPlace + warp - 10] = 0x7fffffff;
+                if (lane == 0) words[kTags + warp - 10] = live + 1;
+                __syncwarp();
+                mine = true;
+              }
+              if (odd) atomicMin(const_cast<int*>(&words[kNanPlace + warp - 10]), pos0 + r);
+              const RowFactors f = row_factors(byte & 255);
+              uint2 v[4] = {row_values(codes.x, f), row_values(codes.y, f), row_values(codes.z, f), row_values(codes.w, f)};
+              if (byte == 0x100) v[0] = v[1] = v[2] = v[3] = make_uint2(0, 0);
+              const uint32_t line = to + (col >> 2) * 16384 + r * 128, piece = 2 * col & 7;
+              asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(line + ((piece ^ (r & 7)) << 4)), "r"(v[0].x), "r"(v[0].y), "r"(v[1].x), "r"(v[1].y) : "memory");
+              asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(line + (((piece + 1) ^ (r & 7)) << 4)), "r"(v[2].x), "r"(v[2].y), "r"(v[3].x), "r"(v[3].y) : "memory");
+            }
+            fence_proxy_async();
+            __syncwarp();
+            if (lane == 0) {
+              mbar_arrive(c_empty + 8 * code.slot);
+              mbar_arrive(which ? v_clean + 8 * value.slot : k_full + 8 * key.slot);
+            }
+            code.next();
+            if (which) value.next(); else key.next();
+          }
+        }
+        __threadfence_block();
+        __syncwarp();
+        if (lane == 0) words[kHelped + warp - 10] = live + 1;
+        ++live;
+      }
+      more = next_item<Tiles>(w, c);
     }
   } else if (warp >= 10) {
     // ---------------- helpers: blocks of v that some row does not see all of ----------------
@@ -376,9 +481,9 @@ attend_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constan
                 if (odd_pair<T>(v[b].x) || odd_pair<T>(v[b].y) || odd_pair<T>(v[b].z) || odd_pair<T>(v[b].w)) odd |= 1u << b;
               if (!__any_sync(0xffffffffu, odd)) continue;
               if (!mine) {                            // the items before this one are written: what the set held goes
-                if (!(ok = wait_count(6, 8, live, 34))) break;
+                if (!(ok = wait_count(kWritten, 8, live, 34))) break;
                 for (int n = lane; n < 3 * D; n += 32) set[n] = 0xffff;
-                if (lane == 0) words[2 + warp - 10] = live + 1;
+                if (lane == 0) words[kTags + warp - 10] = live + 1;
                 __syncwarp();
                 mine = true;
               }
@@ -413,7 +518,7 @@ attend_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constan
         }
         __threadfence_block();
         __syncwarp();
-        if (lane == 0) words[4 + warp - 10] = live + 1;
+        if (lane == 0) words[kHelped + warp - 10] = live + 1;
         ++live;
       }
       more = next_item<Tiles>(w, c);
@@ -484,7 +589,8 @@ attend_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constan
     mbar_drain(done, 0);
   }
   } else {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
+    if constexpr (kE4m3) asm volatile("setmaxnreg.inc.sync.aligned.u32 192;");
+    else asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
     // ---------------- rows ----------------
     const int x = warp >> 2, r = (warp & 3) * 32 + lane;
     const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
@@ -579,8 +685,8 @@ attend_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constan
         if (!(ok = wait(o_full + 8 * x, o_ph, 42))) break;
         o_ph ^= 1u;
         tc_fence_after();
-        if (!(ok = wait_count(4, kHelpers, live + 1, 43))) break;
-        for (int n = 0; n < kHelpers; ++n) odd[n] = words[2 + n] == live + 1;
+        if (!(ok = wait_count(kHelped, kHelpers, live + 1, 43))) break;
+        for (int n = 0; n < kHelpers; ++n) odd[n] = words[kTags + n] == live + 1;
       }
       const bool sector = (reinterpret_cast<uintptr_t>(p.out) & 31) == 0;
       const bool whole = it.begin == 0 && c.end == c.units;
@@ -601,7 +707,12 @@ attend_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constan
         }
 #pragma unroll
         for (int n = 0; n < kHelpers; ++n)
-          if (odd[n]) {
+          if (kE4m3 && odd[n]) {
+            if (words[kNanPlace + n] <= limit) {
+#pragma unroll
+              for (int j = 0; j < 64; ++j) o[j >> 5][j & 31] = 0x7fc00000u;
+            }
+          } else if (!kE4m3 && odd[n]) {
             const uint16_t* const set = special + n * 3 * D + i * 64;
             const int seen = limit - place_of(first_item_limit);
 #pragma unroll
@@ -643,7 +754,7 @@ attend_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constan
       if (it.live) {
         __threadfence_block();
         __syncwarp();
-        if (lane == 0) words[6 + warp] = live + 1;
+        if (lane == 0) words[kWritten + warp] = live + 1;
         ++live;
       }
       more = again;
@@ -700,18 +811,19 @@ __global__ void __launch_bounds__(256) attend_tc_join_kernel(const JoinParams p)
                                                         pack2<T>(v[j + 4] * inv, v[j + 5] * inv), pack2<T>(v[j + 6] * inv, v[j + 7] * inv));
 }
 
-template <typename T, int D, bool PAGED>
+template <typename T, int D, int SOURCE>
 int launch_one(const RowsParams& p, const CUtensorMap (&maps)[3], int ctas, cudaStream_t stream) {
   static bool done[kMaxDevices] = {};
   const int dev = current_device();
   if (dev < 0) return QMM_ERR_DEVICE;
-  auto kernel = attend_tc_kernel<T, D, PAGED>;
+  auto kernel = attend_tc_kernel<T, D, SOURCE>;
+  using L = TcLayout<D, SOURCE>;
   if (!done[dev]) {
-    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, TcLayout<D>::kBytes);
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kBytes);
     if (e != cudaSuccess) return fail(QMM_ERR_CUDA, "cudaFuncSetAttribute: %s", cudaGetErrorString(e));
     done[dev] = true;
   }
-  launch_early(kernel, ctas, kThreads, TcLayout<D>::kBytes, stream, maps[0], maps[1], maps[2], p);
+  launch_early(kernel, ctas, L::kThreads, L::kBytes, stream, maps[0], maps[1], maps[2], p);
   count_launch();
   if (int rc = check_launch("attend_tc_kernel")) return rc;
   if (ctas < 2) return QMM_OK;
@@ -721,10 +833,12 @@ int launch_one(const RowsParams& p, const CUtensorMap (&maps)[3], int ctas, cuda
   return check_launch("attend_tc_join_kernel");
 }
 
-template <typename T>
-int launch_of(const RowsParams& p, const CUtensorMap (&maps)[3], int head_dim, bool paged, int ctas, cudaStream_t stream) {
-  if (head_dim == 64) return paged ? launch_one<T, 64, true>(p, maps, ctas, stream) : launch_one<T, 64, false>(p, maps, ctas, stream);
-  return paged ? launch_one<T, 128, true>(p, maps, ctas, stream) : launch_one<T, 128, false>(p, maps, ctas, stream);
+template <typename T, int D>
+int launch_of(const RowsParams& p, const CUtensorMap (&maps)[3], int source, int ctas, cudaStream_t stream) {
+  if (source == kRowsSource) return launch_one<T, D, kRowsSource>(p, maps, ctas, stream);
+  if (source == kPages16) return launch_one<T, D, kPages16>(p, maps, ctas, stream);
+  if constexpr (std::is_same<T, __nv_bfloat16>::value) return launch_one<T, D, kPages8>(p, maps, ctas, stream);
+  return fail(QMM_ERR_UNSUPPORTED, "attention: an e4m3 cache is attended with bf16 queries");
 }
 
 }  // namespace
@@ -735,22 +849,25 @@ int64_t attend_tc_workspace(int head_dim, int ctas) {
   return ctas * (sizeof(JoinNote) + 2ll * (head_dim == 64 ? partial_floats<256, 64>() : partial_floats<256, 128>()) * 4);
 }
 
-int launch_attend_tc(const RowsParams& given, int elem, int head_dim, bool paged, int ctas, cudaStream_t stream) {
+int launch_attend_tc(const RowsParams& given, int elem, int head_dim, int source, int ctas, cudaStream_t stream) {
   RowsParams p = given;
   AttentionWork& w = p.work;
   w.tile_tokens = 128 / w.group;
   CUtensorMap maps[3];
   if (int rc = tensor_map_3d(&maps[0], elem, p.q, head_dim, w.heads, w.tokens, p.q_head * 2, p.q_row * 2, 64, w.group, w.tile_tokens)) return rc;
-  if (paged) {
+  if (source != kRowsSource) {
     const int page = 1 << p.cache.page_shift, rows = page < kBlock ? page : kBlock;
     const uint64_t all = static_cast<uint64_t>(p.cache.pages) * w.kv_heads << p.cache.page_shift;
-    if (int rc = tensor_map_2d(&maps[1], elem, p.cache.k, head_dim, all, head_dim * 2, 64, rows, 1)) return rc;
-    if (int rc = tensor_map_2d(&maps[2], elem, p.cache.v, head_dim, all, head_dim * 2, 64, rows, 1)) return rc;
+    const bool codes = source == kPages8;              // as they lie; values in the products' swizzle, 64 elements a row
+    for (int i = 0; i < 2; ++i)
+      if (int rc = tensor_map_2d(&maps[1 + i], codes ? QMM_U8 : elem, i ? p.cache.v : p.cache.k, head_dim, all, head_dim * (codes ? 1 : 2), codes ? head_dim : 64, rows, codes ? 0 : 1))
+        return rc;
   } else {
     if (int rc = tensor_map_3d(&maps[1], elem, p.k, head_dim, w.kv_heads, w.tokens, p.k_head * 2, p.k_row * 2, 64, 1, kBlock)) return rc;
     if (int rc = tensor_map_3d(&maps[2], elem, p.v, head_dim, w.kv_heads, w.tokens, p.v_head * 2, p.v_row * 2, 64, 1, kBlock)) return rc;
   }
-  return elem == QMM_BF16 ? launch_of<__nv_bfloat16>(p, maps, head_dim, paged, ctas, stream) : launch_of<__half>(p, maps, head_dim, paged, ctas, stream);
+  if (elem == QMM_BF16) return head_dim == 64 ? launch_of<__nv_bfloat16, 64>(p, maps, source, ctas, stream) : launch_of<__nv_bfloat16, 128>(p, maps, source, ctas, stream);
+  return head_dim == 64 ? launch_of<__half, 64>(p, maps, source, ctas, stream) : launch_of<__half, 128>(p, maps, source, ctas, stream);
 }
 
 }  // namespace qmm
