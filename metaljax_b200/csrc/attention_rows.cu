@@ -273,15 +273,16 @@ __global__ void __launch_bounds__(kThreads, (RowsLayout<D, SOURCE, RW>::kCtas)) 
 #pragma unroll
         for (int i = 0; i < 16 * kPieces / 32; ++i) {
           const int piece = i * 32 + lane, r = 16 * warp + piece / kPieces, col = piece % kPieces;
-          const uint4 codes = lds128<0>(stage + half * L::kHalf + r * D + col * 16);
+          const uint4 c16 = lds128<0>(stage + half * L::kHalf + r * D + col * 16);
           uint32_t byte = 127;
-          if (pos0 + r < c.span.len) byte = *(smem + (stage - ring) + 2 * L::kHalf + half * kChunk + r);
-          const RowFactors f = row_factors(byte);
-          const uint2 a = row_values(codes.x, f), b = row_values(codes.y, f), d = row_values(codes.z, f), e = row_values(codes.w, f);
+          if (pos0 + r < c.span.len) byte = lds8(stage + 2 * L::kHalf + half * kChunk + r);
+          const uint32_t codes[4] = {c16.x, c16.y, c16.z, c16.w};
+          uint32_t v[8];
+          row_values(codes, row_factors(byte), v);
           const uint32_t row = (half ? values : keys) + r * D * 2;
           const uint32_t at0 = row + (((2 * col) ^ (r & 7)) << 4), at1 = row + (((2 * col + 1) ^ (r & 7)) << 4);
-          asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(at0), "r"(a.x), "r"(a.y), "r"(b.x), "r"(b.y) : "memory");
-          asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(at1), "r"(d.x), "r"(d.y), "r"(e.x), "r"(e.y) : "memory");
+          asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(at0), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]) : "memory");
+          asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(at1), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]) : "memory");
         }
       }
       if constexpr (KW == 4) __syncwarp(); else __syncthreads();

@@ -398,30 +398,39 @@ attend_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constan
             constexpr int kPieces = D / 16;
             // rows of values that some rows see and others do not, or none
             const int some = which ? (first_limit + 1 > pos0 ? first_limit + 1 - pos0 : 0) : kBlock, none = which ? seen - pos0 : kBlock;
-#pragma unroll 2
-            for (int i = (warp - 10) * 32 + lane; i < kBlock * kPieces; i += kHelpers * 32) {
+            auto convert = [&](int i, uint32_t byte, bool zero) {
               const int r = i / kPieces, col = i % kPieces;
-              const uint4 codes = lds128<0>(from + i * 16);
-              uint32_t byte = lds8(exps + r);
-              bool odd = false;
-              if (r >= some) {
-                odd = byte == 255 && r < none;
-                if (odd || r >= none) byte = 0x100;     // zeros
+              const uint4 c16 = lds128<0>(from + i * 16);
+              const uint32_t codes[4] = {c16.x, c16.y, c16.z, c16.w};
+              uint32_t v[8];
+              row_values(codes, row_factors(byte), v);
+              if (zero) {
+#pragma unroll
+                for (int n = 0; n < 8; ++n) v[n] = 0;
               }
-              if (__any_sync(0xffffffffu, odd) && !mine) {
-                if (!(ok = wait_count(kWritten, 8, live, 34))) break;
-                if (lane == 0) words[kNanPlace + warp - 10] = 0x7fffffff;
-                if (lane == 0) words[kTags + warp - 10] = live + 1;
-                __syncwarp();
-                mine = true;
-              }
-              if (odd) atomicMin(const_cast<int*>(&words[kNanPlace + warp - 10]), pos0 + r);
-              const RowFactors f = row_factors(byte & 255);
-              uint2 v[4] = {row_values(codes.x, f), row_values(codes.y, f), row_values(codes.z, f), row_values(codes.w, f)};
-              if (byte == 0x100) v[0] = v[1] = v[2] = v[3] = make_uint2(0, 0);
               const uint32_t line = to + (col >> 2) * 16384 + r * 128, piece = 2 * col & 7;
-              asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(line + ((piece ^ (r & 7)) << 4)), "r"(v[0].x), "r"(v[0].y), "r"(v[1].x), "r"(v[1].y) : "memory");
-              asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(line + (((piece + 1) ^ (r & 7)) << 4)), "r"(v[2].x), "r"(v[2].y), "r"(v[3].x), "r"(v[3].y) : "memory");
+              asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(line + ((piece ^ (r & 7)) << 4)), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]) : "memory");
+              asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(line + (((piece + 1) ^ (r & 7)) << 4)), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]) : "memory");
+            };
+            const int mine0 = (warp - 10) * 32 + lane;
+            if (some >= kBlock && none >= kBlock) {
+#pragma unroll 3
+              for (int i = mine0; i < kBlock * kPieces; i += kHelpers * 32) convert(i, lds8(exps + i / kPieces), false);
+            } else {
+              for (int i = mine0; i < kBlock * kPieces; i += kHelpers * 32) {
+                const int r = i / kPieces;
+                const uint32_t byte = lds8(exps + r);
+                const bool odd = r >= some && r < none && byte == 255;
+                if (__any_sync(0xffffffffu, odd) && !mine) {
+                  if (!(ok = wait_count(kWritten, 8, live, 34))) break;
+                  if (lane == 0) words[kNanPlace + warp - 10] = 0x7fffffff;
+                  if (lane == 0) words[kTags + warp - 10] = live + 1;
+                  __syncwarp();
+                  mine = true;
+                }
+                if (odd) atomicMin(const_cast<int*>(&words[kNanPlace + warp - 10]), pos0 + r);
+                convert(i, byte, odd || r >= none);
+              }
             }
             fence_proxy_async();
             __syncwarp();

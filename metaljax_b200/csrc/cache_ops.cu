@@ -250,18 +250,18 @@ __global__ void __launch_bounds__(kThreads) read_kernel(const ReadParams p) {
         for (int which = 0; which < 2; ++which) {
           uint4* const out = reinterpret_cast<uint4*>(which ? p.v_out : p.k_out) + to;
           if constexpr (E4M3) {
-            const RowFactors f = row_factors(byte[which][b]);
             const uint32_t codes[4] = {w[which][b].x, w[which][b].y, w[which][b].z, w[which][b].w};
+            uint32_t v[8];
+            row_values(codes, row_factors(byte[which][b]), v);
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
-              const uint2 lo = row_values(codes[2 * i], f), hi = row_values(codes[2 * i + 1], f);
-              uint4 v = make_uint4(lo.x, lo.y, hi.x, hi.y);
+              uint4 x = make_uint4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
               if constexpr (!std::is_same<T, __nv_bfloat16>::value) {
                 float e[8];
-                unpack8<__nv_bfloat16>(v, e);
-                v = pack8<T>(e);
+                unpack8<__nv_bfloat16>(x, e);
+                x = pack8<T>(e);
               }
-              out[i] = v;
+              out[i] = x;
             }
           } else {
             *out = w[which][b];

@@ -87,17 +87,18 @@ __device__ __forceinline__ uint32_t mul_bf16x2(uint32_t a, uint32_t b) {
   return *reinterpret_cast<const uint32_t*>(&r);
 }
 
-// Four codes -> four bf16 (two words).
-__device__ __forceinline__ uint2 row_values(uint32_t codes, const RowFactors& f) {
-  const uint32_t x = __byte_perm(codes, 0, 0x1404), y = __byte_perm(codes, 0, 0x3424);     // a code in the upper byte of each half
-  uint32_t a = ((x >> 4) & 0x07f007f0u) | (x & 0x80008000u), b = ((y >> 4) & 0x07f007f0u) | (y & 0x80008000u);
-  a = mul_bf16x2(a, f.first);
-  b = mul_bf16x2(b, f.first);
-  if (f.second != 0x3f803f80u) {
-    a = mul_bf16x2(a, f.second);
-    b = mul_bf16x2(b, f.second);
+// Sixteen codes -> sixteen bf16. Of a byte s eeee mmm the upper byte of the bf16 is s0000eee and the lower one emmm0000, made for four codes at a time.
+__device__ __forceinline__ void row_values(const uint32_t (&codes)[4], const RowFactors& f, uint32_t (&out)[8]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t w = codes[i], upper = ((w & 0x80808080u) | ((w >> 4) & 0x7f7f7f7fu)) & 0x87878787u, lower = (w << 4) & 0xf0f0f0f0u;
+    out[2 * i] = mul_bf16x2(__byte_perm(upper, lower, 0x1504), f.first);
+    out[2 * i + 1] = mul_bf16x2(__byte_perm(upper, lower, 0x3726), f.first);
   }
-  return make_uint2(a, b);
+  if (f.second != 0x3f803f80u) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) out[i] = mul_bf16x2(out[i], f.second);
+  }
 }
 
 // ... without the power of two: code I of two words, as bf16 (2^120 brings the exponent there; subnormal codes among them), and as f16, which holds a code as it is.
