@@ -68,9 +68,46 @@ __device__ __forceinline__ uint4 pack8(const float (&f)[8]) {
   return make_uint4(pack2<T>(f[0], f[1]), pack2<T>(f[2], f[3]), pack2<T>(f[4], f[5]), pack2<T>(f[6], f[7]));
 }
 
-// T: type of the projection's rows; E4M3: the cache holds codes, else values of T.
+// Pairs of floats in one instruction.
+__device__ __forceinline__ uint64_t pair_of(float a, float b) {
+  uint64_t v;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(a), "f"(b));
+  return v;
+}
+__device__ __forceinline__ float2 floats_of(uint64_t v) {
+  float2 f;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(f.x), "=f"(f.y) : "l"(v));
+  return f;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+template <typename T>
+__device__ __forceinline__ void pairs_of(const uint4& w, uint64_t (&f)[4]) {
+  const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 v = unpack2<T>(u[i]);
+    f[i] = pair_of(v.x, v.y);
+  }
+}
+__device__ __forceinline__ float max_nan(float a, float b) {            // NaN if one is
+  float d;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+  return d;
+}
+
+// T: type of the projection's rows; E4M3: the cache holds codes, else values of T. Queries, keys and values are a pass each: what an element and its pair's other
+// one are multiplied with (norm's weight times cosine, and sine) stays in registers for all heads, and the root mean square comes last.
 template <typename T, int D, bool E4M3>
-__global__ void __launch_bounds__(kThreads) append_kernel(const AppendParams p) {
+__global__ void __launch_bounds__(kThreads, 3) append_kernel(const AppendParams p) {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");
   constexpr int kLanes = D / 8, kRows = 32 / kLanes;   // lanes of a head's row; rows of a warp
@@ -79,17 +116,8 @@ __global__ void __launch_bounds__(kThreads) append_kernel(const AppendParams p) 
   const int warp = threadIdx.x >> 5, lane32 = threadIdx.x & 31, lane = lane32 % kLanes, slot = lane32 / kLanes;
   const int id = blockIdx.x * kWarps + warp, token = id / p.token_warps, part = id - token * p.token_warps;
   if (token >= p.tokens) return;
-  const int all = p.heads + 2 * p.c.kv_heads, stride = p.token_warps * kRows;
-  const uint4* const rows = reinterpret_cast<const uint4*>(p.qkv) + token * p.row_stride / 8 + lane;
-  uint4 x[kBatch];
-  auto fetch = [&](int head0) {
-#pragma unroll
-    for (int b = 0; b < kBatch; ++b) {
-      const int head = head0 + b * stride;
-      x[b] = head < all ? __ldg(rows + static_cast<int64_t>(head) * kLanes) : make_uint4(0, 0, 0, 0);
-    }
-  };
-  fetch(part * kRows + slot);
+  const int stride = p.token_warps * kRows;
+  const uint4* const rows = reinterpret_cast<const uint4*>(p.qkv) + token * p.row_stride / 8;
   int seq = token, end = 0, pos;
   if (p.cu_q) {
     seq = warp_sequence_of(p.cu_q, p.seqs, token, &end);
@@ -110,90 +138,130 @@ __global__ void __launch_bounds__(kThreads) append_kernel(const AppendParams p) 
   __syncwarp();
   const int pairs = p.rotary_dim / 16;                 // lanes of the first elements of split pairs
   const bool first = lane < pairs, turned = lane < 2 * pairs;
-  const int partner = first ? lane + pairs : lane - pairs;
-  float2 t[8];                                          // this lane's angles: of eight split pairs, or of four neighbouring ones
+  const int partner = p.interleaved || !turned ? lane : first ? lane + pairs : lane - pairs;
+
+  auto pass = [&](auto kind_of, int begin, int count, const uint8_t* weight) {
+    constexpr int kKind = decltype(kind_of)::value;      // 0 queries, 1 keys, 2 values
+    const bool turns_on = kKind != 2 && pairs > 0, scaled = kKind != 2 && weight != nullptr;
+    uint64_t own[4], across[4];                           // factors of an element and of its pair's other one
+    if (kKind != 2) {
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const int at = p.interleaved ? lane * 4 + (i & 3) : (first ? lane : partner) * 8 + i;
-    t[i] = turned ? turns[warp][at] : make_float2(0.0f, 1.0f);
-    if (!p.interleaved && first) t[i].x = -t[i].x;      // the first of a pair takes the sine with the other sign
-  }
-  for (int head0 = part * kRows + slot; __any_sync(0xffffffffu, head0 < all); head0 += kBatch * stride) {
-    uint4 now[kBatch];
+      for (int i = 0; i < 4; ++i) own[i] = across[i] = pair_of(1.0f, 1.0f);
+      if (scaled) {
+        pairs_of<T>(__ldg(reinterpret_cast<const uint4*>(weight) + lane), own);
+        pairs_of<T>(__ldg(reinterpret_cast<const uint4*>(weight) + partner), across);
+      }
+      if (turned) {
 #pragma unroll
-    for (int b = 0; b < kBatch; ++b) now[b] = x[b];
-    fetch(head0 + kBatch * stride);
-#pragma unroll
-    for (int b = 0; b < kBatch; ++b) {
-      const int head = head0 + b * stride;
-      if (!__any_sync(0xffffffffu, head < all)) break;
-      const bool live = head < all, is_q = head < p.heads, is_v = head >= p.heads + p.c.kv_heads;
-      float f[8];
-      unpack8<T>(now[b], f);
-      if (__any_sync(0xffffffffu, !is_v)) {
-        const uint8_t* const weight = is_v ? nullptr : is_q ? p.q_norm : p.k_norm;
-        if (p.q_norm || p.k_norm) {
-          float ss = 0.0f;
-#pragma unroll
-          for (int i = 0; i < 8; ++i) ss = fmaf(f[i], f[i], ss);
-#pragma unroll
-          for (int o = kLanes / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-          if (weight) {
-            float w[8];
-            unpack8<T>(__ldg(reinterpret_cast<const uint4*>(weight) + lane), w);
-            const float inv = rsqrtf(ss / static_cast<float>(D) + p.eps);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) f[i] = f[i] * inv * w[i];
-          }
-        }
-        if (p.interleaved) {
-          if (turned && !is_v) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const float a = f[2 * i], c = f[2 * i + 1];
-              f[2 * i] = a * t[i].y - c * t[i].x;
-              f[2 * i + 1] = c * t[i].y + a * t[i].x;
-            }
-          }
-        } else if (pairs) {
-          float other[8];
-#pragma unroll
-          for (int i = 0; i < 8; ++i) other[i] = __shfl_sync(0xffffffffu, f[i], turned ? partner : lane, kLanes);
-          if (turned && !is_v) {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) f[i] = fmaf(f[i], t[i].y, other[i] * t[i].x);
+        for (int i = 0; i < 4; ++i) {
+          if (p.interleaved) {
+            const float2 t = turns[warp][lane * 4 + i], v = floats_of(across[i]);
+            across[i] = pair_of(-t.x * v.y, t.x * v.x);
+            own[i] = mul2(own[i], pair_of(t.y, t.y));
+          } else {
+            const float2 a = turns[warp][(first ? lane : partner) * 8 + 2 * i], b = turns[warp][(first ? lane : partner) * 8 + 2 * i + 1];
+            across[i] = mul2(across[i], first ? pair_of(-a.x, -b.x) : pair_of(a.x, b.x));
+            own[i] = mul2(own[i], pair_of(a.y, b.y));
           }
         }
       }
-      const int64_t at = ((page * p.c.kv_heads + (head - p.heads - (is_v ? p.c.kv_heads : 0))) << p.c.page_shift) + row;     // (of keys and values)
-      if constexpr (E4M3) {
-        float big = 0.0f;
-        bool fine = true;
+    }
+    for (int head0 = part * kRows + slot; __any_sync(0xffffffffu, head0 < count); head0 += kBatch * stride) {
+      uint4 x[kBatch];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          big = fmaxf(big, fabsf(f[i]));
-          fine = fine && fabsf(f[i]) <= 3.402823466e38f;
+      for (int b = 0; b < kBatch; ++b) {
+        const int head = head0 + b * stride;
+        x[b] = head < count ? __ldg(rows + static_cast<int64_t>(begin + head) * kLanes + lane) : make_uint4(0, 0, 0, 0);
+      }
+#pragma unroll
+      for (int b = 0; b < kBatch; ++b) {
+        const int head = head0 + b * stride;
+        if (!__any_sync(0xffffffffu, head < count)) break;
+        uint4 out = x[b];
+        uint64_t f[4];
+        if (kKind != 2 || E4M3) {
+          pairs_of<T>(x[b], f);
+          uint64_t inv2 = pair_of(1.0f, 1.0f);
+          if (scaled) {
+            uint64_t ss2 = 0;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) ss2 = fma2(f[i], f[i], ss2);
+            const float2 two = floats_of(ss2);
+            float ss = two.x + two.y;
+#pragma unroll
+            for (int o = kLanes / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+            const float inv = rsqrtf(ss / static_cast<float>(D) + p.eps);
+            inv2 = pair_of(inv, inv);
+          }
+          if (turns_on) {
+            uint64_t g[4];                               // the pairs' other elements
+            if (p.interleaved) {
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                const float2 v = floats_of(f[i]);
+                g[i] = pair_of(v.y, v.x);
+              }
+            } else {
+              const uint4 other = make_uint4(__shfl_sync(0xffffffffu, x[b].x, partner, kLanes), __shfl_sync(0xffffffffu, x[b].y, partner, kLanes),
+                                             __shfl_sync(0xffffffffu, x[b].z, partner, kLanes), __shfl_sync(0xffffffffu, x[b].w, partner, kLanes));
+              pairs_of<T>(other, g);
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const uint64_t y = mul2(f[i], own[i]);
+              f[i] = turned ? fma2(g[i], across[i], y) : y;            // (elements that are not turned: infinities and NaN beside them or not)
+            }
+          } else if (scaled) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) f[i] = mul2(f[i], own[i]);
+          }
+          if (scaled) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) f[i] = mul2(f[i], inv2);
+          }
+          if (!(E4M3 && kKind != 0)) {
+            float2 v[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[i] = floats_of(f[i]);
+            out = make_uint4(pack2<T>(v[0].x, v[0].y), pack2<T>(v[1].x, v[1].y), pack2<T>(v[2].x, v[2].y), pack2<T>(v[3].x, v[3].y));
+          }
         }
-        if (!fine) big = INFINITY;
+        if (kKind == 0) {
+          if (head < count) reinterpret_cast<uint4*>(p.q_out)[(static_cast<int64_t>(token) * p.heads + head) * kLanes + lane] = out;
+          continue;
+        }
+        const int64_t at = ((page * p.c.kv_heads + head) << p.c.page_shift) + row;
+        if constexpr (E4M3) {
+          float big = 0.0f;
 #pragma unroll
-        for (int o = kLanes / 2; o > 0; o >>= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, o));
-        fine = big <= 3.402823466e38f;
-        if (live && !is_q && page >= 0) {
+          for (int i = 0; i < 4; ++i) {
+            const float2 v = floats_of(f[i]);
+            big = max_nan(big, max_nan(fabsf(v.x), fabsf(v.y)));
+          }
+#pragma unroll
+          for (int o = kLanes / 2; o > 0; o >>= 1) big = max_nan(big, __shfl_xor_sync(0xffffffffu, big, o));
+          const bool fine = big <= 3.402823466e38f;
           const int e = fine ? row_exponent(big) : 0;
           const float down = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);      // 2^-e: a normal number, and the product is exact
           uint32_t u[4];
 #pragma unroll
-          for (int i = 0; i < 4; ++i) u[i] = fine ? e4m3_pair(f[2 * i] * down, f[2 * i + 1] * down) : 0;
-          reinterpret_cast<uint2*>(is_v ? p.c.v : p.c.k)[at * kLanes + lane] = make_uint2(u[0] | u[1] << 16, u[2] | u[3] << 16);
-          if (lane == 0) (is_v ? p.c.v_exp : p.c.k_exp)[at] = static_cast<uint8_t>(fine ? e + 127 : 255);
+          for (int i = 0; i < 4; ++i) {
+            const float2 v = floats_of(mul2(f[i], pair_of(down, down)));
+            u[i] = fine ? e4m3_pair(v.x, v.y) : 0;
+          }
+          if (head < count && page >= 0) {
+            reinterpret_cast<uint2*>(kKind == 2 ? p.c.v : p.c.k)[at * kLanes + lane] = make_uint2(u[0] | u[1] << 16, u[2] | u[3] << 16);
+            if (lane == 0) (kKind == 2 ? p.c.v_exp : p.c.k_exp)[at] = static_cast<uint8_t>(fine ? e + 127 : 255);
+          }
+        } else if (head < count && page >= 0) {
+          reinterpret_cast<uint4*>(kKind == 2 ? p.c.v : p.c.k)[at * kLanes + lane] = out;
         }
-        if (live && is_q) reinterpret_cast<uint4*>(p.q_out)[(static_cast<int64_t>(token) * p.heads + head) * kLanes + lane] = pack8<T>(f);
-      } else if (live) {
-        if (is_q) reinterpret_cast<uint4*>(p.q_out)[(static_cast<int64_t>(token) * p.heads + head) * kLanes + lane] = pack8<T>(f);
-        else if (page >= 0) reinterpret_cast<uint4*>(is_v ? p.c.v : p.c.k)[at * kLanes + lane] = pack8<T>(f);
       }
     }
-  }
+  };
+  pass(std::integral_constant<int, 0>{}, 0, p.heads, p.q_norm);
+  pass(std::integral_constant<int, 1>{}, p.heads, p.c.kv_heads, p.k_norm);
+  pass(std::integral_constant<int, 2>{}, p.heads + p.c.kv_heads, p.c.kv_heads, nullptr);
 }
 
 struct ReadParams {
