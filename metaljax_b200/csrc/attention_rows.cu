@@ -21,7 +21,7 @@
 #include <type_traits>
 
 #include "attention.h"
-#include "qmm_ptx.cuh"
+#include "qmm_tcgen05.cuh"
 
 namespace qmm {
 namespace {
@@ -55,6 +55,11 @@ __device__ __forceinline__ uint32_t lds16(uint32_t addr) {
   asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(addr));
   return v;
 }
+__device__ __forceinline__ float remote_ld32(uint32_t addr) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+  return v;
+}
 __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -86,7 +91,10 @@ struct RowsLayout {
   static constexpr int kBytes = kRing + kValues + kSpecials + kStats + 64;
 };
 
-template <typename T, int D, int RW, int SOURCE>
+// CTAS > 1: a cluster of CTAS for every sequence and key head (one new token each), which leave their parts in shared memory and join a share of the rows each.
+template <int D>
+constexpr int part_bytes() { return 16 * D * 4 + 2 * 16 * 4; }           // behind RowsLayout: 16 rows' sums, then their maxima and their sums of weights
+template <typename T, int D, int RW, int SOURCE, int CTAS>
 __global__ void __launch_bounds__(kThreads, (RowsLayout<D, SOURCE, RW>::kCtas)) attend_rows_kernel(const RowsParams p) {
   using L = RowsLayout<D, SOURCE, RW>;
   constexpr bool kPaged = SOURCE != kRowsSource, kE4m3 = L::kE4m3;
@@ -98,6 +106,9 @@ __global__ void __launch_bounds__(kThreads, (RowsLayout<D, SOURCE, RW>::kCtas)) 
   int* const special = reinterpret_cast<int*>(smem + L::kRing + L::kValues);           // first positions of +inf, -inf, NaN in each column of v
   int* const any_special = special + 3 * D;
   float* const stats = reinterpret_cast<float*>(smem + L::kRing + L::kValues + L::kSpecials);
+  constexpr bool kCluster = CTAS > 1;
+  static_assert(!kCluster || RW == 1, "a part has 16 rows");
+  [[maybe_unused]] float* const own_part = reinterpret_cast<float*>(smem + L::kBytes);
   const uint32_t ring = smem_u32(smem);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int rw = warp / KW, kw = warp % KW;
@@ -105,13 +116,26 @@ __global__ void __launch_bounds__(kThreads, (RowsLayout<D, SOURCE, RW>::kCtas)) 
 
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  if (tid == 0) p.notes[blockIdx.x].parts = 0;
-  // every warp works out where this CTA begins by itself
   UnitCursor c;
-  int64_t share;
-  if (!find_share<Tiles>(w, blockIdx.x, gridDim.x, p.least, &c, &share)) return;
+  [[maybe_unused]] int64_t share = 0;
+  if constexpr (kCluster) {
+    const int item = blockIdx.x / CTAS, rank = blockIdx.x % CTAS;
+    c.s = item / w.kv_heads;
+    c.h = item - c.s * w.kv_heads;
+    c.t = 0;
+    c.span = span_of(w, c.s);
+    c.units = Tiles::units(w, c.span, 0);
+    const int per = (c.units + CTAS - 1) / CTAS;
+    c.u = rank * per < c.units ? rank * per : c.units;
+    c.end = c.u + per < c.units ? c.u + per : c.units;
+    c.room = 0;                                         // (no next item)
+  } else {
+    if (tid == 0) p.notes[blockIdx.x].parts = 0;
+    // every warp works out where this CTA begins by itself
+    if (!find_share<Tiles>(w, blockIdx.x, gridDim.x, p.least, &c, &share)) return;
+  }
   UnitCursor load = c;                                  // where the copies are
-  bool loading = true;
+  bool loading = c.u < c.end;
 
   // ---- copies: a warp asks for rows 16 * warp .. of a chunk (which lie in one page) ----
   int pages = 0, pages_at = 0;                          // lane i: the page of this warp's rows of chunk pages_at + i
@@ -254,7 +278,7 @@ __global__ void __launch_bounds__(kThreads, (RowsLayout<D, SOURCE, RW>::kCtas)) 
   for (int i = tid; i < 3 * D; i += kThreads) special[i] = INT_MAX;
   __syncthreads();
 
-  for (int done = 0;; ++done) {
+  for (int done = 0; !kCluster || c.u < c.end; ++done) {
     asm volatile("cp.async.wait_group %0;" ::"n"(L::kStages - 2) : "memory");
     if constexpr (KW == 4) __syncwarp(); else __syncthreads();
     request(done + L::kStages - 1);
@@ -570,7 +594,13 @@ __global__ void __launch_bounds__(kThreads, (RowsLayout<D, SOURCE, RW>::kCtas)) 
             if (special[2 * D + d + e] <= seen) v[e] = NAN;
           }
         }
-        if (first && last) {
+        if constexpr (kCluster) {
+          *reinterpret_cast<float4*>(own_part + r * D + d) = make_float4(v[0], v[1], v[2], v[3]);
+          if (d == 0) {
+            own_part[16 * D + r] = mm;
+            own_part[16 * D + 16 + r] = ll;
+          }
+        } else if (first && last) {
           // no weight at all: a row that sees nothing is zero; one that sees only scores of -inf has no softmax
           const float inv = ll == 0.0f ? (seen < 0 ? 0.0f : NAN) : 1.0f / ll;
           uint2 out;
@@ -591,12 +621,50 @@ __global__ void __launch_bounds__(kThreads, (RowsLayout<D, SOURCE, RW>::kCtas)) 
       for (int i = tid; i < 3 * D; i += kThreads) special[i] = INT_MAX;
       if (tid == 0) *any_special = 0;
     }
+    if constexpr (kCluster) break;
     __syncthreads();
     if (c.end < c.units && tid == 0) p.notes[blockIdx.x] = note_of(c, begun, share);
     if (!next_item<Tiles>(w, c)) break;
     begin_item();
   }
   asm volatile("cp.async.wait_all;" ::: "memory");
+  if constexpr (kCluster) {
+    const int rank = blockIdx.x % CTAS;
+    if (begun == c.end)                                   // a CTA without positions: no weight, and zeros
+      for (int i = tid; i < 16 * D + 32; i += kThreads) own_part[i] = i >= 16 * D && i < 16 * D + 16 ? -INFINITY : 0.0f;
+    tc::cluster_barrier();                                // the parts are there
+    constexpr int kVec = D / 4;
+    const int group = w.group;
+    for (int i = tid; i < (group - rank + CTAS - 1) / CTAS * kVec; i += kThreads) {
+      const int r = rank + i / kVec * CTAS, d = i % kVec * 4;
+      float m_of[CTAS], l_of[CTAS], mm = -INFINITY, ll = 0.0f, v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+      float4 x[CTAS];
+#pragma unroll
+      for (int k = 0; k < CTAS; ++k) {
+        const uint32_t at = tc::in_cta(smem_u32(own_part), k);
+        x[k] = tc::remote_ld128(at + (r * D + d) * 4);
+        m_of[k] = remote_ld32(at + (16 * D + r) * 4);
+        l_of[k] = remote_ld32(at + (16 * D + 16 + r) * 4);
+        mm = fmaxf(mm, m_of[k]);
+      }
+      const float base = mm == -INFINITY ? 0.0f : mm;
+#pragma unroll
+      for (int k = 0; k < CTAS; ++k) {
+        const float f = ex2(m_of[k] - base);
+        ll = fmaf(f, l_of[k], ll);
+        v[0] = fmaf(f, x[k].x, v[0]);
+        v[1] = fmaf(f, x[k].y, v[1]);
+        v[2] = fmaf(f, x[k].z, v[2]);
+        v[3] = fmaf(f, x[k].w, v[3]);
+      }
+      const float inv = ll == 0.0f ? (c.span.len < 1 ? 0.0f : NAN) : 1.0f / ll;
+      uint2 out;
+      out.x = pack2<T>(v[0] * inv, v[1] * inv);
+      out.y = pack2<T>(v[2] * inv, v[3] * inv);
+      *reinterpret_cast<uint2*>(p.out + (static_cast<int64_t>(c.span.q0) * w.heads + c.h * group + r) * D * 2 + d * 2) = out;
+    }
+    tc::cluster_barrier();                                // ... and have been read
+  }
 }
 
 // Items whose units fell to several CTAs: block (b, y) joins eight rows of the one that CTA b began and did not finish, a warp each.
@@ -669,11 +737,11 @@ int launch_one(const RowsParams& p, cudaStream_t stream) {
   const int dev = current_device();
   if (dev < 0) return QMM_ERR_DEVICE;
   if (!done[dev]) {
-    const cudaError_t e = cudaFuncSetAttribute(attend_rows_kernel<T, D, RW, SOURCE>, cudaFuncAttributeMaxDynamicSharedMemorySize, RowsLayout<D, SOURCE, RW>::kBytes);
+    const cudaError_t e = cudaFuncSetAttribute(attend_rows_kernel<T, D, RW, SOURCE, 1>, cudaFuncAttributeMaxDynamicSharedMemorySize, RowsLayout<D, SOURCE, RW>::kBytes);
     if (e != cudaSuccess) return fail(QMM_ERR_CUDA, "cudaFuncSetAttribute: %s", cudaGetErrorString(e));
     done[dev] = true;
   }
-  launch_early(attend_rows_kernel<T, D, RW, SOURCE>, ctas, kThreads, RowsLayout<D, SOURCE, RW>::kBytes, stream, p);
+  launch_early(attend_rows_kernel<T, D, RW, SOURCE, 1>, ctas, kThreads, RowsLayout<D, SOURCE, RW>::kBytes, stream, p);
   count_launch();
   if (int rc = check_launch("attend_rows_kernel")) return rc;
   if (ctas < 2) return QMM_OK;
@@ -683,8 +751,48 @@ int launch_one(const RowsParams& p, cudaStream_t stream) {
   return check_launch("attend_join_kernel");
 }
 
+template <typename T, int D, int SOURCE, int CTAS>
+int launch_cluster(const RowsParams& p, int items, cudaStream_t stream) {
+  static bool done[kMaxDevices] = {};
+  const int dev = current_device();
+  if (dev < 0) return QMM_ERR_DEVICE;
+  auto kernel = attend_rows_kernel<T, D, 1, SOURCE, CTAS>;
+  constexpr int kBytes = RowsLayout<D, SOURCE, 1>::kBytes + part_bytes<D>();
+  if (!done[dev]) {
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kBytes);
+    if (e != cudaSuccess) return fail(QMM_ERR_CUDA, "cudaFuncSetAttribute: %s", cudaGetErrorString(e));
+    done[dev] = true;
+  }
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(items * CTAS);
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = kBytes;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = CTAS;
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
+  cudaLaunchKernelEx(&cfg, kernel, p);
+  count_launch();
+  return check_launch("attend_rows_kernel");
+}
+
 template <typename T, int D, int SOURCE>
 int launch_rows_of(const RowsParams& p, int rows, cudaStream_t stream) {
+  // A new token each of a few sequences: a cluster of CTAs for every sequence and key head, one launch, which wants neither the order of all units (2 us) nor a second
+  // launch to join (3.5 us). Eight CTAs where two an SM are enough for all, else four. It pays while the longest sequence that a table has room for is short: without
+  // shares by weight, no more CTAs take part in it (8 key heads of 128, us, bf16 clusters / shares: 1 sequence of 2000 positions 8.5 / 12.3, 8000 14.7 / 16.2, 16000
+  // 19.6 / 19.3; 8 of 4000 11.4 / 15.3; with a second wave 16 of 4000 28.5 / 28.9), and codes, which want three CTAs an SM, sooner not (1 of 2000 10.0 / 13.8, 4000
+  // 14.7 / 16.3, 8000 21.4 / 20.0).
+  const int64_t items = static_cast<int64_t>(p.work.seqs) * p.work.kv_heads, room = 2 * device_sm_count();
+  if (!p.work.cu_q && rows <= 16 && p.work.longest <= (SOURCE == kPages8 ? 4096 : 8192)) {
+    if (items * 8 <= room) return launch_cluster<T, D, SOURCE, 8>(p, static_cast<int>(items), stream);
+    if (items * 4 <= room) return launch_cluster<T, D, SOURCE, 4>(p, static_cast<int>(items), stream);
+  }
   if (rows <= 16) return launch_one<T, D, 1, SOURCE>(p, stream);
   if (rows <= 32) return launch_one<T, D, 2, SOURCE>(p, stream);
   return launch_one<T, D, 4, SOURCE>(p, stream);

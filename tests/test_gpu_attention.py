@@ -104,6 +104,46 @@ def test_one_token_each(dim, dtype, cache, group, kv):
     _check_paged([1] * len(lens), lens, group * kv, kv, dim, 32, dtype, cache, cu=False, seed=group)
 
 
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("dtype, cache", CACHES)
+@pytest.mark.parametrize("group, kv", [(1, 4), (3, 6), (16, 4), (5, 9)])
+@pytest.mark.parametrize("longest", [60, 640, 8193])
+def test_one_token_however_sequences_are_shared(dim, dtype, cache, group, kv, longest):
+    """Clusters of eight CTAs, of four, and shares by weight; CTAs without positions among them."""
+    lens = [longest, 0, 1, 59, 57, 3, 16, 33, longest // 3]
+    _check_paged([1] * len(lens), lens, group * kv, kv, dim, 64, dtype, cache, cu=False, seed=kv)
+
+
+@pytest.mark.parametrize("at", [0, 299, 300, 700])
+def test_infinite_values_and_scores_of_one_token(at):
+    """In a row's sum, on whichever CTA: +inf, NaN, both infinities; keys whose scores are -inf have no weight; none else: no softmax."""
+    gen = _gen(at)
+    lens = [701] * 4
+    cache, table, ks, vs = _paged(lens, 1, 128, 64, BF, gen)
+    page, off = table.long()[:, at // 64], at % 64
+    cache.v[page[0], 0, off, 5] = torch.inf
+    cache.v[page[1], 0, off, 5] = torch.nan
+    cache.v[page[1], 0, off, 6] = torch.inf
+    other = table.long()[1, (700 - at) // 64]
+    cache.v[other, 0, (700 - at) % 64, 6] = -torch.inf
+    cache.k[table[2].long(), :, :, 0] = -torch.inf
+    cache.k[page[2], 0, off, 0] = 0.0
+    cache.k[table[3].long(), :, :, 0] = -torch.inf
+    q = torch.randn((4, 2, 128), generator=gen, device=DEV).to(BF)
+    q[:, :, 0] = 1.0
+    got = attention.paged_attention(q, cache, table, R.lengths(lens, DEV))
+    for s in range(2):
+        want, size = R.attend(q[s: s + 1].double(), ks[s], vs[s], 700, True, 128 ** -0.5)
+        keep = torch.ones(128, dtype=torch.bool, device=DEV)
+        keep[5:7] = False
+        R.close(got[s: s + 1, :, keep], want[..., keep], size[..., keep], BF)
+    assert bool((got[0, :, 5] == torch.inf).all()) and bool(got[1, :, 5].isnan().all())
+    if at != 700 - at:
+        assert bool(got[1, :, 6].isnan().all())
+    assert torch.equal(got[2], vs[2][at].to(BF).expand(2, -1))
+    assert bool(got[3].isnan().all())
+
+
 @pytest.mark.parametrize("page", [16, 32, 64, 128, 256])
 @pytest.mark.parametrize("dtype, cache", CACHES)
 def test_pages_of_every_size(page, dtype, cache):
