@@ -87,17 +87,17 @@ int attend(const char* what, const qmm_paged_cache* cache, const CacheView* view
     p.cache = *view;
     p.work.longest = static_cast<int64_t>(cache->table_width) << view->page_shift;
   }
-  const int64_t rows = (a->cu_q ? a->tokens : 1) * p.work.group;
+  const int64_t rows = a->cu_q ? (a->tokens * p.work.group + a->seqs - 1) / a->seqs : p.work.group;
   const int source = !view ? 0 : cache->elem == QMM_E4M3 ? 2 : 1;
-  // Rows of queries that a sequence and key head have on average: from 32 on the kernel of 2 x 128 rows is no slower (8 sequences of 2000 to 4000 positions: 20
-  // rows 29 against 32 us, 35 rows 24 and 24, 64 rows 36 and 36; of 250 to 500: 18 against 17, 17 and 16, 23 against 17), and from some hundred on several times as fast.
-  const bool tc = a->cu_q && a->tokens * p.work.group > 32 * a->seqs &&
+  // Up to 32 rows of queries that a sequence and key head have on average the stream of mma.sync tiles is no slower, from some hundred on the kernel of 2 x 128 rows
+  // several times as fast (8 sequences of 2000 to 4000 positions: 20 rows 22 against 32 us, 35 rows 24 and 24, 64 rows 36 and 36).
+  const bool tc = a->cu_q && rows > 32 &&
                   (!view || (static_cast<uint64_t>(p.cache.pages) * p.work.kv_heads << p.cache.page_shift) < (1ull << 31));
   p.least = 4;
   const int ctas = tc ? attend_tc_ctas() : attend_rows_ctas();
   p.partial = reinterpret_cast<float*>(p.notes + ctas);
   if (tc) return launch_attend_tc(p, a->elem, a->head_dim, source, ctas, stream);
-  return launch_attend_rows(p, a->elem, a->head_dim, source, rows < 64 ? static_cast<int>(rows) : 64, stream);
+  return launch_attend_rows(p, a->elem, a->head_dim, source, static_cast<int>(rows), stream);
 }
 
 }  // namespace

@@ -800,7 +800,7 @@ int launch_rows_of(const RowsParams& p, int rows, cudaStream_t stream) {
 
 template <typename T, int D>
 int launch_source(const RowsParams& p, int source, int rows, cudaStream_t stream) {
-  if (source == kRowsSource) return launch_one<T, D, 4, kRowsSource>(p, stream);
+  if (source == kRowsSource) return launch_one<T, D, 2, kRowsSource>(p, stream);
   if (source == kPages16) return launch_rows_of<T, D, kPages16>(p, rows, stream);
   if constexpr (std::is_same<T, __nv_bfloat16>::value) return launch_rows_of<T, D, kPages8>(p, rows, stream);
   return fail(QMM_ERR_UNSUPPORTED, "attention: an e4m3 cache is attended with bf16 queries");
