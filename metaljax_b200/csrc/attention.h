@@ -30,6 +30,8 @@ int attend_rows_ctas();             // at most
 int64_t attend_rows_workspace(int head_dim, int ctas);
 // `source`: 0 rows, 1 pages of 16-bit values, 2 pages of e4m3 codes; `rows`: query rows that a sequence and key head have on average, which tiles of 16, 32 or 64 rows are
 // chosen by (more of them are more tiles).
+// CTAs of a cluster that takes a sequence's tiles of a key head, or 0: shares by weight.
+int attend_cluster_ctas(const RowsParams& p, int source, int rows);
 int launch_attend_rows(const RowsParams& p, int elem, int head_dim, int source, int rows, cudaStream_t stream);
 
 // 128-row halves on tcgen05. A cache's rows have to be fewer than 2^31.

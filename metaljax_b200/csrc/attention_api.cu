@@ -91,7 +91,7 @@ int attend(const char* what, const qmm_paged_cache* cache, const CacheView* view
   const int source = !view ? 0 : cache->elem == QMM_E4M3 ? 2 : 1;
   // Up to 32 rows of queries that a sequence and key head have on average the stream of mma.sync tiles is no slower, from some hundred on the kernel of 2 x 128 rows
   // several times as fast (8 sequences of 2000 to 4000 positions: 20 rows 22 against 32 us, 35 rows 24 and 24, 64 rows 36 and 36).
-  const bool tc = a->cu_q && rows > 32 &&
+  const bool tc = a->cu_q && rows > 32 && !attend_cluster_ctas(p, source, rows < 65 ? static_cast<int>(rows) : 65) &&
                   (!view || (static_cast<uint64_t>(p.cache.pages) * p.work.kv_heads << p.cache.page_shift) < (1ull << 31));
   p.least = 4;
   const int ctas = tc ? attend_tc_ctas() : attend_rows_ctas();

@@ -6,10 +6,10 @@
 // One pass: a warp holds 16 rows' queries as A fragments, takes scores of its positions of a chunk, the running maximum m and sum l of
 // 2^(s - m), and adds 2^(s - m) v to its 16 x D sums in registers. RW warps share a tile's rows; the KW = 4 / RW
 // warps on the same rows take 64 / KW positions of a chunk each, and are joined when the item ends. With one row of 16 (RW = 1) a warp reads only what it has asked
-// for itself, and the CTA does not meet but at the ends of items.
+// for itself, and the CTA does not meet but at the ends of items. Pages of bf16 are bound by the memory: the same 64 sequences 206 us, 6.5 TB/s.
 //
 // e4m3 codes: with one row of 16 a warp takes them straight into its B fragments as f16, one conversion a pair (a bf16 takes five
-// instructions a pair, which bound this form: 249 us for 64 sequences of 2000 to 8000 positions, against 197): of keys four codes of a row a step (the queries' elements in the order that makes),
+// instructions a pair, with which 64 sequences of 2000 to 8000 positions took 249 us; now 171, 3.9 TB/s, bound by instructions: 687 for 16 positions): of keys four codes of a row a step (the queries' elements in the order that makes),
 // of values the codes of its four positions, paired by a byte permutation. The queries become f16 under a power of two, the rows' powers of two go to the
 // scores and to the weights. Where warps share positions, the one that asked for a chunk's rows turns them into bf16 (exactly) next to the chunk in
 // shared memory.
@@ -91,9 +91,55 @@ struct RowsLayout {
   static constexpr int kBytes = kRing + kValues + kSpecials + kStats + 64;
 };
 
-// CTAS > 1: a cluster of CTAS for every sequence and key head (one new token each), which leave their parts in shared memory and join a share of the rows each.
-template <int D>
-constexpr int part_bytes() { return 16 * D * 4 + 2 * 16 * 4; }           // behind RowsLayout: 16 rows' sums, then their maxima and their sums of weights
+// Four elements of a row's result. No weight at all: a row that sees nothing is zero; one that sees only scores of -inf has no softmax.
+template <typename T>
+__device__ __forceinline__ void store_row(const RowsParams& p, const UnitCursor& c, int tok, int g, int d, int dim, const float (&v)[4], float l, int seen) {
+  const float inv = l == 0.0f ? (seen < 0 ? 0.0f : NAN) : 1.0f / l;
+  uint2 out;
+  out.x = pack2<T>(v[0] * inv, v[1] * inv);
+  out.y = pack2<T>(v[2] * inv, v[3] * inv);
+  *reinterpret_cast<uint2*>(p.out + (((static_cast<int64_t>(c.span.q0) + tok) * p.work.heads + c.h * p.work.group + g) * dim + d) * 2) = out;
+}
+
+// CTAS = 1: shares by weight, which attend_join_kernel joins. CTAS > 1: clusters of CTAS take whole items (in turn, if there are more than clusters), every CTA an
+// equal run of the units, and join them out of one another's shared memory: the first stages of the ring, and maxima and sums of weights behind everything else.
+template <typename Tiles>
+__device__ __forceinline__ bool cluster_item(const AttentionWork& w, int item, int rank, int ctas, UnitCursor* at) {
+  int n = item / w.kv_heads;                            // tile of all sequences'
+  at->h = item - n * w.kv_heads;
+  if (!w.cu_q) {
+    at->span.n = 1;
+    const int per = Tiles::tiles(w, at->span);
+    at->s = n / per;
+    if (at->s >= w.seqs) return false;
+    at->t = n - at->s * per;
+    at->span = span_of(w, at->s);
+  } else {
+    for (int base = 0;; base += 32) {
+      if (base >= w.seqs) return false;
+      SeqSpan span = {0, 0, 0};
+      if (base + (threadIdx.x & 31) < w.seqs) span = span_of(w, base + (threadIdx.x & 31));
+      const int tiles = Tiles::tiles(w, span);
+      const int64_t upto = warp_scan<int64_t>(tiles);
+      const unsigned past = __ballot_sync(0xffffffffu, upto > n);
+      if (past) {
+        const int l = __ffs(past) - 1;
+        at->s = base + l;
+        at->t = n - static_cast<int>(__shfl_sync(0xffffffffu, upto - tiles, l));
+        at->span = {__shfl_sync(0xffffffffu, span.q0, l), __shfl_sync(0xffffffffu, span.n, l), __shfl_sync(0xffffffffu, span.len, l)};
+        break;
+      }
+      n -= static_cast<int>(__shfl_sync(0xffffffffu, upto, 31));
+    }
+  }
+  at->units = Tiles::units(w, at->span, at->t);
+  const int each = (at->units + ctas - 1) / ctas;
+  at->u = rank * each < at->units ? rank * each : at->units;
+  at->end = at->u + each < at->units ? at->u + each : at->units;
+  at->room = 0;                                         // (no item behind it)
+  return true;
+}
+
 template <typename T, int D, int RW, int SOURCE, int CTAS>
 __global__ void __launch_bounds__(kThreads, (RowsLayout<D, SOURCE, RW>::kCtas)) attend_rows_kernel(const RowsParams p) {
   using L = RowsLayout<D, SOURCE, RW>;
@@ -107,8 +153,10 @@ __global__ void __launch_bounds__(kThreads, (RowsLayout<D, SOURCE, RW>::kCtas)) 
   int* const any_special = special + 3 * D;
   float* const stats = reinterpret_cast<float*>(smem + L::kRing + L::kValues + L::kSpecials);
   constexpr bool kCluster = CTAS > 1;
-  static_assert(!kCluster || RW == 1, "a part has 16 rows");
-  [[maybe_unused]] float* const own_part = reinterpret_cast<float*>(smem + L::kBytes);
+  static_assert(!kCluster || (R * D * 4 <= (kE4m3 && !kDirect ? L::kRing : L::kStage) && 4 * (kDirect ? 8 : 16) * D * 4 <= (kE4m3 && !kDirect ? L::kValues : L::kStage)),
+                "a part, and what it is made of, in the ring");
+  [[maybe_unused]] float* const part_rows = reinterpret_cast<float*>(smem);
+  [[maybe_unused]] float* const part_stats = reinterpret_cast<float*>(smem + L::kBytes);          // R maxima, R sums of weights
   const uint32_t ring = smem_u32(smem);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int rw = warp / KW, kw = warp % KW;
@@ -119,16 +167,7 @@ __global__ void __launch_bounds__(kThreads, (RowsLayout<D, SOURCE, RW>::kCtas)) 
   UnitCursor c;
   [[maybe_unused]] int64_t share = 0;
   if constexpr (kCluster) {
-    const int item = blockIdx.x / CTAS, rank = blockIdx.x % CTAS;
-    c.s = item / w.kv_heads;
-    c.h = item - c.s * w.kv_heads;
-    c.t = 0;
-    c.span = span_of(w, c.s);
-    c.units = Tiles::units(w, c.span, 0);
-    const int per = (c.units + CTAS - 1) / CTAS;
-    c.u = rank * per < c.units ? rank * per : c.units;
-    c.end = c.u + per < c.units ? c.u + per : c.units;
-    c.room = 0;                                         // (no next item)
+    if (!cluster_item<Tiles>(w, blockIdx.x / CTAS, blockIdx.x % CTAS, CTAS, &c)) return;
   } else {
     if (tid == 0) p.notes[blockIdx.x].parts = 0;
     // every warp works out where this CTA begins by itself
@@ -195,8 +234,6 @@ __global__ void __launch_bounds__(kThreads, (RowsLayout<D, SOURCE, RW>::kCtas)) 
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
-
-  look_up();
 
   uint32_t q[D / 16][4];
   float o[D / 8][4];
@@ -271,380 +308,380 @@ __global__ void __launch_bounds__(kThreads, (RowsLayout<D, SOURCE, RW>::kCtas)) 
     }
   };
 
-  begin_item();                                          // (its queries before the stream of keys and values, which they would wait behind)
+  for (int item = blockIdx.x / CTAS;;) {                  // (CTAS = 1: once, with a share's items below)
+    look_up();
+    begin_item();                                          // (its queries before the stream of keys and values, which they would wait behind)
 #pragma unroll
-  for (int i = 0; i < L::kStages - 1; ++i) request(i);
-  if (tid == 0) *any_special = 0;
-  for (int i = tid; i < 3 * D; i += kThreads) special[i] = INT_MAX;
-  __syncthreads();
+    for (int i = 0; i < L::kStages - 1; ++i) request(i);
+    if (tid == 0) *any_special = 0;
+    for (int i = tid; i < 3 * D; i += kThreads) special[i] = INT_MAX;
+    __syncthreads();
 
-  for (int done = 0; !kCluster || c.u < c.end; ++done) {
-    asm volatile("cp.async.wait_group %0;" ::"n"(L::kStages - 2) : "memory");
-    if constexpr (KW == 4) __syncwarp(); else __syncthreads();
-    request(done + L::kStages - 1);
-    const uint32_t stage = ring + (done % L::kStages) * L::kStage;
-    const int pos0 = c.u * kChunk;
-    uint32_t keys = stage, values = stage + L::kHalf;
-    if constexpr (kE4m3 && !kDirect) {
-      // this warp's 16 rows of both as bf16
-      keys = ring + L::kRing;
-      values = keys + kChunk * D * 2;
-      if constexpr (KW != 4) __syncthreads();             // (the last chunk's are read by other warps)
-      constexpr int kPieces = D / 16;
-      static_assert(16 * kPieces % 32 == 0, "whole passes of a warp");
+    for (int done = 0; !kCluster || c.u < c.end; ++done) {
+      asm volatile("cp.async.wait_group %0;" ::"n"(L::kStages - 2) : "memory");
+      if constexpr (KW == 4) __syncwarp(); else __syncthreads();
+      request(done + L::kStages - 1);
+      const uint32_t stage = ring + (done % L::kStages) * L::kStage;
+      const int pos0 = c.u * kChunk;
+      uint32_t keys = stage, values = stage + L::kHalf;
+      if constexpr (kE4m3 && !kDirect) {
+        // this warp's 16 rows of both as bf16
+        keys = ring + L::kRing;
+        values = keys + kChunk * D * 2;
+        if constexpr (KW != 4) __syncthreads();             // (the last chunk's are read by other warps)
+        constexpr int kPieces = D / 16;
+        static_assert(16 * kPieces % 32 == 0, "whole passes of a warp");
 #pragma unroll
-      for (int half = 0; half < 2; ++half) {
+        for (int half = 0; half < 2; ++half) {
 #pragma unroll
+          for (int i = 0; i < 16 * kPieces / 32; ++i) {
+            const int piece = i * 32 + lane, r = 16 * warp + piece / kPieces, col = piece % kPieces;
+            const uint4 c16 = lds128<0>(stage + half * L::kHalf + r * D + col * 16);
+            uint32_t byte = 127;
+            if (pos0 + r < c.span.len) byte = lds8(stage + 2 * L::kHalf + half * kChunk + r);
+            const uint32_t codes[4] = {c16.x, c16.y, c16.z, c16.w};
+            uint32_t v[8];
+            row_values(codes, row_factors(byte), v);
+            const uint32_t row = (half ? values : keys) + r * D * 2;
+            const uint32_t at0 = row + (((2 * col) ^ (r & 7)) << 4), at1 = row + (((2 * col + 1) ^ (r & 7)) << 4);
+            asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(at0), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]) : "memory");
+            asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(at1), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]) : "memory");
+          }
+        }
+        if constexpr (KW == 4) __syncwarp(); else __syncthreads();
+      }
+      // a chunk with positions that are this sequence's, but not every row's (codes by themselves are always numbers)
+      if (!kDirect && pos0 + kChunk - 1 > tile_first_limit && tile_first_limit < c.span.len - 1) {
+        constexpr int kPieces = D / 8;
         for (int i = 0; i < 16 * kPieces / 32; ++i) {
           const int piece = i * 32 + lane, r = 16 * warp + piece / kPieces, col = piece % kPieces;
-          const uint4 c16 = lds128<0>(stage + half * L::kHalf + r * D + col * 16);
-          uint32_t byte = 127;
-          if (pos0 + r < c.span.len) byte = lds8(stage + 2 * L::kHalf + half * kChunk + r);
-          const uint32_t codes[4] = {c16.x, c16.y, c16.z, c16.w};
-          uint32_t v[8];
-          row_values(codes, row_factors(byte), v);
-          const uint32_t row = (half ? values : keys) + r * D * 2;
-          const uint32_t at0 = row + (((2 * col) ^ (r & 7)) << 4), at1 = row + (((2 * col + 1) ^ (r & 7)) << 4);
-          asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(at0), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]) : "memory");
-          asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(at1), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]) : "memory");
+          const uint32_t at = values + r * D * 2 + ((col ^ (r & 7)) << 4);
+          const uint4 v = lds128<0>(at);
+          if (odd_pair<T>(v.x) || odd_pair<T>(v.y) || odd_pair<T>(v.z) || odd_pair<T>(v.w)) {
+            uint32_t u[4] = {v.x, v.y, v.z, v.w};
+            for (int e = 0; e < 8; ++e) {
+              const float2 pair = unpack2<T>(u[e >> 1]);
+              const float x = e & 1 ? pair.y : pair.x;
+              if (!(fabsf(x) <= 3.402823466e38f)) {
+                atomicMin(special + (x > 0.0f ? 0 : x < 0.0f ? D : 2 * D) + col * 8 + e, pos0 + r);
+                *any_special = 1;
+                u[e >> 1] &= e & 1 ? 0x0000ffffu : 0xffff0000u;
+              }
+            }
+            asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(u[0]), "r"(u[1]), "r"(u[2]), "r"(u[3]) : "memory");
+          }
         }
+        if constexpr (KW == 4) __syncwarp(); else __syncthreads();
       }
-      if constexpr (KW == 4) __syncwarp(); else __syncthreads();
-    }
-    // a chunk with positions that are this sequence's, but not every row's (codes by themselves are always numbers)
-    if (!kDirect && pos0 + kChunk - 1 > tile_first_limit && tile_first_limit < c.span.len - 1) {
-      constexpr int kPieces = D / 8;
-      for (int i = 0; i < 16 * kPieces / 32; ++i) {
-        const int piece = i * 32 + lane, r = 16 * warp + piece / kPieces, col = piece % kPieces;
-        const uint32_t at = values + r * D * 2 + ((col ^ (r & 7)) << 4);
-        const uint4 v = lds128<0>(at);
-        if (odd_pair<T>(v.x) || odd_pair<T>(v.y) || odd_pair<T>(v.z) || odd_pair<T>(v.w)) {
-          uint32_t u[4] = {v.x, v.y, v.z, v.w};
-          for (int e = 0; e < 8; ++e) {
-            const float2 pair = unpack2<T>(u[e >> 1]);
-            const float x = e & 1 ? pair.y : pair.x;
-            if (!(fabsf(x) <= 3.402823466e38f)) {
-              atomicMin(special + (x > 0.0f ? 0 : x < 0.0f ? D : 2 * D) + col * 8 + e, pos0 + r);
-              *any_special = 1;
-              u[e >> 1] &= e & 1 ? 0x0000ffffu : 0xffff0000u;
+      // ---- scores of this warp's positions ----
+      float s[SN / 8][4];
+#pragma unroll
+      for (int n = 0; n < SN / 8; ++n)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s[n][i] = 0.0f;
+      float k_scale[SN / 8][2], v_scale[SN / 8][2];         // (codes: of the thread's columns; positions behind the end: 1)
+      [[maybe_unused]] bool wide = false;
+      [[maybe_unused]] float s2[SN / 8][4] = {};            // (two chains of products)
+      if constexpr (kDirect) {
+        // The weights of the values are f16 too: p * 2^(e - v_top + 6), e a row's exponent. Rows more than 2^12 below the largest would lose bits where that one's
+        // weight is small: then these positions' products are taken in bf16 (`wide`).
+        const uint32_t bytes = stage + 2 * L::kHalf + kw * SN;
+        const bool there = lane < SN && kw * SN + lane < c.span.len - pos0;
+        const int k_byte = there ? static_cast<int>(lds8(bytes + lane)) : 127, v_byte = there ? static_cast<int>(lds8(bytes + kChunk + lane)) : 255;
+        const int high = __reduce_max_sync(0xffffffffu, v_byte == 255 ? -1000 : v_byte - 127), low = __reduce_min_sync(0xffffffffu, v_byte == 255 ? 1000 : v_byte - 127);
+        if (high > v_top) {
+          if (v_top > -1000) {
+            const float down = high - v_top > 126 ? 0.0f : __uint_as_float(static_cast<uint32_t>(127 + v_top - high) << 23);
+#pragma unroll
+            for (int n = 0; n < D / 8; ++n)
+#pragma unroll
+              for (int i = 0; i < 4; ++i) o[n][i] *= down;
+          }
+          v_top = high;
+          // 2^(6 - v_top), in two steps that are both in range
+          const int near = v_top > 64 ? 64 : v_top < -64 ? -64 : v_top;
+          v_unit = __uint_as_float(static_cast<uint32_t>(127 + 6 - near) << 23);
+          v_rest = __uint_as_float(static_cast<uint32_t>(127 + near - (v_top < -127 ? -127 : v_top)) << 23);
+        }
+        wide = v_top - low > 12;
+        // ordinary rows: all there, and numbers
+        const bool plain = __all_sync(0xffffffffu, lane >= SN || (there && k_byte != 255 && k_byte != 0 && v_byte != 255 && v_byte != 0));
+#pragma unroll
+        for (int n = 0; n < SN / 8; ++n) {
+          const uint32_t k2 = lds16(bytes + n * 8 + (lane & 3) * 2), v2 = lds16(bytes + kChunk + n * 8 + (lane & 3) * 2);
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const uint32_t kb = e ? k2 >> 8 : k2 & 255, vb = e ? v2 >> 8 : v2 & 255;
+            if (plain) {
+              k_scale[n][e] = __uint_as_float(kb << 23) * q_scale;
+              v_scale[n][e] = __uint_as_float(vb << 23) * v_unit * v_rest;
+            } else {
+              const bool in = kw * SN + n * 8 + (lane & 3) * 2 + e < c.span.len - pos0;
+              k_scale[n][e] = (in ? row_scale(kb) : 1.0f) * q_scale;
+              v_scale[n][e] = (in ? row_scale(vb) : 0.0f) * v_unit * v_rest;
             }
           }
-          asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(u[0]), "r"(u[1]), "r"(u[2]), "r"(u[3]) : "memory");
-        }
-      }
-      if constexpr (KW == 4) __syncwarp(); else __syncthreads();
-    }
-    // ---- scores of this warp's positions ----
-    float s[SN / 8][4];
+          const int r = kw * SN + n * 8 + (lane >> 2);
 #pragma unroll
-    for (int n = 0; n < SN / 8; ++n)
+          for (int h = 0; h < D / 64; ++h) {
+            const int piece = h * 4 + (lane & 3);
+            const uint4 codes = lds128<0>(keys + r * D + ((D == 128 ? piece ^ ((r & 1) << 2) : piece) << 4));
+            const uint32_t word[4] = {codes.x, codes.y, codes.z, codes.w};
 #pragma unroll
-      for (int i = 0; i < 4; ++i) s[n][i] = 0.0f;
-    float k_scale[SN / 8][2], v_scale[SN / 8][2];         // (codes: of the thread's columns; positions behind the end: 1)
-    [[maybe_unused]] bool wide = false;
-    [[maybe_unused]] float s2[SN / 8][4] = {};            // (two chains of products)
-    if constexpr (kDirect) {
-      // The weights of the values are f16 too: p * 2^(e - v_top + 6), e a row's exponent. Rows more than 2^12 below the largest would lose bits where that one's
-      // weight is small: then these positions' products are taken in bf16 (`wide`).
-      const uint32_t bytes = stage + 2 * L::kHalf + kw * SN;
-      const bool there = lane < SN && kw * SN + lane < c.span.len - pos0;
-      const int k_byte = there ? static_cast<int>(lds8(bytes + lane)) : 127, v_byte = there ? static_cast<int>(lds8(bytes + kChunk + lane)) : 255;
-      const int high = __reduce_max_sync(0xffffffffu, v_byte == 255 ? -1000 : v_byte - 127), low = __reduce_min_sync(0xffffffffu, v_byte == 255 ? 1000 : v_byte - 127);
-      if (high > v_top) {
-        if (v_top > -1000) {
-          const float down = high - v_top > 126 ? 0.0f : __uint_as_float(static_cast<uint32_t>(127 + v_top - high) << 23);
+            for (int i = 0; i < 4; ++i) mma16816<MT>(h == 0 ? s[n] : s2[n], q[h * 4 + i], code_half2(word[i]), code_half2(word[i] >> 16));
+          }
+          if constexpr (D == 128) {
 #pragma unroll
-          for (int n = 0; n < D / 8; ++n)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) o[n][i] *= down;
-        }
-        v_top = high;
-        // 2^(6 - v_top), in two steps that are both in range
-        const int near = v_top > 64 ? 64 : v_top < -64 ? -64 : v_top;
-        v_unit = __uint_as_float(static_cast<uint32_t>(127 + 6 - near) << 23);
-        v_rest = __uint_as_float(static_cast<uint32_t>(127 + near - (v_top < -127 ? -127 : v_top)) << 23);
-      }
-      wide = v_top - low > 12;
-      // ordinary rows: all there, and numbers
-      const bool plain = __all_sync(0xffffffffu, lane >= SN || (there && k_byte != 255 && k_byte != 0 && v_byte != 255 && v_byte != 0));
-#pragma unroll
-      for (int n = 0; n < SN / 8; ++n) {
-        const uint32_t k2 = lds16(bytes + n * 8 + (lane & 3) * 2), v2 = lds16(bytes + kChunk + n * 8 + (lane & 3) * 2);
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const uint32_t kb = e ? k2 >> 8 : k2 & 255, vb = e ? v2 >> 8 : v2 & 255;
-          if (plain) {
-            k_scale[n][e] = __uint_as_float(kb << 23) * q_scale;
-            v_scale[n][e] = __uint_as_float(vb << 23) * v_unit * v_rest;
-          } else {
-            const bool in = kw * SN + n * 8 + (lane & 3) * 2 + e < c.span.len - pos0;
-            k_scale[n][e] = (in ? row_scale(kb) : 1.0f) * q_scale;
-            v_scale[n][e] = (in ? row_scale(vb) : 0.0f) * v_unit * v_rest;
+            for (int i = 0; i < 4; ++i) s[n][i] += s2[n][i];
           }
         }
-        const int r = kw * SN + n * 8 + (lane >> 2);
+      } else
 #pragma unroll
-        for (int h = 0; h < D / 64; ++h) {
-          const int piece = h * 4 + (lane & 3);
-          const uint4 codes = lds128<0>(keys + r * D + ((D == 128 ? piece ^ ((r & 1) << 2) : piece) << 4));
-          const uint32_t word[4] = {codes.x, codes.y, codes.z, codes.w};
+      for (int n = 0; n < SN / 16; ++n) {
+        const int r = kw * SN + n * 16 + (lane & 7) + ((lane >> 4) << 3);
 #pragma unroll
-          for (int i = 0; i < 4; ++i) mma16816<MT>(h == 0 ? s[n] : s2[n], q[h * 4 + i], code_half2(word[i]), code_half2(word[i] >> 16));
-        }
-        if constexpr (D == 128) {
-#pragma unroll
-          for (int i = 0; i < 4; ++i) s[n][i] += s2[n][i];
+        for (int kk = 0; kk < D / 16; ++kk) {
+          uint32_t b[4];
+          ldmatrix4(b, keys + r * D * 2 + (((kk * 2 + ((lane >> 3) & 1)) ^ (r & 7)) << 4));
+          mma16816<MT>(s[2 * n], q[kk], b[0], b[1]);
+          mma16816<MT>(s[2 * n + 1], q[kk], b[2], b[3]);
         }
       }
-    } else
-#pragma unroll
-    for (int n = 0; n < SN / 16; ++n) {
-      const int r = kw * SN + n * 16 + (lane & 7) + ((lane >> 4) << 3);
-#pragma unroll
-      for (int kk = 0; kk < D / 16; ++kk) {
-        uint32_t b[4];
-        ldmatrix4(b, keys + r * D * 2 + (((kk * 2 + ((lane >> 3) & 1)) ^ (r & 7)) << 4));
-        mma16816<MT>(s[2 * n], q[kk], b[0], b[1]);
-        mma16816<MT>(s[2 * n + 1], q[kk], b[2], b[3]);
-      }
-    }
-    const int warp_pos = pos0 + kw * SN;
-    const bool edge = warp_pos + SN - 1 > tile_first_limit || tile_rows < R;
-    float top[2] = {-INFINITY, -INFINITY};
-#pragma unroll
-    for (int n = 0; n < SN / 8; ++n)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        s[n][i] *= kDirect ? k_scale[n][i & 1] : p.scale_log2;
-      }
-    if (edge) {
+      const int warp_pos = pos0 + kw * SN;
+      const bool edge = warp_pos + SN - 1 > tile_first_limit || tile_rows < R;
+      float top[2] = {-INFINITY, -INFINITY};
 #pragma unroll
       for (int n = 0; n < SN / 8; ++n)
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          if (warp_pos + n * 8 + (lane & 3) * 2 + (i & 1) > limit[i >> 1]) s[n][i] = -INFINITY;
-    }
-#pragma unroll
-    for (int n = 0; n < SN / 8; ++n)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) top[i >> 1] = fmaxf(top[i >> 1], s[n][i]);
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      top[i] = fmaxf(top[i], __shfl_xor_sync(0xffffffffu, top[i], 1));
-      top[i] = fmaxf(top[i], __shfl_xor_sync(0xffffffffu, top[i], 2));
-    }
-    // the maximum is followed loosely: sums are scaled down when a row's has risen by more than a factor of 2^8, for all rows of the warp at once
-    if (__any_sync(0xffffffffu, top[0] > m[0] + 8.0f || top[1] > m[1] + 8.0f)) {
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const float now = fmaxf(m[i], top[i]), shrink = ex2(m[i] - (now == -INFINITY ? 0.0f : now));
-        m[i] = now;
-        l[i] *= shrink;
-#pragma unroll
-        for (int n = 0; n < D / 8; ++n) {
-          o[n][2 * i] *= shrink;
-          o[n][2 * i + 1] *= shrink;
-        }
-      }
-    }
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const float base = m[i] == -INFINITY ? 0.0f : m[i];
-#pragma unroll
-      for (int n = 0; n < SN / 8; ++n)
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const float x = ex2(s[n][2 * i + e] - base);
-          l[i] += x;
-          s[n][2 * i + e] = kDirect ? x * v_scale[n][e] : x;           // (the values' power of two goes to their weights)
-        }
-    }
-    if (kDirect && edge) {                                // a masked weight is zero whatever that is
-#pragma unroll
-      for (int n = 0; n < SN / 8; ++n)
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          if (warp_pos + n * 8 + (lane & 3) * 2 + (i & 1) > limit[i >> 1]) s[n][i] = 0.0f;
-    }
-    // ---- weights times values ----
-#pragma unroll
-    for (int n = 0; n < SN / 16; ++n) {
-      const uint32_t a[4] = {pack2<MT>(s[2 * n][0], s[2 * n][1]), pack2<MT>(s[2 * n][2], s[2 * n][3]), pack2<MT>(s[2 * n + 1][0], s[2 * n + 1][1]),
-                             pack2<MT>(s[2 * n + 1][2], s[2 * n + 1][3])};
-      if constexpr (kDirect) {
-        // a thread's D / 8 codes of the four positions that its B fragments hold: column `lane / 4` of every fragment
-        const int r = kw * SN + n * 16 + (lane & 3) * 2, g = lane >> 2;
-        uint32_t codes[4][D / 32];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const int row = r + (i & 1) + (i >> 1) * 8;
-          const uint32_t at = values + row * D;
-          if constexpr (D == 128) {
-            const uint4 v = lds128<0>(at + ((g ^ (row & 6)) << 4));
-            codes[i][0] = v.x;
-            codes[i][1] = v.y;
-            codes[i][2] = v.z;
-            codes[i][3] = v.w;
-          } else {
-            const uint2 v = lds64<0>(at + (((g >> 1) ^ (row & 2)) << 4) + (g & 1) * 8);
-            codes[i][0] = v.x;
-            codes[i][1] = v.y;
-          }
+          s[n][i] *= kDirect ? k_scale[n][i & 1] : p.scale_log2;
         }
-        if (!wide) {
+      if (edge) {
 #pragma unroll
-          for (int x = 0; x < D / 32; ++x) {
-            mma16816<MT>(o[4 * x], a, code_half2<0>(codes[0][x], codes[1][x]), code_half2<0>(codes[2][x], codes[3][x]));
-            mma16816<MT>(o[4 * x + 1], a, code_half2<1>(codes[0][x], codes[1][x]), code_half2<1>(codes[2][x], codes[3][x]));
-            mma16816<MT>(o[4 * x + 2], a, code_half2<2>(codes[0][x], codes[1][x]), code_half2<2>(codes[2][x], codes[3][x]));
-            mma16816<MT>(o[4 * x + 3], a, code_half2<3>(codes[0][x], codes[1][x]), code_half2<3>(codes[2][x], codes[3][x]));
-          }
-        } else {
-          const uint32_t b[4] = {pack2<T>(s[2 * n][0], s[2 * n][1]), pack2<T>(s[2 * n][2], s[2 * n][3]), pack2<T>(s[2 * n + 1][0], s[2 * n + 1][1]),
-                                 pack2<T>(s[2 * n + 1][2], s[2 * n + 1][3])};
+        for (int n = 0; n < SN / 8; ++n)
 #pragma unroll
-          for (int x = 0; x < D / 32; ++x) {
-            mma16816<T>(o[4 * x], b, code_pair<0>(codes[0][x], codes[1][x]), code_pair<0>(codes[2][x], codes[3][x]));
-            mma16816<T>(o[4 * x + 1], b, code_pair<1>(codes[0][x], codes[1][x]), code_pair<1>(codes[2][x], codes[3][x]));
-            mma16816<T>(o[4 * x + 2], b, code_pair<2>(codes[0][x], codes[1][x]), code_pair<2>(codes[2][x], codes[3][x]));
-            mma16816<T>(o[4 * x + 3], b, code_pair<3>(codes[0][x], codes[1][x]), code_pair<3>(codes[2][x], codes[3][x]));
-          }
-        }
-      } else {
-        const int r = kw * SN + n * 16 + (lane & 7) + (((lane >> 3) & 1) << 3);
-#pragma unroll
-        for (int dd = 0; dd < D / 16; ++dd) {
-          uint32_t b[4];
-          ldmatrix4t(b, values + r * D * 2 + (((dd * 2 + (lane >> 4)) ^ (r & 7)) << 4));
-          mma16816<MT>(o[2 * dd], a, b[0], b[1]);
-          mma16816<MT>(o[2 * dd + 1], a, b[2], b[3]);
-        }
+          for (int i = 0; i < 4; ++i)
+            if (warp_pos + n * 8 + (lane & 3) * 2 + (i & 1) > limit[i >> 1]) s[n][i] = -INFINITY;
       }
-    }
-    ++c.u;
-    if (c.u < c.end) continue;
-
-    // ---- the item, or this CTA's part of it, ends: its warps' sums meet where the chunk was (e4m3: where its values were) ----
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      l[i] += __shfl_xor_sync(0xffffffffu, l[i], 1);
-      l[i] += __shfl_xor_sync(0xffffffffu, l[i], 2);
-    }
-    if constexpr (kDirect) {
-      const float unit = v_top > -1000 ? ldexpf(1.0f, v_top - 6) : 1.0f;
+      for (int n = 0; n < SN / 8; ++n)
 #pragma unroll
-      for (int n = 0; n < D / 8; ++n)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) o[n][i] *= unit;
-    }
-    __syncthreads();
-    float* const sums = reinterpret_cast<float*>(kE4m3 && !kDirect ? smem + L::kRing : smem + (stage - ring));
-    constexpr int kPasses = kDirect ? 2 : 1, kPart = 16 / kPasses;       // a stage of codes holds eight rows of each warp's sums, the other places all sixteen
-    const bool first = begun == 0, last = c.u == c.units;
-    const bool odd = *any_special != 0;
-    float* const part = p.partial + (2 * static_cast<int64_t>(blockIdx.x) + (first ? 1 : 0)) * partial_floats<R, D>();
-    constexpr int kVec = D / 4;                           // threads of a row
-#pragma unroll
-    for (int pass = 0; pass < kPasses; ++pass) {
-      if (pass * kPart >= tile_rows) break;
-      if (pass) __syncthreads();
+        for (int i = 0; i < 4; ++i) top[i >> 1] = fmaxf(top[i >> 1], s[n][i]);
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        const int r = (lane >> 2) + 8 * i, sr = warp * kPart + (kDirect ? lane >> 2 : r);
-        if (pass == 0 && (lane & 3) == 0) {
-          stats[warp * 16 + r] = m[i];
-          stats[kChunk + warp * 16 + r] = l[i];
+        top[i] = fmaxf(top[i], __shfl_xor_sync(0xffffffffu, top[i], 1));
+        top[i] = fmaxf(top[i], __shfl_xor_sync(0xffffffffu, top[i], 2));
+      }
+      // the maximum is followed loosely: sums are scaled down when a row's has risen by more than a factor of 2^8, for all rows of the warp at once
+      if (__any_sync(0xffffffffu, top[0] > m[0] + 8.0f || top[1] > m[1] + 8.0f)) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const float now = fmaxf(m[i], top[i]), shrink = ex2(m[i] - (now == -INFINITY ? 0.0f : now));
+          m[i] = now;
+          l[i] *= shrink;
+#pragma unroll
+          for (int n = 0; n < D / 8; ++n) {
+            o[n][2 * i] *= shrink;
+            o[n][2 * i + 1] *= shrink;
+          }
         }
-        if (kDirect && i != pass) continue;
+      }
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const float base = m[i] == -INFINITY ? 0.0f : m[i];
+#pragma unroll
+        for (int n = 0; n < SN / 8; ++n)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const float x = ex2(s[n][2 * i + e] - base);
+            l[i] += x;
+            s[n][2 * i + e] = kDirect ? x * v_scale[n][e] : x;           // (the values' power of two goes to their weights)
+          }
+      }
+      if (kDirect && edge) {                                // a masked weight is zero whatever that is
+#pragma unroll
+        for (int n = 0; n < SN / 8; ++n)
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (warp_pos + n * 8 + (lane & 3) * 2 + (i & 1) > limit[i >> 1]) s[n][i] = 0.0f;
+      }
+      // ---- weights times values ----
+#pragma unroll
+      for (int n = 0; n < SN / 16; ++n) {
+        const uint32_t a[4] = {pack2<MT>(s[2 * n][0], s[2 * n][1]), pack2<MT>(s[2 * n][2], s[2 * n][3]), pack2<MT>(s[2 * n + 1][0], s[2 * n + 1][1]),
+                               pack2<MT>(s[2 * n + 1][2], s[2 * n + 1][3])};
+        if constexpr (kDirect) {
+          // a thread's D / 8 codes of the four positions that its B fragments hold: column `lane / 4` of every fragment
+          const int r = kw * SN + n * 16 + (lane & 3) * 2, g = lane >> 2;
+          uint32_t codes[4][D / 32];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int row = r + (i & 1) + (i >> 1) * 8;
+            const uint32_t at = values + row * D;
+            if constexpr (D == 128) {
+              const uint4 v = lds128<0>(at + ((g ^ (row & 6)) << 4));
+              codes[i][0] = v.x;
+              codes[i][1] = v.y;
+              codes[i][2] = v.z;
+              codes[i][3] = v.w;
+            } else {
+              const uint2 v = lds64<0>(at + (((g >> 1) ^ (row & 2)) << 4) + (g & 1) * 8);
+              codes[i][0] = v.x;
+              codes[i][1] = v.y;
+            }
+          }
+          if (!wide) {
+#pragma unroll
+            for (int x = 0; x < D / 32; ++x) {
+              mma16816<MT>(o[4 * x], a, code_half2<0>(codes[0][x], codes[1][x]), code_half2<0>(codes[2][x], codes[3][x]));
+              mma16816<MT>(o[4 * x + 1], a, code_half2<1>(codes[0][x], codes[1][x]), code_half2<1>(codes[2][x], codes[3][x]));
+              mma16816<MT>(o[4 * x + 2], a, code_half2<2>(codes[0][x], codes[1][x]), code_half2<2>(codes[2][x], codes[3][x]));
+              mma16816<MT>(o[4 * x + 3], a, code_half2<3>(codes[0][x], codes[1][x]), code_half2<3>(codes[2][x], codes[3][x]));
+            }
+          } else {
+            const uint32_t b[4] = {pack2<T>(s[2 * n][0], s[2 * n][1]), pack2<T>(s[2 * n][2], s[2 * n][3]), pack2<T>(s[2 * n + 1][0], s[2 * n + 1][1]),
+                                   pack2<T>(s[2 * n + 1][2], s[2 * n + 1][3])};
+#pragma unroll
+            for (int x = 0; x < D / 32; ++x) {
+              mma16816<T>(o[4 * x], b, code_pair<0>(codes[0][x], codes[1][x]), code_pair<0>(codes[2][x], codes[3][x]));
+              mma16816<T>(o[4 * x + 1], b, code_pair<1>(codes[0][x], codes[1][x]), code_pair<1>(codes[2][x], codes[3][x]));
+              mma16816<T>(o[4 * x + 2], b, code_pair<2>(codes[0][x], codes[1][x]), code_pair<2>(codes[2][x], codes[3][x]));
+              mma16816<T>(o[4 * x + 3], b, code_pair<3>(codes[0][x], codes[1][x]), code_pair<3>(codes[2][x], codes[3][x]));
+            }
+          }
+        } else {
+          const int r = kw * SN + n * 16 + (lane & 7) + (((lane >> 3) & 1) << 3);
+#pragma unroll
+          for (int dd = 0; dd < D / 16; ++dd) {
+            uint32_t b[4];
+            ldmatrix4t(b, values + r * D * 2 + (((dd * 2 + (lane >> 4)) ^ (r & 7)) << 4));
+            mma16816<MT>(o[2 * dd], a, b[0], b[1]);
+            mma16816<MT>(o[2 * dd + 1], a, b[2], b[3]);
+          }
+        }
+      }
+      ++c.u;
+      if (c.u < c.end) continue;
+
+      // ---- the item, or this CTA's part of it, ends: its warps' sums meet where the chunk was (e4m3: where its values were) ----
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        l[i] += __shfl_xor_sync(0xffffffffu, l[i], 1);
+        l[i] += __shfl_xor_sync(0xffffffffu, l[i], 2);
+      }
+      if constexpr (kDirect) {
+        const float unit = v_top > -1000 ? ldexpf(1.0f, v_top - 6) : 1.0f;
 #pragma unroll
         for (int n = 0; n < D / 8; ++n)
-          *reinterpret_cast<float2*>(sums + sr * D + ((n * 8 + (lane & 3) * 2) ^ ((sr & 3) << 3))) = make_float2(o[n][2 * i], o[n][2 * i + 1]);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) o[n][i] *= unit;
       }
       __syncthreads();
-      const int row_end = kDirect && tile_rows > (pass + 1) * kPart ? (pass + 1) * kPart : tile_rows;
-      for (int i = pass * kPart * kVec + tid; i < row_end * kVec; i += kThreads) {
-        const int r = i / kVec, d = (i % kVec) * 4;
-        const int tok = (c.t * R + r) / w.group, g = c.t * R + r - tok * w.group;
-        const int seen = w.causal ? c.span.len - c.span.n + tok : c.span.len - 1;
-        float mm = -INFINITY, ll = 0.0f, v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+      float* const sums = reinterpret_cast<float*>(smem + (kE4m3 && !kDirect ? L::kRing : kCluster ? L::kStage : stage - ring));
+      constexpr int kPasses = kDirect ? 2 : 1, kPart = 16 / kPasses;       // a stage of codes holds eight rows of each warp's sums, the other places all sixteen
+      const bool first = begun == 0, last = c.u == c.units;
+      const bool odd = *any_special != 0;
+      float* const part = p.partial + (2 * static_cast<int64_t>(blockIdx.x) + (first ? 1 : 0)) * partial_floats<R, D>();
+      constexpr int kVec = D / 4;                           // threads of a row
 #pragma unroll
-        for (int k = 0; k < KW; ++k) mm = fmaxf(mm, stats[((r / 16) * KW + k) * 16 + r % 16]);
-        const float base = mm == -INFINITY ? 0.0f : mm;
+      for (int pass = 0; pass < kPasses; ++pass) {
+        if (pass * kPart >= tile_rows) break;
+        if (pass) __syncthreads();
 #pragma unroll
-        for (int k = 0; k < KW; ++k) {
-          const int at = ((r / 16) * KW + k) * 16 + r % 16, sr = ((r / 16) * KW + k) * kPart + r % kPart;
-          const float f = ex2(stats[at] - base);
-          ll = fmaf(f, stats[kChunk + at], ll);
-          if constexpr (kDirect) {                        // fragment t, column n: element n * D / 8 + t
+        for (int i = 0; i < 2; ++i) {
+          const int r = (lane >> 2) + 8 * i, sr = warp * kPart + (kDirect ? lane >> 2 : r);
+          if (pass == 0 && (lane & 3) == 0) {
+            stats[warp * 16 + r] = m[i];
+            stats[kChunk + warp * 16 + r] = l[i];
+          }
+          if (kDirect && i != pass) continue;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) v[e] = fmaf(f, sums[sr * D + (((d + e) % (D / 8) * 8 + d / (D / 8)) ^ ((sr & 3) << 3))], v[e]);
+          for (int n = 0; n < D / 8; ++n)
+            *reinterpret_cast<float2*>(sums + sr * D + ((n * 8 + (lane & 3) * 2) ^ ((sr & 3) << 3))) = make_float2(o[n][2 * i], o[n][2 * i + 1]);
+        }
+        __syncthreads();
+        const int row_end = kDirect && tile_rows > (pass + 1) * kPart ? (pass + 1) * kPart : tile_rows;
+        for (int i = pass * kPart * kVec + tid; i < row_end * kVec; i += kThreads) {
+          const int r = i / kVec, d = (i % kVec) * 4;
+          const int tok = (c.t * R + r) / w.group, g = c.t * R + r - tok * w.group;
+          const int seen = w.causal ? c.span.len - c.span.n + tok : c.span.len - 1;
+          float mm = -INFINITY, ll = 0.0f, v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+          for (int k = 0; k < KW; ++k) mm = fmaxf(mm, stats[((r / 16) * KW + k) * 16 + r % 16]);
+          const float base = mm == -INFINITY ? 0.0f : mm;
+#pragma unroll
+          for (int k = 0; k < KW; ++k) {
+            const int at = ((r / 16) * KW + k) * 16 + r % 16, sr = ((r / 16) * KW + k) * kPart + r % kPart;
+            const float f = ex2(stats[at] - base);
+            ll = fmaf(f, stats[kChunk + at], ll);
+            if constexpr (kDirect) {                        // fragment t, column n: element n * D / 8 + t
+#pragma unroll
+              for (int e = 0; e < 4; ++e) v[e] = fmaf(f, sums[sr * D + (((d + e) % (D / 8) * 8 + d / (D / 8)) ^ ((sr & 3) << 3))], v[e]);
+            } else {
+              const float4 x = *reinterpret_cast<const float4*>(sums + sr * D + (d ^ ((sr & 3) << 3)));
+              v[0] = fmaf(f, x.x, v[0]);
+              v[1] = fmaf(f, x.y, v[1]);
+              v[2] = fmaf(f, x.z, v[2]);
+              v[3] = fmaf(f, x.w, v[3]);
+            }
+          }
+          if (odd) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              if (special[d + e] <= seen) v[e] += INFINITY;
+              if (special[D + d + e] <= seen) v[e] -= INFINITY;
+              if (special[2 * D + d + e] <= seen) v[e] = NAN;
+            }
+          }
+          if constexpr (kCluster) {
+            *reinterpret_cast<float4*>(part_rows + r * D + d) = make_float4(v[0], v[1], v[2], v[3]);
+            if (d == 0) {
+              part_stats[r] = mm;
+              part_stats[R + r] = ll;
+            }
+          } else if (first && last) {
+            store_row<T>(p, c, tok, g, d, D, v, ll, seen);
           } else {
-            const float4 x = *reinterpret_cast<const float4*>(sums + sr * D + (d ^ ((sr & 3) << 3)));
-            v[0] = fmaf(f, x.x, v[0]);
-            v[1] = fmaf(f, x.y, v[1]);
-            v[2] = fmaf(f, x.z, v[2]);
-            v[3] = fmaf(f, x.w, v[3]);
-          }
-        }
-        if (odd) {
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            if (special[d + e] <= seen) v[e] += INFINITY;
-            if (special[D + d + e] <= seen) v[e] -= INFINITY;
-            if (special[2 * D + d + e] <= seen) v[e] = NAN;
-          }
-        }
-        if constexpr (kCluster) {
-          *reinterpret_cast<float4*>(own_part + r * D + d) = make_float4(v[0], v[1], v[2], v[3]);
-          if (d == 0) {
-            own_part[16 * D + r] = mm;
-            own_part[16 * D + 16 + r] = ll;
-          }
-        } else if (first && last) {
-          // no weight at all: a row that sees nothing is zero; one that sees only scores of -inf has no softmax
-          const float inv = ll == 0.0f ? (seen < 0 ? 0.0f : NAN) : 1.0f / ll;
-          uint2 out;
-          out.x = pack2<T>(v[0] * inv, v[1] * inv);
-          out.y = pack2<T>(v[2] * inv, v[3] * inv);
-          *reinterpret_cast<uint2*>(p.out + ((static_cast<int64_t>(c.span.q0) + tok) * w.heads + c.h * w.group + g) * D * 2 + d * 2) = out;
-        } else {
-          *reinterpret_cast<float4*>(part + r * D + d) = make_float4(v[0], v[1], v[2], v[3]);
-          if (d == 0) {
-            part[R * D + r] = mm;
-            part[R * D + R + r] = ll;
+            *reinterpret_cast<float4*>(part + r * D + d) = make_float4(v[0], v[1], v[2], v[3]);
+            if (d == 0) {
+              part[R * D + r] = mm;
+              part[R * D + R + r] = ll;
+            }
           }
         }
       }
-    }
-    if (odd) {
+      if (odd) {
+        __syncthreads();
+        for (int i = tid; i < 3 * D; i += kThreads) special[i] = INT_MAX;
+        if (tid == 0) *any_special = 0;
+      }
+      if constexpr (kCluster) break;
       __syncthreads();
-      for (int i = tid; i < 3 * D; i += kThreads) special[i] = INT_MAX;
-      if (tid == 0) *any_special = 0;
+      if (c.end < c.units && tid == 0) p.notes[blockIdx.x] = note_of(c, begun, share);
+      if (!next_item<Tiles>(w, c)) break;
+      begin_item();
     }
-    if constexpr (kCluster) break;
-    __syncthreads();
-    if (c.end < c.units && tid == 0) p.notes[blockIdx.x] = note_of(c, begun, share);
-    if (!next_item<Tiles>(w, c)) break;
-    begin_item();
-  }
-  asm volatile("cp.async.wait_all;" ::: "memory");
-  if constexpr (kCluster) {
-    const int rank = blockIdx.x % CTAS;
-    if (begun == c.end)                                   // a CTA without positions: no weight, and zeros
-      for (int i = tid; i < 16 * D + 32; i += kThreads) own_part[i] = i >= 16 * D && i < 16 * D + 16 ? -INFINITY : 0.0f;
-    tc::cluster_barrier();                                // the parts are there
+    asm volatile("cp.async.wait_all;" ::: "memory");
+    if constexpr (!kCluster) return;
+    if (begun == c.end) {                                   // a CTA without positions: no weight, and zeros
+      for (int i = tid; i < R * D; i += kThreads) part_rows[i] = 0.0f;
+      for (int i = tid; i < 2 * R; i += kThreads) part_stats[i] = i < R ? -INFINITY : 0.0f;
+    }
+    tc::cluster_barrier();                                  // the parts are there
     constexpr int kVec = D / 4;
-    const int group = w.group;
-    for (int i = tid; i < (group - rank + CTAS - 1) / CTAS * kVec; i += kThreads) {
+    const int rank = blockIdx.x % CTAS;
+    for (int i = tid; i < (tile_rows - rank + CTAS - 1) / CTAS * kVec; i += kThreads) {
       const int r = rank + i / kVec * CTAS, d = i % kVec * 4;
+      const int tok = (c.t * R + r) / w.group, g = c.t * R + r - tok * w.group;
+      const int seen = w.causal ? c.span.len - c.span.n + tok : c.span.len - 1;
       float m_of[CTAS], l_of[CTAS], mm = -INFINITY, ll = 0.0f, v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
       float4 x[CTAS];
 #pragma unroll
       for (int k = 0; k < CTAS; ++k) {
-        const uint32_t at = tc::in_cta(smem_u32(own_part), k);
-        x[k] = tc::remote_ld128(at + (r * D + d) * 4);
-        m_of[k] = remote_ld32(at + (16 * D + r) * 4);
-        l_of[k] = remote_ld32(at + (16 * D + 16 + r) * 4);
+        const uint32_t stats_at = tc::in_cta(smem_u32(part_stats), k) + r * 4;
+        x[k] = tc::remote_ld128(tc::in_cta(ring, k) + (r * D + d) * 4);
+        m_of[k] = remote_ld32(stats_at);
+        l_of[k] = remote_ld32(stats_at + R * 4);
         mm = fmaxf(mm, m_of[k]);
       }
       const float base = mm == -INFINITY ? 0.0f : mm;
@@ -657,13 +694,13 @@ __global__ void __launch_bounds__(kThreads, (RowsLayout<D, SOURCE, RW>::kCtas)) 
         v[2] = fmaf(f, x[k].z, v[2]);
         v[3] = fmaf(f, x[k].w, v[3]);
       }
-      const float inv = ll == 0.0f ? (c.span.len < 1 ? 0.0f : NAN) : 1.0f / ll;
-      uint2 out;
-      out.x = pack2<T>(v[0] * inv, v[1] * inv);
-      out.y = pack2<T>(v[2] * inv, v[3] * inv);
-      *reinterpret_cast<uint2*>(p.out + (static_cast<int64_t>(c.span.q0) * w.heads + c.h * group + r) * D * 2 + d * 2) = out;
+      store_row<T>(p, c, tok, g, d, D, v, ll, seen);
     }
-    tc::cluster_barrier();                                // ... and have been read
+    tc::cluster_barrier();                                  // ... and have been read
+    item += gridDim.x / CTAS;
+    if (!cluster_item<Tiles>(w, item, rank, CTAS, &c)) return;
+    load = c;
+    loading = c.u < c.end;
   }
 }
 
@@ -751,20 +788,22 @@ int launch_one(const RowsParams& p, cudaStream_t stream) {
   return check_launch("attend_join_kernel");
 }
 
-template <typename T, int D, int SOURCE, int CTAS>
-int launch_cluster(const RowsParams& p, int items, cudaStream_t stream) {
+template <typename T, int D, int RW, int SOURCE, int CTAS>
+int launch_clusters(const RowsParams& p, cudaStream_t stream) {
   static bool done[kMaxDevices] = {};
   const int dev = current_device();
   if (dev < 0) return QMM_ERR_DEVICE;
-  auto kernel = attend_rows_kernel<T, D, 1, SOURCE, CTAS>;
-  constexpr int kBytes = RowsLayout<D, SOURCE, 1>::kBytes + part_bytes<D>();
+  auto kernel = attend_rows_kernel<T, D, RW, SOURCE, CTAS>;
+  constexpr int kBytes = RowsLayout<D, SOURCE, RW>::kBytes + 2 * 16 * RW * 4;
   if (!done[dev]) {
     const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kBytes);
     if (e != cudaSuccess) return fail(QMM_ERR_CUDA, "cudaFuncSetAttribute: %s", cudaGetErrorString(e));
     done[dev] = true;
   }
+  // (a sequence's last tile may be short; items beyond what the device holds at once are taken in turn)
+  const int64_t items = (p.work.tokens * p.work.group / (16 * RW) + p.work.seqs) * p.work.kv_heads, room = 2 * device_sm_count() / CTAS;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(items * CTAS);
+  cfg.gridDim = dim3(static_cast<unsigned>(items < room ? items : room) * CTAS);
   cfg.blockDim = dim3(kThreads);
   cfg.dynamicSmemBytes = kBytes;
   cfg.stream = stream;
@@ -781,21 +820,19 @@ int launch_cluster(const RowsParams& p, int items, cudaStream_t stream) {
   return check_launch("attend_rows_kernel");
 }
 
+template <typename T, int D, int RW, int SOURCE>
+int launch_tiles(const RowsParams& p, cudaStream_t stream) {
+  const int ctas = attend_cluster_ctas(p, SOURCE, 16 * RW);
+  if (ctas == 8) return launch_clusters<T, D, RW, SOURCE, 8>(p, stream);
+  if (ctas == 4) return launch_clusters<T, D, RW, SOURCE, 4>(p, stream);
+  return launch_one<T, D, RW, SOURCE>(p, stream);
+}
+
 template <typename T, int D, int SOURCE>
 int launch_rows_of(const RowsParams& p, int rows, cudaStream_t stream) {
-  // A new token each of a few sequences: a cluster of CTAs for every sequence and key head, one launch, which wants neither the order of all units (2 us) nor a second
-  // launch to join (3.5 us). Eight CTAs where two an SM are enough for all, else four. It pays while the longest sequence that a table has room for is short: without
-  // shares by weight, no more CTAs take part in it (8 key heads of 128, us, bf16 clusters / shares: 1 sequence of 2000 positions 8.5 / 12.3, 8000 14.7 / 16.2, 16000
-  // 19.6 / 19.3; 8 of 4000 11.4 / 15.3; with a second wave 16 of 4000 28.5 / 28.9), and codes, which want three CTAs an SM, sooner not (1 of 2000 10.0 / 13.8, 4000
-  // 14.7 / 16.3, 8000 21.4 / 20.0).
-  const int64_t items = static_cast<int64_t>(p.work.seqs) * p.work.kv_heads, room = 2 * device_sm_count();
-  if (!p.work.cu_q && rows <= 16 && p.work.longest <= (SOURCE == kPages8 ? 4096 : 8192)) {
-    if (items * 8 <= room) return launch_cluster<T, D, SOURCE, 8>(p, static_cast<int>(items), stream);
-    if (items * 4 <= room) return launch_cluster<T, D, SOURCE, 4>(p, static_cast<int>(items), stream);
-  }
-  if (rows <= 16) return launch_one<T, D, 1, SOURCE>(p, stream);
-  if (rows <= 32) return launch_one<T, D, 2, SOURCE>(p, stream);
-  return launch_one<T, D, 4, SOURCE>(p, stream);
+  if (rows <= 16) return launch_tiles<T, D, 1, SOURCE>(p, stream);
+  if (rows <= 32) return launch_tiles<T, D, 2, SOURCE>(p, stream);
+  return launch_tiles<T, D, 4, SOURCE>(p, stream);
 }
 
 template <typename T, int D>
@@ -807,6 +844,19 @@ int launch_source(const RowsParams& p, int source, int rows, cudaStream_t stream
 }
 
 }  // namespace
+
+// Clusters want neither the order of all units (2 us) nor a second launch to join (3.5 us): eight CTAs a sequence and key head where the device holds as many for all, at
+// two an SM, else four. They pay while no CTA has many positions to do: without shares by weight no others help it, and codes want three CTAs an SM. Measured with 8
+// key heads of 128, us, clusters / shares, tiles of 16 rows: 1 sequence of 2000 positions 8.5 / 12.3, 8000 15.0 / 16.2, 16000 19.6 / 19.3; 8 of 1000 to 4000 11 / 12.8,
+// 2000 to 8000 17 / 16.4; of codes: 1 of 4000 13.8 / 16.3, 8000 21.4 / 20.0; 8 of 500 to 2000 16 / 17.6, 1000 to 4000 25.8 / 21.6. Tiles of 32 rows: 1 of 4000 15.6 /
+// 17.2, 8000 23.0 / 20.7; 8 of 2000 17.5 / 20.9, 1000 to 4000 24.9 / 22.2. Tiles of 64 rows, against the kernel of 2 x 128: 1 of 4000 20.9 / 23.6; 8 of 2000 25.4 / 29.9;
+// 8 of 500 to 2000 with 40 rows on average and up to 76 in two tiles 26.5 / 21.7.
+int attend_cluster_ctas(const RowsParams& p, int source, int rows) {
+  const int64_t items = static_cast<int64_t>(p.work.seqs) * p.work.kv_heads, room = 2 * device_sm_count();
+  const int ctas = items * 8 <= room ? 8 : 4;
+  const bool few = source == kPages16 && rows <= 16 ? p.work.longest <= 1024 * ctas : p.work.longest <= 512 * ctas;
+  return source != kRowsSource && rows <= 64 && items * ctas <= room && few ? ctas : 0;
+}
 
 int attend_rows_ctas() { return 3 * device_sm_count(); }
 

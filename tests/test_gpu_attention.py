@@ -114,6 +114,16 @@ def test_one_token_however_sequences_are_shared(dim, dtype, cache, group, kv, lo
     _check_paged([1] * len(lens), lens, group * kv, kv, dim, 64, dtype, cache, cu=False, seed=kv)
 
 
+@pytest.mark.parametrize("dtype, cache", CACHES)
+@pytest.mark.parametrize("group, kv", [(2, 1), (5, 2), (7, 6)])
+@pytest.mark.parametrize("news", [[1, 1, 0, 3, 1, 2], [5] * 9, [1, 12, 0, 1, 1, 1, 1], [9, 40, 1]])
+@pytest.mark.parametrize("longest", [41, 700, 8200])
+def test_few_tokens_however_sequences_are_shared(dtype, cache, group, kv, news, longest):
+    """Tiles of 16, 32 and 64 rows; sequences of none, of one and of many; CTAs without positions; positions that only some rows see."""
+    lens = [max(n, (longest * (3 + 5 * i % 7)) // 9 if i else longest) for i, n in enumerate(news)]
+    _check_paged(news, lens, group * kv, kv, 128, 64, dtype, cache, seed=kv + len(news), strided=kv == 2)
+
+
 @pytest.mark.parametrize("at", [0, 299, 300, 700])
 def test_infinite_values_and_scores_of_one_token(at):
     """In a row's sum, on whichever CTA: +inf, NaN, both infinities; keys whose scores are -inf have no weight; none else: no softmax."""
