@@ -162,6 +162,7 @@ int qmm_decode_attention(const void* qkv, void* k_cache, void* v_cache, void* ou
  * smallest whole number for which the row's largest magnitude is at most 448 * 2^e (between -117 and
  * 119; 0 for a row of zeros), element x is e4m3(x / 2^e), rounded to nearest even, and the row's E8M0
  * byte is e + 127. A row with an infinity or a NaN in it has the byte 255 and reads as NaN throughout.
+ * Bytes are so 10 to 246 or 255, and codes numbers (not 0x7f, 0xff): of a cache filled otherwise nothing else is read right.
  * The values of such a cache are exact in bf16, which is what q has to be with it. */
 typedef struct {
   uint32_t struct_size;     /* sizeof(qmm_paged_cache) */
@@ -212,7 +213,8 @@ int qmm_cache_read(const qmm_paged_cache* cache, int64_t seqs, const int32_t* cu
 typedef struct {
   uint32_t struct_size;     /* sizeof(qmm_attention_args) */
   int32_t elem;             /* QMM_BF16 or QMM_F16: of q, out, k and v */
-  const void* q;            /* [tokens, heads, head_dim]; strides in elements, multiples of 8; head_dim contiguous */
+  const void* q;            /* [tokens, heads, head_dim]; strides in elements, multiples of 8; head_dim contiguous; q_row a multiple of q_head, no less than
+                               heads of them, and so for k and v (the stride of a dimension of one is not read) */
   int64_t q_row, q_head;
   const void* k;            /* qmm_prompt_attention: [tokens, kv_heads, head_dim]; NULL for qmm_paged_attention */
   int64_t k_row, k_head;

@@ -123,13 +123,15 @@ def _on(device):
 
 
 def _heads_of(name, t, device, dtype):
-    """`[tokens, heads, head_dim]` as the kernels read it: rows of a head side by side, 16-byte steps."""
+    """`[tokens, heads, head_dim]` as the kernels read it (a copy, if it lies otherwise): rows of a head side by side, 16-byte steps, tokens
+    a whole number of heads apart."""
     if t.dim() != 3 or t.dtype != dtype or t.device != device:
         raise ValueError(f"{name}: [tokens, heads, head_dim] of {dtype} on {device} is wanted")
-    d = t.shape[2]
-    if (t.stride(2) != 1 and d > 1) or t.stride(0) % 8 or t.stride(1) % 8 or t.data_ptr() % 16 or t.stride(0) < 0 or t.stride(1) < 0:
-        t = t.clone(memory_format=torch.contiguous_format)
-    return t
+    (n, h, d), (row, head, one) = t.shape, t.stride()
+    lies = (one == 1 or d == 1) and row % 8 == 0 and head % 8 == 0 and t.data_ptr() % 16 == 0 and (n == 1 or row >= d)
+    if lies and h > 1:
+        lies = head >= d and (n == 1 or (row >= head * h and row % head == 0))
+    return t if lies else t.clone(memory_format=torch.contiguous_format)
 
 
 def _output(out, like, shape):

@@ -16,7 +16,6 @@ struct RowsParams {
   float* partial;
   int64_t q_row, q_head, k_row, k_head, v_row, v_head;       // elements
   float scale_log2;
-  int32_t least;               // weights of a CTA's share (attention_plan.cuh)
 };
 
 struct JoinParams {

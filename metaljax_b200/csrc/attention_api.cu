@@ -47,6 +47,13 @@ int check_attention(const char* what, const qmm_attention_args* a) {
   return QMM_OK;
 }
 
+// Rows of heads as copies of whole tiles want them: tokens a whole number of heads apart, no two elements in one place. (A dimension of one has no stride.)
+bool lies(int64_t tokens, int64_t heads, int64_t dim, int64_t* row, int64_t* head) {
+  if (tokens <= 1) *row = heads == 1 ? dim : heads * *head;
+  if (heads == 1) *head = *row;
+  return *row % 8 == 0 && *head % 8 == 0 && *head >= dim && *row >= heads * *head && *row % *head == 0;
+}
+
 int64_t workspace_of(const qmm_attention_args* a) {
   const int64_t rows = attend_rows_workspace(a->head_dim, attend_rows_ctas()), tc = attend_tc_workspace(a->head_dim, attend_tc_ctas());
   return rows > tc ? rows : tc;
@@ -57,10 +64,18 @@ int attend(const char* what, const qmm_paged_cache* cache, const CacheView* view
   if (!(a->scale > 0.0f) || !std::isfinite(a->scale)) return fail(QMM_ERR_UNSUPPORTED, "%s: scale must be a positive number", what);
   if (a->tokens == 0 || a->seqs == 0) return QMM_OK;
   if (!a->q || !a->out) return fail(QMM_ERR_NULL, "%s: q and out are required", what);
-  if (!aligned16(a->q) || !aligned16(a->out) || (a->q_row | a->q_head) % 8) return fail(QMM_ERR_LAYOUT, "%s: q and out must be 16-byte aligned, strides multiples of 8", what);
+  RowsParams p = {};
+  p.q_row = a->q_row;
+  p.q_head = a->q_head;
+  p.k_row = a->k_row;
+  p.k_head = a->k_head;
+  p.v_row = a->v_row;
+  p.v_head = a->v_head;
+  if (!aligned16(a->q) || !aligned16(a->out) || !lies(a->tokens, a->heads, a->head_dim, &p.q_row, &p.q_head) ||
+      (!view && (!lies(a->tokens, a->kv_heads, a->head_dim, &p.k_row, &p.k_head) || !lies(a->tokens, a->kv_heads, a->head_dim, &p.v_row, &p.v_head))))
+    return fail(QMM_ERR_LAYOUT, "%s: 16-byte aligned tensors are wanted, strides multiples of 8, tokens a whole number of heads apart", what);
   if (!a->workspace || a->workspace_bytes < workspace_of(a)) return fail(QMM_ERR_TOO_LARGE, "%s: the workspace is too small", what);
   if (!aligned16(a->workspace)) return fail(QMM_ERR_LAYOUT, "%s: the workspace must be 16-byte aligned", what);
-  RowsParams p = {};
   p.work.cu_q = a->cu_q;
   p.work.kv_lens = a->kv_lens;
   p.work.tokens = a->tokens;
@@ -76,12 +91,6 @@ int attend(const char* what, const qmm_paged_cache* cache, const CacheView* view
   p.v = static_cast<const uint8_t*>(a->v);
   p.out = static_cast<uint8_t*>(a->out);
   p.notes = static_cast<JoinNote*>(a->workspace);
-  p.q_row = a->q_row;
-  p.q_head = a->q_head;
-  p.k_row = a->k_row;
-  p.k_head = a->k_head;
-  p.v_row = a->v_row;
-  p.v_head = a->v_head;
   p.scale_log2 = a->scale * 1.4426950408889634f;
   if (view) {
     p.cache = *view;
@@ -93,7 +102,6 @@ int attend(const char* what, const qmm_paged_cache* cache, const CacheView* view
   // several times as fast (8 sequences of 2000 to 4000 positions: 20 rows 22 against 32 us, 35 rows 24 and 24, 64 rows 36 and 36).
   const bool tc = a->cu_q && rows > 32 && !attend_cluster_ctas(p, source, rows < 65 ? static_cast<int>(rows) : 65) &&
                   (!view || (static_cast<uint64_t>(p.cache.pages) * p.work.kv_heads << p.cache.page_shift) < (1ull << 31));
-  p.least = 4;
   const int ctas = tc ? attend_tc_ctas() : attend_rows_ctas();
   p.partial = reinterpret_cast<float*>(p.notes + ctas);
   if (tc) return launch_attend_tc(p, a->elem, a->head_dim, source, ctas, stream);
@@ -151,8 +159,7 @@ extern "C" int qmm_prompt_attention(const qmm_attention_args* a, void* stream) {
   if (a->kv_lens) return fail(QMM_ERR_UNSUPPORTED, "prompt_attention: a prompt's keys are its own tokens' (kv_lens is NULL)");
   if (a->tokens && a->seqs) {
     if (!a->cu_q || !a->k || !a->v) return fail(QMM_ERR_NULL, "prompt_attention: cu_q, k and v are required");
-    if (!aligned16(a->k) || !aligned16(a->v) || (a->k_row | a->k_head | a->v_row | a->v_head) % 8)
-      return fail(QMM_ERR_LAYOUT, "prompt_attention: k and v must be 16-byte aligned, strides multiples of 8");
+    if (!aligned16(a->k) || !aligned16(a->v)) return fail(QMM_ERR_LAYOUT, "prompt_attention: k and v must be 16-byte aligned");
   }
   return attend("prompt_attention", nullptr, nullptr, a, static_cast<cudaStream_t>(stream));
 }

@@ -9,9 +9,9 @@
 // for itself, and the CTA does not meet but at the ends of items. Pages of bf16 are bound by the memory: the same 64 sequences 206 us, 6.5 TB/s.
 //
 // e4m3 codes: with one row of 16 a warp takes them straight into its B fragments as f16, one conversion a pair (a bf16 takes five
-// instructions a pair, with which 64 sequences of 2000 to 8000 positions took 249 us; now 171, 3.9 TB/s, bound by instructions: 687 for 16 positions): of keys four codes of a row a step (the queries' elements in the order that makes),
-// of values the codes of its four positions, paired by a byte permutation. The queries become f16 under a power of two, the rows' powers of two go to the
-// scores and to the weights. Where warps share positions, the one that asked for a chunk's rows turns them into bf16 (exactly) next to the chunk in
+// instructions a pair, with which 64 sequences of 2000 to 8000 positions took 249 us; now 171, 3.9 TB/s, bound by instructions: 687 for 16
+// positions): of keys four codes of a row a step (the queries' elements in the order that makes), of values the codes of its four positions,
+// paired by a byte permutation. The queries become f16 under a power of two, the rows' powers of two go to the scores and to the weights. Where warps share positions, the one that asked for a chunk's rows turns them into bf16 (exactly) next to the chunk in
 // shared memory.
 //
 // Masked positions: scores are selected, not added to. A value that is no number at a masked position would still be 0 * NaN in the sum, so
@@ -171,7 +171,7 @@ __global__ void __launch_bounds__(kThreads, (RowsLayout<D, SOURCE, RW>::kCtas)) 
   } else {
     if (tid == 0) p.notes[blockIdx.x].parts = 0;
     // every warp works out where this CTA begins by itself
-    if (!find_share<Tiles>(w, blockIdx.x, gridDim.x, p.least, &c, &share)) return;
+    if (!find_share<Tiles>(w, blockIdx.x, gridDim.x, &c, &share)) return;
   }
   UnitCursor load = c;                                  // where the copies are
   bool loading = c.u < c.end;

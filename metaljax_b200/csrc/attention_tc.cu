@@ -251,7 +251,7 @@ attend_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constan
   asm volatile("griddepcontrol.wait;" ::: "memory");
   UnitCursor c;
   int64_t share;
-  bool more = find_share<Tiles>(w, blockIdx.x, gridDim.x, p.least, &c, &share);
+  bool more = find_share<Tiles>(w, blockIdx.x, gridDim.x, &c, &share);
   // every lane waits, and all go on or none does
   auto wait = [&](uint32_t bar, uint32_t parity, int where) -> bool { return __all_sync(0xffffffffu, wait_phase(bar, parity, abort_at, where)); };
   // ... for `n` counters of this CTA, a lane each
@@ -278,325 +278,325 @@ attend_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constan
   bool ok = true;
   // registers a thread at the launch: 168 (128 x 104 + 256 x 200 = 384 x 168), or with more helpers 128 (256 x 64 + 256 x 192 = 512 x 128)
   if (warp >= 8) {
-  if constexpr (kE4m3) asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
-  else asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");
-  if (warp == 9) {
-    // ---------------- copies ----------------
-    if (lane == 0) p.notes[blockIdx.x].parts = 0;         // (also where this CTA gives up)
-    Slot<L::kKeys> key = {0, 0};
-    Slot<L::kValues> value = {0, 0};
-    [[maybe_unused]] Slot<kE4m3 ? L::kCodes : 1> code = {0, 0};
-    int items[2] = {0, 0};
-    const int page_size = 1 << p.cache.page_shift;
-    const int per_block = PAGED ? (page_size < kBlock ? kBlock / page_size : 1) : 1;       // pages of a block
-    while (ok && more) {
-      const Part it = part_of(w, c);
-      if (it.live) {
-        for (int x = 0; x < 2; ++x) {
-          if (it.last[x] == it.begin) continue;
-          if (!(ok = wait(q_empty + 8 * x, (items[x] & 1) ^ 1, 31))) break;
-          ++items[x];
-          if (lane == 0) {
-            mbar_expect_tx(q_full + 8 * x, (D / 64) * w.tile_tokens * w.group * 128);
-            for (int i = 0; i < D / 64; ++i)
-              tma_load_3d(&q_map, base + x * L::kTile + i * 16384, q_full + 8 * x, i * 64, c.h * w.group, c.span.q0 + (2 * c.t + x) * w.tile_tokens);
-          }
-          __syncwarp();
-        }
-        if (!ok) break;
-        int64_t page = 0;
-        auto look_up = [&](int u) {                    // lane i: page i of block u
-          if constexpr (PAGED) {
-            const int pos = u * kBlock + lane * page_size;
-            page = 0;
-            if (lane < per_block && u < it.load_end && pos < c.span.len) page = page_of(p.cache, c.s, pos, w.status);
-            if (page < 0) page = 0;
-          }
-        };
-        look_up(it.begin);
-        for (int u = it.begin; ok && u < it.load_end; ++u) {
-          int there = 1;                                // pages of the block that the sequence has
-          if constexpr (PAGED) {
-            const int pages = (c.span.len - u * kBlock + page_size - 1) >> p.cache.page_shift;
-            there = pages < per_block ? pages : per_block;
-          }
-          const int64_t here = page;
-          look_up(u + 1);
-#pragma unroll
-          for (int which = 0; which < 2; ++which) {
-            if constexpr (kE4m3) {
-              if (!(ok = wait(c_empty + 8 * code.slot, code.phase ^ 1u, 32))) break;
-              const uint32_t dst = base + L::kCodeRing + code.slot * (kBlock * D), exps = base + L::kExps + code.slot * kBlock, bar = c_full + 8 * code.slot;
-              const int rows = page_size < kBlock ? page_size : kBlock;
-              if (lane == 0) mbar_expect_tx(bar, there * rows * (D + 1));
-              __syncwarp();
-              if (lane < there) {
-                const int64_t row = ((here * w.kv_heads + c.h) << p.cache.page_shift) + ((u * kBlock) & (page_size - 1));
-                tma_load_2d(which ? &v_map : &k_map, dst + lane * rows * D, bar, 0, static_cast<int>(row));
-                bulk_load(exps + lane * rows, (which ? p.cache.v_exp : p.cache.k_exp) + row, rows, bar);
-              }
-              __syncwarp();
-              code.next();
-              continue;
-            }
-            const uint32_t slot = which ? value.slot : key.slot;
-            if (!(ok = wait((which ? v_empty : k_empty) + 8 * slot, (which ? value.phase : key.phase) ^ 1u, 32))) break;
-            const uint32_t dst = (which ? value_ring : key_ring) + slot * L::kTile, bar = (which ? v_full : k_full) + 8 * slot;
-            if constexpr (PAGED) {
-              const int rows = page_size < kBlock ? page_size : kBlock;
-              if (lane == 0) mbar_expect_tx(bar, there * rows * D * 2);
-              __syncwarp();
-              if (lane < there) {
-                const int row = static_cast<int>(((here * w.kv_heads + c.h) << p.cache.page_shift) + ((u * kBlock) & (page_size - 1)));
-                for (int i = 0; i < D / 64; ++i) tma_load_2d(which ? &v_map : &k_map, dst + i * 16384 + lane * rows * 128, bar, i * 64, row);
-              }
-            } else if (lane == 0) {
-              mbar_expect_tx(bar, kBlock * D * 2);
-              for (int i = 0; i < D / 64; ++i) tma_load_3d(which ? &v_map : &k_map, dst + i * 16384, bar, i * 64, c.h, c.span.q0 + u * kBlock);
+    if constexpr (kE4m3) asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
+    else asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");
+    if (warp == 9) {
+      // ---------------- copies ----------------
+      if (lane == 0) p.notes[blockIdx.x].parts = 0;         // (also where this CTA gives up)
+      Slot<L::kKeys> key = {0, 0};
+      Slot<L::kValues> value = {0, 0};
+      [[maybe_unused]] Slot<kE4m3 ? L::kCodes : 1> code = {0, 0};
+      int items[2] = {0, 0};
+      const int page_size = 1 << p.cache.page_shift;
+      const int per_block = PAGED ? (page_size < kBlock ? kBlock / page_size : 1) : 1;       // pages of a block
+      while (ok && more) {
+        const Part it = part_of(w, c);
+        if (it.live) {
+          for (int x = 0; x < 2; ++x) {
+            if (it.last[x] == it.begin) continue;
+            if (!(ok = wait(q_empty + 8 * x, (items[x] & 1) ^ 1, 31))) break;
+            ++items[x];
+            if (lane == 0) {
+              mbar_expect_tx(q_full + 8 * x, (D / 64) * w.tile_tokens * w.group * 128);
+              for (int i = 0; i < D / 64; ++i)
+                tma_load_3d(&q_map, base + x * L::kTile + i * 16384, q_full + 8 * x, i * 64, c.h * w.group, c.span.q0 + (2 * c.t + x) * w.tile_tokens);
             }
             __syncwarp();
-            if (which) value.next(); else key.next();
+          }
+          if (!ok) break;
+          int64_t page = 0;
+          auto look_up = [&](int u) {                    // lane i: page i of block u
+            if constexpr (PAGED) {
+              const int pos = u * kBlock + lane * page_size;
+              page = 0;
+              if (lane < per_block && u < it.load_end && pos < c.span.len) page = page_of(p.cache, c.s, pos, w.status);
+              if (page < 0) page = 0;
+            }
+          };
+          look_up(it.begin);
+          for (int u = it.begin; ok && u < it.load_end; ++u) {
+            int there = 1;                                // pages of the block that the sequence has
+            if constexpr (PAGED) {
+              const int pages = (c.span.len - u * kBlock + page_size - 1) >> p.cache.page_shift;
+              there = pages < per_block ? pages : per_block;
+            }
+            const int64_t here = page;
+            look_up(u + 1);
+#pragma unroll
+            for (int which = 0; which < 2; ++which) {
+              if constexpr (kE4m3) {
+                if (!(ok = wait(c_empty + 8 * code.slot, code.phase ^ 1u, 32))) break;
+                const uint32_t dst = base + L::kCodeRing + code.slot * (kBlock * D), exps = base + L::kExps + code.slot * kBlock, bar = c_full + 8 * code.slot;
+                const int rows = page_size < kBlock ? page_size : kBlock;
+                if (lane == 0) mbar_expect_tx(bar, there * rows * (D + 1));
+                __syncwarp();
+                if (lane < there) {
+                  const int64_t row = ((here * w.kv_heads + c.h) << p.cache.page_shift) + ((u * kBlock) & (page_size - 1));
+                  tma_load_2d(which ? &v_map : &k_map, dst + lane * rows * D, bar, 0, static_cast<int>(row));
+                  bulk_load(exps + lane * rows, (which ? p.cache.v_exp : p.cache.k_exp) + row, rows, bar);
+                }
+                __syncwarp();
+                code.next();
+                continue;
+              }
+              const uint32_t slot = which ? value.slot : key.slot;
+              if (!(ok = wait((which ? v_empty : k_empty) + 8 * slot, (which ? value.phase : key.phase) ^ 1u, 32))) break;
+              const uint32_t dst = (which ? value_ring : key_ring) + slot * L::kTile, bar = (which ? v_full : k_full) + 8 * slot;
+              if constexpr (PAGED) {
+                const int rows = page_size < kBlock ? page_size : kBlock;
+                if (lane == 0) mbar_expect_tx(bar, there * rows * D * 2);
+                __syncwarp();
+                if (lane < there) {
+                  const int row = static_cast<int>(((here * w.kv_heads + c.h) << p.cache.page_shift) + ((u * kBlock) & (page_size - 1)));
+                  for (int i = 0; i < D / 64; ++i) tma_load_2d(which ? &v_map : &k_map, dst + i * 16384 + lane * rows * 128, bar, i * 64, row);
+                }
+              } else if (lane == 0) {
+                mbar_expect_tx(bar, kBlock * D * 2);
+                for (int i = 0; i < D / 64; ++i) tma_load_3d(which ? &v_map : &k_map, dst + i * 16384, bar, i * 64, c.h, c.span.q0 + u * kBlock);
+              }
+              __syncwarp();
+              if (which) value.next(); else key.next();
+            }
           }
         }
+        if (c.end < c.units && lane == 0) p.notes[blockIdx.x] = note_of(c, it.begin, share);
+        more = next_item<Tiles>(w, c);
       }
-      if (c.end < c.units && lane == 0) p.notes[blockIdx.x] = note_of(c, it.begin, share);
-      more = next_item<Tiles>(w, c);
-    }
-    if (!ok) {                                          // given up: what is on its way lands first
-      auto drain = [&](uint32_t bars_of, int n, uint32_t slot, uint32_t phase) {
-        for (int i = 0; i < n; ++i) mbar_drain(bars_of + 8 * i, i < static_cast<int>(slot) ? phase : phase ^ 1u);
-      };
-      if constexpr (kE4m3) {
-        drain(c_full, L::kCodes, code.slot, code.phase);
-      } else {
-        drain(k_full, L::kKeys, key.slot, key.phase);
-        drain(v_full, L::kValues, value.slot, value.phase);
+      if (!ok) {                                          // given up: what is on its way lands first
+        auto drain = [&](uint32_t bars_of, int n, uint32_t slot, uint32_t phase) {
+          for (int i = 0; i < n; ++i) mbar_drain(bars_of + 8 * i, i < static_cast<int>(slot) ? phase : phase ^ 1u);
+        };
+        if constexpr (kE4m3) {
+          drain(c_full, L::kCodes, code.slot, code.phase);
+        } else {
+          drain(k_full, L::kKeys, key.slot, key.phase);
+          drain(v_full, L::kValues, value.slot, value.phase);
+        }
+        for (int x = 0; x < 2; ++x)
+          if (items[x]) mbar_drain(q_full + 8 * x, (items[x] - 1) & 1);
       }
-      for (int x = 0; x < 2; ++x)
-        if (items[x]) mbar_drain(q_full + 8 * x, (items[x] - 1) & 1);
-    }
-  } else if (kE4m3 && warp >= 10) {
-    // ---------------- helpers: codes into bf16, in the products' layout ----------------
-    Slot<L::kKeys> key = {0, 0};
-    Slot<L::kValues> value = {0, 0};
-    Slot<kE4m3 ? L::kCodes : 1> code = {0, 0};
-    int live = 0;
-    while (ok && more) {
-      const Part it = part_of(w, c);
-      if (it.live) {
-        const int first_limit = w.causal ? c.span.len - c.span.n + c.t * 2 * w.tile_tokens : c.span.len - 1;
-        const int seen = it.seen[0] > it.seen[1] ? it.seen[0] : it.seen[1];
-        bool mine = false;                              // the first row of no numbers is this item's
-        for (int u = it.begin; ok && u < it.load_end; ++u) {
+    } else if (kE4m3 && warp >= 10) {
+      // ---------------- helpers: codes into bf16, in the products' layout ----------------
+      Slot<L::kKeys> key = {0, 0};
+      Slot<L::kValues> value = {0, 0};
+      Slot<kE4m3 ? L::kCodes : 1> code = {0, 0};
+      int live = 0;
+      while (ok && more) {
+        const Part it = part_of(w, c);
+        if (it.live) {
+          const int first_limit = w.causal ? c.span.len - c.span.n + c.t * 2 * w.tile_tokens : c.span.len - 1;
+          const int seen = it.seen[0] > it.seen[1] ? it.seen[0] : it.seen[1];
+          bool mine = false;                              // the first row of no numbers is this item's
+          for (int u = it.begin; ok && u < it.load_end; ++u) {
 #pragma unroll 1
-          for (int which = 0; which < 2; ++which) {
-            if (!(ok = wait(c_full + 8 * code.slot, code.phase, 33))) break;
-            if (!(ok = wait((which ? v_empty : k_empty) + 8 * (which ? value.slot : key.slot), (which ? value.phase : key.phase) ^ 1u, 45))) break;
-            const uint32_t from = base + L::kCodeRing + code.slot * (kBlock * D), exps = base + L::kExps + code.slot * kBlock;
-            const uint32_t to = which ? value_ring + value.slot * L::kTile : key_ring + key.slot * L::kTile;
-            const int pos0 = u * kBlock;
-            constexpr int kPieces = D / 16;
-            // rows of values that some rows see and others do not, or none
-            const int some = which ? (first_limit + 1 > pos0 ? first_limit + 1 - pos0 : 0) : kBlock, none = which ? seen - pos0 : kBlock;
-            auto convert = [&](int i, uint32_t byte, bool zero) {
-              const int r = i / kPieces, col = i % kPieces;
-              const uint4 c16 = lds128<0>(from + i * 16);
-              const uint32_t codes[4] = {c16.x, c16.y, c16.z, c16.w};
-              uint32_t v[8];
-              row_values(codes, row_factors(byte), v);
-              if (zero) {
+            for (int which = 0; which < 2; ++which) {
+              if (!(ok = wait(c_full + 8 * code.slot, code.phase, 33))) break;
+              if (!(ok = wait((which ? v_empty : k_empty) + 8 * (which ? value.slot : key.slot), (which ? value.phase : key.phase) ^ 1u, 45))) break;
+              const uint32_t from = base + L::kCodeRing + code.slot * (kBlock * D), exps = base + L::kExps + code.slot * kBlock;
+              const uint32_t to = which ? value_ring + value.slot * L::kTile : key_ring + key.slot * L::kTile;
+              const int pos0 = u * kBlock;
+              constexpr int kPieces = D / 16;
+              // rows of values that some rows see and others do not, or none
+              const int some = which ? (first_limit + 1 > pos0 ? first_limit + 1 - pos0 : 0) : kBlock, none = which ? seen - pos0 : kBlock;
+              auto convert = [&](int i, uint32_t byte, bool zero) {
+                const int r = i / kPieces, col = i % kPieces;
+                const uint4 c16 = lds128<0>(from + i * 16);
+                const uint32_t codes[4] = {c16.x, c16.y, c16.z, c16.w};
+                uint32_t v[8];
+                row_values(codes, row_factors(byte), v);
+                if (zero) {
 #pragma unroll
-                for (int n = 0; n < 8; ++n) v[n] = 0;
-              }
-              const uint32_t line = to + (col >> 2) * 16384 + r * 128, piece = 2 * col & 7;
-              asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(line + ((piece ^ (r & 7)) << 4)), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]) : "memory");
-              asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(line + (((piece + 1) ^ (r & 7)) << 4)), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]) : "memory");
-            };
-            const int mine0 = (warp - 10) * 32 + lane;
-            if (some >= kBlock && none >= kBlock) {
+                  for (int n = 0; n < 8; ++n) v[n] = 0;
+                }
+                const uint32_t line = to + (col >> 2) * 16384 + r * 128, piece = 2 * col & 7;
+                asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(line + ((piece ^ (r & 7)) << 4)), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]) : "memory");
+                asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(line + (((piece + 1) ^ (r & 7)) << 4)), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]) : "memory");
+              };
+              const int mine0 = (warp - 10) * 32 + lane;
+              if (some >= kBlock && none >= kBlock) {
 #pragma unroll 3
-              for (int i = mine0; i < kBlock * kPieces; i += kHelpers * 32) convert(i, lds8(exps + i / kPieces), false);
-            } else {
-              for (int i = mine0; i < kBlock * kPieces; i += kHelpers * 32) {
-                const int r = i / kPieces;
-                const uint32_t byte = lds8(exps + r);
-                const bool odd = r >= some && r < none && byte == 255;
-                if (__any_sync(0xffffffffu, odd) && !mine) {
+                for (int i = mine0; i < kBlock * kPieces; i += kHelpers * 32) convert(i, lds8(exps + i / kPieces), false);
+              } else {
+                for (int i = mine0; i < kBlock * kPieces; i += kHelpers * 32) {
+                  const int r = i / kPieces;
+                  const uint32_t byte = lds8(exps + r);
+                  const bool odd = r >= some && r < none && byte == 255;
+                  if (__any_sync(0xffffffffu, odd) && !mine) {
+                    if (!(ok = wait_count(kWritten, 8, live, 34))) break;
+                    if (lane == 0) words[kNanPlace + warp - 10] = 0x7fffffff;
+                    if (lane == 0) words[kTags + warp - 10] = live + 1;
+                    __syncwarp();
+                    mine = true;
+                  }
+                  if (odd) atomicMin(const_cast<int*>(&words[kNanPlace + warp - 10]), pos0 + r);
+                  convert(i, byte, odd || r >= none);
+                }
+              }
+              fence_proxy_async();
+              __syncwarp();
+              if (lane == 0) {
+                mbar_arrive(c_empty + 8 * code.slot);
+                mbar_arrive(which ? v_clean + 8 * value.slot : k_full + 8 * key.slot);
+              }
+              code.next();
+              if (which) value.next(); else key.next();
+            }
+          }
+          __threadfence_block();
+          __syncwarp();
+          if (lane == 0) words[kHelped + warp - 10] = live + 1;
+          ++live;
+        }
+        more = next_item<Tiles>(w, c);
+      }
+    } else if (warp >= 10) {
+      // ---------------- helpers: blocks of v that some row does not see all of ----------------
+      Slot<L::kValues> at = {0, 0};
+      int live = 0;
+      while (ok && more) {
+        const Part it = part_of(w, c);
+        if (it.live) {
+          const int first_limit = w.causal ? c.span.len - c.span.n + c.t * 2 * w.tile_tokens : c.span.len - 1;
+          const int place0 = place_of(first_limit);
+          uint16_t* const set = special + (warp - 10) * 3 * D;
+          bool mine = false;                              // the set is this item's
+          for (int u = it.begin; ok && u < it.load_end; ++u) {
+            const uint32_t slot = at.slot;
+            if (!(ok = wait(v_full + 8 * slot, at.phase, 33))) break;
+            const int pos0 = u * kBlock;
+            if (pos0 + kBlock - 1 > first_limit) {
+              constexpr int kPieces = D / 8;
+              const int some = first_limit + 1 > pos0 ? first_limit + 1 - pos0 : 0;                                   // rows up to here: seen by all
+              const int seen = it.seen[0] > it.seen[1] ? it.seen[0] : it.seen[1];
+              const int none = seen - pos0 < kBlock ? seen - pos0 : kBlock;                                           // from here on: by none
+              auto place = [&](int i) {
+                const int r = i / kPieces, col = i % kPieces;
+                return value_ring + slot * L::kTile + (col >> 3) * 16384 + r * 128 + (((col & 7) ^ (r & 7)) << 4);
+              };
+              const int mine0 = (warp - 10) * 32 + lane;
+              for (int i = none * kPieces + mine0; i < kBlock * kPieces; i += kHelpers * 32)
+                asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(place(i)), "r"(0) : "memory");
+              constexpr int kBatch = 4;
+              for (int i0 = some * kPieces; i0 < none * kPieces; i0 += kBatch * kHelpers * 32) {
+                uint4 v[kBatch];
+                unsigned odd = 0;
+#pragma unroll
+                for (int b = 0; b < kBatch; ++b) {
+                  const int i = i0 + b * kHelpers * 32 + mine0;
+                  v[b] = i < none * kPieces ? lds128<0>(place(i)) : make_uint4(0, 0, 0, 0);
+                }
+#pragma unroll
+                for (int b = 0; b < kBatch; ++b)
+                  if (odd_pair<T>(v[b].x) || odd_pair<T>(v[b].y) || odd_pair<T>(v[b].z) || odd_pair<T>(v[b].w)) odd |= 1u << b;
+                if (!__any_sync(0xffffffffu, odd)) continue;
+                if (!mine) {                            // the items before this one are written: what the set held goes
                   if (!(ok = wait_count(kWritten, 8, live, 34))) break;
-                  if (lane == 0) words[kNanPlace + warp - 10] = 0x7fffffff;
+                  for (int n = lane; n < 3 * D; n += 32) set[n] = 0xffff;
                   if (lane == 0) words[kTags + warp - 10] = live + 1;
                   __syncwarp();
                   mine = true;
                 }
-                if (odd) atomicMin(const_cast<int*>(&words[kNanPlace + warp - 10]), pos0 + r);
-                convert(i, byte, odd || r >= none);
-              }
-            }
-            fence_proxy_async();
-            __syncwarp();
-            if (lane == 0) {
-              mbar_arrive(c_empty + 8 * code.slot);
-              mbar_arrive(which ? v_clean + 8 * value.slot : k_full + 8 * key.slot);
-            }
-            code.next();
-            if (which) value.next(); else key.next();
-          }
-        }
-        __threadfence_block();
-        __syncwarp();
-        if (lane == 0) words[kHelped + warp - 10] = live + 1;
-        ++live;
-      }
-      more = next_item<Tiles>(w, c);
-    }
-  } else if (warp >= 10) {
-    // ---------------- helpers: blocks of v that some row does not see all of ----------------
-    Slot<L::kValues> at = {0, 0};
-    int live = 0;
-    while (ok && more) {
-      const Part it = part_of(w, c);
-      if (it.live) {
-        const int first_limit = w.causal ? c.span.len - c.span.n + c.t * 2 * w.tile_tokens : c.span.len - 1;
-        const int place0 = place_of(first_limit);
-        uint16_t* const set = special + (warp - 10) * 3 * D;
-        bool mine = false;                              // the set is this item's
-        for (int u = it.begin; ok && u < it.load_end; ++u) {
-          const uint32_t slot = at.slot;
-          if (!(ok = wait(v_full + 8 * slot, at.phase, 33))) break;
-          const int pos0 = u * kBlock;
-          if (pos0 + kBlock - 1 > first_limit) {
-            constexpr int kPieces = D / 8;
-            const int some = first_limit + 1 > pos0 ? first_limit + 1 - pos0 : 0;                                   // rows up to here: seen by all
-            const int seen = it.seen[0] > it.seen[1] ? it.seen[0] : it.seen[1];
-            const int none = seen - pos0 < kBlock ? seen - pos0 : kBlock;                                           // from here on: by none
-            auto place = [&](int i) {
-              const int r = i / kPieces, col = i % kPieces;
-              return value_ring + slot * L::kTile + (col >> 3) * 16384 + r * 128 + (((col & 7) ^ (r & 7)) << 4);
-            };
-            const int mine0 = (warp - 10) * 32 + lane;
-            for (int i = none * kPieces + mine0; i < kBlock * kPieces; i += kHelpers * 32)
-              asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(place(i)), "r"(0) : "memory");
-            constexpr int kBatch = 4;
-            for (int i0 = some * kPieces; i0 < none * kPieces; i0 += kBatch * kHelpers * 32) {
-              uint4 v[kBatch];
-              unsigned odd = 0;
+                for (int l = 0; l < 32; ++l) {          // a lane at a time: two may have the same column
+                  if (l == lane && odd) {
 #pragma unroll
-              for (int b = 0; b < kBatch; ++b) {
-                const int i = i0 + b * kHelpers * 32 + mine0;
-                v[b] = i < none * kPieces ? lds128<0>(place(i)) : make_uint4(0, 0, 0, 0);
-              }
+                    for (int b = 0; b < kBatch; ++b) {
+                      if (!(odd >> b & 1)) continue;
+                      const int i = i0 + b * kHelpers * 32 + mine0, r = i / kPieces, col = i % kPieces;
+                      uint32_t word[4] = {v[b].x, v[b].y, v[b].z, v[b].w};
 #pragma unroll
-              for (int b = 0; b < kBatch; ++b)
-                if (odd_pair<T>(v[b].x) || odd_pair<T>(v[b].y) || odd_pair<T>(v[b].z) || odd_pair<T>(v[b].w)) odd |= 1u << b;
-              if (!__any_sync(0xffffffffu, odd)) continue;
-              if (!mine) {                            // the items before this one are written: what the set held goes
-                if (!(ok = wait_count(kWritten, 8, live, 34))) break;
-                for (int n = lane; n < 3 * D; n += 32) set[n] = 0xffff;
-                if (lane == 0) words[kTags + warp - 10] = live + 1;
-                __syncwarp();
-                mine = true;
-              }
-              for (int l = 0; l < 32; ++l) {          // a lane at a time: two may have the same column
-                if (l == lane && odd) {
-#pragma unroll
-                  for (int b = 0; b < kBatch; ++b) {
-                    if (!(odd >> b & 1)) continue;
-                    const int i = i0 + b * kHelpers * 32 + mine0, r = i / kPieces, col = i % kPieces;
-                    uint32_t word[4] = {v[b].x, v[b].y, v[b].z, v[b].w};
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) {
-                      const float2 pair = unpack2<T>(word[e >> 1]);
-                      const float x = e & 1 ? pair.y : pair.x;
-                      if (!(fabsf(x) <= 3.402823466e38f)) {
-                        uint16_t* const first = set + (x > 0.0f ? 0 : x < 0.0f ? D : 2 * D) + col * 8 + e;
-                        if (pos0 + r - place0 < *first) *first = static_cast<uint16_t>(pos0 + r - place0);
-                        word[e >> 1] &= e & 1 ? 0x0000ffffu : 0xffff0000u;
+                      for (int e = 0; e < 8; ++e) {
+                        const float2 pair = unpack2<T>(word[e >> 1]);
+                        const float x = e & 1 ? pair.y : pair.x;
+                        if (!(fabsf(x) <= 3.402823466e38f)) {
+                          uint16_t* const first = set + (x > 0.0f ? 0 : x < 0.0f ? D : 2 * D) + col * 8 + e;
+                          if (pos0 + r - place0 < *first) *first = static_cast<uint16_t>(pos0 + r - place0);
+                          word[e >> 1] &= e & 1 ? 0x0000ffffu : 0xffff0000u;
+                        }
                       }
+                      asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(place(i)), "r"(word[0]), "r"(word[1]), "r"(word[2]), "r"(word[3]) : "memory");
                     }
-                    asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(place(i)), "r"(word[0]), "r"(word[1]), "r"(word[2]), "r"(word[3]) : "memory");
                   }
+                  __syncwarp();
                 }
-                __syncwarp();
               }
+              fence_proxy_async();
             }
-            fence_proxy_async();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(v_clean + 8 * slot);
+            at.next();
           }
+          __threadfence_block();
           __syncwarp();
-          if (lane == 0) mbar_arrive(v_clean + 8 * slot);
-          at.next();
+          if (lane == 0) words[kHelped + warp - 10] = live + 1;
+          ++live;
         }
-        __threadfence_block();
-        __syncwarp();
-        if (lane == 0) words[kHelped + warp - 10] = live + 1;
-        ++live;
+        more = next_item<Tiles>(w, c);
       }
-      more = next_item<Tiles>(w, c);
-    }
-  } else {
-    // ---------------- the MMAs' issuer ----------------
-    constexpr uint32_t kFmt = kBf16 ? 1 : 0;
-    const uint32_t id_scores = instr_desc(kFmt, 128) | (static_cast<uint32_t>(kBlock / 8) << 17);
-    const uint32_t id_values = instr_desc(kFmt, 128) | (static_cast<uint32_t>(D / 8) << 17) | (1u << 16);       // B is MN-major
-    Slot<L::kKeys> key = {0, 0};
-    Slot<L::kValues> value = {0, 0};
-    uint32_t items[2] = {0, 0}, p_ph[2] = {0, 0};
-    auto scores = [&](int x, uint32_t key_slot, bool last) {
-      mma_scores<D>(tmem + x * 128, desc_low(base + x * L::kTile), desc_low(key_ring + key_slot * L::kTile), kDescHigh, id_scores);
-      tc_commit<false>(s_full + 8 * x, 0);
-      if (last) tc_commit<false>(q_empty + 8 * x, 0);    // the next item's queries may come
-    };
-    while (ok && more) {
-      const Part it = part_of(w, c);
-      if (it.live) {
-        if (!(ok = wait(k_full + 8 * key.slot, key.phase, 36))) break;
-        for (int x = 0; x < 2; ++x) {
-          if (it.last[x] == it.begin) continue;
-          if (!(ok = wait(q_full + 8 * x, items[x] & 1, 35))) break;
-          tc_fence_after();
-          scores(x, key.slot, it.begin + 1 == it.last[x]);
-        }
-        if (!ok) break;
-        tc_commit<false>(k_empty + 8 * key.slot, 0);
-        key.next();
-        for (int u = it.begin; ok && u < it.load_end; ++u) {
-          const bool next = u + 1 < it.load_end;
-          if (!(ok = wait(v_clean + 8 * value.slot, value.phase, 37))) break;
-          if (next && !(ok = wait(k_full + 8 * key.slot, key.phase, 38))) break;
+    } else {
+      // ---------------- the MMAs' issuer ----------------
+      constexpr uint32_t kFmt = kBf16 ? 1 : 0;
+      const uint32_t id_scores = instr_desc(kFmt, 128) | (static_cast<uint32_t>(kBlock / 8) << 17);
+      const uint32_t id_values = instr_desc(kFmt, 128) | (static_cast<uint32_t>(D / 8) << 17) | (1u << 16);       // B is MN-major
+      Slot<L::kKeys> key = {0, 0};
+      Slot<L::kValues> value = {0, 0};
+      uint32_t items[2] = {0, 0}, p_ph[2] = {0, 0};
+      auto scores = [&](int x, uint32_t key_slot, bool last) {
+        mma_scores<D>(tmem + x * 128, desc_low(base + x * L::kTile), desc_low(key_ring + key_slot * L::kTile), kDescHigh, id_scores);
+        tc_commit<false>(s_full + 8 * x, 0);
+        if (last) tc_commit<false>(q_empty + 8 * x, 0);    // the next item's queries may come
+      };
+      while (ok && more) {
+        const Part it = part_of(w, c);
+        if (it.live) {
+          if (!(ok = wait(k_full + 8 * key.slot, key.phase, 36))) break;
           for (int x = 0; x < 2; ++x) {
-            if (u >= it.last[x]) continue;
-            if (u == it.begin) {                        // the rows' last item has been read out of O
-              if (!(ok = wait(o_free + 8 * x, (items[x] & 1) ^ 1, 39))) break;
-            }
-            for (int part = 0; part < 2; ++part) {      // P comes in two parts of 64 positions
-              if (!(ok = wait(p_full + 16 * x + 8 * part, p_ph[x], 40))) break;
-              tc_fence_after();
-              mma_values(tmem + 256 + x * D, tmem + x * 128 + part * 32, desc_low_mn(value_ring + value.slot * L::kTile + part * 8192), kDescHigh, id_values,
-                         part | (u > it.begin));
-            }
-            if (!ok) break;
-            p_ph[x] ^= 1u;
-            if (u + 1 < it.last[x]) {
-              scores(x, key.slot, u + 2 == it.last[x]);
-            } else {
-              tc_commit<false>(o_full + 8 * x, 0);
-              ++items[x];
-            }
+            if (it.last[x] == it.begin) continue;
+            if (!(ok = wait(q_full + 8 * x, items[x] & 1, 35))) break;
+            tc_fence_after();
+            scores(x, key.slot, it.begin + 1 == it.last[x]);
           }
           if (!ok) break;
-          tc_commit<false>(v_empty + 8 * value.slot, 0);
-          value.next();
-          if (next) {
-            tc_commit<false>(k_empty + 8 * key.slot, 0);
-            key.next();
+          tc_commit<false>(k_empty + 8 * key.slot, 0);
+          key.next();
+          for (int u = it.begin; ok && u < it.load_end; ++u) {
+            const bool next = u + 1 < it.load_end;
+            if (!(ok = wait(v_clean + 8 * value.slot, value.phase, 37))) break;
+            if (next && !(ok = wait(k_full + 8 * key.slot, key.phase, 38))) break;
+            for (int x = 0; x < 2; ++x) {
+              if (u >= it.last[x]) continue;
+              if (u == it.begin) {                        // the rows' last item has been read out of O
+                if (!(ok = wait(o_free + 8 * x, (items[x] & 1) ^ 1, 39))) break;
+              }
+              for (int part = 0; part < 2; ++part) {      // P comes in two parts of 64 positions
+                if (!(ok = wait(p_full + 16 * x + 8 * part, p_ph[x], 40))) break;
+                tc_fence_after();
+                mma_values(tmem + 256 + x * D, tmem + x * 128 + part * 32, desc_low_mn(value_ring + value.slot * L::kTile + part * 8192), kDescHigh, id_values,
+                           part | (u > it.begin));
+              }
+              if (!ok) break;
+              p_ph[x] ^= 1u;
+              if (u + 1 < it.last[x]) {
+                scores(x, key.slot, u + 2 == it.last[x]);
+              } else {
+                tc_commit<false>(o_full + 8 * x, 0);
+                ++items[x];
+              }
+            }
+            if (!ok) break;
+            tc_commit<false>(v_empty + 8 * value.slot, 0);
+            value.next();
+            if (next) {
+              tc_commit<false>(k_empty + 8 * key.slot, 0);
+              key.next();
+            }
           }
         }
+        more = next_item<Tiles>(w, c);
       }
-      more = next_item<Tiles>(w, c);
+      // The arrivals of all MMAs so far, given up or not, reach their barriers before the CTA leaves.
+      tc_commit<false>(done, 0);
+      mbar_drain(done, 0);
     }
-    // The arrivals of all MMAs so far, given up or not, reach their barriers before the CTA leaves.
-    tc_commit<false>(done, 0);
-    mbar_drain(done, 0);
-  }
   } else {
     if constexpr (kE4m3) asm volatile("setmaxnreg.inc.sync.aligned.u32 192;");
     else asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");

@@ -628,9 +628,12 @@ PyObject* read_pages(PyObject*, PyObject* const* a, Py_ssize_t n) {
 
 bool is_half(const at::Tensor* t) { return t->scalar_type() == at::kBFloat16 || t->scalar_type() == at::kHalf; }
 
-// q, k or v: heads' elements side by side, strides and address in steps of 16 bytes.
+// q, k or v: heads' elements side by side, address and strides in steps of 16 bytes, tokens a whole number of heads apart (the library looks at that).
 bool heads_of(const at::Tensor* t, at::ScalarType type) {
-  return t && t->dim() == 3 && t->scalar_type() == type && t->stride(2) == 1 && t->stride(0) % 8 == 0 && t->stride(1) % 8 == 0 && t->stride(0) >= 0 && t->stride(1) >= 0 && aligned(t);
+  if (!t || t->dim() != 3 || t->scalar_type() != type || t->stride(2) != 1 || !aligned(t)) return false;
+  const int64_t row = t->stride(0), head = t->stride(1);
+  return row % 8 == 0 && head % 8 == 0 && (t->size(1) == 1 || (head >= t->size(2) && (t->size(0) == 1 || (row >= head * t->size(1) && row % head == 0)))) &&
+         (t->size(0) == 1 || row >= t->size(2));
 }
 
 // The rest of both forms: result and workspace, and the call.

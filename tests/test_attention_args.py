@@ -153,6 +153,15 @@ def test_statuses_of_append(args, status):
     assert _lib.lib().qmm_cache_append(ctypes.byref(c), ctypes.byref(a), None) == status, _lib.lib().qmm_last_error()
 
 
+@pytest.mark.parametrize("args", [
+    {"q_head": 32}, {"q_head": 0}, {"q_row": 0}, {"q_row": 192}, {"q_row": 264}, {"k_head": 0}, {"k_row": 64}, {"v_row": 136}, {"q_row": 64, "q_head": 128},
+])
+def test_heads_that_overlap_or_lie_between_steps_are_refused(args):
+    """(their tensors are copied by the Python calls)"""
+    _, a = _args(None, **{"kv_lens": None, "cu_q": 256, "k": 256, "v": 256, "k_row": 128, "k_head": 64, "v_row": 128, "v_head": 64, **args})
+    assert _lib.lib().qmm_prompt_attention(ctypes.byref(a), None) == 4, _lib.lib().qmm_last_error()
+
+
 def test_nothing_to_do_is_no_error():
     c, a = _args(None, tokens=0, seqs=0, q=None, out=None, kv_lens=None)
     assert _lib.lib().qmm_paged_attention(ctypes.byref(c), ctypes.byref(a), None) == 0

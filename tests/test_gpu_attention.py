@@ -645,6 +645,31 @@ def test_rows_that_are_not_aligned():
     assert torch.equal(a, b) and all(torch.equal(m, n) for m, n in zip(*(attention.read_pages(c, table, cu, 59) for c in caches)))
 
 
+@pytest.mark.parametrize("news", [[200, 90], [3, 4]])
+def test_layouts_of_heads(news):
+    """Heads before tokens, heads that share their rows, rows a fraction of a head apart, dimensions of one with any stride."""
+    gen = _gen(31)
+    t, heads, kv, dim = sum(news), 4, 2, 64
+    cu = R.starts(news, DEV)
+    q, k, v = (torch.randn((t, h, dim), generator=gen, device=DEV).to(BF) for h in (heads, kv, kv))
+    want = attention.prompt_attention(q, k, v, cu)
+    first = [x.transpose(0, 1).contiguous().transpose(0, 1) for x in (q, k, v)]
+    assert torch.equal(attention.prompt_attention(*first, cu), want)
+    padded = []
+    for x in (q, k, v):
+        rows = torch.full((t, x.shape[1] * dim + 8), torch.nan, dtype=BF, device=DEV)
+        rows[:, :-8] = x.flatten(1)
+        padded.append(rows[:, :-8].unflatten(1, (-1, dim)))
+    assert torch.equal(attention.prompt_attention(*padded, cu), want)
+    one = [x[:, :1] for x in (k, v)]
+    shared = attention.prompt_attention(q, *(x.expand(-1, 2, -1) for x in one), cu)
+    assert torch.equal(shared, attention.prompt_attention(q, *(x.expand(-1, 2, -1).contiguous() for x in one), cu))
+    assert torch.equal(shared, attention.prompt_attention(q, *one, cu))
+    assert torch.equal(shared, attention.prompt_attention(q, *(x.as_strided(x.shape, (x.stride(0), 8, 1)) for x in one), cu))
+    last = [x[t - 1:].as_strided((1,) + tuple(x.shape[1:]), (16, dim, 1)) for x in (q, k, v)]
+    assert torch.equal(attention.prompt_attention(*last, R.starts([1], DEV)), last[2].repeat_interleave(2, dim=1))
+
+
 @pytest.mark.parametrize("offset", [8, 16, 24])
 def test_results_at_every_alignment(offset):
     """Results, queries, keys, values and caches that begin at any multiple of 16 bytes."""
