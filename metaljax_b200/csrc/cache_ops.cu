@@ -16,7 +16,7 @@ namespace {
 
 constexpr int kThreads = 256, kWarps = kThreads / 32;
 
-// One warp: sequence of packed row `row`, as sequence_of.
+// One warp: sequence of packed row `row`: the last s with starts[s] <= row, or -1 for a row of none.
 __device__ __forceinline__ int warp_sequence_of(const int32_t* __restrict__ starts, int seqs, int row, int* end) {
   const int lane = threadIdx.x & 31;
   int lo = 0, n = seqs + 1;                            // among starts[lo .. lo + n), of which the first is <= row

@@ -1,4 +1,4 @@
-// What the kernels on a paged cache share: sequences and positions of packed rows, page lookup with its checks, and the rows of an e4m3 cache.
+// What the kernels on a paged cache share: page lookup with its checks, and the rows of an e4m3 cache.
 // Device code, but for the view.
 #pragma once
 
@@ -26,17 +26,6 @@ struct CacheView {
 };
 
 __device__ __forceinline__ void report_index(int* status) { atomicCAS(status, 0, QMM_DEVICE_BAD_INDEX); }
-
-// Sequence of packed row `row`: the last s with starts[s] <= row, or -1 for a row of none.
-__device__ __forceinline__ int sequence_of(const int32_t* __restrict__ starts, int seqs, int row) {
-  if (row < starts[0] || row >= starts[seqs]) return -1;
-  int lo = 0, hi = seqs;                               // starts[lo] <= row < starts[hi]
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (starts[mid] <= row) lo = mid; else hi = mid;
-  }
-  return lo;
-}
 
 // Page of a position, or -1 (reported): no such entry, or a page that the cache does not have.
 __device__ __forceinline__ int64_t page_of(const CacheView& c, int seq, int pos, int* status) {
