@@ -781,7 +781,10 @@ int launch_one(const RowsParams& p, cudaStream_t stream) {
   launch_early(attend_rows_kernel<T, D, RW, SOURCE, 1>, ctas, kThreads, RowsLayout<D, SOURCE, RW>::kBytes, stream, p);
   count_launch();
   if (int rc = check_launch("attend_rows_kernel")) return rc;
-  if (ctas < 2) return QMM_OK;
+  // sequences of one chunk at most: nothing to join
+  const int64_t longest = SOURCE == kRowsSource ? p.work.tokens : p.work.longest;
+  if (ctas < 2 || longest <= kChunk) return QMM_OK;
+  static_assert(RowTiles<16 * RW, kChunk>::kWhole == 2, "items of one unit are whole");
   JoinParams j = {p.work, p.out, p.notes, p.partial};
   launch_early(attend_join_kernel<T, D, 16 * RW>, dim3(ctas - 1, 16 * RW / kJoinRows), kJoinThreads, 0, stream, j);
   count_launch();

@@ -835,7 +835,9 @@ int launch_one(const RowsParams& p, const CUtensorMap (&maps)[3], int ctas, cuda
   launch_early(kernel, ctas, L::kThreads, L::kBytes, stream, maps[0], maps[1], maps[2], p);
   count_launch();
   if (int rc = check_launch("attend_tc_kernel")) return rc;
-  if (ctas < 2) return QMM_OK;
+  // items too short to be cut, however sequences are: nothing to join, and the launch that would find that out (2 us) is left out
+  const int64_t longest = SOURCE == kRowsSource ? p.work.tokens : p.work.longest;
+  if (ctas < 2 || longest <= (Tiles::kWhole - 1) * kBlock) return QMM_OK;
   JoinParams j = {p.work, p.out, p.notes, p.partial};
   launch_early(attend_tc_join_kernel<T, D>, dim3(ctas - 1, D / kJoinColumns), 256, 0, stream, j);
   count_launch();
