@@ -70,8 +70,8 @@ struct RowTiles {
   }
 };
 
-// 16 prompts of some 700 tokens with heads of 64 / 4 of some 150 / one of 8192, us: kCost 3 and kWhole 8 46 / 15 / 477; kCost 2 44 / 20 / 477;
-// kWhole 4 47 / 15 / 478, 16 (kCost 2) 44 / 20 / 480. (Taken with whole items at the CTA of their middle, which is no faster than that of their beginning.)
+// 16 prompts of some 700 tokens with heads of 64 / 4 of some 150 / one of 8192 / 8 chunks of 64 over up to 8000, us: kCost 3 and kWhole 8 46.0 / 16 / 469 / 64; kCost 2
+// 45.1 / 16 / 470 / 65, 1 45.3 / 16 / 497 / 69; kCost 2 and kWhole 5 47.0 / 16 / 469 / 63.
 template <int B>
 struct TokenTiles {
   static constexpr int kCost = 3, kWhole = 8;
@@ -139,10 +139,11 @@ __device__ __forceinline__ int64_t lane_weights(const AttentionWork& w, int base
   return sum;
 }
 
-// Weights of a CTA's share: at least kLeast, a single unit with what its item costs (less makes parts to join out of nothing). (Divisions of 64
+// Weights of a CTA's share: at least a single unit with what its item costs (less makes parts to join out of nothing). (Divisions of 64
 // bits are calls, and spill what is live around them.)
-constexpr int kLeast = 4;
+template <typename Tiles>
 __device__ __forceinline__ int64_t quota_of(int64_t total, int ctas) {
+  constexpr int kLeast = Tiles::kCost + 1;
   int shift = 0;
   while ((total + ctas) >> shift >> 32) shift += 8;     // (a larger share than need be where weights pass 2^32)
   const int64_t q = shift ? (static_cast<int64_t>(static_cast<uint32_t>(total >> shift) / ctas) + 1) << shift : static_cast<uint32_t>(total + ctas - 1) / ctas;
@@ -228,7 +229,7 @@ __device__ __forceinline__ bool find_share(const AttentionWork& w, int cta, int 
     if (__all_sync(0xffffffffu, small)) {
       const int total = __reduce_add_sync(0xffffffffu, sum);
       int quota = static_cast<int>(static_cast<unsigned>(total + ctas - 1) / static_cast<unsigned>(ctas));
-      if (quota < kLeast) quota = kLeast;
+      if (quota < Tiles::kCost + 1) quota = Tiles::kCost + 1;
       *share = quota;
       if (static_cast<int64_t>(quota) * cta >= total) return false;
       int left = quota * cta;
@@ -254,7 +255,7 @@ __device__ __forceinline__ bool find_share(const AttentionWork& w, int cta, int 
   }
   int64_t total = 0;
   for (int base = 0; base < w.seqs; base += 32) total += warp_sum(lane_weights<Tiles>(w, base)) * w.kv_heads;
-  const int64_t quota = quota_of(total, ctas);
+  const int64_t quota = quota_of<Tiles>(total, ctas);
   *share = quota;
   int64_t left = quota * cta;
   if (left >= total) return false;
