@@ -106,6 +106,8 @@ __device__ __forceinline__ float max_nan(float a, float b) {            // NaN i
 
 // T: type of the projection's rows; E4M3: the cache holds codes, else values of T. Queries, keys and values are a pass each: what an element and its pair's other
 // one are multiplied with (norm's weight times cosine, and sine) stays in registers for all heads, and the root mean square comes last.
+// Bound by instructions at three CTAs an SM (some 6700 tokens of 32 + 2 x 8 heads of 128 with norms into e4m3 50 us, 3.9 TB/s; 8192 into bf16 44, 4.5 TB/s). Before heads were
+// asked for a batch ahead, with four rows a batch: 52.7; four CTAs 53.6, with two rows 58.1; two CTAs with six 60.4; two warps a token 72.
 template <typename T, int D, bool E4M3>
 __global__ void __launch_bounds__(kThreads, 3) append_kernel(const AppendParams p) {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
@@ -118,6 +120,14 @@ __global__ void __launch_bounds__(kThreads, 3) append_kernel(const AppendParams 
   if (token >= p.tokens) return;
   const int stride = p.token_warps * kRows;
   const uint4* const rows = reinterpret_cast<const uint4*>(p.qkv) + token * p.row_stride / 8;
+  // Pieces of this warp's next heads, asked for a batch ahead, also of the next pass; the first ones before it is known where the token stands.
+  uint4 x[kBatch];
+  const int head_at = part * kRows + slot;
+  auto ask = [&](int begin, int count, int head) {
+    return head < count ? __ldg(rows + static_cast<int64_t>(begin + head) * kLanes + lane) : make_uint4(0, 0, 0, 0);
+  };
+#pragma unroll
+  for (int b = 0; b < kBatch; ++b) x[b] = ask(0, p.heads, head_at + b * stride);
   int seq = token, end = 0, pos;
   if (p.cu_q) {
     seq = warp_sequence_of(p.cu_q, p.seqs, token, &end);
@@ -140,7 +150,7 @@ __global__ void __launch_bounds__(kThreads, 3) append_kernel(const AppendParams 
   const bool first = lane < pairs, turned = lane < 2 * pairs;
   const int partner = p.interleaved || !turned ? lane : first ? lane + pairs : lane - pairs;
 
-  auto pass = [&](auto kind_of, int begin, int count, const uint8_t* weight) {
+  auto pass = [&](auto kind_of, int begin, int count, const uint8_t* weight, int next_begin, int next_count) {
     constexpr int kKind = decltype(kind_of)::value;      // 0 queries, 1 keys, 2 values
     const bool turns_on = kKind != 2 && pairs > 0, scaled = kKind != 2 && weight != nullptr;
     uint64_t own[4], across[4];                           // factors of an element and of its pair's other one
@@ -166,21 +176,18 @@ __global__ void __launch_bounds__(kThreads, 3) append_kernel(const AppendParams 
         }
       }
     }
-    for (int head0 = part * kRows + slot; __any_sync(0xffffffffu, head0 < count); head0 += kBatch * stride) {
-      uint4 x[kBatch];
+    for (int head0 = head_at;; head0 += kBatch * stride) {
+      const bool more = __any_sync(0xffffffffu, head0 + kBatch * stride < count);
 #pragma unroll
       for (int b = 0; b < kBatch; ++b) {
         const int head = head0 + b * stride;
-        x[b] = head < count ? __ldg(rows + static_cast<int64_t>(begin + head) * kLanes + lane) : make_uint4(0, 0, 0, 0);
-      }
-#pragma unroll
-      for (int b = 0; b < kBatch; ++b) {
-        const int head = head0 + b * stride;
-        if (!__any_sync(0xffffffffu, head < count)) break;
-        uint4 out = x[b];
+        const uint4 mine = x[b];
+        x[b] = more ? ask(begin, count, head + kBatch * stride) : ask(next_begin, next_count, head_at + b * stride);
+        if (!__any_sync(0xffffffffu, head < count)) continue;
+        uint4 out = mine;
         uint64_t f[4];
         if (kKind != 2 || E4M3) {
-          pairs_of<T>(x[b], f);
+          pairs_of<T>(mine, f);
           uint64_t inv2 = pair_of(1.0f, 1.0f);
           if (scaled) {
             uint64_t ss2 = 0;
@@ -202,8 +209,8 @@ __global__ void __launch_bounds__(kThreads, 3) append_kernel(const AppendParams 
                 g[i] = pair_of(v.y, v.x);
               }
             } else {
-              const uint4 other = make_uint4(__shfl_sync(0xffffffffu, x[b].x, partner, kLanes), __shfl_sync(0xffffffffu, x[b].y, partner, kLanes),
-                                             __shfl_sync(0xffffffffu, x[b].z, partner, kLanes), __shfl_sync(0xffffffffu, x[b].w, partner, kLanes));
+              const uint4 other = make_uint4(__shfl_sync(0xffffffffu, mine.x, partner, kLanes), __shfl_sync(0xffffffffu, mine.y, partner, kLanes),
+                                             __shfl_sync(0xffffffffu, mine.z, partner, kLanes), __shfl_sync(0xffffffffu, mine.w, partner, kLanes));
               pairs_of<T>(other, g);
             }
 #pragma unroll
@@ -257,11 +264,12 @@ __global__ void __launch_bounds__(kThreads, 3) append_kernel(const AppendParams 
           reinterpret_cast<uint4*>(kKind == 2 ? p.c.v : p.c.k)[at * kLanes + lane] = out;
         }
       }
+      if (!more) break;
     }
   };
-  pass(std::integral_constant<int, 0>{}, 0, p.heads, p.q_norm);
-  pass(std::integral_constant<int, 1>{}, p.heads, p.c.kv_heads, p.k_norm);
-  pass(std::integral_constant<int, 2>{}, p.heads + p.c.kv_heads, p.c.kv_heads, nullptr);
+  pass(std::integral_constant<int, 0>{}, 0, p.heads, p.q_norm, p.heads, p.c.kv_heads);
+  pass(std::integral_constant<int, 1>{}, p.heads, p.c.kv_heads, p.k_norm, p.heads + p.c.kv_heads, p.c.kv_heads);
+  pass(std::integral_constant<int, 2>{}, p.heads + p.c.kv_heads, p.c.kv_heads, nullptr, 0, 0);
 }
 
 struct ReadParams {

@@ -45,11 +45,9 @@ __device__ __forceinline__ int64_t page_of(const CacheView& c, int seq, int pos,
 // ---- rows of an e4m3 cache ----
 // The exponent e of a row whose largest magnitude is `big` (finite): the smallest whole number with big <= 448 * 2^e, 448 = 1.75 * 2^8.
 __device__ __forceinline__ int row_exponent(float big) {
-  if (big == 0.0f) return 0;
-  int x;
-  const float m = frexpf(big, &x);                     // big = m * 2^x, m in [0.5, 1); 448 = 0.875 * 2^9
-  const int e = x - (m > 0.875f ? 8 : 9);
-  return e < -117 ? -117 : e > 119 ? 119 : e;
+  const uint32_t bits = __float_as_uint(big);          // 1.m * 2^(x - 127); what is smaller than 2^-126 has a row of the least exponent
+  const int e = static_cast<int>(bits >> 23) - 127 - 8 + ((bits & 0x7fffffu) > 0x600000u ? 1 : 0);
+  return bits == 0 ? 0 : e < -117 ? -117 : e > 119 ? 119 : e;
 }
 
 __device__ __forceinline__ uint32_t e4m3_pair(float lo, float hi) {
