@@ -1,6 +1,6 @@
 // Attention of query tiles of 16, 32 or 64 rows over keys and values in pages (16-bit or e4m3) or in rows, on mma.sync: what one new token a
 // sequence, or a few, take. With few rows a key is used for too little arithmetic to be anything but a stream, so the kernel is
-// built like one: 128 threads, two CTAs an SM, chunks of 64 positions on their way (cp.async, 16-byte pieces under an XOR swizzle that makes
+// built like one: 128 threads, two CTAs an SM (three of codes), shares of the work by weight or clusters by item, chunks of 64 positions on their way (cp.async, 16-byte pieces under an XOR swizzle that makes
 // ldmatrix conflict-free) while one is worked on, also across the ends of items.
 //
 // One pass: a warp holds 16 rows' queries as A fragments, takes scores of its positions of a chunk, the running maximum m and sum l of

@@ -106,7 +106,7 @@ __device__ __forceinline__ float max_nan(float a, float b) {            // NaN i
 
 // T: type of the projection's rows; E4M3: the cache holds codes, else values of T. Queries, keys and values are a pass each: what an element and its pair's other
 // one are multiplied with (norm's weight times cosine, and sine) stays in registers for all heads, and the root mean square comes last.
-// Bound by instructions at three CTAs an SM (some 6700 tokens of 32 + 2 x 8 heads of 128 with norms into e4m3 50 us, 3.9 TB/s; 8192 into bf16 44, 4.5 TB/s). Before heads were
+// Bound by instructions at three CTAs an SM (some 6700 tokens of 32 + 2 x 8 heads of 128 with norms into e4m3 49.7 us, 4.1 TB/s; 8192 into bf16 44, 4.5 TB/s). Before heads were
 // asked for a batch ahead, with four rows a batch: 52.7; four CTAs 53.6, with two rows 58.1; two CTAs with six 60.4; two warps a token 72.
 template <typename T, int D, bool E4M3>
 __global__ void __launch_bounds__(kThreads, 3) append_kernel(const AppendParams p) {
