@@ -91,6 +91,8 @@ class PagedCache:
         _index("page_table", table, self.k.device, 2)
         if table.stride(1) != 1 and table.shape[1] > 1:
             raise ValueError("page_table: a sequence's entries have to lie side by side")
+        if table.shape[0] > 1 and table.stride(0) < table.shape[1]:
+            table = table.contiguous()                          # (rows that share memory, as those of one expanded row do)
         c = _lib.PagedCacheArgs()
         c.struct_size, c.elem = ctypes.sizeof(c), _CACHE_ELEM[self.k.dtype]
         c.k, c.v = self.k.data_ptr(), self.v.data_ptr()
@@ -98,7 +100,8 @@ class PagedCache:
             c.k_exp, c.v_exp = self.k_exp.data_ptr(), self.v_exp.data_ptr()
         c.pages, c.kv_heads, c.page_size, c.head_dim = self.k.shape
         c.table, c.table_width = table.data_ptr(), table.shape[1]
-        c.table_stride = max(table.stride(0), table.shape[1]) if table.shape[0] > 1 else table.shape[1]
+        c.table_stride = table.stride(0) if table.shape[0] > 1 else table.shape[1]
+        c.table_tensor = table                                  # (as long as the call needs it)
         return c
 
 

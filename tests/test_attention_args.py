@@ -180,3 +180,21 @@ def test_rotary_frequencies():
     for bad in ((63, {}), (64, {"factor": 0.0}), (64, {"bands": (4.0, 1.0, 8192)})):
         with pytest.raises(ValueError):
             attention.rotary_frequencies(bad[0], device="cpu", **bad[1])
+
+
+@pytest.mark.parametrize("table", [
+    torch.tensor([[2, 0, 3]], dtype=torch.int32).expand(4, 3),                                            # one row for all sequences
+    torch.arange(5, dtype=torch.int32).as_strided((2, 4), (1, 1)),                                        # rows that overlap
+    torch.tensor([[2]], dtype=torch.int32).expand(3, 1),
+    torch.arange(12, dtype=torch.int32).view(3, 4)[:, :2],                                                # rows further apart than they are long
+    torch.arange(12, dtype=torch.int32).view(3, 4)[1:2],
+])
+def test_tables_as_the_kernels_read_them(table):
+    """Entry i of sequence s is at s * table_stride + i, whatever the tensor's strides."""
+    c = _cache()._with(table)
+    assert c.table_stride >= c.table_width == table.shape[1]
+    held = (table if c.table == table.data_ptr() else c.table_tensor).untyped_storage()
+    last = c.table + 4 * ((table.shape[0] - 1) * c.table_stride + c.table_width)
+    assert held.data_ptr() <= c.table and last <= held.data_ptr() + held.nbytes(), "entries behind the table's memory"
+    at = ctypes.cast(c.table, ctypes.POINTER(ctypes.c_int32))
+    assert [[at[s * c.table_stride + i] for i in range(table.shape[1])] for s in range(table.shape[0])] == table.tolist()

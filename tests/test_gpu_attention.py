@@ -707,3 +707,31 @@ def test_no_sequences():
     q = torch.zeros((0, 4, 64), dtype=BF, device=DEV)
     assert attention.paged_attention(q, cache, torch.zeros((0, 1), dtype=torch.int32, device=DEV), none).shape == q.shape
     assert attention.prompt_attention(q, q[:, :2], q[:, :2], torch.zeros((1,), dtype=torch.int32, device=DEV)).shape == q.shape
+
+
+@pytest.mark.parametrize("cache_dtype", [BF, E4M3])
+@pytest.mark.parametrize("new", [1, 4, 40])
+def test_tables_whose_rows_share_memory(cache_dtype, new):
+    """Several sequences over one prefix: one row of pages expanded to all of them, rows that overlap, and the same rows written out."""
+    gen = _gen(41)
+    seqs, heads, kv, dim, page = 5, 8, 2, 128, 32
+    cache, row, _, _ = _paged([320], kv, dim, page, cache_dtype, gen)
+    lens, cu = R.lengths([320, 100, 41, 64, 57], DEV), R.starts([new] * seqs, DEV)
+    flat = row[0].clone()                                          # ten pages: rows of six entries that begin one behind the other
+    q = torch.randn((seqs * new, heads, dim), generator=gen, device=DEV).to(BF)
+    few = R.lengths([192, 100, 41, 64, 57], DEV)
+    for table, n in ((row.expand(seqs, -1), lens), (row[:, :1].expand(seqs, -1), R.lengths([32] * seqs, DEV)), (flat.as_strided((seqs, 6), (1, 1)), few)):
+        whole = table.contiguous()
+        assert table.stride(0) < table.shape[1] <= whole.stride(0)
+        assert torch.equal(attention.paged_attention(q, cache, table, n, cu), attention.paged_attention(q, cache, whole, n, cu))
+        cu_kv, total = R.starts(n.tolist(), DEV), int(n.sum())
+        assert all(torch.equal(a, b) for a, b in zip(attention.read_pages(cache, table, cu_kv, total), attention.read_pages(cache, whole, cu_kv, total)))
+    # appended through one row of the table: position 10 s of the pages that all sequences share
+    x = torch.randn((seqs, (heads + 2 * kv) * dim), generator=gen, device=DEV).to(BF)
+    at = R.lengths([10 * s + 1 for s in range(seqs)], DEV)
+    caches = [PagedCache(*(t if t is None else t.clone() for t in (cache.k, cache.v, cache.k_exp, cache.v_exp))) for _ in range(2)]
+    a, b = (attention.append(x, c, t, at, heads=heads) for c, t in zip(caches, (row.expand(seqs, -1), row.repeat(seqs, 1))))
+    assert torch.equal(a, b)
+    for name in ("k", "v") + (("k_exp", "v_exp") if cache_dtype == E4M3 else ()):
+        m, n = (getattr(c, name).view(torch.uint8) for c in caches)
+        assert torch.equal(m, n) and not torch.equal(m, getattr(cache, name).view(torch.uint8))
