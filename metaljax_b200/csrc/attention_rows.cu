@@ -11,7 +11,7 @@
 // e4m3 codes: with one row of 16 a warp takes them straight into its B fragments as f16, one conversion a pair (a bf16 takes five
 // instructions a pair, with which 64 sequences of 2000 to 8000 positions took 249 us; now 171, 3.9 TB/s, bound by instructions: 687 for 16
 // positions): of keys four codes of a row a step (the queries' elements in the order that makes), of values the codes of its four positions,
-// paired by a byte permutation. The queries become f16 under a power of two, the rows' powers of two go to the scores and to the weights. Where warps share positions, the one that asked for a chunk's rows turns them into bf16 (exactly) next to the chunk in
+// paired by a byte permutation. A row's queries become f16 under a power of two of its own, the rows' powers of two go to the scores and to the weights. Where warps share positions, the one that asked for a chunk's rows turns them into bf16 (exactly) next to the chunk in
 // shared memory.
 //
 // Masked positions: scores are selected, not added to. A value that is no number at a masked position would still be 0 * NaN in the sum, so
@@ -241,7 +241,7 @@ __global__ void __launch_bounds__(kThreads, (RowsLayout<D, SOURCE, RW>::kCtas)) 
   int limit[2];                                          // last position that the thread's two rows see (-1: none)
   int tile_first_limit = 0, tile_rows = 0;
   int begun = 0;                                         // first unit of this item here
-  [[maybe_unused]] float q_scale = 0.0f;                 // (codes) the queries' power of two and the scale
+  [[maybe_unused]] float q_scale[2] = {};                // (codes) the power of two of the queries of the thread's two rows, and the scale
   [[maybe_unused]] float v_unit = 1.0f, v_rest = 1.0f;
   [[maybe_unused]] int v_top = 0;                        // (codes) the largest exponent of a row of values so far: the sums are in units of 2^v_top
 
@@ -250,7 +250,7 @@ __global__ void __launch_bounds__(kThreads, (RowsLayout<D, SOURCE, RW>::kCtas)) 
     const int row0 = c.t * R, rows = c.span.n * w.group - row0;
     tile_rows = rows < R ? rows : R;
     tile_first_limit = w.causal ? c.span.len - c.span.n + row0 / w.group : c.span.len - 1;
-    [[maybe_unused]] float big = 0.0f;
+    [[maybe_unused]] float big[2] = {};
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       const int r = rw * 16 + (lane >> 2) + 8 * i;
@@ -271,8 +271,8 @@ __global__ void __launch_bounds__(kThreads, (RowsLayout<D, SOURCE, RW>::kCtas)) 
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
             const float2 f = unpack2<T>(e ? x.y : x.x);
-            if (fabsf(f.x) <= 3.402823466e38f) big = fmaxf(big, fabsf(f.x));
-            if (fabsf(f.y) <= 3.402823466e38f) big = fmaxf(big, fabsf(f.y));
+            if (fabsf(f.x) <= 3.402823466e38f) big[i] = fmaxf(big[i], fabsf(f.x));
+            if (fabsf(f.y) <= 3.402823466e38f) big[i] = fmaxf(big[i], fabsf(f.y));
           }
         }
       } else {
@@ -288,21 +288,24 @@ __global__ void __launch_bounds__(kThreads, (RowsLayout<D, SOURCE, RW>::kCtas)) 
 #pragma unroll
       for (int i = 0; i < 4; ++i) o[n][i] = 0.0f;
     if constexpr (kDirect) {
-      // f16 under a power of two that brings the tile's largest element to [2^14, 2^15): elements down to 2^-31 of it keep all their bits
+      // f16 under a power of two for each row, that brings its largest element to [2^14, 2^15): elements down to 2^-31 of it keep all their bits
 #pragma unroll
-      for (int x = 16; x > 0; x >>= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, x));
-      int e = 0;
-      if (big > 0.0f) frexpf(big, &e);
-      e = e < -100 ? -100 : e;
-      const float up = __uint_as_float(static_cast<uint32_t>(15 - e + 127) << 23);
-      q_scale = __uint_as_float(static_cast<uint32_t>(e - 15 + 127) << 23) * p.scale_log2;
+      for (int i = 0; i < 2; ++i) {
+        big[i] = fmaxf(big[i], __shfl_xor_sync(0xffffffffu, big[i], 1));
+        big[i] = fmaxf(big[i], __shfl_xor_sync(0xffffffffu, big[i], 2));
+        int e = 0;
+        if (big[i] > 0.0f) frexpf(big[i], &e);
+        e = e < -100 ? -100 : e;
+        const float up = __uint_as_float(static_cast<uint32_t>(15 - e + 127) << 23);
+        q_scale[i] = __uint_as_float(static_cast<uint32_t>(e - 15 + 127) << 23) * p.scale_log2;
 #pragma unroll
-      for (int kk = 0; kk < D / 16; ++kk)
+        for (int kk = 0; kk < D / 16; ++kk)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float2 f = unpack2<T>(q[kk][i]);
-          q[kk][i] = pack2<__half>(f.x * up, f.y * up);
-        }
+          for (int j = i; j < 4; j += 2) {
+            const float2 f = unpack2<T>(q[kk][j]);
+            q[kk][j] = pack2<__half>(f.x * up, f.y * up);
+          }
+      }
       v_top = -1000;
       v_unit = v_rest = 1.0f;
     }
@@ -413,11 +416,11 @@ __global__ void __launch_bounds__(kThreads, (RowsLayout<D, SOURCE, RW>::kCtas)) 
           for (int e = 0; e < 2; ++e) {
             const uint32_t kb = e ? k2 >> 8 : k2 & 255, vb = e ? v2 >> 8 : v2 & 255;
             if (plain) {
-              k_scale[n][e] = __uint_as_float(kb << 23) * q_scale;
+              k_scale[n][e] = __uint_as_float(kb << 23);
               v_scale[n][e] = __uint_as_float(vb << 23) * v_unit * v_rest;
             } else {
               const bool in = kw * SN + n * 8 + (lane & 3) * 2 + e < c.span.len - pos0;
-              k_scale[n][e] = (in ? row_scale(kb) : 1.0f) * q_scale;
+              k_scale[n][e] = in ? row_scale(kb) : 1.0f;
               v_scale[n][e] = (in ? row_scale(vb) : 0.0f) * v_unit * v_rest;
             }
           }
@@ -454,7 +457,7 @@ __global__ void __launch_bounds__(kThreads, (RowsLayout<D, SOURCE, RW>::kCtas)) 
       for (int n = 0; n < SN / 8; ++n)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          s[n][i] *= kDirect ? k_scale[n][i & 1] : p.scale_log2;
+          s[n][i] *= kDirect ? k_scale[n][i & 1] * q_scale[i >> 1] : p.scale_log2;
         }
       if (edge) {
 #pragma unroll

@@ -735,3 +735,31 @@ def test_tables_whose_rows_share_memory(cache_dtype, new):
     for name in ("k", "v") + (("k_exp", "v_exp") if cache_dtype == E4M3 else ()):
         m, n = (getattr(c, name).view(torch.uint8) for c in caches)
         assert torch.equal(m, n) and not torch.equal(m, getattr(cache, name).view(torch.uint8))
+
+
+# ---- e4m3 pages: heads, rows and positions have nothing to do with one another ----
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("news, heads", [([1, 1, 1], 4), ([1, 1, 1], 16), ([3, 1, 2], 4)])
+@pytest.mark.parametrize("longest", [300, 9000])
+def test_e4m3_heads_of_very_different_sizes(dim, news, heads, longest):
+    """Queries of one head 2^45 or 2^100 above the others, far below them, of zeros or with infinities: the other heads' results are as good as
+    without it, and so is its own where it has one."""
+    gen = _gen(51)
+    lens = [longest, 64, 77]
+    cache, table, ks, vs = _paged(lens, 1, dim, 64, E4M3, gen)
+    q = torch.randn((sum(news), heads, dim), generator=gen, device=DEV).to(BF)
+    cu = None if max(news) == 1 else R.starts(news, DEV)
+    for change in (1.0, 2.0 ** 45, 2.0 ** 100, torch.inf, 0.0, 2.0 ** -60):
+        x = q.clone()
+        x[:, 1] *= change
+        keep = torch.ones(heads, dtype=torch.bool, device=DEV)
+        keep[1] = change <= 1
+        got = attention.paged_attention(x, cache, table, R.lengths(lens, DEV), cu)
+        at = 0
+        for s, n in enumerate(news):
+            k, v = (y.expand(-1, heads, -1)[:, keep] for y in (ks[s], vs[s]))
+            want, size = R.attend_fast(x[at: at + n, keep].double(), k, v, lens[s] - n, True, dim ** -0.5)
+            R.close(got[at: at + n, keep], want, size, BF, products=16.0 * 8)          # (keys here are up to eight times N(0, 1))
+            at += n
