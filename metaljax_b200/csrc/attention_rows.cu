@@ -103,6 +103,7 @@ __device__ __forceinline__ void store_row(const RowsParams& p, const UnitCursor&
 
 // CTAS = 1: shares by weight, which attend_join_kernel joins. CTAS > 1: clusters of CTAS take whole items (in turn, if there are more than clusters), every CTA an
 // equal run of the units, and join them out of one another's shared memory: the first stages of the ring, and maxima and sums of weights behind everything else.
+// (They are two an SM at most, and have the registers of two: 8 sequences of up to 2000 positions of codes, two tokens each, 18.1 us, with those of three 21.2.)
 template <typename Tiles>
 __device__ __forceinline__ bool cluster_item(const AttentionWork& w, int item, int rank, int ctas, UnitCursor* at) {
   int n = item / w.kv_heads;                            // tile of all sequences'
@@ -141,7 +142,7 @@ __device__ __forceinline__ bool cluster_item(const AttentionWork& w, int item, i
 }
 
 template <typename T, int D, int RW, int SOURCE, int CTAS>
-__global__ void __launch_bounds__(kThreads, (RowsLayout<D, SOURCE, RW>::kCtas)) attend_rows_kernel(const RowsParams p) {
+__global__ void __launch_bounds__(kThreads, (CTAS > 1 ? 2 : RowsLayout<D, SOURCE, RW>::kCtas)) attend_rows_kernel(const RowsParams p) {
   using L = RowsLayout<D, SOURCE, RW>;
   constexpr bool kPaged = SOURCE != kRowsSource, kE4m3 = L::kE4m3;
   constexpr int R = 16 * RW, KW = 4 / RW, SN = kChunk / KW;               // rows of a tile; warps on the same rows; a warp's positions of a chunk
@@ -242,8 +243,15 @@ __global__ void __launch_bounds__(kThreads, (RowsLayout<D, SOURCE, RW>::kCtas)) 
   int tile_first_limit = 0, tile_rows = 0;
   int begun = 0;                                         // first unit of this item here
   [[maybe_unused]] float q_scale[2] = {};                // (codes) the power of two of the queries of the thread's two rows, and the scale
-  [[maybe_unused]] float v_unit = 1.0f, v_rest = 1.0f;
-  [[maybe_unused]] int v_top = 0;                        // (codes) the largest exponent of a row of values so far: the sums are in units of 2^v_top
+  // (codes) The weights of the values, p * 2^e with e a row's exponent, are f16 too, times a power of two for each row of queries, `v_unit`, which its sums have as
+  // well: 2^(6 - t), where 2^(t - 4) is about the largest weight that this row has had (0: none yet). So a weight loses bits 2^18 below the largest and is lost
+  // 2^27 below it, however far the rows' exponents are apart, and rows that a query does not see, or gives no weight, count for nothing. No weight is above
+  // 2^(e + 8): while e <= t + 1 none is above f16's range, and the weights themselves are looked at in chunks with a larger exponent only.
+  constexpr int kNone = -1000;
+  [[maybe_unused]] float v_unit[2] = {};
+  [[maybe_unused]] int t_low = kNone, t_high = kNone;     // the least and the largest t of the warp's rows (t_low kNone: one has none, or they are to be looked at)
+  auto unit_of = [](int t) { return __uint_as_float(static_cast<uint32_t>(133 - t) << 23); };
+  auto exponent_of = [](float unit) { return 133 - static_cast<int>(__float_as_uint(unit) >> 23); };
 
   auto begin_item = [&]() {
     begun = c.u;
@@ -306,8 +314,8 @@ __global__ void __launch_bounds__(kThreads, (RowsLayout<D, SOURCE, RW>::kCtas)) 
             q[kk][j] = pack2<__half>(f.x * up, f.y * up);
           }
       }
-      v_top = -1000;
-      v_unit = v_rest = 1.0f;
+      v_unit[0] = v_unit[1] = 0.0f;
+      t_low = t_high = kNone;
     }
   };
 
@@ -382,47 +390,27 @@ __global__ void __launch_bounds__(kThreads, (RowsLayout<D, SOURCE, RW>::kCtas)) 
       for (int n = 0; n < SN / 8; ++n)
 #pragma unroll
         for (int i = 0; i < 4; ++i) s[n][i] = 0.0f;
-      float k_scale[SN / 8][2], v_scale[SN / 8][2];         // (codes: of the thread's columns; positions behind the end: 1)
-      [[maybe_unused]] bool wide = false;
+      [[maybe_unused]] float k_scale[SN / 8][2], v_scale[SN / 8][2];        // (codes: of the thread's columns; positions behind the end: 1 and 0)
+      [[maybe_unused]] uint32_t v_bytes[SN / 8];
+      [[maybe_unused]] bool plain = true;
+      [[maybe_unused]] int low = 0, high = 0;               // (codes) exponents of this warp's rows of values
       [[maybe_unused]] float s2[SN / 8][4] = {};            // (two chains of products)
       if constexpr (kDirect) {
-        // The weights of the values are f16 too: p * 2^(e - v_top + 6), e a row's exponent. Rows more than 2^12 below the largest would lose bits where that one's
-        // weight is small: then these positions' products are taken in bf16 (`wide`).
         const uint32_t bytes = stage + 2 * L::kHalf + kw * SN;
         const bool there = lane < SN && kw * SN + lane < c.span.len - pos0;
         const int k_byte = there ? static_cast<int>(lds8(bytes + lane)) : 127, v_byte = there ? static_cast<int>(lds8(bytes + kChunk + lane)) : 255;
-        const int high = __reduce_max_sync(0xffffffffu, v_byte == 255 ? -1000 : v_byte - 127), low = __reduce_min_sync(0xffffffffu, v_byte == 255 ? 1000 : v_byte - 127);
-        if (high > v_top) {
-          if (v_top > -1000) {
-            const float down = high - v_top > 126 ? 0.0f : __uint_as_float(static_cast<uint32_t>(127 + v_top - high) << 23);
-#pragma unroll
-            for (int n = 0; n < D / 8; ++n)
-#pragma unroll
-              for (int i = 0; i < 4; ++i) o[n][i] *= down;
-          }
-          v_top = high;
-          // 2^(6 - v_top), in two steps that are both in range
-          const int near = v_top > 64 ? 64 : v_top < -64 ? -64 : v_top;
-          v_unit = __uint_as_float(static_cast<uint32_t>(127 + 6 - near) << 23);
-          v_rest = __uint_as_float(static_cast<uint32_t>(127 + near - (v_top < -127 ? -127 : v_top)) << 23);
-        }
-        wide = v_top - low > 12;
+        high = __reduce_max_sync(0xffffffffu, v_byte == 255 ? kNone : v_byte - 127);
+        low = __reduce_min_sync(0xffffffffu, v_byte == 255 ? 1000 : v_byte - 127);
         // ordinary rows: all there, and numbers
-        const bool plain = __all_sync(0xffffffffu, lane >= SN || (there && k_byte != 255 && k_byte != 0 && v_byte != 255 && v_byte != 0));
+        plain = __all_sync(0xffffffffu, lane >= SN || (there && k_byte != 255 && k_byte != 0 && v_byte != 255 && v_byte != 0));
 #pragma unroll
         for (int n = 0; n < SN / 8; ++n) {
-          const uint32_t k2 = lds16(bytes + n * 8 + (lane & 3) * 2), v2 = lds16(bytes + kChunk + n * 8 + (lane & 3) * 2);
+          const uint32_t k2 = lds16(bytes + n * 8 + (lane & 3) * 2);
+          v_bytes[n] = lds16(bytes + kChunk + n * 8 + (lane & 3) * 2);
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
-            const uint32_t kb = e ? k2 >> 8 : k2 & 255, vb = e ? v2 >> 8 : v2 & 255;
-            if (plain) {
-              k_scale[n][e] = __uint_as_float(kb << 23);
-              v_scale[n][e] = __uint_as_float(vb << 23) * v_unit * v_rest;
-            } else {
-              const bool in = kw * SN + n * 8 + (lane & 3) * 2 + e < c.span.len - pos0;
-              k_scale[n][e] = in ? row_scale(kb) : 1.0f;
-              v_scale[n][e] = (in ? row_scale(vb) : 0.0f) * v_unit * v_rest;
-            }
+            const uint32_t kb = e ? k2 >> 8 : k2 & 255;
+            k_scale[n][e] = plain ? __uint_as_float(kb << 23) : kw * SN + n * 8 + (lane & 3) * 2 + e < c.span.len - pos0 ? row_scale(kb) : 1.0f;
           }
           const int r = kw * SN + n * 8 + (lane >> 2);
 #pragma unroll
@@ -451,7 +439,7 @@ __global__ void __launch_bounds__(kThreads, (RowsLayout<D, SOURCE, RW>::kCtas)) 
         }
       }
       const int warp_pos = pos0 + kw * SN;
-      const bool edge = warp_pos + SN - 1 > tile_first_limit || tile_rows < R;
+      const bool edge = warp_pos + SN - 1 > tile_first_limit;          // (rows behind the tile's last: whatever their sums are, none reads them)
       float top[2] = {-INFINITY, -INFINITY};
 #pragma unroll
       for (int n = 0; n < SN / 8; ++n)
@@ -479,15 +467,33 @@ __global__ void __launch_bounds__(kThreads, (RowsLayout<D, SOURCE, RW>::kCtas)) 
       if (__any_sync(0xffffffffu, top[0] > m[0] + 8.0f || top[1] > m[1] + 8.0f)) {
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          const float now = fmaxf(m[i], top[i]), shrink = ex2(m[i] - (now == -INFINITY ? 0.0f : now));
-          m[i] = now;
+          const float now = fmaxf(m[i], top[i]), base = now == -INFINITY ? 0.0f : now;
+          float shrink = ex2(m[i] - base);
           l[i] *= shrink;
+          if constexpr (kDirect) {                          // the weights so far shrink, and their power of two with them
+            if (v_unit[i] > 0.0f && now > m[i]) {
+              const int t = exponent_of(v_unit[i]), fall = min(static_cast<int>(fminf(now - m[i], 300.0f)), t + 117);
+              v_unit[i] = unit_of(t - fall);
+              shrink = ex2(m[i] - base + static_cast<float>(fall));
+            }
+          }
+          m[i] = now;
 #pragma unroll
           for (int n = 0; n < D / 8; ++n) {
             o[n][2 * i] *= shrink;
             o[n][2 * i + 1] *= shrink;
           }
         }
+        t_low = kNone;
+      }
+      if constexpr (kDirect) {
+#pragma unroll
+        for (int n = 0; n < SN / 8; ++n)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const uint32_t vb = e ? v_bytes[n] >> 8 : v_bytes[n] & 255;
+            v_scale[n][e] = plain ? __uint_as_float(vb << 23) : warp_pos + n * 8 + (lane & 3) * 2 + e < c.span.len ? row_scale(vb) : 0.0f;
+          }
       }
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
@@ -508,11 +514,68 @@ __global__ void __launch_bounds__(kThreads, (RowsLayout<D, SOURCE, RW>::kCtas)) 
           for (int i = 0; i < 4; ++i)
             if (warp_pos + n * 8 + (lane & 3) * 2 + (i & 1) > limit[i >> 1]) s[n][i] = 0.0f;
       }
+      // Rows of values more than 2^14 below t would lose bits where their weights are small: rows of queries that see one take this chunk's weights in bf16.
+      [[maybe_unused]] bool wide[2] = {false, false}, any_wide = false, all_wide = false;
+      if constexpr (kDirect) {
+        const bool apart = warp_pos + SN - 1 > tile_first_limit && tile_first_limit < c.span.len - 1;        // positions that only some rows see: all that follows is by what a row sees
+        if (high > t_low + 1 || t_high - low > 14 || apart) {
+          int least = 1000, most = kNone, mine[2];
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            float big = 0.0f;
+#pragma unroll
+            for (int n = 0; n < SN / 8; ++n) big = fmaxf(big, fmaxf(s[n][2 * i], s[n][2 * i + 1]));
+            big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 1));
+            big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 2));
+            const int old = v_unit[i] > 0.0f ? exponent_of(v_unit[i]) : kNone, t = max(static_cast<int>(__float_as_uint(big) >> 23) - 127 + 4, -117);
+            mine[i] = old;
+            if (big > 0.0f && t > old) {
+              if (old != kNone) {
+                const float down = t - old > 126 ? 0.0f : __uint_as_float(static_cast<uint32_t>(127 - (t - old)) << 23);
+#pragma unroll
+                for (int n = 0; n < D / 8; ++n) {
+                  o[n][2 * i] *= down;
+                  o[n][2 * i + 1] *= down;
+                }
+              }
+              v_unit[i] = unit_of(t);
+              mine[i] = t;
+            }
+            if (limit[i] >= 0) {
+              least = min(least, mine[i]);
+              most = max(most, mine[i]);
+            }
+          }
+          t_low = __reduce_min_sync(0xffffffffu, least);
+          t_high = __reduce_max_sync(0xffffffffu, most);
+          if (t_high - low > 14) {
+            // the least exponent of the first 1, 2, .. 16 positions, in a lane each
+            const int byte = lane < SN && warp_pos + lane < c.span.len ? static_cast<int>(lds8(stage + 2 * L::kHalf + kChunk + kw * SN + lane)) : 255;
+            int upto = byte == 255 ? 1000 : byte - 127;
+#pragma unroll
+            for (int d = 1; d < SN; d <<= 1) {
+              const int x = __shfl_up_sync(0xffffffffu, upto, d);
+              if (lane >= d) upto = min(upto, x);
+            }
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              const int last = limit[i] - warp_pos, seen = __shfl_sync(0xffffffffu, upto, last < 0 ? 0 : last < SN ? last : SN - 1);
+              wide[i] = last >= 0 && mine[i] - seen > 14;
+            }
+            any_wide = __any_sync(0xffffffffu, wide[0] || wide[1]);
+            all_wide = __all_sync(0xffffffffu, (wide[0] || limit[0] < 0) && (wide[1] || limit[1] < 0));
+          }
+        }
+#pragma unroll
+        for (int n = 0; n < SN / 8; ++n)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) s[n][i] *= v_unit[i >> 1];
+      }
       // ---- weights times values ----
 #pragma unroll
       for (int n = 0; n < SN / 16; ++n) {
-        const uint32_t a[4] = {pack2<MT>(s[2 * n][0], s[2 * n][1]), pack2<MT>(s[2 * n][2], s[2 * n][3]), pack2<MT>(s[2 * n + 1][0], s[2 * n + 1][1]),
-                               pack2<MT>(s[2 * n + 1][2], s[2 * n + 1][3])};
+        uint32_t a[4] = {pack2<MT>(s[2 * n][0], s[2 * n][1]), pack2<MT>(s[2 * n][2], s[2 * n][3]), pack2<MT>(s[2 * n + 1][0], s[2 * n + 1][1]),
+                         pack2<MT>(s[2 * n + 1][2], s[2 * n + 1][3])};
         if constexpr (kDirect) {
           // a thread's D / 8 codes of the four positions that its B fragments hold: column `lane / 4` of every fragment
           const int r = kw * SN + n * 16 + (lane & 3) * 2, g = lane >> 2;
@@ -533,23 +596,28 @@ __global__ void __launch_bounds__(kThreads, (RowsLayout<D, SOURCE, RW>::kCtas)) 
               codes[i][1] = v.y;
             }
           }
-          if (!wide) {
+          if (any_wide) {
+            uint32_t b[4];
 #pragma unroll
-            for (int x = 0; x < D / 32; ++x) {
-              mma16816<MT>(o[4 * x], a, code_half2<0>(codes[0][x], codes[1][x]), code_half2<0>(codes[2][x], codes[3][x]));
-              mma16816<MT>(o[4 * x + 1], a, code_half2<1>(codes[0][x], codes[1][x]), code_half2<1>(codes[2][x], codes[3][x]));
-              mma16816<MT>(o[4 * x + 2], a, code_half2<2>(codes[0][x], codes[1][x]), code_half2<2>(codes[2][x], codes[3][x]));
-              mma16816<MT>(o[4 * x + 3], a, code_half2<3>(codes[0][x], codes[1][x]), code_half2<3>(codes[2][x], codes[3][x]));
+            for (int i = 0; i < 4; ++i) {
+              b[i] = wide[i & 1] ? pack2<T>(s[2 * n + (i >> 1)][(i & 1) * 2], s[2 * n + (i >> 1)][(i & 1) * 2 + 1]) : 0;
+              if (wide[i & 1]) a[i] = 0;
             }
-          } else {
-            const uint32_t b[4] = {pack2<T>(s[2 * n][0], s[2 * n][1]), pack2<T>(s[2 * n][2], s[2 * n][3]), pack2<T>(s[2 * n + 1][0], s[2 * n + 1][1]),
-                                   pack2<T>(s[2 * n + 1][2], s[2 * n + 1][3])};
 #pragma unroll
             for (int x = 0; x < D / 32; ++x) {
               mma16816<T>(o[4 * x], b, code_pair<0>(codes[0][x], codes[1][x]), code_pair<0>(codes[2][x], codes[3][x]));
               mma16816<T>(o[4 * x + 1], b, code_pair<1>(codes[0][x], codes[1][x]), code_pair<1>(codes[2][x], codes[3][x]));
               mma16816<T>(o[4 * x + 2], b, code_pair<2>(codes[0][x], codes[1][x]), code_pair<2>(codes[2][x], codes[3][x]));
               mma16816<T>(o[4 * x + 3], b, code_pair<3>(codes[0][x], codes[1][x]), code_pair<3>(codes[2][x], codes[3][x]));
+            }
+          }
+          if (!all_wide) {
+#pragma unroll
+            for (int x = 0; x < D / 32; ++x) {
+              mma16816<MT>(o[4 * x], a, code_half2<0>(codes[0][x], codes[1][x]), code_half2<0>(codes[2][x], codes[3][x]));
+              mma16816<MT>(o[4 * x + 1], a, code_half2<1>(codes[0][x], codes[1][x]), code_half2<1>(codes[2][x], codes[3][x]));
+              mma16816<MT>(o[4 * x + 2], a, code_half2<2>(codes[0][x], codes[1][x]), code_half2<2>(codes[2][x], codes[3][x]));
+              mma16816<MT>(o[4 * x + 3], a, code_half2<3>(codes[0][x], codes[1][x]), code_half2<3>(codes[2][x], codes[3][x]));
             }
           }
         } else {
@@ -573,11 +641,21 @@ __global__ void __launch_bounds__(kThreads, (RowsLayout<D, SOURCE, RW>::kCtas)) 
         l[i] += __shfl_xor_sync(0xffffffffu, l[i], 2);
       }
       if constexpr (kDirect) {
-        const float unit = v_top > -1000 ? ldexpf(1.0f, v_top - 6) : 1.0f;
+        // In units of one, and both sums with the maximum under a power of two that leaves them 2^12 below the largest value: what joins up to as many of them
+        // stays in float32's range as the result does. (Of small values less: one factor in range.)
 #pragma unroll
-        for (int n = 0; n < D / 8; ++n)
+        for (int i = 0; i < 2; ++i) {
+          const int t = v_unit[i] > 0.0f ? exponent_of(v_unit[i]) : 6;
+          const int below = min(12 + min(max(static_cast<int>(__float_as_uint(l[i]) >> 23) - 126, 0), 48), t + 120);
+          const float unit = __uint_as_float(static_cast<uint32_t>(127 + t - 6 - below) << 23);
+          l[i] *= __uint_as_float(static_cast<uint32_t>(127 - below) << 23);
+          m[i] += static_cast<float>(below);
 #pragma unroll
-          for (int i = 0; i < 4; ++i) o[n][i] *= unit;
+          for (int n = 0; n < D / 8; ++n) {
+            o[n][2 * i] *= unit;
+            o[n][2 * i + 1] *= unit;
+          }
+        }
       }
       __syncthreads();
       float* const sums = reinterpret_cast<float*>(smem + (kE4m3 && !kDirect ? L::kRing : kCluster ? L::kStage : stage - ring));

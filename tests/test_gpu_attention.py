@@ -763,3 +763,69 @@ def test_e4m3_heads_of_very_different_sizes(dim, news, heads, longest):
             want, size = R.attend_fast(x[at: at + n, keep].double(), k, v, lens[s] - n, True, dim ** -0.5)
             R.close(got[at: at + n, keep], want, size, BF, products=16.0 * 8)          # (keys here are up to eight times N(0, 1))
             at += n
+
+
+@pytest.mark.parametrize("byte", [140, 187, 246, 10, 255])
+@pytest.mark.parametrize("news, group", [([2, 3], 4), ([4, 1], 4), ([2, 2], 1), ([7, 3], 2), ([16, 9], 1)])
+@pytest.mark.parametrize("longest", [130, 2000, 9000])
+def test_e4m3_positions_that_a_token_does_not_see_leave_its_bits(byte, news, group, longest):
+    """The last new tokens' rows of values under other powers of two, from the least to the largest, and as no numbers: the tokens before
+    them have the bits that they have without."""
+    gen = _gen(52)
+    lens, kv, dim = [longest, longest // 3 + 20], 2, 128
+    cache, table, ks, _ = _paged(lens, kv, dim, 64, E4M3, gen)
+    q = torch.randn((sum(news), group * kv, dim), generator=gen, device=DEV).to(BF)
+    args = (cache, table, R.lengths(lens, DEV), R.starts(news, DEV))
+    first = attention.paged_attention(q, *args)
+    for back in (1, 2):
+        kept = cache.v_exp.clone()
+        for s, n in enumerate(lens):
+            if back < news[s]:
+                pos = n - back
+                cache.v_exp[table[s, pos // 64].long(), 0, pos % 64] = byte
+        got = attention.paged_attention(q, *args)
+        vs = attention.read_pages(cache, table, R.starts(lens, DEV), sum(lens))[1].split(lens)
+        cache.v_exp.copy_(kept)
+        at = 0
+        for s, n in enumerate(news):
+            unseen = max(0, n - back) if back < n else n
+            assert torch.equal(got[at: at + unseen], first[at: at + unseen])
+            assert torch.equal(got[at: at + n, group:], first[at: at + n, group:])          # (the other key head)
+            if unseen < n:                                           # ... and those that see them the sums of what stands there
+                want, size = R.attend_fast(q[at + unseen: at + n].double(), ks[s], vs[s].double(), lens[s] - n + unseen, True, dim ** -0.5)
+                R.close(got[at + unseen: at + n], want, size.nan_to_num(0, 0, 0), BF, products=16.0 * 8)
+            at += n
+
+
+@pytest.mark.parametrize("heads", [4, 16])
+@pytest.mark.parametrize("at, span", [(0, 1), (5, 1), (150, 1), (298, 1), (0, 64), (64, 64), (192, 64)])
+def test_e4m3_large_values_of_small_weight(heads, at, span):
+    """Rows of values far above the others, at positions whose weights make up for it, or are nothing: their share of the sums is their weights',
+    and the other rows keep theirs, whether they come before them or behind."""
+    gen = _gen(53)
+    # powers of two: of the other rows, of these, and (downwards) of these rows' weights
+    cases = [(0, 30, 30.0), (0, 45, 44.0), (0, 60, 62.0), (0, 100, 90.0), (0, 117, 117.0), (0, 117, 124.0), (0, 117, 300.0), (0, 13, 40.0), (-60, 110, 300.0), (-100, 60, 300.0),
+             (-60, 50, 112.0), (-40, 80, 118.0)]
+    dim, n = 128, 300
+    cache, table, ks, vs = _paged([n] * len(cases), 1, dim, 32, E4M3, gen)
+    pos = torch.arange(n, device=DEV)
+    here = (pos >= at) & (pos < at + span)
+    for s, (base, up, _) in enumerate(cases):
+        where, off = table[s].long()[pos // 32], pos % 32
+        k = torch.zeros((n, 1, dim), device=DEV)                 # keys of one element, zero in the rows in question: their scores are `low` powers of two below
+        k[~here, :, 0] = 8.0
+        codes, exps = R.quantize(k)
+        cache.k.view(torch.uint8)[where, :, off], cache.k_exp[where, :, off] = codes.view(torch.uint8), exps
+        ks[s] = R.dequantized(codes, exps)
+        assert torch.equal(ks[s], k.double())
+        cache.v_exp[where, 0, off] = torch.where(here, torch.full_like(pos, 127 + up), cache.v_exp[where, 0, off].long() + base).to(torch.uint8)
+        vs[s] = R.dequantized(cache.v[where, :, off], cache.v_exp[where, :, off])
+    scale = 1.0 / 8
+    q = torch.zeros((len(cases), heads, dim), device=DEV)
+    q[:, :, 0] = torch.tensor([low for _, _, low in cases], device=DEV)[:, None] * 0.6875         # (about ln 2, in five bits: a score of 0.6875 * low)
+    q = q.to(BF)
+    got = attention.paged_attention(q, cache, table, R.lengths([n] * len(cases), DEV), scale=scale)
+    for s in range(len(cases)):
+        want, size = R.attend_fast(q[s: s + 1].double(), ks[s], vs[s], n - 1, True, scale)
+        # (scores of one exact product, up to 207; in powers of two up to 298, a float32 with a step of 2^-15: far below the bound's part for products of 300)
+        R.close(got[s: s + 1], want, size, BF, products=300.0)
