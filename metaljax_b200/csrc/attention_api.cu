@@ -125,7 +125,7 @@ extern "C" int qmm_cache_append(const qmm_paged_cache* cache, const qmm_append_a
   if (a->rotary_dim < 0 || a->rotary_dim > cache->head_dim || a->rotary_dim % 16) return fail(QMM_ERR_SHAPE, "cache_append: rotary_dim is a multiple of 16 up to head_dim");
   if (a->tokens == 0 || a->seqs == 0) return QMM_OK;
   if (!a->qkv || !a->q_out || !a->kv_lens || (a->rotary_dim && !a->freqs)) return fail(QMM_ERR_NULL, "cache_append: qkv, q_out, kv_lens and (with rotary_dim) freqs are required");
-  if (a->row_stride % 8 || a->row_stride < static_cast<int64_t>(a->heads + 2 * cache->kv_heads) * cache->head_dim)
+  if (a->row_stride % 8 || a->row_stride < (a->heads + 2 * static_cast<int64_t>(cache->kv_heads)) * cache->head_dim)
     return fail(QMM_ERR_LAYOUT, "cache_append: rows of qkv are a multiple of 8 elements apart, and no less than they are long");
   if (!aligned16(a->qkv) || !aligned16(a->q_out) || !aligned16(a->q_norm) || !aligned16(a->k_norm))
     return fail(QMM_ERR_LAYOUT, "cache_append: pointers must be 16-byte aligned");

@@ -198,3 +198,12 @@ def test_tables_as_the_kernels_read_them(table):
     assert held.data_ptr() <= c.table and last <= held.data_ptr() + held.nbytes(), "entries behind the table's memory"
     at = ctypes.cast(c.table, ctypes.POINTER(ctypes.c_int32))
     assert [[at[s * c.table_stride + i] for i in range(table.shape[1])] for s in range(table.shape[0])] == table.tolist()
+
+
+def test_rows_of_more_heads_than_32_bits_count_are_refused():
+    """A row of qkv of heads + 2 kv_heads, counted in 64 bits: no such row fits a stride of 512."""
+    c, _ = _args({"pages": 1, "kv_heads": 1 << 30})
+    a = _lib.AppendArgs()
+    a.struct_size, a.qkv, a.row_stride, a.q_out, a.tokens, a.seqs, a.heads = ctypes.sizeof(a), 256, 512, 256, 2, 2, 4
+    a.freqs, a.kv_lens = 256, 256
+    assert _lib.lib().qmm_cache_append(ctypes.byref(c), ctypes.byref(a), None) == 4, _lib.lib().qmm_last_error()
