@@ -154,9 +154,11 @@ int qmm_decode_attention(const void* qkv, void* k_cache, void* v_cache, void* ou
  * kv_lens[s] positions, so that token i of n stands at position kv_lens[s] - n + i. Rows behind
  * cu_q[seqs] belong to no sequence and are left as they are. Lengths, starts and tables are int32
  * on the device and are read by the kernels: nothing is copied to the host, and a captured call
- * may be replayed with other lengths. A page outside the cache, a length that its table has no
- * room for and a token before position 0 are reported (QMM_DEVICE_BAD_INDEX, as QMM_ERR_SHAPE from
- * qmm_poll_status) and never followed: such a page is read as page 0, and not written.
+ * may be replayed with other lengths. A page outside the cache and a length that its table has no
+ * room for are reported (QMM_DEVICE_BAD_INDEX, as QMM_ERR_SHAPE from qmm_poll_status) and never
+ * followed: such a page is read as page 0, and not written. A token before position 0 (a length
+ * below the number of new tokens) is reported and not written by qmm_cache_append; attention gives
+ * it zeros and reports nothing.
  *
  * An e4m3 cache holds a row (one position of one head) as codes under one power of two: with e the
  * smallest whole number for which the row's largest magnitude is at most 448 * 2^e (between -117 and
@@ -209,7 +211,11 @@ int qmm_cache_read(const qmm_paged_cache* cache, int64_t seqs, const int32_t* cu
 
 /* out[t, h] = sum_j softmax_j(scale * q[t, h] . k[j, h / group]) v[j, h / group] over the positions j of t's sequence that t sees:
  * those up to its own (causal), or all. What stands at other positions has no influence, whatever it is; a token that sees
- * none is zero. float32 sums and statistics; the weights of the values are rounded to q's type. */
+ * none is zero. float32 sums and statistics: weights below 2^-126 of the largest count for nothing, and the sums of weights times
+ * values, in parts of the positions too, are to stay in float32's range. The weights of the values are rounded to q's type. With an
+ * e4m3 cache and few query rows (16 or fewer a key head and sequence on average) queries and weights are held as f16 under powers of two of
+ * their own row: elements more than 2^31 below the largest of a query lose bits, and weights (times their value row's power of two) more than
+ * 2^18 below the largest that their row has had do, and are gone 2^27 below it. */
 typedef struct {
   uint32_t struct_size;     /* sizeof(qmm_attention_args) */
   int32_t elem;             /* QMM_BF16 or QMM_F16: of q, out, k and v */

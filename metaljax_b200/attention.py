@@ -166,7 +166,8 @@ def append(qkv, cache: PagedCache, page_table, kv_lens, cu_q=None, *, heads: int
     head divided by its root mean square (plus `eps` under the root) and multiplied by them. `freqs` (float64, see
     `rotary_frequencies`): the first `2 * len(freqs)` elements rotated, pairs half of that apart, or neighbours
     (`interleaved`). float32 arithmetic with angles from float64; rounded once, to the result's type or
-    the e4m3 cache's codes. Rows behind the last sequence are neither read nor written."""
+    the e4m3 cache's codes. Rows behind the last sequence are neither read nor written. A token before position 0 is
+    reported, and not written. (The queries of f16 rows have to be made bf16 to be attended over an e4m3 cache.)"""
     done = _lib.native().append(qkv, cache.k, cache.v, cache.k_exp, cache.v_exp, page_table, kv_lens, cu_q, heads, freqs, interleaved, q_norm, k_norm, eps, out)
     if done is not None:
         return _native(done)
@@ -284,8 +285,10 @@ def prompt_attention(q, k, v, cu_seqlens, *, causal: bool = True, scale=None, ou
 def paged_attention(q, cache: PagedCache, page_table, kv_lens, cu_q=None, *, causal: bool = True, scale=None, out=None):
     """Attention of new tokens over a cache that holds them already (`append`): `q` `[tokens, heads, head_dim]`, those of sequence s
     being rows `cu_q[s]` to `cu_q[s + 1] - 1` (None: one token each) and the last ones of its `kv_lens[s]` positions. A token
-    sees the positions up to its own, or (not `causal`) all of them; one that sees none is zero. q has the cache's type,
-    bf16 with an e4m3 cache. Returns `[tokens, heads, head_dim]`; rows that belong to no sequence are not written."""
+    sees the positions up to its own, or (not `causal`) all of them; one that sees none (before position 0, too: nothing is
+    reported) is zero. q has the cache's type, bf16 with an e4m3 cache. Returns `[tokens, heads, head_dim]`; rows that belong to
+    no sequence are not written. The kernel is chosen by how many new tokens a sequence has on average: many single tokens and a long
+    chunk are better made two calls."""
     done = _lib.native().paged_attention(q, cache.k, cache.v, cache.k_exp, cache.v_exp, page_table, kv_lens, cu_q, causal, scale, out)
     if done is not None:
         return _native(done)

@@ -9,7 +9,7 @@
 // for itself, and the CTA does not meet but at the ends of items. Pages of bf16 are bound by the memory: the same 64 sequences 206 us, 6.5 TB/s.
 //
 // e4m3 codes: with one row of 16 a warp takes them straight into its B fragments as f16, one conversion a pair (a bf16 takes five
-// instructions a pair, with which 64 sequences of 2000 to 8000 positions took 249 us; now 171, 3.9 TB/s, bound by instructions: 687 for 16
+// instructions a pair, with which 64 sequences of 2000 to 8000 positions took 249 us; now 171, 3.9 TB/s, bound by instructions: 680 for 16
 // positions): of keys four codes of a row a step (the queries' elements in the order that makes), of values the codes of its four positions,
 // paired by a byte permutation. A row's queries become f16 under a power of two of its own, the rows' powers of two go to the scores and to the weights. Where warps share positions, the one that asked for a chunk's rows turns them into bf16 (exactly) next to the chunk in
 // shared memory.
@@ -931,10 +931,12 @@ int launch_source(const RowsParams& p, int source, int rows, cudaStream_t stream
 
 // Clusters want neither the order of all units (2 us) nor a second launch to join (3.5 us): eight CTAs a sequence and key head where the device holds as many for all, at
 // two an SM, else four. They pay while no CTA has many positions to do: without shares by weight no others help it, and codes want three CTAs an SM. Measured with 8
-// key heads of 128, us, clusters / shares, tiles of 16 rows: 1 sequence of 2000 positions 8.5 / 12.3, 8000 15.0 / 16.2, 16000 19.6 / 19.3; 8 of 1000 to 4000 11 / 12.8,
-// 2000 to 8000 17 / 16.4; of codes: 1 of 4000 13.8 / 16.3, 8000 21.4 / 20.0; 8 of 500 to 2000 16 / 17.6, 1000 to 4000 25.8 / 21.6. Tiles of 32 rows: 1 of 4000 15.6 /
-// 17.2, 8000 23.0 / 20.7; 8 of 2000 17.5 / 20.9, 1000 to 4000 24.9 / 22.2. Tiles of 64 rows, against the kernel of 2 x 128: 1 of 4000 20.9 / 23.6; 8 of 2000 25.4 / 29.9;
-// 8 of 500 to 2000 with 40 rows on average and up to 76 in two tiles 26.5 / 21.7.
+// key heads of 128, us, clusters / shares, two calls' inputs in turn. Tiles of 16 rows: 1 sequence of 2000 positions 8.1 / 11.7, 8000 15.6 / 16.2, 16000 26.9 / 23.6; 8 of
+// 500 to 2000 11.6 / 12.8, 1000 to 4000 20.6 / 21.1, 2000 to 8000 36.0 / 35.1; of codes: 1 of 2000 10.8 / 15.3, 4000 15.0 / 16.5, 8000 23.6 / 20.1; 8 of 500 to 2000 16.2 / 18.1,
+// 1000 to 4000 26.0 / 22.2. (Heads of 64: 1 of 8000 11.4 / 13.2, 16000 17.9 / 16.0; 8 of 1000 to 4000 13.9 / 14.0; of codes: 1 of 4000 12.7 / 13.2, 8000 20.0 / 15.4; 8 of
+// 500 to 2000 13.4 / 14.1, 1000 to 4000 22.0 / 16.6.) Tiles of 32 rows: 1 of 4000 15.5 / 17.0, 8000 23.2 / 20.0; 8 of 2000 19.6 / 24.0, 1000 to 4000 27.1 / 28.1; of codes
+// 22.1 / 20.7, 36.3 / 23.8, 24.9 / 29.2, 40.4 / 35.7. Tiles of 64 rows, against the kernel of 2 x 128: 1 of 4000 21.1 / 23.2; 8 of 2000 26.6 / 31.4; of codes 29.2 / 28.8,
+// 32.0 / 38.7; 8 of 500 to 2000 with 40 rows on average and up to 76 in two tiles 26.5 / 21.7.
 int attend_cluster_ctas(const RowsParams& p, int source, int rows) {
   const int64_t items = static_cast<int64_t>(p.work.seqs) * p.work.kv_heads, room = 2 * device_sm_count();
   const int ctas = items * 8 <= room ? 8 : 4;

@@ -139,7 +139,8 @@ __global__ void __launch_bounds__(kThreads, 3) append_kernel(const AppendParams 
   const int64_t page = page_of(p.c, seq, pos, p.status);
   const int row = pos & ((1 << p.c.page_shift) - 1);
   for (int i = lane32; i < p.rotary_dim / 2; i += 32) {
-    // a fraction of a turn, exact to 2^-30 for positions up to 2^31; sine and cosine rounded once (from a fraction in 32 bits a third more of an e4m3 cache's codes of keys
+    // a fraction of a turn, off by some 2^-52 of the number of turns: 2^-35 at position 2^20, 2^-25 at 2^30, the last that a table allows, where a radian is a
+    // position; sine and cosine rounded once (from a fraction in 32 bits a third more of an e4m3 cache's codes of keys
     // were a step off: 15 in five million, now 10)
     const double turned = static_cast<double>(pos) * (__ldg(p.freqs + i) * 0.15915494309189533576888376337251);
     double s, c;

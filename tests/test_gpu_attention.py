@@ -829,3 +829,14 @@ def test_e4m3_large_values_of_small_weight(heads, at, span):
         want, size = R.attend_fast(q[s: s + 1].double(), ks[s], vs[s], n - 1, True, scale)
         # (scores of one exact product, up to 207; in powers of two up to 298, a float32 with a step of 2^-15: far below the bound's part for products of 300)
         R.close(got[s: s + 1], want, size, BF, products=300.0)
+
+
+@pytest.mark.parametrize("dtype, cache", CACHES)
+@pytest.mark.parametrize("group, kv, dim", [(33, 2, 128), (40, 1, 64), (64, 3, 128)])
+@pytest.mark.parametrize("longest", [70, 900, 9000])
+def test_more_query_heads_than_two_tiles_of_16(dtype, cache, group, kv, dim, longest):
+    """Up to 64 query heads a key head, one token each with and without starts, and a few."""
+    lens = [longest, 1, 0, 17, longest // 2]
+    for cu in (False, True):
+        _check_paged([1] * len(lens), lens, group * kv, kv, dim, 32, dtype, cache, cu=cu, seed=group)
+    _check_paged([3, 1, 0, 2, 5], lens[:2] + [4] + lens[3:], group * kv, kv, dim, 32, dtype, cache, seed=group)
